@@ -15,6 +15,7 @@
 #include <mutex>
 #include <string>
 
+#include "../../include/rwkv7m_lm_head.h"
 #include "../../include/rwkv7m_screening.h"
 #include "../../include/rwkv7m_timemix.h"
 #include "../../include/rwkv7m_wkv.h"
@@ -785,6 +786,136 @@ int output_backward_impl(
     return hip_status("time-mix consumer backward launch",
                       rwkv7m::launch_timemix_output_backward(
                           dtype == RWKV7M_DTYPE_BF16, int(d.N), A, stream));
+}
+
+}  // namespace
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Operators around the language model's head (include/rwkv7m_lm_head.h)
+// ---------------------------------------------------------------------------
+
+// Dtype and sizes of `outer * inner` strided rows of `n` elements.
+int lm_rows(const char* fn, const char* what, int dtype, int64_t outer,
+            int64_t inner, int64_t n, int64_t outer_stride,
+            int64_t inner_stride, int64_t* rows, rwkv7m::LmRows* out) {
+    const std::string f(fn);
+    if (dtype != RWKV7M_DTYPE_F32 && dtype != RWKV7M_DTYPE_BF16)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    f + ": " + what + " must be bfloat16 or float32 (dtype=" +
+                        std::to_string(dtype) + ")");
+    if (outer < 0 || inner < 0 || outer_stride < 0 || inner_stride < 0)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    f + ": negative dimension or stride");
+    if (n < 1)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    f + ": a row must have at least one element, got " +
+                        std::to_string(n));
+    const int64_t lim = int64_t(1) << 40, bytes = int64_t(1) << 46;
+    if (n > (int64_t(1) << 30) || outer > lim || inner > lim ||
+        (inner > 0 && outer > lim / inner) ||
+        (outer > 0 && inner > 0 && outer * inner > bytes / n) ||
+        (outer > 1 && outer_stride > bytes / (outer - 1)) ||
+        (inner > 1 && inner_stride > bytes / (inner - 1)))
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": sizes too large");
+    *rows = outer * inner;
+    out->inner = inner > 0 ? inner : 1;
+    out->outer_stride = outer_stride;
+    out->inner_stride = inner_stride;
+    return RWKV7M_OK;
+}
+
+int lm_dtype(const char* fn, const char* what, int dtype) {
+    if (dtype != RWKV7M_DTYPE_F32 && dtype != RWKV7M_DTYPE_BF16)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    std::string(fn) + ": " + what +
+                        " must be bfloat16 or float32 (dtype=" +
+                        std::to_string(dtype) + ")");
+    return RWKV7M_OK;
+}
+
+// Each pointer is required (non-NULL) and aligned to `size` bytes.
+int lm_need(const char* fn, int64_t size, std::initializer_list<Named> ptrs) {
+    for (const Named& x : ptrs) {
+        if (x.p == nullptr)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": " + x.name + " is NULL");
+        if (reinterpret_cast<uintptr_t>(x.p) % uintptr_t(size))
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": " + x.name + " is not " +
+                            std::to_string(size) + "-byte aligned");
+    }
+    return RWKV7M_OK;
+}
+
+// The same for a pointer that may be NULL.
+int lm_may(const char* fn, int64_t size, std::initializer_list<Named> ptrs) {
+    for (const Named& x : ptrs)
+        if (x.p) RWKV7M_TRY(lm_need(fn, size, {x}));
+    return RWKV7M_OK;
+}
+
+int64_t lm_size(int dtype) { return dtype == RWKV7M_DTYPE_BF16 ? 2 : 4; }
+
+int lm_temperature(const char* fn, double t) {
+    // (below 1e-30 log2(e) / t overflows; above 1e30 it is lost to fp32)
+    if (!(t >= 1e-30 && t <= 1e30))
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    std::string(fn) +
+                        ": temperature must be positive and finite");
+    return RWKV7M_OK;
+}
+
+// No C++ exception leaves a C entry point.
+template <typename F>
+int lm_guard(F body) {
+    try {
+        g_last_error.clear();
+        return body();
+    } catch (...) {
+        return RWKV7M_ERR_HIP;
+    }
+}
+
+int lm_distill_args(const char* fn, int dtype, int teacher_dtype,
+                    int64_t outer, int64_t inner, int64_t V,
+                    int64_t outer_stride, int64_t inner_stride, int64_t K,
+                    const void* logits, const int64_t* ids,
+                    const void* teacher, const float* weight,
+                    double temperature, void* dlogits,
+                    rwkv7m::LmDistillArgs* A) {
+    RWKV7M_TRY(lm_rows(fn, "logits", dtype, outer, inner, V, outer_stride,
+                       inner_stride, &A->rows, &A->xr));
+    RWKV7M_TRY(lm_dtype(fn, "teacher logits", teacher_dtype));
+    RWKV7M_TRY(lm_temperature(fn, temperature));
+    if (K < 0 || K > RWKV7M_MAX_TEACHER_K)
+        return fail(K < 0 ? RWKV7M_ERR_INVALID_ARGUMENT
+                          : RWKV7M_ERR_UNSUPPORTED,
+                    std::string(fn) + ": K=" + std::to_string(K) +
+                        " teacher alternatives are not supported (0 to " +
+                        std::to_string(RWKV7M_MAX_TEACHER_K) + ")");
+    if (A->rows > 0) {
+        RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"logits", logits}}));
+        if (K > 0) {
+            RWKV7M_TRY(lm_need(fn, 8, {{"teacher_ids", ids}}));
+            RWKV7M_TRY(lm_need(fn, lm_size(teacher_dtype),
+                               {{"teacher_logits", teacher}}));
+        }
+        RWKV7M_TRY(lm_may(fn, 4, {{"weight", weight}}));
+        RWKV7M_TRY(lm_may(fn, lm_size(dtype), {{"dlogits", dlogits}}));
+    }
+    A->V = V;
+    A->K = K;
+    A->x = logits;
+    A->ids = ids;
+    A->teacher = teacher;
+    A->weight = weight;
+    A->mean_weight = A->rows > 0 ? float(1.0 / double(A->rows)) : 0.f;
+    A->c = float(1.4426950408889634 / temperature);
+    A->temperature = float(temperature);
+    A->dlogits = dlogits;
+    return RWKV7M_OK;
 }
 
 }  // namespace
@@ -1582,6 +1713,231 @@ int rwkv7m_screen_write_backward(
                       rwkv7m::launch_screen_write(
                           dtype == RWKV7M_DTYPE_BF16, true, A,
                           static_cast<hipStream_t>(stream)));
+}
+
+int rwkv7m_layer_norm(int dtype, int param_dtype, int64_t outer, int64_t inner,
+                      int64_t C, int64_t outer_stride, int64_t inner_stride,
+                      const void* x, const void* weight, const void* bias,
+                      double eps, void* y, float* mean, float* rstd,
+                      void* stream) {
+    const char* fn = "rwkv7m_layer_norm";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmNormArgs A{};
+        RWKV7M_TRY(lm_rows(fn, "x", dtype, outer, inner, C, outer_stride,
+                           inner_stride, &A.rows, &A.xr));
+        RWKV7M_TRY(lm_dtype(fn, "weight and bias", param_dtype));
+        RWKV7M_TRY(tm_eps(fn, eps));
+        if ((mean == nullptr) != (rstd == nullptr))
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": mean and rstd go together");
+        if (A.rows == 0) return RWKV7M_OK;
+        RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"x", x}, {"y", y}}));
+        RWKV7M_TRY(lm_may(fn, lm_size(param_dtype),
+                          {{"weight", weight}, {"bias", bias}}));
+        RWKV7M_TRY(lm_may(fn, 4, {{"mean", mean}, {"rstd", rstd}}));
+        A.C = C;
+        A.x = x;
+        A.weight = weight;
+        A.bias = bias;
+        A.param_bf16 = param_dtype == RWKV7M_DTYPE_BF16;
+        A.eps = float(eps);
+        A.y = y;
+        A.mean = mean;
+        A.rstd = rstd;
+        return hip_status("layer norm launch",
+                          rwkv7m::launch_lm_norm(
+                              dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
+}
+
+int64_t rwkv7m_layer_norm_workspace_floats(int64_t rows, int64_t C) {
+    if (rows < 0 || C < 1 || C > (int64_t(1) << 30)) return -1;
+    return rwkv7m::lm_norm_workspace_floats(rows, C);
+}
+
+int rwkv7m_layer_norm_backward(int dtype, int param_dtype, int64_t outer,
+                               int64_t inner, int64_t C, int64_t outer_stride,
+                               int64_t inner_stride, const void* x,
+                               const void* weight, const float* mean,
+                               const float* rstd, const void* dy, void* dx,
+                               void* dweight, void* dbias, float* workspace,
+                               int64_t workspace_floats, void* stream) {
+    const char* fn = "rwkv7m_layer_norm_backward";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmNormArgs A{};
+        RWKV7M_TRY(lm_rows(fn, "x", dtype, outer, inner, C, outer_stride,
+                           inner_stride, &A.rows, &A.xr));
+        RWKV7M_TRY(lm_dtype(fn, "weight and bias", param_dtype));
+        const int64_t psize = lm_size(param_dtype);
+        RWKV7M_TRY(lm_may(fn, psize, {{"weight", weight},
+                                      {"dweight", dweight},
+                                      {"dbias", dbias}}));
+        if (A.rows > 0) {
+            RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"x", x}, {"dy", dy}}));
+            RWKV7M_TRY(lm_need(fn, 4, {{"mean", mean}, {"rstd", rstd}}));
+            RWKV7M_TRY(lm_may(fn, lm_size(dtype), {{"dx", dx}}));
+            const int64_t floats = dweight || dbias
+                ? rwkv7m::lm_norm_workspace_floats(A.rows, C) : 0;
+            if (workspace_floats < floats)
+                return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                            std::string(fn) + ": workspace holds " +
+                                std::to_string(workspace_floats) +
+                                " floats, needs " + std::to_string(floats));
+            if (floats > 0)
+                RWKV7M_TRY(lm_need(fn, 16, {{"workspace", workspace}}));
+        }
+        A.C = C;
+        A.x = x;
+        A.weight = weight;
+        A.param_bf16 = param_dtype == RWKV7M_DTYPE_BF16;
+        A.mean = const_cast<float*>(mean);
+        A.rstd = const_cast<float*>(rstd);
+        A.dy = dy;
+        A.dx = dx;
+        A.dweight = dweight;
+        A.dbias = dbias;
+        A.workspace = workspace;
+        return hip_status("layer norm backward launch",
+                          rwkv7m::launch_lm_norm_backward(
+                              dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
+}
+
+int rwkv7m_token_logprobs(int dtype, int64_t outer, int64_t inner, int64_t V,
+                          int64_t outer_stride, int64_t inner_stride,
+                          const void* logits, const int64_t* tokens,
+                          int64_t top_k, double temperature, float* logprobs,
+                          float* entropy, int64_t* top_ids,
+                          float* top_logprobs, float* stats, void* stream) {
+    const char* fn = "rwkv7m_token_logprobs";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmScoreArgs A{};
+        RWKV7M_TRY(lm_rows(fn, "logits", dtype, outer, inner, V, outer_stride,
+                           inner_stride, &A.rows, &A.xr));
+        RWKV7M_TRY(lm_temperature(fn, temperature));
+        if (top_k < 0 || top_k > V)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": top_k=" + std::to_string(top_k) +
+                            " is not within 0 and V=" + std::to_string(V));
+        if (top_k > RWKV7M_MAX_TOP_K)
+            return fail(RWKV7M_ERR_UNSUPPORTED,
+                        std::string(fn) + ": top_k=" + std::to_string(top_k) +
+                            " is not supported (at most " +
+                            std::to_string(RWKV7M_MAX_TOP_K) + ")");
+        if (A.rows == 0) return RWKV7M_OK;
+        RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"logits", logits}}));
+        RWKV7M_TRY(lm_need(fn, 8, {{"tokens", tokens}}));
+        RWKV7M_TRY(lm_need(fn, 4, {{"logprobs", logprobs},
+                                   {"entropy", entropy}}));
+        if (top_k > 0) {
+            RWKV7M_TRY(lm_need(fn, 8, {{"top_ids", top_ids}}));
+            RWKV7M_TRY(lm_need(fn, 4, {{"top_logprobs", top_logprobs}}));
+        }
+        RWKV7M_TRY(lm_may(fn, 4, {{"stats", stats}}));
+        A.V = V;
+        A.x = logits;
+        A.tokens = tokens;
+        A.top_k = int(top_k);
+        A.c = float(1.4426950408889634 / temperature);
+        A.logprobs = logprobs;
+        A.entropy = entropy;
+        A.top_ids = top_ids;
+        A.top_logprobs = top_logprobs;
+        A.stats = stats;
+        return hip_status("token log probabilities launch",
+                          rwkv7m::launch_lm_score(
+                              dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
+}
+
+int rwkv7m_token_logprobs_backward(
+    int dtype, int64_t outer, int64_t inner, int64_t V, int64_t outer_stride,
+    int64_t inner_stride, const void* logits, const int64_t* tokens,
+    double temperature, const float* stats, const float* entropy,
+    const float* d_logprobs, const float* d_entropy, void* dlogits,
+    void* stream) {
+    const char* fn = "rwkv7m_token_logprobs_backward";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmScoreArgs A{};
+        RWKV7M_TRY(lm_rows(fn, "logits", dtype, outer, inner, V, outer_stride,
+                           inner_stride, &A.rows, &A.xr));
+        RWKV7M_TRY(lm_temperature(fn, temperature));
+        if (A.rows == 0) return RWKV7M_OK;
+        RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"logits", logits},
+                                                {"dlogits", dlogits}}));
+        RWKV7M_TRY(lm_need(fn, 8, {{"tokens", tokens}}));
+        RWKV7M_TRY(lm_need(fn, 4, {{"stats", stats}, {"entropy", entropy}}));
+        RWKV7M_TRY(lm_may(fn, 4, {{"d_logprobs", d_logprobs},
+                                  {"d_entropy", d_entropy}}));
+        A.V = V;
+        A.x = logits;
+        A.tokens = tokens;
+        A.c = float(1.4426950408889634 / temperature);
+        A.stats = const_cast<float*>(stats);
+        A.entropy = const_cast<float*>(entropy);
+        A.d_logprobs = d_logprobs;
+        A.d_entropy = d_entropy;
+        A.dlogits = dlogits;
+        return hip_status("token log probabilities backward launch",
+                          rwkv7m::launch_lm_score_backward(
+                              dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
+}
+
+int rwkv7m_distill_loss(int dtype, int teacher_dtype, int64_t outer,
+                        int64_t inner, int64_t V, int64_t outer_stride,
+                        int64_t inner_stride, int64_t K, const void* logits,
+                        const int64_t* teacher_ids, const void* teacher_logits,
+                        const float* weight, double temperature, float* loss,
+                        float* row_losses, void* dlogits, void* stream) {
+    const char* fn = "rwkv7m_distill_loss";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmDistillArgs A{};
+        RWKV7M_TRY(lm_distill_args(fn, dtype, teacher_dtype, outer, inner, V,
+                                   outer_stride, inner_stride, K, logits,
+                                   teacher_ids, teacher_logits, weight,
+                                   temperature, dlogits, &A));
+        RWKV7M_TRY(lm_need(fn, 4, {{"loss", loss}}));
+        if (A.rows > 0)
+            RWKV7M_TRY(lm_need(fn, 4, {{"row_losses", row_losses}}));
+        A.loss = loss;
+        A.row_losses = row_losses;
+        return hip_status("distillation loss launch",
+                          rwkv7m::launch_lm_distill(
+                              dtype == RWKV7M_DTYPE_BF16,
+                              teacher_dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
+}
+
+int rwkv7m_distill_loss_backward(
+    int dtype, int teacher_dtype, int64_t outer, int64_t inner, int64_t V,
+    int64_t outer_stride, int64_t inner_stride, int64_t K, const void* logits,
+    const int64_t* teacher_ids, const void* teacher_logits,
+    const float* weight, double temperature, const float* scale,
+    int holds_unit, void* dlogits, void* stream) {
+    const char* fn = "rwkv7m_distill_loss_backward";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmDistillArgs A{};
+        RWKV7M_TRY(lm_distill_args(fn, dtype, teacher_dtype, outer, inner, V,
+                                   outer_stride, inner_stride, K, logits,
+                                   teacher_ids, teacher_logits, weight,
+                                   temperature, dlogits, &A));
+        if (A.rows == 0) return RWKV7M_OK;
+        RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"dlogits", dlogits}}));
+        RWKV7M_TRY(lm_need(fn, 4, {{"scale", scale}}));
+        A.scale = scale;
+        A.holds_unit = holds_unit != 0;
+        return hip_status("distillation gradient launch",
+                          rwkv7m::launch_lm_distill(
+                              dtype == RWKV7M_DTYPE_BF16,
+                              teacher_dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
 }
 
 }  // extern "C"

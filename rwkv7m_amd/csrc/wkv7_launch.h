@@ -301,6 +301,63 @@ hipError_t launch_timemix_output_backward(bool bf16, int N,
                                           const TmOutputBwdArgs& A,
                                           hipStream_t stream);
 
+// Operators around the language model's head (lm_norm.hip, lm_score.hip,
+// lm_distill.hip).  Row r of x or logits starts at (r / inner) * outer_stride
+// + (r % inner) * inner_stride elements; every other array is contiguous.
+struct LmRows {
+    int64_t inner, outer_stride, inner_stride;
+};
+struct LmNormArgs {
+    int64_t rows, C;
+    LmRows xr;
+    const void *x, *weight, *bias;  // weight and bias may be 0
+    int param_bf16;
+    float eps;
+    void* y;
+    float *mean, *rstd;   // [rows]; forward: may be 0
+    const void* dy;       // backward: the rest
+    void *dx, *dweight, *dbias;  // each may be 0
+    float* workspace;     // lm_norm_workspace_floats(rows, C) floats
+};
+struct LmScoreArgs {
+    int64_t rows, V;
+    LmRows xr;
+    const void* x;
+    const int64_t* tokens;
+    int top_k;
+    float c;  // log2(e) / temperature
+    float *logprobs, *entropy;
+    int64_t* top_ids;
+    float* top_logprobs;
+    float* stats;  // [rows][2]: the largest logit, log sum e; forward: may be 0
+    const float *d_logprobs, *d_entropy;  // may be 0
+    void* dlogits;
+};
+struct LmDistillArgs {
+    int64_t rows, V, K;
+    LmRows xr;
+    const void* x;
+    const int64_t* ids;
+    const void* teacher;
+    const float* weight;  // may be 0: mean_weight each
+    float mean_weight;
+    float c, temperature;  // c = log2(e) / temperature
+    float *loss, *row_losses;  // 0 in the backward
+    void* dlogits;             // may be 0
+    const float* scale;        // may be 0: 1
+    int holds_unit;
+};
+int64_t lm_norm_workspace_floats(int64_t rows, int64_t C);
+hipError_t launch_lm_norm(bool bf16, const LmNormArgs& A, hipStream_t stream);
+hipError_t launch_lm_norm_backward(bool bf16, const LmNormArgs& A,
+                                   hipStream_t stream);
+hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
+                           hipStream_t stream);
+hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
+                                    hipStream_t stream);
+hipError_t launch_lm_distill(bool bf16, bool teacher_bf16,
+                             const LmDistillArgs& A, hipStream_t stream);
+
 // One token (T = 1) for N = 64 without checkpoints; s_t may alias s0.
 hipError_t launch_decode(const SeqFwdArgs& p, hipStream_t stream);
 hipError_t launch_seq_backward(const SeqBwdArgs& p, hipStream_t stream);

@@ -47,8 +47,7 @@ LIB_PATH = os.path.join(_PKG_DIR, "librwkv7m_wkv.so")
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 
-# Every symbol declared in include/rwkv7m_wkv.h, include/rwkv7m_timemix.h
-# and include/rwkv7m_screening.h.
+# Every symbol declared in include/*.h.
 EXPORTED_SYMBOLS = (
     "rwkv7m_abi_version",
     "rwkv7m_last_error",
@@ -89,6 +88,13 @@ EXPORTED_SYMBOLS = (
     "rwkv7m_screen_write_keys",
     "rwkv7m_screen_write_scan_backward",
     "rwkv7m_screen_write_queries",
+    "rwkv7m_layer_norm",
+    "rwkv7m_layer_norm_workspace_floats",
+    "rwkv7m_layer_norm_backward",
+    "rwkv7m_token_logprobs",
+    "rwkv7m_token_logprobs_backward",
+    "rwkv7m_distill_loss",
+    "rwkv7m_distill_loss_backward",
 )
 
 LAYOUTS = ("tbhn", "bthn")
@@ -197,6 +203,24 @@ def load_library(path: str | None = None):
                 ("write_queries", [i64] * 4 + [vp] * 2 + [f64] + [vp] * 3),
                 ("stats", [i64] * 4 + [vp] * 6 + [f64] * 2 + [vp] * 4)):
             fn = getattr(lib, "rwkv7m_screen_" + name)
+            fn.restype = i32
+            fn.argtypes = args
+        lib.rwkv7m_layer_norm_workspace_floats.restype = i64
+        lib.rwkv7m_layer_norm_workspace_floats.argtypes = [i64] * 2
+        for name, args in (
+                ("layer_norm", [i32] * 2 + [i64] * 5 + [vp] * 3 + [f64] +
+                 [vp] * 4),
+                ("layer_norm_backward", [i32] * 2 + [i64] * 5 + [vp] * 9 +
+                 [i64, vp]),
+                ("token_logprobs", [i32] + [i64] * 5 + [vp] * 2 +
+                 [i64, f64] + [vp] * 6),
+                ("token_logprobs_backward", [i32] + [i64] * 5 + [vp] * 2 +
+                 [f64] + [vp] * 6),
+                ("distill_loss", [i32] * 2 + [i64] * 6 + [vp] * 4 + [f64] +
+                 [vp] * 4),
+                ("distill_loss_backward", [i32] * 2 + [i64] * 6 + [vp] * 4 +
+                 [f64, vp, i32, vp, vp])):
+            fn = getattr(lib, "rwkv7m_" + name)
             fn.restype = i32
             fn.argtypes = args
         if path is None:
