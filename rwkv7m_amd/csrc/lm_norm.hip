@@ -1,12 +1,24 @@
 // Layer norm over the last axis, forward and backward
 // (include/rwkv7m_lm_head.h has the formulas).
+//
+// Bound by memory: about 8 operations an element forward and 14 backward
+// against 4 and 6 bytes.  A row is read once and held in registers, as the
+// 16-byte vectors it came in, by a group of TPR threads (16 for up to 128
+// bf16 elements, a wave, a workgroup of 4 or of 16 waves), NV vectors each;
+// the variance is the mean of the squared deviations, from the registers.
+// Rows longer than 16 waves hold (kLongest) are walked again from the L2.
+// Workgroups stay for many rows, with the parameters, and in the backward
+// their gradients' sums, in registers; each workgroup writes one partial row
+// of those sums and a second kernel adds the partial rows in a fixed order.
+//
+// A row whose length is no multiple of the vector ends in a vector moved back
+// to end with it (its first `dup` elements are the vector before's): every
+// access is whole, and what the two write twice is the same value.
 
 #include "lm_rows.h"
 
 namespace rwkv7m {
 namespace {
-
-constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 __device__ __forceinline__ float param(const void* p, bool bf16, int64_t i,
                                        float absent) {
@@ -15,8 +27,228 @@ __device__ __forceinline__ float param(const void* p, bool bf16, int64_t i,
                 : static_cast<const float*>(p)[i];
 }
 
+__device__ __forceinline__ void store_param(void* p, bool bf16, int64_t i,
+                                            float x) {
+    if (bf16)
+        store_f(static_cast<bf16_t*>(p) + i, x);
+    else
+        store_f(static_cast<float*>(p) + i, x);
+}
+
+// Where a thread's vectors lie in a row of C elements.
+template <typename E, int TPR, int NV, bool TAIL>
+struct Place {
+    static constexpr int n = Vec<E>::n;
+    int C, lane;
+
+    __device__ __forceinline__ bool has(int i) const {
+        return (i * TPR + lane) * n < C;
+    }
+    __device__ __forceinline__ int at(int i) const {
+        const int a = (i * TPR + lane) * n;
+        return TAIL && a + n > C ? C - n : a;
+    }
+    __device__ __forceinline__ int dup(int i) const {
+        return TAIL ? (i * TPR + lane) * n - at(i) : 0;
+    }
+};
+
+// Sums over the TPR threads of a row, the same in each of them.  Where a row
+// is more than a wave's the two buffers of `s` take turns: one barrier a sum.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sums(float (&x)[K],
+                                         float (*s)[K][TPR / 64 + 1],
+                                         int& turn) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] = lanes_sum<TPR < 64 ? TPR : 64>(x[k]);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        if (threadIdx.x % 64 == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) s[turn][k][threadIdx.x / 64] = x[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            x[k] = s[turn][k][0];
+#pragma unroll
+            for (int w = 1; w < W; ++w) x[k] += s[turn][k][w];
+        }
+        turn ^= 1;
+    }
+}
+
+template <typename E, int TPR, int NV, bool TAIL>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(
+    LmNormArgs A) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1, n = Vec<E>::n;
+    __shared__ float s[2][1][TPR / 64 + 1];
+    int turn = 0;
+    const Place<E, TPR, NV, TAIL> at{int(A.C), int(threadIdx.x % TPR)};
+    const float inv = 1.f / float(A.C);
+    float w[NV][n], b[NV][n];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (at.has(i))
+#pragma unroll
+            for (int j = 0; j < n; ++j) {
+                w[i][j] = param(A.weight, A.param_bf16, at.at(i) + j, 1.f);
+                b[i][j] = param(A.bias, A.param_bf16, at.at(i) + j, 0.f);
+            }
+    for (int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
+         row < A.rows; row += int64_t(gridDim.x) * RPB) {
+        const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
+        E* y = static_cast<E*>(A.y) + row * A.C;
+        Vec<E> v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i)) v[i].load(x + at.at(i));
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i))
+#pragma unroll
+                for (int j = 0; j < n; ++j)
+                    sum[0] += j < at.dup(i) ? 0.f : v[i].get(j);
+        row_sums<TPR>(sum, s, turn);
+        const float mean = sum[0] * inv;
+        sum[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i))
+#pragma unroll
+                for (int j = 0; j < n; ++j) {
+                    const float d = j < at.dup(i) ? 0.f : v[i].get(j) - mean;
+                    sum[0] = __builtin_fmaf(d, d, sum[0]);
+                }
+        row_sums<TPR>(sum, s, turn);
+        const float rstd = 1.f / sqrtf(sum[0] * inv + A.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i)) {
+                Vec<E> o;
+#pragma unroll
+                for (int j = 0; j < n; j += 2)
+                    o.set2(j,
+                           __builtin_fmaf((v[i].get(j) - mean) * rstd, w[i][j],
+                                          b[i][j]),
+                           __builtin_fmaf((v[i].get(j + 1) - mean) * rstd,
+                                          w[i][j + 1], b[i][j + 1]));
+                o.store(y + at.at(i));
+            }
+        if (A.mean && threadIdx.x % TPR == 0) {
+            A.mean[row] = mean;
+            A.rstd[row] = rstd;
+        }
+    }
+}
+
+// dx, and the workgroup's partial row of the parameters' gradients:
+// workspace[block][0 / 1][C] (weight, bias).
+template <typename E, int TPR, int NV, bool TAIL>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(
+    LmNormArgs A) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1, n = Vec<E>::n;
+    constexpr int kCols = RPB > 1 ? TPR * NV * n : 1;
+    __shared__ float s[2][2][TPR / 64 + 1];
+    __shared__ float part[2][kCols];
+    int turn = 0;
+    const Place<E, TPR, NV, TAIL> at{int(A.C), int(threadIdx.x % TPR)};
+    const float inv = 1.f / float(A.C);
+    float w[NV][n], dw[NV][n] = {}, db[NV][n] = {};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (at.has(i))
+#pragma unroll
+            for (int j = 0; j < n; ++j)
+                w[i][j] = param(A.weight, A.param_bf16, at.at(i) + j, 1.f);
+    for (int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
+         row < A.rows; row += int64_t(gridDim.x) * RPB) {
+        const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
+        const E* dy = static_cast<const E*>(A.dy) + row * A.C;
+        const float mean = A.mean[row], rstd = A.rstd[row];
+        Vec<E> vx[NV], vd[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i)) {
+                vx[i].load(x + at.at(i));
+                vd[i].load(dy + at.at(i));
+            }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i))
+#pragma unroll
+                for (int j = 0; j < n; ++j) {
+                    const float xh = (vx[i].get(j) - mean) * rstd;
+                    const float d = j < at.dup(i) ? 0.f : vd[i].get(j);
+                    const float g = d * w[i][j];
+                    sum[0] += g;
+                    sum[1] = __builtin_fmaf(g, xh, sum[1]);
+                    dw[i][j] = __builtin_fmaf(d, xh, dw[i][j]);
+                    db[i][j] += d;
+                }
+        row_sums<TPR>(sum, s, turn);
+        const float sg = sum[0] * inv, sgx = sum[1] * inv;
+        if (A.dx) {
+            E* dx = static_cast<E*>(A.dx) + row * A.C;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (at.has(i)) {
+                    Vec<E> o;
+                    float r[n];
+#pragma unroll
+                    for (int j = 0; j < n; ++j) {
+                        const float xh = (vx[i].get(j) - mean) * rstd;
+                        r[j] = rstd * (__builtin_fmaf(vd[i].get(j), w[i][j],
+                                                      -sg) -
+                                       xh * sgx);
+                    }
+#pragma unroll
+                    for (int j = 0; j < n; j += 2) o.set2(j, r[j], r[j + 1]);
+                    o.store(dx + at.at(i));
+                }
+        }
+    }
+    if (!A.workspace) return;
+    float* out = A.workspace + int64_t(blockIdx.x) * 2 * A.C;
+    if constexpr (RPB > 1) {
+        // the row groups' sums one after the other, the first group's last
+        for (int g = RPB - 1; g > 0; --g) {
+            const bool mine = int(threadIdx.x) / TPR == g;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (mine && at.has(i))
+#pragma unroll
+                    for (int j = 0; j < n; ++j) {
+                        const int c = (i * TPR + at.lane) * n + j;
+                        const bool more = g < RPB - 1;
+                        part[0][c] = dw[i][j] + (more ? part[0][c] : 0.f);
+                        part[1][c] = db[i][j] + (more ? part[1][c] : 0.f);
+                    }
+            __syncthreads();
+        }
+        if (int(threadIdx.x) >= TPR) return;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (at.has(i))
+#pragma unroll
+            for (int j = 0; j < n; ++j) {
+                if (j < at.dup(i)) continue;
+                const int c = (i * TPR + at.lane) * n + j;
+                out[at.at(i) + j] = dw[i][j] + (RPB > 1 ? part[0][c] : 0.f);
+                out[A.C + at.at(i) + j] =
+                    db[i][j] + (RPB > 1 ? part[1][c] : 0.f);
+            }
+}
+
+// Any length, element by element: rows shorter than a vector, and those
+// longer than kLongest (their second and third reads come from the L2).
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
 template <typename E>
-__global__ __launch_bounds__(kThreads) void norm_fwd_kernel(LmNormArgs A) {
+__global__ __launch_bounds__(kThreads) void norm_fwd_any_kernel(LmNormArgs A) {
     __shared__ float s[kWaves];
     const float n = 1.f / float(A.C);
     for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
@@ -29,14 +261,14 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(LmNormArgs A) {
         float sq = 0.f;
         for (int64_t i = threadIdx.x; i < A.C; i += kThreads) {
             const float d = load_f(x + i) - mean;
-            sq += d * d;
+            sq = __builtin_fmaf(d, d, sq);
         }
-        const float rstd =
-            1.f / sqrtf(block_sum<kWaves>(sq, s) * n + A.eps);
+        const float rstd = 1.f / sqrtf(block_sum<kWaves>(sq, s) * n + A.eps);
         for (int64_t i = threadIdx.x; i < A.C; i += kThreads)
-            store_f(y + i, (load_f(x + i) - mean) * rstd *
-                                   param(A.weight, A.param_bf16, i, 1.f) +
-                               param(A.bias, A.param_bf16, i, 0.f));
+            store_f(y + i,
+                    __builtin_fmaf((load_f(x + i) - mean) * rstd,
+                                   param(A.weight, A.param_bf16, i, 1.f),
+                                   param(A.bias, A.param_bf16, i, 0.f)));
         if (threadIdx.x == 0 && A.mean) {
             A.mean[row] = mean;
             A.rstd[row] = rstd;
@@ -44,112 +276,156 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(LmNormArgs A) {
     }
 }
 
+// The workgroup's partial row is kept in the workspace itself: each thread
+// adds its rows to its own columns.
 template <typename E>
-__global__ __launch_bounds__(kThreads) void norm_dx_kernel(LmNormArgs A) {
+__global__ __launch_bounds__(kThreads) void norm_bwd_any_kernel(LmNormArgs A) {
     __shared__ float s[kWaves];
     const float n = 1.f / float(A.C);
+    float* part = A.workspace + int64_t(blockIdx.x) * 2 * A.C;
+    bool first = true;
     for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
         const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
         const E* dy = static_cast<const E*>(A.dy) + row * A.C;
-        E* dx = static_cast<E*>(A.dx) + row * A.C;
         const float mean = A.mean[row], rstd = A.rstd[row];
         float sg = 0.f, sgx = 0.f;
         for (int64_t i = threadIdx.x; i < A.C; i += kThreads) {
-            const float g =
-                load_f(dy + i) * param(A.weight, A.param_bf16, i, 1.f);
+            const float d = load_f(dy + i);
+            const float xh = (load_f(x + i) - mean) * rstd;
+            const float g = d * param(A.weight, A.param_bf16, i, 1.f);
             sg += g;
-            sgx += g * ((load_f(x + i) - mean) * rstd);
+            sgx = __builtin_fmaf(g, xh, sgx);
+            if (A.workspace) {
+                part[i] = __builtin_fmaf(d, xh, first ? 0.f : part[i]);
+                part[A.C + i] = d + (first ? 0.f : part[A.C + i]);
+            }
         }
+        first = false;
+        if (!A.dx) continue;
         sg = block_sum<kWaves>(sg, s) * n;
         sgx = block_sum<kWaves>(sgx, s) * n;
+        E* dx = static_cast<E*>(A.dx) + row * A.C;
         for (int64_t i = threadIdx.x; i < A.C; i += kThreads) {
             const float g =
                 load_f(dy + i) * param(A.weight, A.param_bf16, i, 1.f);
-            const float xh = (load_f(x + i) - mean) * rstd;
-            store_f(dx + i, rstd * (g - sg - xh * sgx));
+            store_f(dx + i, rstd * (g - sg - (load_f(x + i) - mean) * rstd *
+                                                 sgx));
         }
     }
 }
 
-// Partial parameter gradients: block (column tile, g) sums the rows
-// g, g + groups, ... into part[g][0 / 1][C] (weight, bias).
+// dweight and dbias from the partial rows [parts][2 C]: a block sums 64
+// columns over 16 interleaved shares of the rows.
+__global__ __launch_bounds__(1024) void norm_sum_kernel(LmNormArgs A,
+                                                        int parts) {
+    __shared__ float s[16][64];
+    const int64_t c = int64_t(blockIdx.x) * 64 + threadIdx.x % 64;
+    const int share = threadIdx.x / 64;
+    float x = 0.f;
+    if (c < 2 * A.C)
+        for (int p = share; p < parts; p += 16)
+            x += A.workspace[int64_t(p) * 2 * A.C + c];
+    s[share][threadIdx.x % 64] = x;
+    __syncthreads();
+    if (share != 0 || c >= 2 * A.C) return;
+    for (int k = 1; k < 16; ++k) x += s[k][threadIdx.x];
+    void* out = c < A.C ? A.dweight : A.dbias;
+    if (out) store_param(out, A.param_bf16, c < A.C ? c : c - A.C, x);
+}
+
+// Elements a row may have for the widest group (16 waves, 4 vectors each).
 template <typename E>
-__global__ __launch_bounds__(kThreads) void norm_part_kernel(LmNormArgs A,
-                                                             int groups) {
-    const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-    if (c >= A.C) return;
-    float dw = 0.f, db = 0.f;
-    for (int64_t row = blockIdx.y; row < A.rows; row += groups) {
-        const float x = load_f(static_cast<const E*>(A.x) +
-                               row_offset(A.xr, row) + c);
-        const float dy = load_f(static_cast<const E*>(A.dy) + row * A.C + c);
-        dw += dy * ((x - A.mean[row]) * A.rstd[row]);
-        db += dy;
-    }
-    float* p = A.workspace + int64_t(blockIdx.y) * 2 * A.C;
-    p[c] = dw;
-    p[A.C + c] = db;
+constexpr int64_t kLongest = 1024 * 4 * Vec<E>::n;
+
+// The group that holds a row of C elements: a wave as long as its threads
+// hold the row in 4 vectors, then 4, then 16 waves.
+template <typename E>
+int threads_per_row(int64_t C) {
+    const int64_t n = Vec<E>::n;
+    if (C < n || C > kLongest<E>) return 0;
+    return C <= 16 * n ? 16 : C <= 64 * 4 * n ? 64 : C <= 256 * 4 * n ? 256
+                                                                      : 1024;
 }
 
-__global__ __launch_bounds__(kThreads) void norm_sum_kernel(LmNormArgs A,
-                                                            int groups) {
-    const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-    if (c >= A.C) return;
-    float dw = 0.f, db = 0.f;
-    for (int g = 0; g < groups; ++g) {
-        dw += A.workspace[int64_t(g) * 2 * A.C + c];
-        db += A.workspace[int64_t(g) * 2 * A.C + A.C + c];
-    }
-    for (int k = 0; k < 2; ++k) {
-        void* out = k ? A.dbias : A.dweight;
-        if (!out) continue;
-        if (A.param_bf16)
-            store_f(static_cast<bf16_t*>(out) + c, k ? db : dw);
-        else
-            store_f(static_cast<float*>(out) + c, k ? db : dw);
+// Workgroups of the backward: two a CU (each CU's registers hold two
+// workgroups' sums at least), fewer where the rows are few.
+int64_t backward_blocks(int64_t rows, int tpr) {
+    const int64_t groups = tpr && tpr < 256 ? 256 / tpr : 1;
+    const int64_t blocks = (rows + groups - 1) / groups;
+    return blocks < 512 ? blocks : 512;
+}
+
+using NormKernel = void (*)(LmNormArgs);
+
+template <typename E, bool BWD, int TPR, int NV>
+NormKernel pick_tail(int64_t C) {
+    const bool tail = C % Vec<E>::n != 0;
+    if (BWD)
+        return tail ? norm_bwd_kernel<E, TPR, NV, true>
+                    : norm_bwd_kernel<E, TPR, NV, false>;
+    return tail ? norm_fwd_kernel<E, TPR, NV, true>
+                : norm_fwd_kernel<E, TPR, NV, false>;
+}
+
+template <typename E, bool BWD, int TPR>
+NormKernel pick_vectors(int64_t C) {
+    switch ((C + TPR * Vec<E>::n - 1) / (TPR * Vec<E>::n)) {
+    case 1: return pick_tail<E, BWD, TPR, 1>(C);
+    case 2: return pick_tail<E, BWD, TPR, 2>(C);
+    case 3: return pick_tail<E, BWD, TPR, 3>(C);
+    default: return pick_tail<E, BWD, TPR, 4>(C);
     }
 }
 
-int row_groups(int64_t rows) {
-    return int(rows < 1 ? 0 : rows < 256 ? rows : 256);
-}
-
-unsigned row_grid(int64_t rows) {
-    return unsigned(rows < (1 << 20) ? rows : 1 << 20);
+template <typename E, bool BWD>
+NormKernel pick(int64_t C) {
+    switch (threads_per_row<E>(C)) {
+    case 16: return pick_tail<E, BWD, 16, 1>(C);
+    case 64: return pick_vectors<E, BWD, 64>(C);
+    case 256: return pick_vectors<E, BWD, 256>(C);
+    case 1024: return pick_vectors<E, BWD, 1024>(C);
+    default: return BWD ? norm_bwd_any_kernel<E> : norm_fwd_any_kernel<E>;
+    }
 }
 
 }  // namespace
 
 int64_t lm_norm_workspace_floats(int64_t rows, int64_t C) {
-    return 2 * C * row_groups(rows);
+    // (a row group's share is at least one row in every variant)
+    return 2 * C * (rows < 512 ? rows : 512);
 }
 
 hipError_t launch_lm_norm(bool bf16, const LmNormArgs& A, hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    hipLaunchKernelGGL(bf16 ? norm_fwd_kernel<bf16_t> : norm_fwd_kernel<float>,
-                       dim3(row_grid(A.rows)), dim3(kThreads), 0, stream, A);
+    const int tpr =
+        bf16 ? threads_per_row<bf16_t>(A.C) : threads_per_row<float>(A.C);
+    const int64_t groups = tpr && tpr < 256 ? 256 / tpr : 1;
+    int64_t blocks = (A.rows + groups - 1) / groups;
+    if (blocks > 1024) blocks = 1024;
+    const auto kern = bf16 ? pick<bf16_t, false>(A.C) : pick<float, false>(A.C);
+    hipLaunchKernelGGL(kern, dim3(unsigned(blocks)),
+                       dim3(tpr > 256 ? tpr : 256), 0, stream, A);
     return hipGetLastError();
 }
 
 hipError_t launch_lm_norm_backward(bool bf16, const LmNormArgs& A,
                                    hipStream_t stream) {
-    if (A.rows > 0 && A.dx)
-        hipLaunchKernelGGL(
-            bf16 ? norm_dx_kernel<bf16_t> : norm_dx_kernel<float>,
-            dim3(row_grid(A.rows)), dim3(kThreads), 0, stream, A);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || (!A.dweight && !A.dbias)) return e;
-    const int groups = row_groups(A.rows);
-    const unsigned tiles = unsigned((A.C + kThreads - 1) / kThreads);
-    if (groups > 0)
-        hipLaunchKernelGGL(
-            bf16 ? norm_part_kernel<bf16_t> : norm_part_kernel<float>,
-            dim3(tiles, unsigned(groups)), dim3(kThreads), 0, stream, A,
-            groups);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(norm_sum_kernel, dim3(tiles), dim3(kThreads), 0, stream,
-                       A, groups);
+    const bool params = A.dweight || A.dbias;
+    const int tpr =
+        bf16 ? threads_per_row<bf16_t>(A.C) : threads_per_row<float>(A.C);
+    const int64_t blocks = backward_blocks(A.rows, tpr);
+    if (A.rows > 0 && (A.dx || params)) {
+        LmNormArgs B = A;
+        if (!params) B.workspace = nullptr;
+        const auto kern =
+            bf16 ? pick<bf16_t, true>(A.C) : pick<float, true>(A.C);
+        hipLaunchKernelGGL(kern, dim3(unsigned(blocks)),
+                           dim3(tpr > 256 ? tpr : 256), 0, stream, B);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !params) return e;
+    hipLaunchKernelGGL(norm_sum_kernel, dim3(unsigned((2 * A.C + 63) / 64)),
+                       dim3(1024), 0, stream, A, int(blocks));
     return hipGetLastError();
 }
 

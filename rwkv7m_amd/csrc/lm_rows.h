@@ -15,7 +15,50 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ int64_t row_offset(const LmRows& R, int64_t row) {
+    if (row < R.inner) return row * R.inner_stride;  // (no division)
     return row / R.inner * R.outer_stride + row % R.inner * R.inner_stride;
+}
+
+// 16 bytes of adjacent elements, at their element's own alignment: gfx950
+// takes such a load or store as one instruction at any address.
+template <typename E>
+struct Vec {
+    static constexpr int n = 16 / int(sizeof(E));
+    typedef uint32_t raw_t __attribute__((ext_vector_type(4), aligned(2)));
+    raw_t raw;
+
+    __device__ __forceinline__ void load(const E* p) {
+        raw = *reinterpret_cast<const raw_t*>(p);
+    }
+    __device__ __forceinline__ void store(E* p) const {
+        *reinterpret_cast<raw_t*>(p) = raw;
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(E) == 4) return __uint_as_float(raw[j]);
+        const uint32_t u = raw[j >> 1];
+        return __uint_as_float(j & 1 ? u & 0xffff0000u : u << 16);
+    }
+    // Element pair j, j + 1 (j even), rounded to nearest even in bf16.
+    __device__ __forceinline__ void set2(int j, float a, float b) {
+        if constexpr (sizeof(E) == 4) {
+            raw[j] = __float_as_uint(a);
+            raw[j + 1] = __float_as_uint(b);
+        } else {
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            const f32x2 f = {a, b};
+            raw[j >> 1] = __builtin_bit_cast(
+                uint32_t, __builtin_convertvector(f, bf16x2));
+        }
+    }
+};
+
+// The sum over aligned groups of G lanes (16, 64), the same in each of them.
+template <int G>
+__device__ __forceinline__ float lanes_sum(float x) {
+    x = group_sum<16>(x);
+    if constexpr (G == 64) x = add_swap<32>(add_swap<16>(x));
+    return x;
 }
 
 // The larger of two, a NaN if either is one (v_maximum3_f32).
