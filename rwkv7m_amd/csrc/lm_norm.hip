@@ -27,6 +27,33 @@ __device__ __forceinline__ float param(const void* p, bool bf16, int64_t i,
                 : static_cast<const float*>(p)[i];
 }
 
+// N parameters from element i on, in 16-byte loads (8 for 4 bf16).
+template <int N>
+__device__ __forceinline__ void params(const void* p, bool bf16, int64_t i,
+                                       float absent, float (&f)[N]) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = absent;
+    } else if (bf16) {
+        typedef uint32_t half_t
+            __attribute__((ext_vector_type(N / 2), aligned(2)));
+        const half_t v = *reinterpret_cast<const half_t*>(
+            static_cast<const bf16_t*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            f[j] = __uint_as_float(j & 1 ? v[j / 2] & 0xffff0000u
+                                         : v[j / 2] << 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            Vec<float> v;
+            v.load(static_cast<const float*>(p) + i + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[j + k] = v.get(k);
+        }
+    }
+}
+
 __device__ __forceinline__ void store_param(void* p, bool bf16, int64_t i,
                                             float x) {
     if (bf16)
@@ -53,48 +80,51 @@ struct Place {
     }
 };
 
+template <int TPR>
+constexpr int kFwdThreads = TPR > 256 ? TPR : 256;
+constexpr int kBwdThreads = 1024;
+
 // Sums over the TPR threads of a row, the same in each of them.  Where a row
-// is more than a wave's the two buffers of `s` take turns: one barrier a sum.
-template <int TPR, int K>
-__device__ __forceinline__ void row_sums(float (&x)[K],
-                                         float (*s)[K][TPR / 64 + 1],
+// is more than a wave's the two buffers of `s` (a value a wave of the
+// workgroup) take turns: one barrier a call.
+template <int TPR, int K, int W>
+__device__ __forceinline__ void row_sums(float (&x)[K], float (*s)[K][W],
                                          int& turn) {
 #pragma unroll
     for (int k = 0; k < K; ++k) x[k] = lanes_sum<TPR < 64 ? TPR : 64>(x[k]);
     if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
+        const int wave = threadIdx.x / 64, first = wave / (TPR / 64) *
+                                                   (TPR / 64);
         if (threadIdx.x % 64 == 0) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) s[turn][k][threadIdx.x / 64] = x[k];
+            for (int k = 0; k < K; ++k) s[turn][k][wave] = x[k];
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            x[k] = s[turn][k][0];
+            x[k] = s[turn][k][first];
 #pragma unroll
-            for (int w = 1; w < W; ++w) x[k] += s[turn][k][w];
+            for (int w = 1; w < TPR / 64; ++w) x[k] += s[turn][k][first + w];
         }
         turn ^= 1;
     }
 }
 
 template <typename E, int TPR, int NV, bool TAIL>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(
+__global__ __launch_bounds__(kFwdThreads<TPR>) void norm_fwd_kernel(
     LmNormArgs A) {
-    constexpr int RPB = TPR < 256 ? 256 / TPR : 1, n = Vec<E>::n;
-    __shared__ float s[2][1][TPR / 64 + 1];
+    constexpr int RPB = kFwdThreads<TPR> / TPR, n = Vec<E>::n;
+    __shared__ float s[2][1][kFwdThreads<TPR> / 64];
     int turn = 0;
     const Place<E, TPR, NV, TAIL> at{int(A.C), int(threadIdx.x % TPR)};
     const float inv = 1.f / float(A.C);
     float w[NV][n], b[NV][n];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if (at.has(i))
-#pragma unroll
-            for (int j = 0; j < n; ++j) {
-                w[i][j] = param(A.weight, A.param_bf16, at.at(i) + j, 1.f);
-                b[i][j] = param(A.bias, A.param_bf16, at.at(i) + j, 0.f);
-            }
+        if (at.has(i)) {
+            params(A.weight, A.param_bf16, at.at(i), 1.f, w[i]);
+            params(A.bias, A.param_bf16, at.at(i), 0.f, b[i]);
+        }
     for (int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
          row < A.rows; row += int64_t(gridDim.x) * RPB) {
         const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
@@ -143,45 +173,74 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(
     }
 }
 
+// One row's operands of the backward, as they came (zeros past the last row).
+template <typename E, int NV>
+struct BwdRow {
+    Vec<E> x[NV], dy[NV];
+    float mean, rstd;
+
+    template <typename P>
+    __device__ __forceinline__ void load(const LmNormArgs& A, int64_t row,
+                                         const P& at) {
+        mean = rstd = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i].raw = dy[i].raw = 0;
+        if (row >= A.rows) return;
+        const E* px = static_cast<const E*>(A.x) + row_offset(A.xr, row);
+        const E* pd = static_cast<const E*>(A.dy) + row * A.C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i)) {
+                x[i].load(px + at.at(i));
+                dy[i].load(pd + at.at(i));
+            }
+        mean = A.mean[row];
+        rstd = A.rstd[row];
+    }
+};
+
 // dx, and the workgroup's partial row of the parameters' gradients:
-// workspace[block][0 / 1][C] (weight, bias).
+// workspace[block][0 / 1][C] (weight, bias).  One workgroup of 16 waves a CU,
+// kBwdThreads / TPR rows at a time, so that there are few partial rows
+// (their 16 C bytes, written and read again, are what a workgroup adds to
+// the 6 C of each of its rows in bf16).
 template <typename E, int TPR, int NV, bool TAIL>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(
-    LmNormArgs A) {
-    constexpr int RPB = TPR < 256 ? 256 / TPR : 1, n = Vec<E>::n;
+__global__ __launch_bounds__(kBwdThreads) void norm_bwd_kernel(LmNormArgs A) {
+    constexpr int RPB = kBwdThreads / TPR, n = Vec<E>::n;
     constexpr int kCols = RPB > 1 ? TPR * NV * n : 1;
-    __shared__ float s[2][2][TPR / 64 + 1];
-    __shared__ float part[2][kCols];
+    // A thread with one vector a row asks for the next row's while it works
+    // on this one's ([32768, 2048] bf16: 84 against 87 us); with two the
+    // waves have enough in flight without ([16384, 4096]: 83 against 81).
+    constexpr bool kAhead = NV == 1;
+    __shared__ float s[2][2][kBwdThreads / 64];
+    __shared__ float part[RPB][2][kCols];
     int turn = 0;
     const Place<E, TPR, NV, TAIL> at{int(A.C), int(threadIdx.x % TPR)};
+    const int group = threadIdx.x / TPR;
+    const int64_t step = int64_t(gridDim.x) * RPB;
     const float inv = 1.f / float(A.C);
     float w[NV][n], dw[NV][n] = {}, db[NV][n] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if (at.has(i))
-#pragma unroll
-            for (int j = 0; j < n; ++j)
-                w[i][j] = param(A.weight, A.param_bf16, at.at(i) + j, 1.f);
-    for (int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
-         row < A.rows; row += int64_t(gridDim.x) * RPB) {
-        const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
-        const E* dy = static_cast<const E*>(A.dy) + row * A.C;
-        const float mean = A.mean[row], rstd = A.rstd[row];
-        Vec<E> vx[NV], vd[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (at.has(i)) {
-                vx[i].load(x + at.at(i));
-                vd[i].load(dy + at.at(i));
-            }
+        if (at.has(i)) params(A.weight, A.param_bf16, at.at(i), 1.f, w[i]);
+    BwdRow<E, NV> v, next;
+    if constexpr (kAhead) v.load(A, int64_t(blockIdx.x) * RPB + group, at);
+    // (the workgroup's threads make the same number of turns)
+    for (int64_t base = int64_t(blockIdx.x) * RPB; base < A.rows;
+         base += step) {
+        const int64_t row = base + group;
+        if constexpr (kAhead)
+            next.load(A, row + step, at);
+        else
+            v.load(A, row, at);
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (at.has(i))
 #pragma unroll
                 for (int j = 0; j < n; ++j) {
-                    const float xh = (vx[i].get(j) - mean) * rstd;
-                    const float d = j < at.dup(i) ? 0.f : vd[i].get(j);
+                    const float xh = (v.x[i].get(j) - v.mean) * v.rstd;
+                    const float d = j < at.dup(i) ? 0.f : v.dy[i].get(j);
                     const float g = d * w[i][j];
                     sum[0] += g;
                     sum[1] = __builtin_fmaf(g, xh, sum[1]);
@@ -190,7 +249,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(
                 }
         row_sums<TPR>(sum, s, turn);
         const float sg = sum[0] * inv, sgx = sum[1] * inv;
-        if (A.dx) {
+        if (A.dx && row < A.rows) {
             E* dx = static_cast<E*>(A.dx) + row * A.C;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -199,48 +258,50 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(
                     float r[n];
 #pragma unroll
                     for (int j = 0; j < n; ++j) {
-                        const float xh = (vx[i].get(j) - mean) * rstd;
-                        r[j] = rstd * (__builtin_fmaf(vd[i].get(j), w[i][j],
-                                                      -sg) -
-                                       xh * sgx);
+                        const float xh = (v.x[i].get(j) - v.mean) * v.rstd;
+                        r[j] = v.rstd * (__builtin_fmaf(v.dy[i].get(j),
+                                                        w[i][j], -sg) -
+                                         xh * sgx);
                     }
 #pragma unroll
                     for (int j = 0; j < n; j += 2) o.set2(j, r[j], r[j + 1]);
                     o.store(dx + at.at(i));
                 }
         }
+        if constexpr (kAhead) v = next;
     }
     if (!A.workspace) return;
     float* out = A.workspace + int64_t(blockIdx.x) * 2 * A.C;
     if constexpr (RPB > 1) {
-        // the row groups' sums one after the other, the first group's last
-        for (int g = RPB - 1; g > 0; --g) {
-            const bool mine = int(threadIdx.x) / TPR == g;
+        // the row groups' sums side by side, added in the groups' order
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (mine && at.has(i))
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i))
 #pragma unroll
-                    for (int j = 0; j < n; ++j) {
-                        const int c = (i * TPR + at.lane) * n + j;
-                        const bool more = g < RPB - 1;
-                        part[0][c] = dw[i][j] + (more ? part[0][c] : 0.f);
-                        part[1][c] = db[i][j] + (more ? part[1][c] : 0.f);
+                for (int j = 0; j < n; ++j)
+                    if (j >= at.dup(i)) {
+                        part[group][0][at.at(i) + j] = dw[i][j];
+                        part[group][1][at.at(i) + j] = db[i][j];
                     }
-            __syncthreads();
-        }
-        if (int(threadIdx.x) >= TPR) return;
-    }
+        __syncthreads();
+        for (int k = 0; k < 2; ++k)
+            for (int c = threadIdx.x; c < A.C; c += kBwdThreads) {
+                float x = part[0][k][c];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (at.has(i))
-#pragma unroll
-            for (int j = 0; j < n; ++j) {
-                if (j < at.dup(i)) continue;
-                const int c = (i * TPR + at.lane) * n + j;
-                out[at.at(i) + j] = dw[i][j] + (RPB > 1 ? part[0][c] : 0.f);
-                out[A.C + at.at(i) + j] =
-                    db[i][j] + (RPB > 1 ? part[1][c] : 0.f);
+                for (int r = 1; r < RPB; ++r) x += part[r][k][c];
+                out[k * A.C + c] = x;
             }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.has(i))
+#pragma unroll
+                for (int j = 0; j < n; ++j)
+                    if (j >= at.dup(i)) {
+                        out[at.at(i) + j] = dw[i][j];
+                        out[A.C + at.at(i) + j] = db[i][j];
+                    }
+    }
 }
 
 // Any length, element by element: rows shorter than a vector, and those
@@ -323,6 +384,7 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(LmNormArgs A,
     const int share = threadIdx.x / 64;
     float x = 0.f;
     if (c < 2 * A.C)
+#pragma unroll 8
         for (int p = share; p < parts; p += 16)
             x += A.workspace[int64_t(p) * 2 * A.C + c];
     s[share][threadIdx.x % 64] = x;
@@ -333,26 +395,28 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(LmNormArgs A,
     if (out) store_param(out, A.param_bf16, c < A.C ? c : c - A.C, x);
 }
 
-// Elements a row may have for the widest group (16 waves, 4 vectors each).
-template <typename E>
-constexpr int64_t kLongest = 1024 * 4 * Vec<E>::n;
+// Vectors a thread of a group below the widest holds.
+constexpr int64_t kFwdVectors = 4, kBwdVectors = 2;
+constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 256;
 
-// The group that holds a row of C elements: a wave as long as its threads
-// hold the row in 4 vectors, then 4, then 16 waves.
+// Elements a row may have for the widest group (16 waves of 2 vectors each).
 template <typename E>
-int threads_per_row(int64_t C) {
-    const int64_t n = Vec<E>::n;
+constexpr int64_t kLongest = 1024 * 2 * Vec<E>::n;
+
+// The group that holds a row of C elements: a quarter of a wave, a wave, 4
+// or 16 waves; 0: none.
+template <typename E>
+int threads_per_row(int64_t C, bool backward) {
+    const int64_t n = Vec<E>::n, nv = backward ? kBwdVectors : kFwdVectors;
     if (C < n || C > kLongest<E>) return 0;
-    return C <= 16 * n ? 16 : C <= 64 * 4 * n ? 64 : C <= 256 * 4 * n ? 256
-                                                                      : 1024;
+    return C <= 16 * n ? 16 : C <= 64 * nv * n ? 64 : C <= 256 * nv * n ? 256
+                                                                        : 1024;
 }
 
-// Workgroups of the backward: two a CU (each CU's registers hold two
-// workgroups' sums at least), fewer where the rows are few.
-int64_t backward_blocks(int64_t rows, int tpr) {
-    const int64_t groups = tpr && tpr < 256 ? 256 / tpr : 1;
-    const int64_t blocks = (rows + groups - 1) / groups;
-    return blocks < 512 ? blocks : 512;
+// Workgroups for `rows` rows, `at_once` in each.
+int64_t row_blocks(int64_t rows, int at_once, int64_t most) {
+    const int64_t blocks = (rows + at_once - 1) / at_once;
+    return blocks < most ? blocks : most;
 }
 
 using NormKernel = void (*)(LmNormArgs);
@@ -360,67 +424,78 @@ using NormKernel = void (*)(LmNormArgs);
 template <typename E, bool BWD, int TPR, int NV>
 NormKernel pick_tail(int64_t C) {
     const bool tail = C % Vec<E>::n != 0;
-    if (BWD)
+    if constexpr (BWD)
         return tail ? norm_bwd_kernel<E, TPR, NV, true>
                     : norm_bwd_kernel<E, TPR, NV, false>;
-    return tail ? norm_fwd_kernel<E, TPR, NV, true>
-                : norm_fwd_kernel<E, TPR, NV, false>;
+    else
+        return tail ? norm_fwd_kernel<E, TPR, NV, true>
+                    : norm_fwd_kernel<E, TPR, NV, false>;
 }
 
 template <typename E, bool BWD, int TPR>
 NormKernel pick_vectors(int64_t C) {
-    switch ((C + TPR * Vec<E>::n - 1) / (TPR * Vec<E>::n)) {
-    case 1: return pick_tail<E, BWD, TPR, 1>(C);
-    case 2: return pick_tail<E, BWD, TPR, 2>(C);
-    case 3: return pick_tail<E, BWD, TPR, 3>(C);
-    default: return pick_tail<E, BWD, TPR, 4>(C);
+    const int64_t nv = (C + TPR * Vec<E>::n - 1) / (TPR * Vec<E>::n);
+    if (nv == 1) return pick_tail<E, BWD, TPR, 1>(C);
+    if (nv == 2) return pick_tail<E, BWD, TPR, 2>(C);
+    if constexpr (!BWD && TPR < 1024) {
+        if (nv == 3) return pick_tail<E, BWD, TPR, 3>(C);
+        return pick_tail<E, BWD, TPR, 4>(C);
     }
+    return nullptr;
 }
 
 template <typename E, bool BWD>
-NormKernel pick(int64_t C) {
-    switch (threads_per_row<E>(C)) {
+NormKernel pick(int64_t C, int tpr) {
+    switch (tpr) {
     case 16: return pick_tail<E, BWD, 16, 1>(C);
     case 64: return pick_vectors<E, BWD, 64>(C);
     case 256: return pick_vectors<E, BWD, 256>(C);
     case 1024: return pick_vectors<E, BWD, 1024>(C);
-    default: return BWD ? norm_bwd_any_kernel<E> : norm_fwd_any_kernel<E>;
+    default:
+        if constexpr (BWD)
+            return norm_bwd_any_kernel<E>;
+        else
+            return norm_fwd_any_kernel<E>;
     }
 }
 
 }  // namespace
 
 int64_t lm_norm_workspace_floats(int64_t rows, int64_t C) {
-    // (a row group's share is at least one row in every variant)
-    return 2 * C * (rows < 512 ? rows : 512);
+    return 2 * C * (rows < kBwdBlocks ? rows : kBwdBlocks);
 }
 
 hipError_t launch_lm_norm(bool bf16, const LmNormArgs& A, hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    const int tpr =
-        bf16 ? threads_per_row<bf16_t>(A.C) : threads_per_row<float>(A.C);
-    const int64_t groups = tpr && tpr < 256 ? 256 / tpr : 1;
-    int64_t blocks = (A.rows + groups - 1) / groups;
-    if (blocks > 1024) blocks = 1024;
-    const auto kern = bf16 ? pick<bf16_t, false>(A.C) : pick<float, false>(A.C);
-    hipLaunchKernelGGL(kern, dim3(unsigned(blocks)),
-                       dim3(tpr > 256 ? tpr : 256), 0, stream, A);
+    const int tpr = bf16 ? threads_per_row<bf16_t>(A.C, false)
+                         : threads_per_row<float>(A.C, false);
+    const int threads = tpr > 256 ? tpr : 256;
+    const NormKernel kern = bf16 ? pick<bf16_t, false>(A.C, tpr)
+                                 : pick<float, false>(A.C, tpr);
+    if (!kern) return hipErrorInvalidValue;
+    const int64_t blocks =
+        row_blocks(A.rows, tpr ? threads / tpr : 1, kFwdBlocks);
+    hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(unsigned(threads)),
+                       0, stream, A);
     return hipGetLastError();
 }
 
 hipError_t launch_lm_norm_backward(bool bf16, const LmNormArgs& A,
                                    hipStream_t stream) {
     const bool params = A.dweight || A.dbias;
-    const int tpr =
-        bf16 ? threads_per_row<bf16_t>(A.C) : threads_per_row<float>(A.C);
-    const int64_t blocks = backward_blocks(A.rows, tpr);
+    const int tpr = bf16 ? threads_per_row<bf16_t>(A.C, true)
+                         : threads_per_row<float>(A.C, true);
+    const int threads = tpr ? kBwdThreads : kThreads;
+    const int64_t blocks =
+        row_blocks(A.rows, tpr ? threads / tpr : 1, kBwdBlocks);
     if (A.rows > 0 && (A.dx || params)) {
         LmNormArgs B = A;
         if (!params) B.workspace = nullptr;
-        const auto kern =
-            bf16 ? pick<bf16_t, true>(A.C) : pick<float, true>(A.C);
+        const NormKernel kern = bf16 ? pick<bf16_t, true>(A.C, tpr)
+                                     : pick<float, true>(A.C, tpr);
+        if (!kern) return hipErrorInvalidValue;
         hipLaunchKernelGGL(kern, dim3(unsigned(blocks)),
-                           dim3(tpr > 256 ? tpr : 256), 0, stream, B);
+                           dim3(unsigned(threads)), 0, stream, B);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !params) return e;
