@@ -19,6 +19,20 @@ __device__ __forceinline__ int64_t row_offset(const LmRows& R, int64_t row) {
     return row / R.inner * R.outer_stride + row % R.inner * R.inner_stride;
 }
 
+// One workgroup a row: a grid of 2^16 columns (a grid has fewer than 2^32
+// threads along an axis) and the row a workgroup of it takes, which may be
+// past the last one.  A loop over rows instead would keep what does not change
+// between them in registers that the row needs.
+inline dim3 row_grid(int64_t rows) {
+    const int64_t most = 1 << 16;
+    return rows <= most ? dim3(unsigned(rows))
+                        : dim3(unsigned(most),
+                               unsigned((rows + most - 1) / most));
+}
+__device__ __forceinline__ int64_t grid_row() {
+    return int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
+}
+
 // 16 bytes of adjacent elements, at their element's own alignment: gfx950
 // takes such a load or store as one instruction at any address.
 template <typename E>
@@ -87,31 +101,167 @@ __device__ __forceinline__ float block_sum(float x, float* s) {
     return block_fold<W>(x, s, [](float a, float b) { return a + b; });
 }
 
-// Softmax statistics of a set of logits x at temperature T, with c = log2(e)
-// / T: d = x - ref, e = 2^(d c), s0 = sum e, s1 = sum e d, where ref is the
-// largest x (0 in a set without one above -inf: there e is 0).  x - ref is
-// taken before the product with c: it is exact or nearly so where e counts,
-// and neither a row of the type's lowest value nor one near its largest
-// overflows.  d is held above -200 / c (2^-200 is 0 in fp32), so that -inf
-// adds nothing rather than NaN; NaN and +inf - inf stay NaN.
-struct SoftStats {
-    float ref, s0, s1;
+// The largest over the wave's lanes, the same in each of them.
+__device__ __forceinline__ float wave_larger(float x) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) x = larger(x, __shfl_xor(x, m));
+    return x;
+}
+
+// f over the W values that a workgroup's waves left in `s` (after a barrier),
+// the same in every lane: each lane takes one of them, so that it needs one
+// register and not W.
+template <int W, typename F>
+__device__ __forceinline__ float waves_fold(const float* s, F f) {
+    float x = s[threadIdx.x % W];
+#pragma unroll
+    for (int m = W / 2; m >= 1; m >>= 1) x = f(x, __shfl_xor(x, m));
+    return x;
+}
+
+template <int W>
+__device__ __forceinline__ float waves_sum(const float* s) {
+    return waves_fold<W>(s, [](float a, float b) { return a + b; });
+}
+
+// Waves a SIMD that a kernel with a Row of NV vectors a thread leaves room for:
+// the row's 4 NV registers and as many as 32 others of the SIMD's 512.
+template <int NV>
+constexpr int kRowWaves = NV <= 8 ? 8 : 4;
+
+// An offset that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint64_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(x)));
+    const uint64_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(x >> 32)));
+    return int64_t(hi << 32 | lo);
+}
+
+// A row of V logits in the registers of the NT threads of a workgroup: NV
+// whole vectors each, vector i * NT + thread, with -inf in the places past
+// the row's whole vectors; thread 0 holds the V % n elements behind them
+// (and -inf) in one more.  What is past the first NV * NT vectors is read
+// again from memory each time the row is walked.
+template <typename E, int NT, int NV>
+struct Row {
+    static constexpr int n = Vec<E>::n;
+    const E* x;
+    int V, whole;  // elements, whole vectors
+    Vec<E> v[NV], rest;
+
+    static __device__ __forceinline__ typename Vec<E>::raw_t nothing() {
+        return sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+    }
+    // vector k of the row, k = i * NT + thread (i the same in every thread)
+    static __device__ __forceinline__ E* at(E* p, int i) {
+        return reinterpret_cast<E*>(reinterpret_cast<char*>(p + i * NT * n) +
+                                    uint32_t(threadIdx.x) * 16u);
+    }
+    __device__ __forceinline__ void load(const E* p, int length) {
+        x = p;
+        V = length;
+        whole = V / n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i].raw = nothing();
+            if (i * NT + int(threadIdx.x) < whole)
+                v[i].load(at(const_cast<E*>(x), i));
+        }
+        rest.raw = nothing();
+        if (threadIdx.x == 0 && whole * n < V) {
+#pragma unroll
+            for (int j = 0; j < n; j += 2) {
+                const int id = whole * n + j;
+                rest.set2(j, id < V ? load_f(x + id) : rest.get(j),
+                          id + 1 < V ? load_f(x + id + 1) : rest.get(j + 1));
+            }
+        }
+    }
+    // f(vector, id of its first element) over the thread's vectors; the id is
+    // V for one of nothing but -inf past the row's whole vectors.  The empty asm keeps the compiler from carrying one walk's unpacked elements
+    // over to the next in two to four times the registers.
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            asm volatile("" : "+v"(v[i].raw));
+            const int k = i * NT + int(threadIdx.x);
+            if (i * NT < whole) f(v[i], k < whole ? k * n : V);
+        }
+#pragma unroll 1
+        for (int i = NV; i * NT < whole; ++i) {
+            if (i * NT + int(threadIdx.x) >= whole) break;
+            Vec<E> a;
+            a.load(at(const_cast<E*>(x), i));
+            f(a, (i * NT + int(threadIdx.x)) * n);
+        }
+        if (whole * n < V && threadIdx.x == 0) {
+            asm volatile("" : "+v"(rest.raw));
+            f(rest, whole * n);
+        }
+    }
+    __device__ __forceinline__ float largest() {
+        float m = -__builtin_inff();
+        each([&](const Vec<E>& a, int) {
+#pragma unroll
+            for (int j = 0; j < n; ++j) m = larger(m, a.get(j));
+        });
+        return m;
+    }
 };
 
-__device__ __forceinline__ float ref_of(float largest) {
-    return largest == -__builtin_inff() ? 0.f : largest;
-}
+// go(KERNEL<E, NT, NV>, NT) with the smallest workgroup that holds a row of V
+// logits: 256 threads up to 8 vectors each (16384 bf16), then 1024; rows past
+// 16 vectors of 1024 threads (131072 bf16) read their rest again each walk.
+#define RWKV7M_LM_ROW_KERNEL(KERNEL, E, V, go)        \
+    do {                                              \
+        constexpr int64_t vec = Vec<E>::n;            \
+        if ((V) <= 256 * 1 * vec)                     \
+            go(KERNEL<E, 256, 1>, 256);               \
+        else if ((V) <= 256 * 2 * vec)                \
+            go(KERNEL<E, 256, 2>, 256);               \
+        else if ((V) <= 256 * 4 * vec)                \
+            go(KERNEL<E, 256, 4>, 256);               \
+        else if ((V) <= 256 * 8 * vec)                \
+            go(KERNEL<E, 256, 8>, 256);               \
+        else if ((V) <= 1024 * 4 * vec)               \
+            go(KERNEL<E, 1024, 4>, 1024);             \
+        else if ((V) <= 1024 * 8 * vec)               \
+            go(KERNEL<E, 1024, 8>, 1024);             \
+        else                                          \
+            go(KERNEL<E, 1024, 16>, 1024);            \
+    } while (0)
 
-__device__ __forceinline__ float soft_d(float x, float ref, float lowest) {
-    return larger(x - ref, lowest);
-}
+// Softmax over a row of logits x at temperature T in base 2: t = x c - refc
+// in one fma, e = 2^t, with c = log2(e) / T and refc = ref c rounded, ref the
+// row's largest.  e is the softmax up to a factor that does not depend on x,
+// so the rounding of refc is no error as long as everything is taken from the
+// same t.  A row with no element above -inf has ref 0, and every e 0.
+// Where ref c is beyond 2^100 (rows of the type's lowest or largest values),
+// an element below the largest is at least 2^76 below it in units of 1 / c,
+// so its e is 0: there c is replaced by a power of two 2^60 below it, whose
+// product with x is exact, does not overflow and says the same.
+struct RowSoftmax {
+    float c, refc, ref;
 
-__device__ __forceinline__ void soft_add(SoftStats& a, float x, float c,
-                                         float lowest) {
-    const float d = soft_d(x, a.ref, lowest);
-    const float e = __builtin_amdgcn_exp2f(d * c);
-    a.s0 += e;
-    a.s1 = __builtin_fmaf(e, d, a.s1);
-}
+    __device__ __forceinline__ RowSoftmax(float largest, float c_) {
+        ref = largest == -__builtin_inff() ? 0.f : largest;
+        c = c_;
+        refc = ref * c;
+        if (fabsf(refc) > 0x1p100f) {
+            c = __uint_as_float(__float_as_uint(c_) & 0x7f800000u) * 0x1p-60f;
+            refc = ref * c;
+        }
+    }
+    __device__ __forceinline__ float t(float x) const {
+        return __builtin_fmaf(x, c, -refc);
+    }
+    __device__ __forceinline__ float e(float x) const {
+        return __builtin_amdgcn_exp2f(t(x));
+    }
+    // log2 of sum 2^((x - ref) c), from s = the sum of e
+    __device__ __forceinline__ float log2_sum(float s) const {
+        return __log2f(s) + __builtin_fmaf(-ref, c, refc);
+    }
+};
 
 }  // namespace rwkv7m

@@ -1,12 +1,27 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of
 // logits, and their backward (include/rwkv7m_lm_head.h has the formulas).
+//
+// Bound by memory: a row is read once.  One workgroup holds a row in its
+// registers as it came (65536 bf16 logits: 1024 threads of 32 registers), so
+// that the largest logit, the sums and the alternatives are three walks over
+// registers and not over memory.
+//
+// The alternatives.  Each thread's largest logit is known from the first
+// walk; the k-th largest over 256 groups of threads is a lower bound T of the
+// row's k-th largest logit, and for logits in no particular order not many
+// more than k of them lie at or above it (-256 log(1 - k / 256) on average).
+// The vectors that hold one go to LDS, their elements at or above T to a list
+// there, and each of those finds its rank by counting the ones before it.
+// Where they are more than LDS has room for (many equal logits, or large ones
+// at the same few threads), or NaN are among them, the list's bound is found
+// exactly, by bisection over the order of the values and then of the ids.
 
 #include "lm_rows.h"
 
 namespace rwkv7m {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kGroups = 256, kVectors = 256, kList = 512;
 
 // The order of the alternatives as an unsigned number: that of the floats,
 // -0 with +0, every NaN above +inf.
@@ -15,95 +30,289 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) {
+    if (k == 0xfffffffeu) return __builtin_nanf("");
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 
-// One workgroup a row.  The alternatives one at a time: the largest (key,
-// lowest id) below the one before.
-template <typename E>
-__global__ __launch_bounds__(kThreads) void score_kernel(LmScoreArgs A) {
-    __shared__ float s[kWaves];
-    __shared__ uint64_t su[kWaves];
-    const float c = A.c, lowest = -200.f / c, inv_t = c * kLn2;
-    for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
-        const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
-        float m = -__builtin_inff();
-        for (int64_t i = threadIdx.x; i < A.V; i += kThreads)
-            m = larger(m, load_f(x + i));
-        m = block_fold<kWaves>(m, s, larger);
-        SoftStats st{ref_of(m), 0.f, 0.f};
-        for (int64_t i = threadIdx.x; i < A.V; i += kThreads)
-            soft_add(st, load_f(x + i), c, lowest);
-        st.s0 = block_sum<kWaves>(st.s0, s);
-        st.s1 = block_sum<kWaves>(st.s1, s);
-        const float ls = kLn2 * __log2f(st.s0);
-        const auto logp = [&](float v) {
-            return __builtin_fmaf(v - st.ref, inv_t, -ls);
-        };
-        const bool empty = m == -__builtin_inff();
-        if (threadIdx.x == 0) {
-            const int64_t tok = A.tokens[row];
-            A.logprobs[row] = tok < 0       ? 0.f
-                              : tok >= A.V  ? __builtin_nanf("")
-                              : empty       ? -__builtin_inff()
-                                            : logp(load_f(x + tok));
-            A.entropy[row] = empty ? 0.f : ls - st.s1 / st.s0 * inv_t;
-            if (A.stats) {
-                A.stats[2 * row] = st.ref;
-                A.stats[2 * row + 1] = empty ? __builtin_inff() : ls;
-            }
+template <int W>
+struct ScoreShared {
+    float largest[W], sums[2][W], at_token;
+    int64_t token;
+    uint32_t groups[kGroups];
+    uint32_t bound;
+    int vectors, listed, counts[2][W];
+    // vectors that hold an element at or above the bound, with the id of
+    // their first element, and those elements, key above the id's complement
+    uint32_t raw[kVectors][4], first[kVectors];
+    uint64_t list[kList];
+};
+
+// The largest 32-bit number with 16 low zeros that at least k of the groups'
+// keys reach: 16 steps of a bisection with the wave's votes.  One wave.
+__device__ __forceinline__ uint32_t group_bound(const uint32_t* groups, int k) {
+    const int lane = threadIdx.x % 64;
+    uint32_t key[kGroups / 64];
+#pragma unroll
+    for (int i = 0; i < kGroups / 64; ++i) key[i] = groups[64 * i + lane];
+    uint32_t bound = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = bound | (1u << bit);
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < kGroups / 64; ++i)
+            count += __popcll(__ballot(key[i] >= t));
+        if (count >= k) bound = t;
+    }
+    return bound;
+}
+
+// How many of the row's first `ids` elements have yes(key, id), over the
+// workgroup; the two buffers of `counts` take turns.  From memory, for the
+// rows that need it.
+template <int W, typename R, typename F>
+__device__ __forceinline__ int count_row(const R& row, int ids,
+                                         ScoreShared<W>& S, int& turn, F yes) {
+    int count = 0;
+#pragma unroll 1
+    for (int id = threadIdx.x; id < ids; id += 64 * W)
+        count += yes(order_key(load_f(row.x + id)), id);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) count += __shfl_xor(count, m);
+    if (threadIdx.x % 64 == 0) S.counts[turn][threadIdx.x / 64] = count;
+    __syncthreads();
+    count = 0;
+    for (int w = 0; w < W; ++w) count += S.counts[turn][w];
+    turn ^= 1;
+    return count;
+}
+
+// Fills the list with the row's first K elements of the order.
+template <int W, typename R, typename P>
+__device__ void list_exactly(const R& row, int K, uint32_t largest,
+                             ScoreShared<W>& S, P put) {
+    // the largest key that K elements reach
+    int turn = 0;
+    uint32_t lo = 0, hi = largest;
+    while (lo < hi) {
+        const uint32_t mid = hi - (hi - lo) / 2;
+        if (count_row<W>(row, row.V, S, turn, [&](uint32_t k, int) {
+                return k >= mid;
+            }) >= K)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const int above = count_row<W>(row, row.V, S, turn,
+                                   [&](uint32_t k, int) { return k > lo; });
+    // the lowest id bound under which the elements of that key make K with
+    // those above it: doubled from 64 until it is one, then bisected
+    const auto enough = [&](int ids) {
+        return above + count_row<W>(row, ids, S, turn, [&](uint32_t k, int) {
+                   return k == lo;
+               }) >= K;
+    };
+    int ilo = 0, ihi = 64;
+    while (ihi < row.V && !enough(ihi)) {
+        ilo = ihi;
+        ihi *= 2;
+    }
+    if (ihi > row.V) ihi = row.V;
+    while (ihi - ilo > 1) {
+        const int mid = ilo + (ihi - ilo) / 2;
+        if (enough(mid))
+            ihi = mid;
+        else
+            ilo = mid;
+    }
+    if (threadIdx.x == 0) S.listed = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int id = threadIdx.x; id < row.V; id += 64 * W) {
+        const uint32_t k = order_key(load_f(row.x + id));
+        if (k > lo || (k == lo && id < ihi)) put(k, id);
+    }
+    __syncthreads();
+}
+
+template <typename E, int NT, int NV>
+__global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
+    LmScoreArgs A) {
+    constexpr int W = NT / 64, n = Vec<E>::n;
+    __shared__ ScoreShared<W> S;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int K = A.top_k, V = int(A.V);
+    const float inv_t = A.c * kLn2, inf = __builtin_inff();
+    const int64_t r = grid_row();
+    if (r >= A.rows) return;
+    Row<E, NT, NV> row;
+    row.load(static_cast<const E*>(A.x) + uniform(row_offset(A.xr, r)), V);
+    const float mine = row.largest();
+    const float wl = wave_larger(mine);
+    if (lane == 0) S.largest[wave] = wl;
+    if (threadIdx.x == 0) S.vectors = S.listed = 0;
+    if (K) {
+        float g = mine;  // the largest of a group of NT / 256 threads
+#pragma unroll
+        for (int m = 1; m < NT / kGroups; m *= 2)
+            g = larger(g, __shfl_xor(g, m));
+        if (threadIdx.x % (NT / kGroups) == 0)
+            S.groups[threadIdx.x / (NT / kGroups)] = order_key(g);
+    }
+    __syncthreads();
+    const float largest = waves_fold<W>(S.largest, larger);
+    if (K && wave == 0) {
+        const uint32_t b = group_bound(S.groups, K);
+        if (lane == 0) S.bound = b;
+    }
+    if (threadIdx.x == NT - 1) {
+        const int64_t tok = A.tokens[r];
+        S.token = tok;
+        if (tok >= 0 && tok < V) S.at_token = load_f(row.x + tok);
+    }
+    const RowSoftmax soft(largest, A.c);
+    float s0 = 0.f, s1 = 0.f;
+    row.each([&](const Vec<E>& a, int) {
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            // (held above -200, where e is 0 already: -inf adds 0, not
+            // 0 * -inf)
+            const float t = larger(soft.t(a.get(j)), -200.f);
+            const float e = __builtin_amdgcn_exp2f(t);
+            s0 += e;
+            s1 = __builtin_fmaf(e, t, s1);
         }
-        uint64_t last = ~uint64_t(0);
-        for (int k = 0; k < A.top_k; ++k) {
-            uint64_t best = 0;
-            for (int64_t i = threadIdx.x; i < A.V; i += kThreads) {
-                const uint64_t key =
-                    uint64_t(order_key(load_f(x + i))) << 32 |
-                    uint32_t(0xffffffffu - uint32_t(i));
-                if (key < last && key > best) best = key;
-            }
-            last = block_fold<kWaves>(
-                best, su,
-                [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-            if (threadIdx.x == 0) {
-                const uint32_t id = 0xffffffffu - uint32_t(last);
-                A.top_ids[row * A.top_k + k] = id;
-                A.top_logprobs[row * A.top_k + k] =
-                    empty ? -__builtin_inff() : logp(load_f(x + id));
-            }
+    });
+    s0 = lanes_sum<64>(s0);
+    s1 = lanes_sum<64>(s1);
+    if (lane == 0) {
+        S.sums[0][wave] = s0;
+        S.sums[1][wave] = s1;
+    }
+    __syncthreads();
+    s0 = waves_sum<W>(S.sums[0]);
+    s1 = waves_sum<W>(S.sums[1]);
+    const bool empty = largest == -inf;
+    const float ls = kLn2 * soft.log2_sum(s0);
+    const auto logp = [&](float x) {
+        return empty ? -inf : __builtin_fmaf(x - soft.ref, inv_t, -ls);
+    };
+    if (threadIdx.x == 0) {
+        A.logprobs[r] = S.token < 0    ? 0.f
+                        : S.token >= V ? __builtin_nanf("")
+                                       : logp(S.at_token);
+        A.entropy[r] = empty ? 0.f : kLn2 * (__log2f(s0) - s1 / s0);
+        if (A.stats) {
+            A.stats[2 * r] = soft.ref;
+            A.stats[2 * r + 1] = empty ? inf : ls;
+        }
+    }
+    if (!K) return;
+    const uint32_t bound = S.bound;
+    // (below the key of -inf: the groups that hold anything are fewer
+    // than k)
+    const float least = bound < 0x00800000u ? -inf : key_value(bound);
+    const auto put = [&](uint32_t key, int id) {
+        const int at = atomicAdd(&S.listed, 1);
+        if (at < kList)
+            S.list[at] = uint64_t(key) << 32 | (0xffffffffu - uint32_t(id));
+    };
+    if (mine >= least)
+        row.each([&](const Vec<E>& a, int id) {
+            float most = a.get(0);
+#pragma unroll
+            for (int j = 1; j < n; ++j) most = larger(most, a.get(j));
+            if (!(most >= least) || id >= V) return;
+            const int at = atomicAdd(&S.vectors, 1);
+            if (at >= kVectors) return;
+            S.first[at] = uint32_t(id);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) S.raw[at][w] = a.raw[w];
+        });
+    __syncthreads();
+    const int vectors = S.vectors;
+    for (int i = threadIdx.x; i < vectors * n && vectors <= kVectors;
+         i += NT) {
+        const E* from = reinterpret_cast<const E*>(S.raw[i / n]);
+        const float x = load_f(from + i % n);
+        const int id = int(S.first[i / n]) + i % n;
+        if (x >= least && id < V) put(order_key(x), id);
+    }
+    __syncthreads();
+    int listed = S.listed;
+    if (vectors > kVectors || listed > kList || largest != largest) {
+        list_exactly<W>(row, K, order_key(largest), S, put);
+        listed = K;
+    }
+    for (int i = threadIdx.x; i < listed; i += NT) {
+        const uint64_t own = S.list[i];
+        int rank = 0;
+        for (int j = 0; j < listed; ++j) rank += S.list[j] > own;
+        if (rank < K) {
+            A.top_ids[r * K + rank] = 0xffffffffu - uint32_t(own);
+            A.top_logprobs[r * K + rank] =
+                logp(key_value(uint32_t(own >> 32)));
         }
     }
 }
 
+// dlogits: a workgroup a tile of kTile vectors a thread of one row.
+constexpr int kBwdThreads = 256, kTile = 4;
+
 template <typename E>
-__global__ __launch_bounds__(kThreads) void score_bwd_kernel(LmScoreArgs A) {
+__global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A) {
+    constexpr int n = Vec<E>::n, kCols = kBwdThreads * kTile * n;
     const float inv_t = A.c * kLn2;
-    for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
-        const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, row);
-        E* dx = static_cast<E*>(A.dlogits) + row * A.V;
-        const int64_t tok = A.tokens[row];
+    const int64_t tiles = (A.V + kCols - 1) / kCols;
+    for (int64_t tile = blockIdx.x; tile < A.rows * tiles; tile += gridDim.x) {
+        const int64_t r = tile / tiles;
+        const int V = int(A.V);
+        const int first = int(tile % tiles) * kCols + int(threadIdx.x) * n;
+        const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, r);
+        E* dx = static_cast<E*>(A.dlogits) + r * A.V;
+        const int64_t tok = A.tokens[r];
         const float dl =
-            A.d_logprobs && tok >= 0 ? A.d_logprobs[row] * inv_t : 0.f;
-        const float de = A.d_entropy ? A.d_entropy[row] * inv_t : 0.f;
-        const float ref = A.stats[2 * row], ls = A.stats[2 * row + 1];
-        const float h = A.entropy[row];
+            A.d_logprobs && tok >= 0 ? A.d_logprobs[r] * inv_t : 0.f;
+        const float de = A.d_entropy ? A.d_entropy[r] * inv_t : 0.f;
+        const float ref = A.stats[2 * r], ls = A.stats[2 * r + 1];
         const bool any = dl != 0.f || de != 0.f;
-        const float nan = tok >= A.V && dl != 0.f ? __builtin_nanf("") : 0.f;
-        for (int64_t i = threadIdx.x; i < A.V; i += kThreads) {
-            float d = 0.f;
-            if (any) {
-                // (held above -150, whose exp is 0 in fp32: -inf gives no NaN)
-                const float lp = larger(
-                    __builtin_fmaf(load_f(x + i) - ref, inv_t, -ls), -150.f);
-                d = nan - __builtin_amdgcn_exp2f(lp * kLog2e) *
-                              (dl + de * (lp + h));
-                if (i == tok) d += dl;
+        // -p (dl + de (lp + h)) = p (lp g1 + g0), NaN for a token past V
+        const float g1 = -de;
+        const float g0 = tok >= V && dl != 0.f ? __builtin_nanf("")
+                                               : -dl - de * A.entropy[r];
+        const auto grad = [&](float v, int id) {
+            // (held above -150, whose exp is 0 in fp32: -inf gives no NaN)
+            const float lp =
+                larger(__builtin_fmaf(v - ref, inv_t, -ls), -150.f);
+            const float d = __builtin_amdgcn_exp2f(lp * kLog2e) *
+                            __builtin_fmaf(lp, g1, g0);
+            return id == tok ? d + dl : d;
+        };
+        Vec<E> v[kTile];
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+            const int at = first + i * kBwdThreads * n;
+            v[i].raw = 0;
+            if (any && at + n <= V) v[i].load(x + at);
+        }
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+            const int at = first + i * kBwdThreads * n;
+            if (at + n <= V) {
+                if (any) {
+#pragma unroll
+                    for (int j = 0; j < n; j += 2)
+                        v[i].set2(j, grad(v[i].get(j), at + j),
+                                  grad(v[i].get(j + 1), at + j + 1));
+                }
+                v[i].store(dx + at);
+            } else {
+                for (int j = at; j < V; ++j)
+                    store_f(dx + j, any ? grad(load_f(x + j), j) : 0.f);
             }
-            store_f(dx + i, d);
         }
     }
-}
-
-unsigned row_grid(int64_t rows) {
-    return unsigned(rows < (1 << 20) ? rows : 1 << 20);
 }
 
 }  // namespace
@@ -111,17 +320,26 @@ unsigned row_grid(int64_t rows) {
 hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
                            hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    hipLaunchKernelGGL(bf16 ? score_kernel<bf16_t> : score_kernel<float>,
-                       dim3(row_grid(A.rows)), dim3(kThreads), 0, stream, A);
+    const auto go = [&](auto kern, unsigned threads) {
+        hipLaunchKernelGGL(kern, row_grid(A.rows), dim3(threads), 0, stream,
+                           A);
+    };
+    if (bf16)
+        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, go);
+    else
+        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, go);
     return hipGetLastError();
 }
 
 hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
                                     hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
+    const int64_t cols = kBwdThreads * kTile * (bf16 ? 8 : 4);
+    const int64_t tiles = A.rows * ((A.V + cols - 1) / cols);
     hipLaunchKernelGGL(
         bf16 ? score_bwd_kernel<bf16_t> : score_bwd_kernel<float>,
-        dim3(row_grid(A.rows)), dim3(kThreads), 0, stream, A);
+        dim3(unsigned(tiles < (1 << 20) ? tiles : 1 << 20)), dim3(kBwdThreads),
+        0, stream, A);
     return hipGetLastError();
 }
 

@@ -910,6 +910,7 @@ int lm_distill_args(const char* fn, int dtype, int teacher_dtype,
     A->x = logits;
     A->ids = ids;
     A->teacher = teacher;
+    A->teacher_bf16 = teacher_dtype == RWKV7M_DTYPE_BF16;
     A->weight = weight;
     A->mean_weight = A->rows > 0 ? float(1.0 / double(A->rows)) : 0.f;
     A->c = float(1.4426950408889634 / temperature);
@@ -1908,8 +1909,7 @@ int rwkv7m_distill_loss(int dtype, int teacher_dtype, int64_t outer,
         A.row_losses = row_losses;
         return hip_status("distillation loss launch",
                           rwkv7m::launch_lm_distill(
-                              dtype == RWKV7M_DTYPE_BF16,
-                              teacher_dtype == RWKV7M_DTYPE_BF16, A,
+                              dtype == RWKV7M_DTYPE_BF16, A,
                               static_cast<hipStream_t>(stream)));
     });
 }
@@ -1934,8 +1934,7 @@ int rwkv7m_distill_loss_backward(
         A.holds_unit = holds_unit != 0;
         return hip_status("distillation gradient launch",
                           rwkv7m::launch_lm_distill(
-                              dtype == RWKV7M_DTYPE_BF16,
-                              teacher_dtype == RWKV7M_DTYPE_BF16, A,
+                              dtype == RWKV7M_DTYPE_BF16, A,
                               static_cast<hipStream_t>(stream)));
     });
 }

@@ -339,6 +339,7 @@ struct LmDistillArgs {
     const void* x;
     const int64_t* ids;
     const void* teacher;
+    int teacher_bf16;
     const float* weight;  // may be 0: mean_weight each
     float mean_weight;
     float c, temperature;  // c = log2(e) / temperature
@@ -355,8 +356,8 @@ hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
                            hipStream_t stream);
 hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
                                     hipStream_t stream);
-hipError_t launch_lm_distill(bool bf16, bool teacher_bf16,
-                             const LmDistillArgs& A, hipStream_t stream);
+hipError_t launch_lm_distill(bool bf16, const LmDistillArgs& A,
+                             hipStream_t stream);
 
 // One token (T = 1) for N = 64 without checkpoints; s_t may alias s0.
 hipError_t launch_decode(const SeqFwdArgs& p, hipStream_t stream);

@@ -541,6 +541,28 @@ def test_distill_without_rows_or_alternatives(lm):
     assert s.top_ids.shape == (2, 0, 2) and s.logprobs.shape == (2, 0)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [9, 2047, 2051, 8203, 16387, 20005, 32769,
+                               40003, 65531, 131075, 140007])
+def test_every_place_of_a_row_counts(lm, V, dtype):
+    """Rows with all their weight at their ends or in the middle: each element
+    there is most of the sum, of the gradient and of the alternatives."""
+    print("case: weight at the ends", V, dtype, flush=True)
+    x = _logits(_gen(V), 4, V, dtype=dtype)
+    ends = list(range(min(V, 12))) + list(range(max(0, V - 12), V))
+    x[0, ends] = 20.0 + torch.arange(float(len(ends))).to(x.dtype) / 8
+    x[1, V - 1] = 30.0
+    x[2, :] = -INF
+    x[2, ends[::2]] = 1.0
+    x[3, V // 2 - 1:V // 2 + 9] = 25.0
+    tok = torch.tensor([V - 1, V - 1, ends[0], V // 2]).cuda()
+    _check_score(lm, x.cuda(), tok, min(V, 30))
+    ids = torch.tensor([[V - 1, 0], [V - 2, V - 1], [ends[0], ends[2]],
+                        [V // 2, V - 1]]).cuda()
+    top = torch.tensor([[1.0, 2.0], [0.5, 0.0], [0.0, 0.0], [3.0, 1.0]]).cuda()
+    _check_distill(lm, x.cuda(), ids, top, None, 1.0)
+
+
 # --- gradients against differences ----------------------------------------
 
 def _against_differences(f, leaves, step=1e-2):
