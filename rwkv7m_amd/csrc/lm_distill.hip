@@ -84,7 +84,7 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void distill_kernel(
     }
     const RowSoftmax soft(largest, A.c), teacher(teacher_largest, A.c);
     float s0 = 0.f;
-    row.each([&](const Vec<E>& a, int) {
+    row.each([&](const Vec<E>& a, int, int) {
 #pragma unroll
         for (int j = 0; j < n; ++j) s0 += soft.e(a.get(j));
     });
@@ -123,15 +123,15 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void distill_kernel(
     const float wt = w * A.temperature * scale;
     const float wp = (s0 == 0.f ? 0.f : wt / s0) + bad;
     if (dx)
-        row.each([&](const Vec<E>& a, int at) {
+        row.each([&](const Vec<E>& a, int id, int from) {
             Vec<E> g;
 #pragma unroll
             for (int j = 0; j < n; j += 2)
                 g.set2(j, wp * soft.e(a.get(j)), wp * soft.e(a.get(j + 1)));
-            if (at + n <= V)
-                g.store(dx + at);
+            if (from == 0)
+                g.store(dx + id);
             else
-                for (int j = 0; at + j < V; ++j) store_f(dx + at + j, g.get(j));
+                for (int j = from; j < n; ++j) store_f(dx + id + j, g.get(j));
         });
     __syncthreads();
     const float kl = waves_sum<4>(S.teacher[2]) + bad;

@@ -138,9 +138,10 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
 
 // A row of V logits in the registers of the NT threads of a workgroup: NV
 // whole vectors each, vector i * NT + thread, with -inf in the places past
-// the row's whole vectors; thread 0 holds the V % n elements behind them
-// (and -inf) in one more.  What is past the first NV * NT vectors is read
-// again from memory each time the row is walked.
+// the row's whole vectors.  Thread 0 holds the V % n elements behind them in
+// one more, which ends with the row (so that it is one load) and has -inf in
+// place of the elements that are the last whole vector's.  What is past the
+// first NV * NT vectors is read again from memory each time the row is walked.
 template <typename E, int NT, int NV>
 struct Row {
     static constexpr int n = Vec<E>::n;
@@ -151,10 +152,11 @@ struct Row {
     static __device__ __forceinline__ typename Vec<E>::raw_t nothing() {
         return sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
     }
-    // vector k of the row, k = i * NT + thread (i the same in every thread)
-    static __device__ __forceinline__ E* at(E* p, int i) {
-        return reinterpret_cast<E*>(reinterpret_cast<char*>(p + i * NT * n) +
-                                    uint32_t(threadIdx.x) * 16u);
+    // vector i * NT + thread of the row (i the same in every thread)
+    __device__ __forceinline__ const E* at(int i) const {
+        return reinterpret_cast<const E*>(
+            reinterpret_cast<const char*>(x + i * NT * n) +
+            uint32_t(threadIdx.x) * 16u);
     }
     __device__ __forceinline__ void load(const E* p, int length) {
         x = p;
@@ -163,45 +165,49 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             v[i].raw = nothing();
-            if (i * NT + int(threadIdx.x) < whole)
-                v[i].load(at(const_cast<E*>(x), i));
+            if (i * NT + int(threadIdx.x) < whole) v[i].load(at(i));
         }
         rest.raw = nothing();
         if (threadIdx.x == 0 && whole * n < V) {
+            if (V >= n) rest.load(x + V - n);
 #pragma unroll
             for (int j = 0; j < n; j += 2) {
-                const int id = whole * n + j;
-                rest.set2(j, id < V ? load_f(x + id) : rest.get(j),
-                          id + 1 < V ? load_f(x + id + 1) : rest.get(j + 1));
+                const auto get = [&](int i) {
+                    if (i < n - V % n) return -__builtin_inff();
+                    return V < n ? load_f(x + V - n + i) : rest.get(i);
+                };
+                rest.set2(j, get(j), get(j + 1));
             }
         }
     }
-    // f(vector, id of its first element) over the thread's vectors; the id is
-    // V for one of nothing but -inf past the row's whole vectors.  The empty asm keeps the compiler from carrying one walk's unpacked elements
-    // over to the next in two to four times the registers.
+    // f(vector, id of its element 0, least j that is an element of the row)
+    // over the thread's vectors; the last is n for one past the row's whole
+    // vectors.  The empty asm keeps the compiler from carrying one walk's
+    // unpacked elements over to the next in two to four times the registers.
     template <typename F>
     __device__ __forceinline__ void each(F f) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             asm volatile("" : "+v"(v[i].raw));
             const int k = i * NT + int(threadIdx.x);
-            if (i * NT < whole) f(v[i], k < whole ? k * n : V);
+            if (i * NT < whole) f(v[i], k * n, k < whole ? 0 : n);
         }
 #pragma unroll 1
         for (int i = NV; i * NT < whole; ++i) {
-            if (i * NT + int(threadIdx.x) >= whole) break;
+            const int k = i * NT + int(threadIdx.x);
+            if (k >= whole) break;
             Vec<E> a;
-            a.load(at(const_cast<E*>(x), i));
-            f(a, (i * NT + int(threadIdx.x)) * n);
+            a.load(at(i));
+            f(a, k * n, 0);
         }
         if (whole * n < V && threadIdx.x == 0) {
             asm volatile("" : "+v"(rest.raw));
-            f(rest, whole * n);
+            f(rest, V - n, n - V % n);
         }
     }
     __device__ __forceinline__ float largest() {
         float m = -__builtin_inff();
-        each([&](const Vec<E>& a, int) {
+        each([&](const Vec<E>& a, int, int) {
 #pragma unroll
             for (int j = 0; j < n; ++j) m = larger(m, a.get(j));
         });

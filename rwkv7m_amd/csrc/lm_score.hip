@@ -43,8 +43,10 @@ struct ScoreShared {
     uint32_t bound;
     int vectors, listed, counts[2][W];
     // vectors that hold an element at or above the bound, with the id of
-    // their first element, and those elements, key above the id's complement
-    uint32_t raw[kVectors][4], first[kVectors];
+    // element 0 and their least element, and those elements, key above the
+    // id's complement
+    uint32_t raw[kVectors][4];
+    int first[kVectors], from[kVectors];
     uint64_t list[kList];
 };
 
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
     }
     const RowSoftmax soft(largest, A.c);
     float s0 = 0.f, s1 = 0.f;
-    row.each([&](const Vec<E>& a, int) {
+    row.each([&](const Vec<E>& a, int, int) {
 #pragma unroll
         for (int j = 0; j < n; ++j) {
             // (held above -200, where e is 0 already: -inf adds 0, not
@@ -219,25 +221,24 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
             S.list[at] = uint64_t(key) << 32 | (0xffffffffu - uint32_t(id));
     };
     if (mine >= least)
-        row.each([&](const Vec<E>& a, int id) {
+        row.each([&](const Vec<E>& a, int id, int from) {
             float most = a.get(0);
 #pragma unroll
             for (int j = 1; j < n; ++j) most = larger(most, a.get(j));
-            if (!(most >= least) || id >= V) return;
+            if (!(most >= least) || from == n) return;
             const int at = atomicAdd(&S.vectors, 1);
             if (at >= kVectors) return;
-            S.first[at] = uint32_t(id);
+            S.first[at] = id;
+            S.from[at] = from;
 #pragma unroll
             for (int w = 0; w < 4; ++w) S.raw[at][w] = a.raw[w];
         });
     __syncthreads();
     const int vectors = S.vectors;
-    for (int i = threadIdx.x; i < vectors * n && vectors <= kVectors;
-         i += NT) {
-        const E* from = reinterpret_cast<const E*>(S.raw[i / n]);
-        const float x = load_f(from + i % n);
-        const int id = int(S.first[i / n]) + i % n;
-        if (x >= least && id < V) put(order_key(x), id);
+    for (int i = threadIdx.x; i < vectors * n && vectors <= kVectors; i += NT) {
+        const int v = i / n, j = i % n;
+        const float x = load_f(reinterpret_cast<const E*>(S.raw[v]) + j);
+        if (x >= least && j >= S.from[v]) put(order_key(x), S.first[v] + j);
     }
     __syncthreads();
     int listed = S.listed;
