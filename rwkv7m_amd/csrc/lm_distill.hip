@@ -16,21 +16,25 @@
 namespace rwkv7m {
 namespace {
 
-constexpr int kMaxK = 256;
+// Threads that hold an alternative: the first 4 waves, or the only one.
+template <int NT>
+constexpr int kTeacher = NT < 256 ? NT : 256;
 
-template <int W>
+template <int NT>
 struct DistillShared {
-    float largest[W], sums[W], teacher[3][4], bad[4];
-    int ids[kMaxK];
-    float q[kMaxK];
+    static constexpr int KT = kTeacher<NT>, KW = KT / 64;
+    float largest[NT / 64], sums[NT / 64], teacher[3][KW], bad[KW];
+    // each alternative's id (-1: none, -2: past the vocabulary), teacher's
+    // logit, then q, and student's logit
+    int ids[KT];
+    float q[KT], student[KT];
 };
 
 template <typename E, int NT, int NV>
 __global__ __launch_bounds__(NT, kRowWaves<NV>) void distill_kernel(
     LmDistillArgs A) {
-    constexpr int W = NT / 64, n = Vec<E>::n;
-    static_assert(kMaxK == 256 && NT >= kMaxK, "an alternative a thread");
-    __shared__ DistillShared<W> S;
+    constexpr int W = NT / 64, KW = kTeacher<NT> / 64, n = Vec<E>::n;
+    __shared__ DistillShared<NT> S;
     const int64_t r = grid_row();
     if (r >= A.rows) return;
     float scale = 1.f;
@@ -43,7 +47,6 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void distill_kernel(
     const float inf = __builtin_inff();
     const float w = A.weight ? A.weight[r] : A.mean_weight;
     E* dx = A.dlogits ? static_cast<E*>(A.dlogits) + r * A.V : nullptr;
-    Row<E, NT, NV> row;
     const auto clear = [&] {
         if (threadIdx.x == 0 && A.row_losses) A.row_losses[r] = 0.f;
         if (!dx) return;
@@ -56,85 +59,85 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void distill_kernel(
         clear();
         return;
     }
-    row.load(static_cast<const E*>(A.x) + uniform(row_offset(A.xr, r)), V);
-    int64_t id = -1;
-    float t = -inf, at_id = 0.f;  // the teacher's logit, the student's
-    if (k < K) {
-        id = A.ids[r * K + k];
-        const int64_t i = r * K + k;
-        if (id >= 0)
-            t = A.teacher_bf16
-                    ? bf16_to_f32(static_cast<const bf16_t*>(A.teacher)[i])
-                    : static_cast<const float*>(A.teacher)[i];
-        if (id >= 0 && id < V) at_id = load_f(row.x + id);
-    }
-    const float mine = row.largest();
-    const float wl = wave_larger(mine);
-    if (lane == 0) S.largest[wave] = wl;
-    if (wave < 4) {
+    Row<E, NT, NV> row(
+        static_cast<const E*>(A.x) + uniform(row_offset(A.xr, r)), V);
+    if (wave < KW) {
+        int id = -1;
+        float t = -inf, at_id = 0.f;
+        if (k < K) {
+            const int64_t i = r * K + k, full = A.ids[i];
+            if (full >= 0) {
+                t = A.teacher_bf16
+                        ? bf16_to_f32(static_cast<const bf16_t*>(A.teacher)[i])
+                        : static_cast<const float*>(A.teacher)[i];
+                id = full < V ? int(full) : -2;
+                if (full < V) at_id = load_f(row.x + id);
+            }
+        }
+        S.ids[k] = id;
+        S.q[k] = t;
+        S.student[k] = at_id;
         const float tl = wave_larger(t);
         if (lane == 0) S.teacher[0][wave] = tl;
     }
+    const float wl = wave_larger(row.largest());
+    if (lane == 0) S.largest[wave] = wl;
     __syncthreads();
-    const float largest = waves_fold<W>(S.largest, larger);
-    const float teacher_largest = waves_fold<4>(S.teacher[0], larger);
+    const float teacher_largest = waves_fold<KW>(S.teacher[0], larger);
     if (teacher_largest == -inf) {
         clear();
         return;
     }
-    const RowSoftmax soft(largest, A.c), teacher(teacher_largest, A.c);
-    float s0 = 0.f;
-    row.each([&](const Vec<E>& a, int, int) {
-#pragma unroll
-        for (int j = 0; j < n; ++j) s0 += soft.e(a.get(j));
-    });
-    s0 = lanes_sum<64>(s0);
-    if (lane == 0) S.sums[wave] = s0;
-    const float te = id >= 0 ? teacher.e(t) : 0.f;
-    if (wave < 4) {
-        const float es = lanes_sum<64>(te);
+    const RowSoftmax soft(waves_fold<W>(S.largest, larger), A.c);
+    const RowSoftmax teacher(teacher_largest, A.c);
+    if (wave < KW) {
+        const float te = teacher.e(S.q[k]);
+        const float es = lanes_sum<64>(S.ids[k] == -1 ? 0.f : te);
         // an id past the vocabulary: NaN for the row
-        const float bad = __any(id >= V) ? __builtin_nanf("") : 0.f;
+        const float bad = __any(S.ids[k] == -2) ? __builtin_nanf("") : 0.f;
         if (lane == 0) {
             S.teacher[1][wave] = es;
             S.bad[wave] = bad;
         }
     }
+    float s0 = soft.e(row.one);
+    row.each([&](const Vec<E>& a, int) {
+#pragma unroll
+        for (int j = 0; j < n; ++j) s0 += soft.e(a.get(j));
+    });
+    s0 = lanes_sum<64>(s0);
+    if (lane == 0) S.sums[wave] = s0;
     __syncthreads();
     s0 = waves_sum<W>(S.sums);
-    const float ts = waves_sum<4>(S.teacher[1]);
-    const float bad = waves_sum<4>(S.bad);
-    const float q = te / ts;
-    if (wave < 4) {
+    const float bad = waves_sum<KW>(S.bad);
+    if (wave < KW) {
+        const float ts = waves_sum<KW>(S.teacher[1]), t = S.q[k];
+        const float q = S.ids[k] == -1 ? 0.f : teacher.e(t) / ts;
         float share = 0.f;
         if (q != 0.f) {
-            // log2 q - log2 p
-            const float lp = largest == -inf
-                                 ? -inf
-                                 : (at_id - soft.ref) * A.c -
-                                       soft.log2_sum(s0);
+            // log2 q - log2 p; a row of nothing but -inf has p = 0
+            const float lp = (S.student[k] - soft.ref) * A.c -
+                             (s0 == 0.f ? inf : soft.log2_sum(s0));
             share = q * ((t - teacher.ref) * A.c - teacher.log2_sum(ts) - lp);
         }
         share = lanes_sum<64>(share);
         if (lane == 0) S.teacher[2][wave] = share;
-        S.ids[k] = id >= 0 && id < V ? int(id) : -1;
         S.q[k] = q;
     }
     const float wt = w * A.temperature * scale;
-    const float wp = (s0 == 0.f ? 0.f : wt / s0) + bad;
-    if (dx)
-        row.each([&](const Vec<E>& a, int id, int from) {
+    const float wp = uniform((s0 == 0.f ? 0.f : wt / s0) + bad);
+    if (dx) {
+        row.each([&](const Vec<E>& a, int i) {
             Vec<E> g;
 #pragma unroll
             for (int j = 0; j < n; j += 2)
                 g.set2(j, wp * soft.e(a.get(j)), wp * soft.e(a.get(j + 1)));
-            if (from == 0)
-                g.store(dx + id);
-            else
-                for (int j = from; j < n; ++j) store_f(dx + id + j, g.get(j));
+            if (i < row.cut.whole) g.store(dx + row.cut.lead + i * n);
         });
+        if (row.has_one()) store_f(dx + row.one_id(), wp * soft.e(row.one));
+    }
     __syncthreads();
-    const float kl = waves_sum<4>(S.teacher[2]) + bad;
+    const float kl = waves_sum<KW>(S.teacher[2]) + bad;
     if (threadIdx.x == 0 && A.row_losses)
         A.row_losses[r] = kl * kLn2 * A.temperature * A.temperature;
     if (!dx || k >= K || S.ids[k] < 0) return;
@@ -146,7 +149,8 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void distill_kernel(
         sum += S.q[j];
     }
     if (first)
-        store_f(dx + S.ids[k], __builtin_fmaf(soft.e(at_id), wp, -sum * wt));
+        store_f(dx + S.ids[k],
+                __builtin_fmaf(soft.e(S.student[k]), wp, -sum * wt));
 }
 
 // loss = sum_r weight[r] row_losses[r], one workgroup, in float64.
@@ -165,14 +169,15 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(LmDistillArgs A) {
 hipError_t launch_lm_distill(bool bf16, const LmDistillArgs& A,
                              hipStream_t stream) {
     if (A.rows > 0) {
+        const bool wave = A.K <= kTeacher<64>;
         const auto go = [&](auto kern, unsigned threads) {
             hipLaunchKernelGGL(kern, row_grid(A.rows), dim3(threads), 0,
                                stream, A);
         };
         if (bf16)
-            RWKV7M_LM_ROW_KERNEL(distill_kernel, bf16_t, A.V, go);
+            RWKV7M_LM_ROW_KERNEL(distill_kernel, bf16_t, A.V, wave, go);
         else
-            RWKV7M_LM_ROW_KERNEL(distill_kernel, float, A.V, go);
+            RWKV7M_LM_ROW_KERNEL(distill_kernel, float, A.V, wave, go);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !A.loss) return e;

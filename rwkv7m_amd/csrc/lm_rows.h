@@ -113,6 +113,7 @@ __device__ __forceinline__ float wave_larger(float x) {
 // register and not W.
 template <int W, typename F>
 __device__ __forceinline__ float waves_fold(const float* s, F f) {
+    static_assert(W >= 1 && W <= 64 && (W & (W - 1)) == 0, "");
     float x = s[threadIdx.x % W];
 #pragma unroll
     for (int m = W / 2; m >= 1; m >>= 1) x = f(x, __shfl_xor(x, m));
@@ -136,78 +137,86 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return int64_t(hi << 32 | lo);
 }
 
+__device__ __forceinline__ float uniform(float x) {
+    return __uint_as_float(uint32_t(
+        __builtin_amdgcn_readfirstlane(int(__float_as_uint(x)))));
+}
+
+// A row of V elements cut at the addresses that are multiples of 16 bytes:
+// `lead` elements, `whole` vectors, `rest` elements (rows whose vectors
+// straddle cost a quarter more time in the load instructions).
+template <typename E>
+struct Cut {
+    static constexpr int n = Vec<E>::n;
+    int lead, whole, rest;
+
+    __device__ __forceinline__ Cut(const E* x, int V) {
+        const uint32_t past = uint32_t(reinterpret_cast<uint64_t>(x)) & 15u;
+        lead = int((16u - past) & 15u) / int(sizeof(E));
+        if (lead > V) lead = V;
+        whole = (V - lead) / n;
+        rest = (V - lead) % n;
+    }
+};
+
 // A row of V logits in the registers of the NT threads of a workgroup: NV
 // whole vectors each, vector i * NT + thread, with -inf in the places past
-// the row's whole vectors.  Thread 0 holds the V % n elements behind them in
-// one more, which ends with the row (so that it is one load) and has -inf in
-// place of the elements that are the last whole vector's.  What is past the
-// first NV * NT vectors is read again from memory each time the row is walked.
+// the row's whole vectors, and the elements before and behind those one to a
+// thread (-inf in the others).  What is past the first NV * NT vectors is read
+// again from memory each time the row is walked.
 template <typename E, int NT, int NV>
 struct Row {
     static constexpr int n = Vec<E>::n;
     const E* x;
-    int V, whole;  // elements, whole vectors
-    Vec<E> v[NV], rest;
+    int V;
+    Cut<E> cut;
+    Vec<E> v[NV];
+    float one;
 
-    static __device__ __forceinline__ typename Vec<E>::raw_t nothing() {
-        return sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+    __device__ __forceinline__ Row(const E* p, int length)
+        : x(p), V(length), cut(p, length) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i].raw = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+            if (i * NT + int(threadIdx.x) < cut.whole) v[i].load(at(i));
+        }
+        one = has_one() ? load_f(x + one_id()) : -__builtin_inff();
     }
     // vector i * NT + thread of the row (i the same in every thread)
     __device__ __forceinline__ const E* at(int i) const {
         return reinterpret_cast<const E*>(
-            reinterpret_cast<const char*>(x + i * NT * n) +
+            reinterpret_cast<const char*>(x + cut.lead + i * NT * n) +
             uint32_t(threadIdx.x) * 16u);
     }
-    __device__ __forceinline__ void load(const E* p, int length) {
-        x = p;
-        V = length;
-        whole = V / n;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            v[i].raw = nothing();
-            if (i * NT + int(threadIdx.x) < whole) v[i].load(at(i));
-        }
-        rest.raw = nothing();
-        if (threadIdx.x == 0 && whole * n < V) {
-            if (V >= n) rest.load(x + V - n);
-#pragma unroll
-            for (int j = 0; j < n; j += 2) {
-                const auto get = [&](int i) {
-                    if (i < n - V % n) return -__builtin_inff();
-                    return V < n ? load_f(x + V - n + i) : rest.get(i);
-                };
-                rest.set2(j, get(j), get(j + 1));
-            }
-        }
+    __device__ __forceinline__ bool has_one() const {
+        return int(threadIdx.x) < cut.lead + cut.rest;
     }
-    // f(vector, id of its element 0, least j that is an element of the row)
-    // over the thread's vectors; the last is n for one past the row's whole
-    // vectors.  The empty asm keeps the compiler from carrying one walk's
-    // unpacked elements over to the next in two to four times the registers.
+    __device__ __forceinline__ int one_id() const {
+        const int t = threadIdx.x;
+        return t < cut.lead ? t : V - cut.rest - cut.lead + t;
+    }
+    // f(vector, its number) over the thread's vectors, the last of which may
+    // be past the row's whole vectors (-inf).  The empty asm keeps the
+    // compiler from carrying one walk's unpacked elements over to the next in
+    // two to four times the registers.
     template <typename F>
     __device__ __forceinline__ void each(F f) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             asm volatile("" : "+v"(v[i].raw));
-            const int k = i * NT + int(threadIdx.x);
-            if (i * NT < whole) f(v[i], k * n, k < whole ? 0 : n);
+            if (i * NT < cut.whole) f(v[i], i * NT + int(threadIdx.x));
         }
 #pragma unroll 1
-        for (int i = NV; i * NT < whole; ++i) {
-            const int k = i * NT + int(threadIdx.x);
-            if (k >= whole) break;
+        for (int i = NV; i * NT < cut.whole; ++i) {
+            if (i * NT + int(threadIdx.x) >= cut.whole) break;
             Vec<E> a;
             a.load(at(i));
-            f(a, k * n, 0);
-        }
-        if (whole * n < V && threadIdx.x == 0) {
-            asm volatile("" : "+v"(rest.raw));
-            f(rest, V - n, n - V % n);
+            f(a, i * NT + int(threadIdx.x));
         }
     }
     __device__ __forceinline__ float largest() {
-        float m = -__builtin_inff();
-        each([&](const Vec<E>& a, int, int) {
+        float m = one;
+        each([&](const Vec<E>& a, int) {
 #pragma unroll
             for (int j = 0; j < n; ++j) m = larger(m, a.get(j));
         });
@@ -216,13 +225,18 @@ struct Row {
 };
 
 // go(KERNEL<E, NT, NV>, NT) with the smallest workgroup that holds a row of V
-// logits: 256 threads up to 8 vectors each (16384 bf16), then 1024; rows past
-// 16 vectors of 1024 threads (131072 bf16) read their rest again each walk.
-#define RWKV7M_LM_ROW_KERNEL(KERNEL, E, V, go)        \
+// logits: where `wave` a wave up to 4 vectors a thread (2048 bf16), 256
+// threads up to 8 (16384), then 1024; rows past 16 vectors of 1024 threads
+// (131072 bf16) read their rest again each walk.
+#define RWKV7M_LM_ROW_KERNEL(KERNEL, E, V, wave, go)  \
     do {                                              \
         constexpr int64_t vec = Vec<E>::n;            \
-        if ((V) <= 256 * 1 * vec)                     \
-            go(KERNEL<E, 256, 1>, 256);               \
+        if ((wave) && (V) <= 64 * 1 * vec)            \
+            go(KERNEL<E, 64, 1>, 64);                 \
+        else if ((wave) && (V) <= 64 * 2 * vec)       \
+            go(KERNEL<E, 64, 2>, 64);                 \
+        else if ((wave) && (V) <= 64 * 4 * vec)       \
+            go(KERNEL<E, 64, 4>, 64);                 \
         else if ((V) <= 256 * 2 * vec)                \
             go(KERNEL<E, 256, 2>, 256);               \
         else if ((V) <= 256 * 4 * vec)                \
@@ -249,14 +263,14 @@ struct Row {
 struct RowSoftmax {
     float c, refc, ref;
 
+    // (largest is the same in every lane)
     __device__ __forceinline__ RowSoftmax(float largest, float c_) {
-        ref = largest == -__builtin_inff() ? 0.f : largest;
+        ref = uniform(largest == -__builtin_inff() ? 0.f : largest);
         c = c_;
-        refc = ref * c;
-        if (fabsf(refc) > 0x1p100f) {
+        if (fabsf(ref * c) > 0x1p100f)
             c = __uint_as_float(__float_as_uint(c_) & 0x7f800000u) * 0x1p-60f;
-            refc = ref * c;
-        }
+        c = uniform(c);
+        refc = uniform(ref * c);
     }
     __device__ __forceinline__ float t(float x) const {
         return __builtin_fmaf(x, c, -refc);

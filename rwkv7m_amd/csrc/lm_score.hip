@@ -21,7 +21,14 @@
 namespace rwkv7m {
 namespace {
 
-constexpr int kGroups = 256, kVectors = 256, kList = 512;
+// Groups of threads whose largest logits bound the alternatives (a wave's
+// threads are their own), and the room in LDS.
+template <int NT>
+constexpr int kGroups = NT < 256 ? NT : 256;
+template <int NT>
+constexpr int kVectors = NT < 256 ? 128 : 256;
+template <int NT>
+constexpr int kList = NT < 256 ? 256 : 512;
 
 // The order of the alternatives as an unsigned number: that of the floats,
 // -0 with +0, every NaN above +inf.
@@ -35,35 +42,35 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-template <int W>
+template <int NT>
 struct ScoreShared {
+    static constexpr int W = NT / 64;
     float largest[W], sums[2][W], at_token;
     int64_t token;
-    uint32_t groups[kGroups];
-    uint32_t bound;
+    uint32_t groups[kGroups<NT>], bound;
     int vectors, listed, counts[2][W];
     // vectors that hold an element at or above the bound, with the id of
-    // element 0 and their least element, and those elements, key above the
-    // id's complement
-    uint32_t raw[kVectors][4];
-    int first[kVectors], from[kVectors];
-    uint64_t list[kList];
+    // their first, and those elements, key above the id's complement
+    uint32_t raw[kVectors<NT>][4];
+    int first[kVectors<NT>];
+    uint64_t list[kList<NT>];
 };
 
 // The largest 32-bit number with 16 low zeros that at least k of the groups'
 // keys reach: 16 steps of a bisection with the wave's votes.  One wave.
+template <int G>
 __device__ __forceinline__ uint32_t group_bound(const uint32_t* groups, int k) {
     const int lane = threadIdx.x % 64;
-    uint32_t key[kGroups / 64];
+    uint32_t key[G / 64];
 #pragma unroll
-    for (int i = 0; i < kGroups / 64; ++i) key[i] = groups[64 * i + lane];
+    for (int i = 0; i < G / 64; ++i) key[i] = groups[64 * i + lane];
     uint32_t bound = 0;
 #pragma unroll 1
     for (int bit = 31; bit >= 16; --bit) {
         const uint32_t t = bound | (1u << bit);
         int count = 0;
 #pragma unroll
-        for (int i = 0; i < kGroups / 64; ++i)
+        for (int i = 0; i < G / 64; ++i)
             count += __popcll(__ballot(key[i] >= t));
         if (count >= k) bound = t;
     }
@@ -73,45 +80,45 @@ __device__ __forceinline__ uint32_t group_bound(const uint32_t* groups, int k) {
 // How many of the row's first `ids` elements have yes(key, id), over the
 // workgroup; the two buffers of `counts` take turns.  From memory, for the
 // rows that need it.
-template <int W, typename R, typename F>
+template <int NT, typename R, typename F>
 __device__ __forceinline__ int count_row(const R& row, int ids,
-                                         ScoreShared<W>& S, int& turn, F yes) {
+                                         ScoreShared<NT>& S, int& turn, F yes) {
     int count = 0;
 #pragma unroll 1
-    for (int id = threadIdx.x; id < ids; id += 64 * W)
+    for (int id = threadIdx.x; id < ids; id += NT)
         count += yes(order_key(load_f(row.x + id)), id);
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) count += __shfl_xor(count, m);
     if (threadIdx.x % 64 == 0) S.counts[turn][threadIdx.x / 64] = count;
     __syncthreads();
     count = 0;
-    for (int w = 0; w < W; ++w) count += S.counts[turn][w];
+    for (int w = 0; w < NT / 64; ++w) count += S.counts[turn][w];
     turn ^= 1;
     return count;
 }
 
 // Fills the list with the row's first K elements of the order.
-template <int W, typename R, typename P>
+template <int NT, typename R, typename P>
 __device__ void list_exactly(const R& row, int K, uint32_t largest,
-                             ScoreShared<W>& S, P put) {
+                             ScoreShared<NT>& S, P put) {
     // the largest key that K elements reach
     int turn = 0;
     uint32_t lo = 0, hi = largest;
     while (lo < hi) {
         const uint32_t mid = hi - (hi - lo) / 2;
-        if (count_row<W>(row, row.V, S, turn, [&](uint32_t k, int) {
+        if (count_row<NT>(row, row.V, S, turn, [&](uint32_t k, int) {
                 return k >= mid;
             }) >= K)
             lo = mid;
         else
             hi = mid - 1;
     }
-    const int above = count_row<W>(row, row.V, S, turn,
+    const int above = count_row<NT>(row, row.V, S, turn,
                                    [&](uint32_t k, int) { return k > lo; });
     // the lowest id bound under which the elements of that key make K with
     // those above it: doubled from 64 until it is one, then bisected
     const auto enough = [&](int ids) {
-        return above + count_row<W>(row, ids, S, turn, [&](uint32_t k, int) {
+        return above + count_row<NT>(row, ids, S, turn, [&](uint32_t k, int) {
                    return k == lo;
                }) >= K;
     };
@@ -131,7 +138,7 @@ __device__ void list_exactly(const R& row, int K, uint32_t largest,
     if (threadIdx.x == 0) S.listed = 0;
     __syncthreads();
 #pragma unroll 1
-    for (int id = threadIdx.x; id < row.V; id += 64 * W) {
+    for (int id = threadIdx.x; id < row.V; id += NT) {
         const uint32_t k = order_key(load_f(row.x + id));
         if (k > lo || (k == lo && id < ihi)) put(k, id);
     }
@@ -142,30 +149,31 @@ template <typename E, int NT, int NV>
 __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
     LmScoreArgs A) {
     constexpr int W = NT / 64, n = Vec<E>::n;
-    __shared__ ScoreShared<W> S;
+    __shared__ ScoreShared<NT> S;
+    constexpr int G = kGroups<NT>;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int K = A.top_k, V = int(A.V);
     const float inv_t = A.c * kLn2, inf = __builtin_inff();
     const int64_t r = grid_row();
     if (r >= A.rows) return;
-    Row<E, NT, NV> row;
-    row.load(static_cast<const E*>(A.x) + uniform(row_offset(A.xr, r)), V);
+    Row<E, NT, NV> row(
+        static_cast<const E*>(A.x) + uniform(row_offset(A.xr, r)), V);
     const float mine = row.largest();
     const float wl = wave_larger(mine);
     if (lane == 0) S.largest[wave] = wl;
     if (threadIdx.x == 0) S.vectors = S.listed = 0;
-    if (K) {
-        float g = mine;  // the largest of a group of NT / 256 threads
+    if (K > 1) {
+        float g = mine;  // the largest of a group of NT / G threads
 #pragma unroll
-        for (int m = 1; m < NT / kGroups; m *= 2)
-            g = larger(g, __shfl_xor(g, m));
-        if (threadIdx.x % (NT / kGroups) == 0)
-            S.groups[threadIdx.x / (NT / kGroups)] = order_key(g);
+        for (int m = 1; m < NT / G; m *= 2) g = larger(g, __shfl_xor(g, m));
+        if (threadIdx.x % (NT / G) == 0)
+            S.groups[threadIdx.x / (NT / G)] = order_key(g);
     }
     __syncthreads();
     const float largest = waves_fold<W>(S.largest, larger);
     if (K && wave == 0) {
-        const uint32_t b = group_bound(S.groups, K);
+        const uint32_t b =
+            K > 1 ? group_bound<G>(S.groups, K) : order_key(largest);
         if (lane == 0) S.bound = b;
     }
     if (threadIdx.x == NT - 1) {
@@ -175,17 +183,18 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
     }
     const RowSoftmax soft(largest, A.c);
     float s0 = 0.f, s1 = 0.f;
-    row.each([&](const Vec<E>& a, int, int) {
+    const auto add = [&](float x) {
+        // (held above -200, where e is 0 already: -inf adds 0, not 0 * -inf)
+        const float t = larger(soft.t(x), -200.f);
+        const float e = __builtin_amdgcn_exp2f(t);
+        s0 += e;
+        s1 = __builtin_fmaf(e, t, s1);
+    };
+    row.each([&](const Vec<E>& a, int) {
 #pragma unroll
-        for (int j = 0; j < n; ++j) {
-            // (held above -200, where e is 0 already: -inf adds 0, not
-            // 0 * -inf)
-            const float t = larger(soft.t(a.get(j)), -200.f);
-            const float e = __builtin_amdgcn_exp2f(t);
-            s0 += e;
-            s1 = __builtin_fmaf(e, t, s1);
-        }
+        for (int j = 0; j < n; ++j) add(a.get(j));
     });
+    add(row.one);
     s0 = lanes_sum<64>(s0);
     s1 = lanes_sum<64>(s1);
     if (lane == 0) {
@@ -217,33 +226,34 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
     const float least = bound < 0x00800000u ? -inf : key_value(bound);
     const auto put = [&](uint32_t key, int id) {
         const int at = atomicAdd(&S.listed, 1);
-        if (at < kList)
+        if (at < kList<NT>)
             S.list[at] = uint64_t(key) << 32 | (0xffffffffu - uint32_t(id));
     };
     if (mine >= least)
-        row.each([&](const Vec<E>& a, int id, int from) {
+        row.each([&](const Vec<E>& a, int k) {
             float most = a.get(0);
 #pragma unroll
             for (int j = 1; j < n; ++j) most = larger(most, a.get(j));
-            if (!(most >= least) || from == n) return;
+            if (!(most >= least) || k >= row.cut.whole) return;
             const int at = atomicAdd(&S.vectors, 1);
-            if (at >= kVectors) return;
-            S.first[at] = id;
-            S.from[at] = from;
+            if (at >= kVectors<NT>) return;
+            S.first[at] = row.cut.lead + k * n;
 #pragma unroll
             for (int w = 0; w < 4; ++w) S.raw[at][w] = a.raw[w];
         });
+    if (row.has_one() && row.one >= least)
+        put(order_key(row.one), row.one_id());
     __syncthreads();
     const int vectors = S.vectors;
-    for (int i = threadIdx.x; i < vectors * n && vectors <= kVectors; i += NT) {
-        const int v = i / n, j = i % n;
-        const float x = load_f(reinterpret_cast<const E*>(S.raw[v]) + j);
-        if (x >= least && j >= S.from[v]) put(order_key(x), S.first[v] + j);
+    for (int i = threadIdx.x; i < vectors * n && vectors <= kVectors<NT>;
+         i += NT) {
+        const float x = load_f(reinterpret_cast<const E*>(S.raw[i / n]) + i % n);
+        if (x >= least) put(order_key(x), S.first[i / n] + i % n);
     }
     __syncthreads();
     int listed = S.listed;
-    if (vectors > kVectors || listed > kList || largest != largest) {
-        list_exactly<W>(row, K, order_key(largest), S, put);
+    if (vectors > kVectors<NT> || listed > kList<NT> || largest != largest) {
+        list_exactly<NT>(row, K, order_key(largest), S, put);
         listed = K;
     }
     for (int i = threadIdx.x; i < listed; i += NT) {
@@ -258,18 +268,18 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
     }
 }
 
-// dlogits: a workgroup a tile of kTile vectors a thread of one row.
+// dlogits: a workgroup a tile of kTile vectors a thread of one row; the first
+// tile's also takes the elements before and behind the row's vectors.
 constexpr int kBwdThreads = 256, kTile = 4;
 
 template <typename E>
-__global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A) {
-    constexpr int n = Vec<E>::n, kCols = kBwdThreads * kTile * n;
+__global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A,
+                                                                int tiles) {
+    constexpr int n = Vec<E>::n;
     const float inv_t = A.c * kLn2;
-    const int64_t tiles = (A.V + kCols - 1) / kCols;
     for (int64_t tile = blockIdx.x; tile < A.rows * tiles; tile += gridDim.x) {
         const int64_t r = tile / tiles;
-        const int V = int(A.V);
-        const int first = int(tile % tiles) * kCols + int(threadIdx.x) * n;
+        const int part = int(tile % tiles), V = int(A.V);
         const E* x = static_cast<const E*>(A.x) + row_offset(A.xr, r);
         E* dx = static_cast<E*>(A.dlogits) + r * A.V;
         const int64_t tok = A.tokens[r];
@@ -290,28 +300,31 @@ __global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A) {
                             __builtin_fmaf(lp, g1, g0);
             return id == tok ? d + dl : d;
         };
+        const Cut<E> cut(x, V);
+        const int first = part * kBwdThreads * kTile + int(threadIdx.x);
         Vec<E> v[kTile];
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            const int at = first + i * kBwdThreads * n;
+            const int k = first + i * kBwdThreads;
             v[i].raw = 0;
-            if (any && at + n <= V) v[i].load(x + at);
+            if (any && k < cut.whole) v[i].load(x + cut.lead + k * n);
         }
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            const int at = first + i * kBwdThreads * n;
-            if (at + n <= V) {
-                if (any) {
+            const int k = first + i * kBwdThreads, at = cut.lead + k * n;
+            if (k >= cut.whole) break;
+            if (any) {
 #pragma unroll
-                    for (int j = 0; j < n; j += 2)
-                        v[i].set2(j, grad(v[i].get(j), at + j),
-                                  grad(v[i].get(j + 1), at + j + 1));
-                }
-                v[i].store(dx + at);
-            } else {
-                for (int j = at; j < V; ++j)
-                    store_f(dx + j, any ? grad(load_f(x + j), j) : 0.f);
+                for (int j = 0; j < n; j += 2)
+                    v[i].set2(j, grad(v[i].get(j), at + j),
+                              grad(v[i].get(j + 1), at + j + 1));
             }
+            v[i].store(dx + at);
+        }
+        if (part == 0 && int(threadIdx.x) < cut.lead + cut.rest) {
+            const int t = threadIdx.x;
+            const int id = t < cut.lead ? t : V - cut.rest + t - cut.lead;
+            store_f(dx + id, any ? grad(load_f(x + id), id) : 0.f);
         }
     }
 }
@@ -326,9 +339,9 @@ hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
                            A);
     };
     if (bf16)
-        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, go);
+        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, true, go);
     else
-        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, go);
+        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, true, go);
     return hipGetLastError();
 }
 
@@ -336,11 +349,11 @@ hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
                                     hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
     const int64_t cols = kBwdThreads * kTile * (bf16 ? 8 : 4);
-    const int64_t tiles = A.rows * ((A.V + cols - 1) / cols);
+    const int64_t tiles = (A.V + cols - 1) / cols, all = A.rows * tiles;
     hipLaunchKernelGGL(
         bf16 ? score_bwd_kernel<bf16_t> : score_bwd_kernel<float>,
-        dim3(unsigned(tiles < (1 << 20) ? tiles : 1 << 20)), dim3(kBwdThreads),
-        0, stream, A);
+        dim3(unsigned(all < (1 << 20) ? all : 1 << 20)), dim3(kBwdThreads), 0,
+        stream, A, int(tiles));
     return hipGetLastError();
 }
 
