@@ -126,9 +126,10 @@ __device__ __forceinline__ float waves_sum(const float* s) {
 }
 
 // Waves a SIMD that a kernel with a Row of NV vectors a thread leaves room for:
-// the row's 4 NV registers and as many as 32 others of the SIMD's 512.
-template <int NV>
-constexpr int kRowWaves = NV <= 8 ? 8 : 4;
+// the row's 4 NV registers and as many as 32 others of the SIMD's 512 (a few
+// more where a wave has the row to itself, which LDS has no room for 8 of).
+template <int NT, int NV>
+constexpr int kRowWaves = NT == 64 ? 6 : NV <= 8 ? 8 : 4;
 
 // An offset that is the same in every lane, in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -225,7 +226,8 @@ struct Row {
 };
 
 // go(KERNEL<E, NT, NV>, NT) with the smallest workgroup that holds a row of V
-// logits: where `wave` a wave up to 4 vectors a thread (2048 bf16), 256
+// logits: where `wave` a wave up to 8 vectors a thread (4096 bf16; no barriers:
+// 60000 such rows are scored in 85 us, by 256 threads each in 109), 256
 // threads up to 8 (16384), then 1024; rows past 16 vectors of 1024 threads
 // (131072 bf16) read their rest again each walk.
 #define RWKV7M_LM_ROW_KERNEL(KERNEL, E, V, wave, go)  \
@@ -237,6 +239,8 @@ struct Row {
             go(KERNEL<E, 64, 2>, 64);                 \
         else if ((wave) && (V) <= 64 * 4 * vec)       \
             go(KERNEL<E, 64, 4>, 64);                 \
+        else if ((wave) && (V) <= 64 * 8 * vec)       \
+            go(KERNEL<E, 64, 8>, 64);                 \
         else if ((V) <= 256 * 2 * vec)                \
             go(KERNEL<E, 256, 2>, 256);               \
         else if ((V) <= 256 * 4 * vec)                \

@@ -7,9 +7,10 @@
 // registers and not over memory.
 //
 // The alternatives.  Each thread's largest logit is known from the first
-// walk; the k-th largest over 256 groups of threads is a lower bound T of the
-// row's k-th largest logit, and for logits in no particular order not many
-// more than k of them lie at or above it (-256 log(1 - k / 256) on average).
+// walk; the k-th largest over g = 256 groups of threads (64 threads in a wave
+// of its own) is a lower bound T of the row's k-th largest logit, and for
+// logits in no particular order not many more than k of them lie at or above
+// it (-g log(1 - k / g) on average).
 // The vectors that hold one go to LDS, their elements at or above T to a list
 // there, and each of those finds its rank by counting the ones before it.
 // Where they are more than LDS has room for (many equal logits, or large ones
@@ -21,10 +22,7 @@
 namespace rwkv7m {
 namespace {
 
-// Groups of threads whose largest logits bound the alternatives (a wave's
-// threads are their own), and the room in LDS.
-template <int NT>
-constexpr int kGroups = NT < 256 ? NT : 256;
+// Room in LDS for the vectors and the elements at or above the bound.
 template <int NT>
 constexpr int kVectors = NT < 256 ? 128 : 256;
 template <int NT>
@@ -47,7 +45,7 @@ struct ScoreShared {
     static constexpr int W = NT / 64;
     float largest[W], sums[2][W], at_token;
     int64_t token;
-    uint32_t groups[kGroups<NT>], bound;
+    uint32_t groups[NT > 64 ? 256 : 1], bound;
     int vectors, listed, counts[2][W];
     // vectors that hold an element at or above the bound, with the id of
     // their first, and those elements, key above the id's complement
@@ -56,23 +54,21 @@ struct ScoreShared {
     uint64_t list[kList<NT>];
 };
 
-// The largest 32-bit number with 16 low zeros that at least k of the groups'
-// keys reach: 16 steps of a bisection with the wave's votes.  One wave.
+// The largest 32-bit number with 16 low zeros that at least k of the 64 G keys
+// reach (G in each lane of the wave), or a smaller one that exactly k reach:
+// at most 16 steps of a bisection with the wave's votes.
 template <int G>
-__device__ __forceinline__ uint32_t group_bound(const uint32_t* groups, int k) {
-    const int lane = threadIdx.x % 64;
-    uint32_t key[G / 64];
-#pragma unroll
-    for (int i = 0; i < G / 64; ++i) key[i] = groups[64 * i + lane];
+__device__ __forceinline__ uint32_t group_bound(const uint32_t (&key)[G],
+                                                int k) {
     uint32_t bound = 0;
 #pragma unroll 1
     for (int bit = 31; bit >= 16; --bit) {
         const uint32_t t = bound | (1u << bit);
         int count = 0;
 #pragma unroll
-        for (int i = 0; i < G / 64; ++i)
-            count += __popcll(__ballot(key[i] >= t));
+        for (int i = 0; i < G; ++i) count += __popcll(__ballot(key[i] >= t));
         if (count >= k) bound = t;
+        if (count == k) break;
     }
     return bound;
 }
@@ -146,11 +142,10 @@ __device__ void list_exactly(const R& row, int K, uint32_t largest,
 }
 
 template <typename E, int NT, int NV>
-__global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
+__global__ __launch_bounds__(NT, kRowWaves<NT, NV>) void score_kernel(
     LmScoreArgs A) {
     constexpr int W = NT / 64, n = Vec<E>::n;
     __shared__ ScoreShared<NT> S;
-    constexpr int G = kGroups<NT>;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int K = A.top_k, V = int(A.V);
     const float inv_t = A.c * kLn2, inf = __builtin_inff();
@@ -162,18 +157,28 @@ __global__ __launch_bounds__(NT, kRowWaves<NV>) void score_kernel(
     const float wl = wave_larger(mine);
     if (lane == 0) S.largest[wave] = wl;
     if (threadIdx.x == 0) S.vectors = S.listed = 0;
-    if (K > 1) {
-        float g = mine;  // the largest of a group of NT / G threads
+    if constexpr (NT > 64) {
+        if (K > 1) {
+            float g = mine;  // the largest of one of 256 groups of threads
 #pragma unroll
-        for (int m = 1; m < NT / G; m *= 2) g = larger(g, __shfl_xor(g, m));
-        if (threadIdx.x % (NT / G) == 0)
-            S.groups[threadIdx.x / (NT / G)] = order_key(g);
+            for (int m = 1; m < NT / 256; m *= 2)
+                g = larger(g, __shfl_xor(g, m));
+            if (threadIdx.x % (NT / 256) == 0)
+                S.groups[threadIdx.x / (NT / 256)] = order_key(g);
+        }
     }
     __syncthreads();
     const float largest = waves_fold<W>(S.largest, larger);
     if (K && wave == 0) {
-        const uint32_t b =
-            K > 1 ? group_bound<G>(S.groups, K) : order_key(largest);
+        uint32_t b = order_key(largest);
+        if (K > 1) {
+            constexpr int G = NT > 64 ? 4 : 1;
+            uint32_t key[G] = {order_key(mine)};
+            if constexpr (NT > 64)
+#pragma unroll
+                for (int i = 0; i < G; ++i) key[i] = S.groups[64 * i + lane];
+            b = group_bound(key, K);
+        }
         if (lane == 0) S.bound = b;
     }
     if (threadIdx.x == NT - 1) {
@@ -334,14 +339,16 @@ __global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A,
 hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
                            hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
+    // a wave's 64 groups bound more alternatives too loosely
+    const bool wave = A.top_k <= 20;
     const auto go = [&](auto kern, unsigned threads) {
         hipLaunchKernelGGL(kern, row_grid(A.rows), dim3(threads), 0, stream,
                            A);
     };
     if (bf16)
-        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, true, go);
+        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, wave, go);
     else
-        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, true, go);
+        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, wave, go);
     return hipGetLastError();
 }
 
