@@ -31,7 +31,7 @@ struct DistillShared {
 };
 
 template <typename E, int NT, int NV>
-__global__ __launch_bounds__(NT, kRowWaves<NT, NV>) void distill_kernel(
+__global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
     LmDistillArgs A) {
     constexpr int W = NT / 64, KW = kTeacher<NT> / 64, n = Vec<E>::n;
     __shared__ DistillShared<NT> S;

@@ -142,7 +142,7 @@ __device__ void list_exactly(const R& row, int K, uint32_t largest,
 }
 
 template <typename E, int NT, int NV>
-__global__ __launch_bounds__(NT, kRowWaves<NT, NV>) void score_kernel(
+__global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     LmScoreArgs A) {
     constexpr int W = NT / 64, n = Vec<E>::n;
     __shared__ ScoreShared<NT> S;
