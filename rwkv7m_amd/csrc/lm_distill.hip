@@ -77,18 +77,18 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
         S.ids[k] = id;
         S.q[k] = t;
         S.student[k] = at_id;
-        const float tl = wave_larger(t);
+        const float tl = lanes_larger<64>(t);
         if (lane == 0) S.teacher[0][wave] = tl;
     }
-    const float wl = wave_larger(row.largest());
+    const float wl = lanes_larger<64>(row.largest());
     if (lane == 0) S.largest[wave] = wl;
     __syncthreads();
-    const float teacher_largest = waves_fold<KW>(S.teacher[0], larger);
+    const float teacher_largest = waves_larger<KW>(S.teacher[0]);
     if (teacher_largest == -inf) {
         clear();
         return;
     }
-    const RowSoftmax soft(waves_fold<W>(S.largest, larger), A.c);
+    const RowSoftmax soft(waves_larger<W>(S.largest), A.c);
     const RowSoftmax teacher(teacher_largest, A.c);
     if (wave < KW) {
         const float te = teacher.e(S.q[k]);

@@ -33,6 +33,11 @@ __device__ __forceinline__ int64_t grid_row() {
     return int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
 }
 
+// The larger of two, a NaN if either is one (v_maximum3_f32).
+__device__ __forceinline__ float larger(float a, float b) {
+    return __builtin_elementwise_maximum(a, b);
+}
+
 // 16 bytes of adjacent elements, at their element's own alignment: gfx950
 // takes such a load or store as one instruction at any address.
 template <typename E>
@@ -67,17 +72,47 @@ struct Vec {
     }
 };
 
-// The sum over aligned groups of G lanes (16, 64), the same in each of them.
-template <int G>
-__device__ __forceinline__ float lanes_sum(float x) {
-    x = group_sum<16>(x);
-    if constexpr (G == 64) x = add_swap<32>(add_swap<16>(x));
+// f over aligned groups of G lanes (4, 16 or 64), the same in each of them:
+// lane rotations and swaps in the instructions themselves, without the LDS
+// traffic and the address registers of shuffles.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf,
+                                                false));
+}
+template <int G, typename T, typename F>
+__device__ __forceinline__ T lanes_fold(T x, F f) {
+    static_assert(sizeof(T) == 4 && (G == 4 || G == 16 || G == 64), "");
+    const auto bits = [](T v) { return __builtin_bit_cast(uint32_t, v); };
+    const auto value = [](uint32_t u) { return __builtin_bit_cast(T, u); };
+    if constexpr (G == 4) {
+        x = f(x, value(dpp<0x4e>(bits(x))));  // lane ^ 2
+        return f(x, value(dpp<0xb1>(bits(x))));  // lane ^ 1
+    }
+    // rotations of a row of 16 lanes: after each, lanes that far apart agree
+    x = f(x, value(dpp<0x128>(bits(x))));
+    x = f(x, value(dpp<0x124>(bits(x))));
+    x = f(x, value(dpp<0x122>(bits(x))));
+    x = f(x, value(dpp<0x121>(bits(x))));
+    if constexpr (G == 64) {
+        const auto a = __builtin_amdgcn_permlane16_swap(bits(x), bits(x),
+                                                        false, false);
+        x = f(value(a[0]), value(a[1]));
+        const auto b = __builtin_amdgcn_permlane32_swap(bits(x), bits(x),
+                                                        false, false);
+        x = f(value(b[0]), value(b[1]));
+    }
     return x;
 }
 
-// The larger of two, a NaN if either is one (v_maximum3_f32).
-__device__ __forceinline__ float larger(float a, float b) {
-    return __builtin_elementwise_maximum(a, b);
+template <int G, typename T>
+__device__ __forceinline__ T lanes_sum(T x) {
+    return lanes_fold<G>(x, [](T a, T b) { return a + b; });
+}
+
+template <int G>
+__device__ __forceinline__ float lanes_larger(float x) {
+    return lanes_fold<G>(x, [](float a, float b) { return larger(a, b); });
 }
 
 // f over one value of each of the workgroup's W waves' lanes, the same in
@@ -101,28 +136,23 @@ __device__ __forceinline__ float block_sum(float x, float* s) {
     return block_fold<W>(x, s, [](float a, float b) { return a + b; });
 }
 
-// The largest over the wave's lanes, the same in each of them.
-__device__ __forceinline__ float wave_larger(float x) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x = larger(x, __shfl_xor(x, m));
-    return x;
-}
-
-// f over the W values that a workgroup's waves left in `s` (after a barrier),
-// the same in every lane: each lane takes one of them, so that it needs one
-// register and not W.
+// f over the W values (4, 16 or 1) that a workgroup's waves left in `s` (after
+// a barrier), the same in every lane.
 template <int W, typename F>
 __device__ __forceinline__ float waves_fold(const float* s, F f) {
-    static_assert(W >= 1 && W <= 64 && (W & (W - 1)) == 0, "");
-    float x = s[threadIdx.x % W];
-#pragma unroll
-    for (int m = W / 2; m >= 1; m >>= 1) x = f(x, __shfl_xor(x, m));
-    return x;
+    if constexpr (W == 1)
+        return s[0];
+    else
+        return lanes_fold<W>(s[threadIdx.x % W], f);
 }
 
 template <int W>
 __device__ __forceinline__ float waves_sum(const float* s) {
     return waves_fold<W>(s, [](float a, float b) { return a + b; });
+}
+template <int W>
+__device__ __forceinline__ float waves_larger(const float* s) {
+    return waves_fold<W>(s, [](float a, float b) { return larger(a, b); });
 }
 
 // Waves a SIMD that a kernel with a Row of NV vectors a thread leaves room for:

@@ -83,8 +83,7 @@ __device__ __forceinline__ int count_row(const R& row, int ids,
 #pragma unroll 1
     for (int id = threadIdx.x; id < ids; id += NT)
         count += yes(order_key(load_f(row.x + id)), id);
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) count += __shfl_xor(count, m);
+    count = lanes_sum<64>(count);
     if (threadIdx.x % 64 == 0) S.counts[turn][threadIdx.x / 64] = count;
     __syncthreads();
     count = 0;
@@ -154,21 +153,19 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     Row<E, NT, NV> row(
         static_cast<const E*>(A.x) + uniform(row_offset(A.xr, r)), V);
     const float mine = row.largest();
-    const float wl = wave_larger(mine);
+    const float wl = lanes_larger<64>(mine);
     if (lane == 0) S.largest[wave] = wl;
     if (threadIdx.x == 0) S.vectors = S.listed = 0;
     if constexpr (NT > 64) {
         if (K > 1) {
-            float g = mine;  // the largest of one of 256 groups of threads
-#pragma unroll
-            for (int m = 1; m < NT / 256; m *= 2)
-                g = larger(g, __shfl_xor(g, m));
+            // the largest of one of 256 groups of threads
+            const float g = NT == 256 ? mine : lanes_larger<4>(mine);
             if (threadIdx.x % (NT / 256) == 0)
                 S.groups[threadIdx.x / (NT / 256)] = order_key(g);
         }
     }
     __syncthreads();
-    const float largest = waves_fold<W>(S.largest, larger);
+    const float largest = waves_larger<W>(S.largest);
     if (K && wave == 0) {
         uint32_t b = order_key(largest);
         if (K > 1) {
