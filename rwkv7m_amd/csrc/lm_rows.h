@@ -190,11 +190,13 @@ struct Cut {
     }
 };
 
+constexpr int kLargestRow = 16;
+
 // A row of V logits in the registers of the NT threads of a workgroup: NV
 // whole vectors each, vector i * NT + thread, with -inf in the places past
 // the row's whole vectors, and the elements before and behind those one to a
-// thread (-inf in the others).  What is past the first NV * NT vectors is read
-// again from memory each time the row is walked.
+// thread (-inf in the others).  What is past the first NV * NT vectors of the
+// largest variant is read again from memory each time the row is walked.
 template <typename E, int NT, int NV>
 struct Row {
     static constexpr int n = Vec<E>::n;
@@ -237,13 +239,22 @@ struct Row {
             asm volatile("" : "+v"(v[i].raw));
             if (i * NT < cut.whole) f(v[i], i * NT + int(threadIdx.x));
         }
+        // (rows of the other variants end within their registers: without
+        // this loop they keep within 64 of them)
+        if constexpr (NV == kLargestRow)
 #pragma unroll 1
-        for (int i = NV; i * NT < cut.whole; ++i) {
-            if (i * NT + int(threadIdx.x) >= cut.whole) break;
-            Vec<E> a;
-            a.load(at(i));
-            f(a, i * NT + int(threadIdx.x));
-        }
+            for (int i = NV; i * NT < cut.whole; i += 4) {
+                Vec<E> a[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    a[u].raw = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+                    if ((i + u) * NT + int(threadIdx.x) < cut.whole)
+                        a[u].load(at(i + u));
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    f(a[u], (i + u) * NT + int(threadIdx.x));
+            }
     }
     __device__ __forceinline__ float largest() {
         float m = one;

@@ -270,13 +270,14 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     }
 }
 
-// dlogits: a workgroup a tile of kTile vectors a thread of one row; the first
-// tile's also takes the elements before and behind the row's vectors.
-constexpr int kBwdThreads = 256, kTile = 4;
+// dlogits: a workgroup a tile of kTile vectors a thread of one row (a wave's
+// where a row is no longer than that); the first tile's also takes the
+// elements before and behind the row's vectors.
+constexpr int kTile = 4;
 
-template <typename E>
-__global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A,
-                                                                int tiles) {
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void score_bwd_kernel(LmScoreArgs A,
+                                                       int tiles) {
     constexpr int n = Vec<E>::n;
     const float inv_t = A.c * kLn2;
     for (int64_t tile = blockIdx.x; tile < A.rows * tiles; tile += gridDim.x) {
@@ -303,17 +304,17 @@ __global__ __launch_bounds__(kBwdThreads) void score_bwd_kernel(LmScoreArgs A,
             return id == tok ? d + dl : d;
         };
         const Cut<E> cut(x, V);
-        const int first = part * kBwdThreads * kTile + int(threadIdx.x);
+        const int first = part * NT * kTile + int(threadIdx.x);
         Vec<E> v[kTile];
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            const int k = first + i * kBwdThreads;
+            const int k = first + i * NT;
             v[i].raw = 0;
             if (any && k < cut.whole) v[i].load(x + cut.lead + k * n);
         }
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            const int k = first + i * kBwdThreads, at = cut.lead + k * n;
+            const int k = first + i * NT, at = cut.lead + k * n;
             if (k >= cut.whole) break;
             if (any) {
 #pragma unroll
@@ -352,12 +353,16 @@ hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
 hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
                                     hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    const int64_t cols = kBwdThreads * kTile * (bf16 ? 8 : 4);
+    // [60000, 1000] bf16: 100 us by 256 threads a row
+    const int64_t n = bf16 ? 8 : 4, threads = A.V <= 64 * kTile * n ? 64 : 256;
+    const int64_t cols = threads * kTile * n;
     const int64_t tiles = (A.V + cols - 1) / cols, all = A.rows * tiles;
-    hipLaunchKernelGGL(
-        bf16 ? score_bwd_kernel<bf16_t> : score_bwd_kernel<float>,
-        dim3(unsigned(all < (1 << 20) ? all : 1 << 20)), dim3(kBwdThreads), 0,
-        stream, A, int(tiles));
+    const auto kern = threads == 64 ? (bf16 ? score_bwd_kernel<bf16_t, 64>
+                                            : score_bwd_kernel<float, 64>)
+                                    : (bf16 ? score_bwd_kernel<bf16_t, 256>
+                                            : score_bwd_kernel<float, 256>);
+    hipLaunchKernelGGL(kern, dim3(unsigned(all < (1 << 20) ? all : 1 << 20)),
+                       dim3(unsigned(threads)), 0, stream, A, int(tiles));
     return hipGetLastError();
 }
 
