@@ -241,21 +241,23 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight,
 
 // --- token log probabilities ------------------------------------------------
 
-// int64 contiguous ids of `shape`.
-Tensor ids_of(const char* what, const Tensor& t, at::IntArrayRef shape) {
+void check_shape(const char* what, const Tensor& t, at::IntArrayRef shape) {
     TORCH_CHECK_VALUE(t.sizes() == shape, what, " must have shape ",
                       shape_of(shape), ", got ", shape_of(t.sizes()));
+}
+
+void check_ids(const char* what, const Tensor& t, at::IntArrayRef shape) {
+    check_shape(what, t, shape);
     TORCH_CHECK_TYPE(t.scalar_type() == at::kLong ||
                          t.scalar_type() == at::kInt,
                      what, " must be int64 or int32, got ", t.scalar_type());
-    return t.to(at::kLong).contiguous();
 }
 
-Tensor weights_of(const char* what, const Tensor& t, at::IntArrayRef shape) {
-    if (!t.defined()) return t;
-    TORCH_CHECK_VALUE(t.sizes() == shape, what, " must have shape ",
-                      shape_of(shape), ", got ", shape_of(t.sizes()));
-    return t.detach().to(at::kFloat).contiguous();
+// What the kernels take: contiguous int64 ids, contiguous fp32 weights.
+Tensor ids64(const Tensor& t) { return t.to(at::kLong).contiguous(); }
+
+Tensor weights32(const Tensor& t) {
+    return t.defined() ? t.detach().to(at::kFloat).contiguous() : t;
 }
 
 // [logprobs, entropy, top_ids, top_logprobs, statistics]; the ids and their
@@ -266,12 +268,13 @@ variable_list score_forward(const Tensor& logits, const Tensor& tokens_,
     const int64_t V = row_width("logits", logits);
     const int code = code_of("logits", logits);
     const auto shape = logits.sizes().slice(0, logits.dim() - 1);
-    const Tensor tokens = ids_of("tokens", tokens_, shape);
-    same_gpu({&logits, &tokens});
+    check_ids("tokens", tokens_, shape);
+    same_gpu({&logits, &tokens_});
     const int64_t most = std::min<int64_t>(V, RWKV7M_MAX_TOP_K);
     TORCH_CHECK_VALUE(top_k >= 0 && top_k <= most, "top_k must be within 0 "
                       "and ", most, " (V=", V, "), got ", top_k);
     const c10::DeviceGuard guard(logits.device());
+    const Tensor tokens = ids64(tokens_);
     const Rows r(logits);
     const auto opts = f32(logits);
     Tensor lp = at::empty(shape, opts), ent = at::empty(shape, opts), ids, top,
@@ -309,11 +312,9 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
             return {Tensor(), Tensor(), Tensor(), Tensor()};
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &stats = saved[2], &ent = saved[3];
-        const auto shape = logits.sizes().slice(0, logits.dim() - 1);
         const c10::DeviceGuard guard(logits.device());
-        const Tensor tokens = ids_of("tokens", saved[1], shape);
-        const Tensor dlp = weights_of("the gradient of logprobs", d[0], shape);
-        const Tensor dent = weights_of("the gradient of entropy", d[1], shape);
+        const Tensor tokens = ids64(saved[1]);
+        const Tensor dlp = weights32(d[0]), dent = weights32(d[1]);
         const Rows r(logits);
         Tensor dx = at::empty(logits.sizes(),
                               logits.options().requires_grad(false));
@@ -346,8 +347,8 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(
 struct Distill {
     int code, tcode;
     int64_t V, K;
-    Tensor ids, teacher, weight;
     c10::DeviceGuard guard;
+    Tensor ids, teacher, weight;
     Rows r;
 
     static const Tensor& checked(const Tensor& logits, const Tensor& ids,
@@ -364,8 +365,8 @@ struct Distill {
                           RWKV7M_MAX_TEACHER_K, " teacher alternatives are "
                           "supported, got ", teacher.size(-1));
         code_of("teacher_logits", teacher);
-        ids_of("teacher_ids", ids, teacher.sizes());
-        weights_of("weight", weight, shape);
+        check_ids("teacher_ids", ids, teacher.sizes());
+        if (weight.defined()) check_shape("weight", weight, shape);
         same_gpu({&logits, &ids, &teacher, &weight});
         return logits;
     }
@@ -375,11 +376,10 @@ struct Distill {
           tcode(code_of("teacher_logits", teacher_)),
           V(logits.size(-1)),
           K(teacher_.size(-1)),
-          ids(ids_of("teacher_ids", ids_, teacher_.sizes())),
-          teacher(teacher_.contiguous()),
-          weight(weights_of("weight", weight_,
-                            logits.sizes().slice(0, logits.dim() - 1))),
           guard(logits.device()),
+          ids(ids64(ids_)),
+          teacher(teacher_.contiguous()),
+          weight(weights32(weight_)),
           r(logits) {}
 };
 
@@ -426,7 +426,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
         const auto saved = ctx->get_saved_variables();
         const Tensor& logits = saved[0];
         const Distill d(logits, saved[1], saved[2], saved[3]);
-        const Tensor scale = weights_of("the gradient of loss", g[0], {});
+        const Tensor scale = weights32(g[0]);
         // a second backward over a retained graph gets a buffer of its own
         Tensor dx;
         const auto kept = ctx->saved_data.find("gradient");

@@ -712,3 +712,61 @@ def test_side_stream_and_graph_replays(lm):
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b), f"replay {rep}"
+
+
+# --- more rows than a grid's columns, parts of the gradients, the example ---
+
+def test_more_rows_than_65536(lm):
+    print("case: 70001 rows", flush=True)
+    rows, V = 70001, 10
+    x = torch.randn(rows, V, generator=_gen(1)).cuda()
+    last = x[-3:].clone()
+    tok = torch.arange(rows, device="cuda") % V
+    a = lm.token_logprobs(x, tok, top_k=3)
+    b = lm.token_logprobs(last, tok[-3:], top_k=3)
+    assert all(torch.equal(p[-3:], q) for p, q in zip(a, b))
+    ids, top = tok[:, None].contiguous(), torch.zeros(rows, 1, device="cuda")
+    w = torch.ones(rows, device="cuda")
+    a = lm.distill_loss(x, ids, top, w)
+    b = lm.distill_loss(last, ids[-3:], top[-3:], w[-3:])
+    assert torch.equal(a.row_losses[-3:], b.row_losses)
+    want = a.row_losses.double().sum()
+    assert abs(float(a.loss.double() - want)) <= 1e-6 * float(want)
+    assert torch.equal(lm.layer_norm(x)[-3:], lm.layer_norm(last))
+
+
+@pytest.mark.parametrize("C", [100, 3000, 20000])
+def test_layer_norm_gradients_one_at_a_time(lm, C):
+    """Each of the three gradients alone is that of all three together."""
+    print("case: layer norm, parts of the gradients", C, flush=True)
+    g = _gen(C)
+    x, w, b = (torch.randn(*s, generator=g).cuda() for s in
+               ((9, C), (C,), (C,)))
+    dy = torch.randn(9, C, generator=g).cuda()
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    every = torch.autograd.grad(lm.layer_norm(*leaves), leaves, dy)
+    for i in range(3):
+        args = [x, w, b]
+        args[i] = leaves[i]
+        got, = torch.autograd.grad(lm.layer_norm(*args), leaves[i], dy)
+        assert torch.equal(got, every[i])
+    got, = torch.autograd.grad(lm.layer_norm(x, None, leaves[2]), leaves[2],
+                               dy)
+    assert torch.equal(got, every[2])
+
+
+def test_the_example_learns(hip_lib):
+    print("case: distill and score example", flush=True)
+    import importlib.util
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location(
+        "distill_and_score",
+        os.path.join(root, "examples", "distill_and_score.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    losses, before, after = mod.run(steps=25, vocab=5003, width=256)
+    assert torch.isfinite(losses).all()
+    assert float(losses[-1]) < 0.7 * float(losses[0])
+    assert float(after.logprobs.mean()) > float(before.logprobs.mean())
+    assert after.top_ids.shape == (4, 64, 3)
