@@ -82,11 +82,13 @@ __device__ __forceinline__ uint32_t dpp(uint32_t x) {
 }
 template <int G, typename T, typename F>
 __device__ __forceinline__ T lanes_fold(T x, F f) {
-    static_assert(sizeof(T) == 4 && (G == 4 || G == 16 || G == 64), "");
+    static_assert(sizeof(T) == 4 && (G == 2 || G == 4 || G == 8 || G == 16 ||
+                                     G == 64), "");
     const auto bits = [](T v) { return __builtin_bit_cast(uint32_t, v); };
     const auto value = [](uint32_t u) { return __builtin_bit_cast(T, u); };
-    if constexpr (G == 4) {
-        x = f(x, value(dpp<0x4e>(bits(x))));  // lane ^ 2
+    if constexpr (G <= 8) {
+        if constexpr (G == 8) x = f(x, value(dpp<0x141>(bits(x))));  // 7 - lane
+        if constexpr (G >= 4) x = f(x, value(dpp<0x4e>(bits(x))));  // lane ^ 2
         return f(x, value(dpp<0xb1>(bits(x))));  // lane ^ 1
     }
     // rotations of a row of 16 lanes: after each, lanes that far apart agree
@@ -159,7 +161,7 @@ __device__ __forceinline__ float waves_larger(const float* s) {
 // the row's 4 NV registers and as many as 32 others of the SIMD's 512 (a few
 // more where a wave has the row to itself, which LDS has no room for 8 of).
 template <int NT, int NV>
-constexpr int kRowWaves = NT == 64 ? 6 : NV <= 8 ? 8 : 4;
+constexpr int kRowWaves = NT == 64 || NT == 512 ? 6 : NV <= 8 ? 8 : 4;
 
 // An offset that is the same in every lane, in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -190,7 +192,7 @@ struct Cut {
     }
 };
 
-constexpr int kLargestRow = 16;
+constexpr int kLargestRow = 1024 * 16;
 
 // A row of V logits in the registers of the NT threads of a workgroup: NV
 // whole vectors each, vector i * NT + thread, with -inf in the places past
@@ -210,16 +212,23 @@ struct Row {
         : x(p), V(length), cut(p, length) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            v[i].raw = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
-            if (i * NT + int(threadIdx.x) < cut.whole) v[i].load(at(i));
+            if ((i + 1) * NT <= cut.whole) {  // (the same in every thread)
+                v[i].load(at(i));
+            } else {
+                v[i].raw = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+                if (i * NT + int(threadIdx.x) < cut.whole) v[i].load(at(i));
+            }
         }
         one = has_one() ? load_f(x + one_id()) : -__builtin_inff();
     }
     // vector i * NT + thread of the row (i the same in every thread)
     __device__ __forceinline__ const E* at(int i) const {
-        return reinterpret_cast<const E*>(
-            reinterpret_cast<const char*>(x + cut.lead + i * NT * n) +
-            uint32_t(threadIdx.x) * 16u);
+        // (a scalar base and a 32-bit offset: the empty asm keeps the two
+        // from being added up in vector registers for each i)
+        int64_t base = int64_t(cut.lead + i * NT * n) * int64_t(sizeof(E));
+        asm volatile("" : "+s"(base));
+        return reinterpret_cast<const E*>(reinterpret_cast<const char*>(x) +
+                                          base + uint32_t(threadIdx.x) * 16u);
     }
     __device__ __forceinline__ bool has_one() const {
         return int(threadIdx.x) < cut.lead + cut.rest;
@@ -241,7 +250,7 @@ struct Row {
         }
         // (rows of the other variants end within their registers: without
         // this loop they keep within 64 of them)
-        if constexpr (NV == kLargestRow)
+        if constexpr (NT * NV == kLargestRow)
 #pragma unroll 1
             for (int i = NV; i * NT < cut.whole; i += 4) {
                 Vec<E> a[4];
@@ -269,9 +278,10 @@ struct Row {
 // go(KERNEL<E, NT, NV>, NT) with the smallest workgroup that holds a row of V
 // logits: where `wave` a wave up to 8 vectors a thread (4096 bf16; no barriers:
 // 60000 such rows are scored in 85 us, by 256 threads each in 109), 256
-// threads up to 8 (16384), then 1024; rows past 16 vectors of 1024 threads
-// (131072 bf16) read their rest again each walk.
-#define RWKV7M_LM_ROW_KERNEL(KERNEL, E, V, wave, go)  \
+// threads up to 8 (16384), 1024 threads with 4 (32768), NT8 threads up to 8192
+// vectors (65536), then 1024; rows past 16 vectors of 1024 threads (131072
+// bf16) read their rest again each walk.
+#define RWKV7M_LM_ROW_KERNEL(KERNEL, E, V, wave, NT8, go) \
     do {                                              \
         constexpr int64_t vec = Vec<E>::n;            \
         if ((wave) && (V) <= 64 * 1 * vec)            \
@@ -291,7 +301,7 @@ struct Row {
         else if ((V) <= 1024 * 4 * vec)               \
             go(KERNEL<E, 1024, 4>, 1024);             \
         else if ((V) <= 1024 * 8 * vec)               \
-            go(KERNEL<E, 1024, 8>, 1024);             \
+            go(KERNEL<E, NT8, 8192 / NT8>, NT8);      \
         else                                          \
             go(KERNEL<E, 1024, 16>, 1024);            \
     } while (0)

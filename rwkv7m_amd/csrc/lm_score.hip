@@ -159,7 +159,8 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     if constexpr (NT > 64) {
         if (K > 1) {
             // the largest of one of 256 groups of threads
-            const float g = NT == 256 ? mine : lanes_larger<4>(mine);
+            float g = mine;
+            if constexpr (NT > 256) g = lanes_larger<NT / 256>(g);
             if (threadIdx.x % (NT / 256) == 0)
                 S.groups[threadIdx.x / (NT / 256)] = order_key(g);
         }
@@ -337,16 +338,19 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(LmScoreArgs A,
 hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
                            hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    // a wave's 64 groups bound more alternatives too loosely
+    // a wave's 64 groups bound more alternatives too loosely; 512 threads hold
+    // 65536 bf16 in 80 registers, so that a CU has three rows at work (1024
+    // threads: two) and more to do while one ranks its alternatives: [4088,
+    // 65536] with 20 of them 104 against 109 us, with 64 of them 108 / 120
     const bool wave = A.top_k <= 20;
     const auto go = [&](auto kern, unsigned threads) {
         hipLaunchKernelGGL(kern, row_grid(A.rows), dim3(threads), 0, stream,
                            A);
     };
     if (bf16)
-        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, wave, go);
+        RWKV7M_LM_ROW_KERNEL(score_kernel, bf16_t, A.V, wave, 512, go);
     else
-        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, wave, go);
+        RWKV7M_LM_ROW_KERNEL(score_kernel, float, A.V, wave, 512, go);
     return hipGetLastError();
 }
 
