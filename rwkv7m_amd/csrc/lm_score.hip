@@ -31,12 +31,11 @@ constexpr int kList = NT < 256 ? 256 : 512;
 // The order of the alternatives as an unsigned number: that of the floats,
 // -0 with +0, every NaN above +inf.
 __device__ __forceinline__ uint32_t order_key(float x) {
-    if (x != x) return 0xfffffffeu;
+    if (x != x) return 0xffff0000u;
     const uint32_t u = __float_as_uint(x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
-    if (k == 0xfffffffeu) return __builtin_nanf("");
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
@@ -73,16 +72,32 @@ __device__ __forceinline__ uint32_t group_bound(const uint32_t (&key)[G],
     return bound;
 }
 
-// How many of the row's first `ids` elements have yes(key, id), over the
-// workgroup; the two buffers of `counts` take turns.  From memory, for the
-// rows that need it.
-template <int NT, typename R, typename F>
-__device__ __forceinline__ int count_row(const R& row, int ids,
+// f(key, id) over the thread's share of the row's first `ids` elements, from
+// memory.
+template <int NT, typename E, typename F>
+__device__ __forceinline__ void walk_memory(const E* x, int ids, F f) {
+    constexpr int n = Vec<E>::n;
+    const Cut<E> cut(x, ids);
+#pragma unroll 2
+    for (int k = threadIdx.x; k < cut.whole; k += NT) {
+        Vec<E> a;
+        a.load(x + cut.lead + k * n);
+#pragma unroll
+        for (int j = 0; j < n; ++j)
+            f(order_key(a.get(j)), cut.lead + k * n + j);
+    }
+    const int t = threadIdx.x, id = t < cut.lead ? t : ids - cut.rest -
+                                                           cut.lead + t;
+    if (t < cut.lead + cut.rest) f(order_key(load_f(x + id)), id);
+}
+
+// How many of the row's first `ids` elements have yes(key), over the
+// workgroup; the two buffers of `counts` take turns.
+template <int NT, typename E, typename F>
+__device__ __forceinline__ int count_row(const E* x, int ids,
                                          ScoreShared<NT>& S, int& turn, F yes) {
     int count = 0;
-#pragma unroll 1
-    for (int id = threadIdx.x; id < ids; id += NT)
-        count += yes(order_key(load_f(row.x + id)), id);
+    walk_memory<NT>(x, ids, [&](uint32_t k, int) { count += yes(k); });
     count = lanes_sum<64>(count);
     if (threadIdx.x % 64 == 0) S.counts[turn][threadIdx.x / 64] = count;
     __syncthreads();
@@ -92,37 +107,51 @@ __device__ __forceinline__ int count_row(const R& row, int ids,
     return count;
 }
 
-// Fills the list with the row's first K elements of the order.
-template <int NT, typename R, typename P>
-__device__ void list_exactly(const R& row, int K, uint32_t largest,
-                             ScoreShared<NT>& S, P put) {
-    // the largest key that K elements reach
+// Fills the list with the row's first K elements of the order.  At least K
+// have keys from `bound` on; `largest` is the row's largest key.  Most often
+// the elements of the bound's own value are too many (equal logits, masks of
+// -inf with fewer than K others): then the first count shows it and no
+// bisection is needed.
+template <int NT, typename E, typename P>
+__device__ void list_exactly(const E* x, int V, int K, uint32_t bound,
+                             uint32_t largest, ScoreShared<NT>& S, P put) {
+    // the largest key that K elements reach, from lo on
     int turn = 0;
-    uint32_t lo = 0, hi = largest;
+    const auto above = [&](uint32_t key) {
+        return count_row<NT>(x, V, S, turn, [&](uint32_t k) { return k > key; });
+    };
+    uint32_t lo = bound, hi = bound | 0xffffu;
+    if (above(hi) >= K) {
+        lo = hi + 1;
+        hi = largest;
+    } else {
+        if (hi > largest) hi = largest;
+        // a bf16 value's key is the only one with its 16 high bits, -inf's is
+        // the lowest
+        if (sizeof(E) == 2 || hi <= 0x007fffffu)
+            lo = hi = hi & 0x80000000u && sizeof(E) == 2 ? hi & 0xffff0000u
+                                                         : hi;
+    }
     while (lo < hi) {
         const uint32_t mid = hi - (hi - lo) / 2;
-        if (count_row<NT>(row, row.V, S, turn, [&](uint32_t k, int) {
-                return k >= mid;
-            }) >= K)
+        if (above(mid - 1) >= K)
             lo = mid;
         else
             hi = mid - 1;
     }
-    const int above = count_row<NT>(row, row.V, S, turn,
-                                   [&](uint32_t k, int) { return k > lo; });
     // the lowest id bound under which the elements of that key make K with
     // those above it: doubled from 64 until it is one, then bisected
+    const int more = K - above(lo);
     const auto enough = [&](int ids) {
-        return above + count_row<NT>(row, ids, S, turn, [&](uint32_t k, int) {
-                   return k == lo;
-               }) >= K;
+        return count_row<NT>(x, ids, S, turn,
+                             [&](uint32_t k) { return k == lo; }) >= more;
     };
     int ilo = 0, ihi = 64;
-    while (ihi < row.V && !enough(ihi)) {
+    while (ihi < V && !enough(ihi)) {
         ilo = ihi;
         ihi *= 2;
     }
-    if (ihi > row.V) ihi = row.V;
+    if (ihi > V) ihi = V;
     while (ihi - ilo > 1) {
         const int mid = ilo + (ihi - ilo) / 2;
         if (enough(mid))
@@ -132,11 +161,9 @@ __device__ void list_exactly(const R& row, int K, uint32_t largest,
     }
     if (threadIdx.x == 0) S.listed = 0;
     __syncthreads();
-#pragma unroll 1
-    for (int id = threadIdx.x; id < row.V; id += NT) {
-        const uint32_t k = order_key(load_f(row.x + id));
+    walk_memory<NT>(x, V, [&](uint32_t k, int id) {
         if (k > lo || (k == lo && id < ihi)) put(k, id);
-    }
+    });
     __syncthreads();
 }
 
@@ -256,7 +283,7 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     __syncthreads();
     int listed = S.listed;
     if (vectors > kVectors<NT> || listed > kList<NT> || largest != largest) {
-        list_exactly<NT>(row, K, order_key(largest), S, put);
+        list_exactly<NT>(row.x, V, K, bound, order_key(largest), S, put);
         listed = K;
     }
     for (int i = threadIdx.x; i < listed; i += NT) {
@@ -342,7 +369,7 @@ hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
     // 65536 bf16 in 80 registers, so that a CU has three rows at work (1024
     // threads: two) and more to do while one ranks its alternatives: [4088,
     // 65536] with 20 of them 104 against 109 us, with 64 of them 108 / 120
-    const bool wave = A.top_k <= 20;
+    const bool wave = A.top_k <= 40;
     const auto go = [&](auto kern, unsigned threads) {
         hipLaunchKernelGGL(kern, row_grid(A.rows), dim3(threads), 0, stream,
                            A);
