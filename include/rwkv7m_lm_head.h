@@ -15,7 +15,8 @@
  * rounded once, to nearest even.  Strides are >= 0 elements; an output shares
  * no byte with an input.  Calls only enqueue work on `stream`, never allocate
  * and never synchronise, so they may be captured in a HIP graph.  Results do
- * not depend on the order in which workgroups run.
+ * not depend on the order in which workgroups run, nor a row's on how many
+ * others there are.
  */
 #ifndef RWKV7M_LM_HEAD_H
 #define RWKV7M_LM_HEAD_H
@@ -98,7 +99,7 @@ int rwkv7m_token_logprobs_backward(
  * teacher_ids int64 and teacher_logits (of `teacher_dtype`) [rows][K]; an id
  * >= V gives NaN; an alternative of -inf has q = 0 and adds nothing.  weight
  * [rows] fp32, or NULL: 1 / rows each.  A row with weight 0, or without an
- * alternative of q > 0, has loss and gradient 0 and its logits are not read.
+ * alternative above -inf, has loss and gradient 0 whatever its logits hold.
  * row_losses [rows] fp32; dlogits [rows][V] of `dtype`, or NULL: the losses
  * alone. */
 int rwkv7m_distill_loss(int dtype, int teacher_dtype, int64_t outer,

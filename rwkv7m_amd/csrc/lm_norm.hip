@@ -4,12 +4,14 @@
 // Bound by memory: about 8 operations an element forward and 14 backward
 // against 4 and 6 bytes.  A row is read once and held in registers, as the
 // 16-byte vectors it came in, by a group of TPR threads (16 for up to 128
-// bf16 elements, a wave, a workgroup of 4 or of 16 waves), NV vectors each;
-// the variance is the mean of the squared deviations, from the registers.
-// Rows longer than 16 waves hold (kLongest) are walked again from the L2.
-// Workgroups stay for many rows, with the parameters, and in the backward
-// their gradients' sums, in registers; each workgroup writes one partial row
-// of those sums and a second kernel adds the partial rows in a fixed order.
+// bf16 elements, a wave, 4 or 16 waves), NV vectors each; the variance is the
+// mean of the squared deviations, from the registers.  Rows longer than 16
+// waves hold (kLongest) are walked again from the L2.  Workgroups stay for
+// many rows, with the parameters, and in the backward their gradients' sums,
+// in registers; each workgroup writes one partial row of those sums and a
+// second kernel adds the partial rows in a fixed order.
+// [32768, 2048] bf16 with fp32 parameters: forward 44 us (6.1 TB/s), backward
+// 80 + 4 us (5.0 TB/s).
 //
 // A row whose length is no multiple of the vector ends in a vector moved back
 // to end with it (its first `dup` elements are the vector before's): every
@@ -395,7 +397,10 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(LmNormArgs A,
     if (out) store_param(out, A.param_bf16, c < A.C ? c : c - A.C, x);
 }
 
-// Vectors a thread of a group below the widest holds.
+// Vectors a thread of a group below the widest holds.  The backward has four
+// arrays of them in fp32 and one workgroup of 16 waves a CU: two, or too few
+// waves have room ([32768, 2048] bf16 by waves of 4 vectors, in workgroups of
+// 4, 94 us; by groups of 4 waves with one vector each 84).
 constexpr int64_t kFwdVectors = 4, kBwdVectors = 2;
 constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 256;
 

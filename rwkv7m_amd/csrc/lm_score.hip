@@ -1,10 +1,15 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of
 // logits, and their backward (include/rwkv7m_lm_head.h has the formulas).
 //
-// Bound by memory: a row is read once.  One workgroup holds a row in its
-// registers as it came (65536 bf16 logits: 1024 threads of 32 registers), so
-// that the largest logit, the sums and the alternatives are three walks over
-// registers and not over memory.
+// Bound by memory: a row is read once, about 10 operations an element.  One
+// workgroup holds a row in its registers as it came (65536 bf16 logits: 512
+// threads of 64 registers), so that the largest logit, the sums and the
+// alternatives are three walks over registers and not over memory.  [4088,
+// 65536] bf16 is read in 91 us (5.9 TB/s), with 10 alternatives in 99 (5.4):
+// what those add is mostly latency, a search of the bound, two passes over LDS
+// and three barriers in which the row's registers wait.  Rows of more than
+// 65536 bf16 leave room for one workgroup a CU, whose loads nothing overlaps:
+// 4.1 TB/s at 131072.
 //
 // The alternatives.  Each thread's largest logit is known from the first
 // walk; the k-th largest over g = 256 groups of threads (64 threads in a wave
@@ -15,7 +20,8 @@
 // there, and each of those finds its rank by counting the ones before it.
 // Where they are more than LDS has room for (many equal logits, or large ones
 // at the same few threads), or NaN are among them, the list's bound is found
-// exactly, by bisection over the order of the values and then of the ids.
+// exactly, by counting and bisection over the order of the values and then of
+// the ids: 0.40 ms for [4088, 65536] of nothing but equal logits.
 
 #include "lm_rows.h"
 
@@ -300,7 +306,8 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
 
 // dlogits: a workgroup a tile of kTile vectors a thread of one row (a wave's
 // where a row is no longer than that); the first tile's also takes the
-// elements before and behind the row's vectors.
+// elements before and behind the row's vectors.  Bound by memory: 12
+// operations and 4 bytes an element in bf16, 5.8 TB/s at [4088, 65536].
 constexpr int kTile = 4;
 
 template <typename E, int NT>
@@ -365,11 +372,13 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(LmScoreArgs A,
 hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
                            hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    // a wave's 64 groups bound more alternatives too loosely; 512 threads hold
-    // 65536 bf16 in 80 registers, so that a CU has three rows at work (1024
-    // threads: two) and more to do while one ranks its alternatives: [4088,
-    // 65536] with 20 of them 104 against 109 us, with 64 of them 108 / 120
+    // A wave's 64 groups bound more alternatives too loosely.
     const bool wave = A.top_k <= 40;
+    // 512 threads hold 65536 bf16 in 80 registers, so that a CU has three rows
+    // at work (1024 threads: two) and more to do while one ranks its
+    // alternatives: [4088, 65536] with 20 of them 100 against 109 us.  A
+    // single row takes 10.2 us so and 8.7 by 1024 threads, but a row's results
+    // would then depend on how many others there are.
     const auto go = [&](auto kern, unsigned threads) {
         hipLaunchKernelGGL(kern, row_grid(A.rows), dim3(threads), 0, stream,
                            A);
