@@ -7,8 +7,8 @@
 // to a CU) and walks them three times: for the largest, for the sum of the
 // exponentials, and for the gradient weight T p, with each exponential
 // computed again rather than kept (the row would take twice the registers).
-// [4088, 65536] bf16 takes 209 us (5.1 TB/s); read again for the gradient it
-// took 1018.  The teacher's alternatives are one to a thread of the first 4
+// [4088, 65536] bf16 takes 209 us (5.1 TB/s) by itself; between backward
+// passes, under a profiler, 211 to 229.  The teacher's alternatives are one to a thread of the first 4
 // waves and stay in LDS; after the gradient's row is out, each writes its
 // entry again with its q taken off, the first of equal ids with all their q,
 // summed in the order of the alternatives.
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
 }
 
 // loss = sum_r weight[r] row_losses[r], one workgroup, in float64: a fixed
-// order, and no error beside the rows' own (4 us at 4088 rows, latency).
+// order, and no error beside the rows' own (5 us at 4088 rows, latency).
 __global__ __launch_bounds__(1024) void distill_sum_kernel(LmDistillArgs A) {
     __shared__ double s[16];
     double x = 0.0;

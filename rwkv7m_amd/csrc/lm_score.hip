@@ -393,7 +393,7 @@ hipError_t launch_lm_score(bool bf16, const LmScoreArgs& A,
 hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
                                     hipStream_t stream) {
     if (A.rows == 0) return hipSuccess;
-    // [60000, 1000] bf16: 100 us by 256 threads a row
+    // [60000, 1000] bf16: 100 us by 256 threads a row, 48 by 64.
     const int64_t n = bf16 ? 8 : 4, threads = A.V <= 64 * kTile * n ? 64 : 256;
     const int64_t cols = threads * kTile * n;
     const int64_t tiles = (A.V + cols - 1) / cols, all = A.rows * tiles;
