@@ -93,7 +93,8 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
     const RowSoftmax soft(waves_larger<W>(S.largest), A.c);
     const RowSoftmax teacher(teacher_largest, A.c);
     if (wave < KW) {
-        const float te = teacher.e(S.q[k]);
+        const float te =
+            __builtin_amdgcn_exp2f(teacher.difference(S.q[k]));
         const float es = lanes_sum<64>(S.ids[k] == -1 ? 0.f : te);
         // an id past the vocabulary: NaN for the row
         const float bad = __any(S.ids[k] == -2) ? __builtin_nanf("") : 0.f;
@@ -102,10 +103,14 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
             S.bad[wave] = bad;
         }
     }
-    float s0 = soft.e(row.one);
-    row.each([&](const Vec<E>& a, int) {
+    float s0 = 0.f;
+    soft.with_t(row, [&](auto t, auto each) {
+        s0 = __builtin_amdgcn_exp2f(t(row.one));
+        each([&](const Vec<E>& a, int) {
 #pragma unroll
-        for (int j = 0; j < n; ++j) s0 += soft.e(a.get(j));
+            for (int j = 0; j < n; ++j)
+                s0 += __builtin_amdgcn_exp2f(t(a.get(j)));
+        });
     });
     s0 = lanes_sum<64>(s0);
     if (lane == 0) S.sums[wave] = s0;
@@ -114,13 +119,14 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
     const float bad = waves_sum<KW>(S.bad);
     if (wave < KW) {
         const float ts = waves_sum<KW>(S.teacher[1]), t = S.q[k];
-        const float q = S.ids[k] == -1 ? 0.f : teacher.e(t) / ts;
+        const float te = __builtin_amdgcn_exp2f(teacher.difference(t));
+        const float q = S.ids[k] == -1 ? 0.f : te / ts;
         float share = 0.f;
         if (q != 0.f) {
             // log2 q - log2 p; a row of nothing but -inf has p = 0
-            const float lp = (S.student[k] - soft.ref) * A.c -
+            const float lp = soft.difference(S.student[k]) -
                              (s0 == 0.f ? inf : soft.log2_sum(s0));
-            share = q * ((t - teacher.ref) * A.c - teacher.log2_sum(ts) - lp);
+            share = q * (teacher.difference(t) - __log2f(ts) - lp);
         }
         share = lanes_sum<64>(share);
         if (lane == 0) S.teacher[2][wave] = share;
@@ -128,16 +134,20 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
     }
     const float wt = w * A.temperature * scale;
     const float wp = uniform((s0 == 0.f ? 0.f : wt / s0) + bad);
-    if (dx) {
-        row.each([&](const Vec<E>& a, int i) {
-            Vec<E> g;
+    if (dx)
+        soft.with_t(row, [&](auto t, auto each) {
+            const auto grad = [&](float x) {
+                return wp * __builtin_amdgcn_exp2f(t(x));
+            };
+            each([&](const Vec<E>& a, int i) {
+                Vec<E> g;
 #pragma unroll
-            for (int j = 0; j < n; j += 2)
-                g.set2(j, wp * soft.e(a.get(j)), wp * soft.e(a.get(j + 1)));
-            if (i < row.cut.whole) g.store(dx + row.cut.lead + i * n);
+                for (int j = 0; j < n; j += 2)
+                    g.set2(j, grad(a.get(j)), grad(a.get(j + 1)));
+                if (i < row.cut.whole) g.store(dx + row.cut.lead + i * n);
+            });
+            if (row.has_one()) store_f(dx + row.one_id(), grad(row.one));
         });
-        if (row.has_one()) store_f(dx + row.one_id(), wp * soft.e(row.one));
-    }
     __syncthreads();
     const float kl = waves_sum<KW>(S.teacher[2]) + bad;
     if (threadIdx.x == 0 && A.row_losses)
@@ -150,9 +160,11 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
         first = first && j >= k;
         sum += S.q[j];
     }
-    if (first)
-        store_f(dx + S.ids[k],
-                __builtin_fmaf(soft.e(S.student[k]), wp, -sum * wt));
+    if (!first) return;
+    soft.with_t(row, [&](auto t, auto) {
+        const float e = __builtin_amdgcn_exp2f(t(S.student[k]));
+        store_f(dx + S.ids[k], __builtin_fmaf(e, wp, -sum * wt));
+    });
 }
 
 // loss = sum_r weight[r] row_losses[r], one workgroup, in float64: a fixed

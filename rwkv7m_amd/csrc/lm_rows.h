@@ -244,13 +244,22 @@ struct Row {
     // f(vector, its number) over the thread's vectors, the last of which may
     // be past the row's whole vectors (-inf).  The empty asm keeps the
     // compiler from carrying one walk's unpacked elements over to the next in
-    // two to four times the registers.
-    template <typename F>
+    // two to four times the registers.  With COPY f gets a copy, for a walk in
+    // a branch beside another one: the asm's results of both would have to
+    // meet in one set of registers behind it, and the row spills.
+    template <bool COPY = false, typename F>
     __device__ __forceinline__ void each(F f) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            asm volatile("" : "+v"(v[i].raw));
-            if (i * NT < cut.whole) f(v[i], i * NT + int(threadIdx.x));
+            if constexpr (COPY) {
+                if (i * NT >= cut.whole) continue;
+                Vec<E> a = v[i];
+                asm volatile("" : "+v"(a.raw));
+                f(a, i * NT + int(threadIdx.x));
+            } else {
+                asm volatile("" : "+v"(v[i].raw));
+                if (i * NT < cut.whole) f(v[i], i * NT + int(threadIdx.x));
+            }
         }
         // (rows of the other variants end within their registers: without
         // this loop they keep within 64 of them)
@@ -310,36 +319,44 @@ struct Row {
             go(KERNEL<E, 1024, 16>, 1024);            \
     } while (0)
 
-// Softmax over a row of logits x at temperature T in base 2: t = x c - refc
-// in one fma, e = 2^t, with c = log2(e) / T and refc = ref c rounded, ref the
-// row's largest.  e is the softmax up to a factor that does not depend on x,
-// so the rounding of refc is no error as long as everything is taken from the
-// same t.  A row with no element above -inf has ref 0, and every e 0.
-// Where ref c is beyond 2^100 (rows of the type's lowest or largest values),
-// an element below the largest is at least 2^76 below it in units of 1 / c,
-// so its e is 0: there c is replaced by a power of two 2^60 below it, whose
-// product with x is exact, does not overflow and says the same.
+// Softmax over a row of logits x at temperature T in base 2: e = 2^t with t =
+// (x - ref) c, c = log2(e) / T and ref the row's largest.  A row with no
+// element above -inf has ref 0, and every e 0.
+// Up to |ref c| = 2^16, one fma an element: t = x c - refc, refc the rounded
+// product, which moves every t by the same 2^-9 or less.  e is then the
+// softmax up to a factor that does not depend on x, and everything is taken
+// from the same t.  That factor grows with |ref c| and leaves fp32's range at
+// 2^31 (logits of -1e10, a temperature of 1e-8), so rows beyond take the
+// difference first: next to ref it is exact, and t is off by its own rounding
+// alone at any size.  Taken so for every row, the added operation costs rows
+// of 4096 to 131072 bf16 3 to 4 % of their scoring's time.
 struct RowSoftmax {
-    float c, refc, ref;
+    float c, ref, refc;
+    bool one_fma;  // (the same in every lane)
 
     // (largest is the same in every lane)
-    __device__ __forceinline__ RowSoftmax(float largest, float c_) {
-        ref = uniform(largest == -__builtin_inff() ? 0.f : largest);
-        c = c_;
-        if (fabsf(ref * c) > 0x1p100f)
-            c = __uint_as_float(__float_as_uint(c_) & 0x7f800000u) * 0x1p-60f;
-        c = uniform(c);
+    __device__ __forceinline__ RowSoftmax(float largest, float c_)
+        : c(c_), ref(uniform(largest == -__builtin_inff() ? 0.f : largest)) {
         refc = uniform(ref * c);
+        one_fma = fabsf(refc) <= 0x1p16f;
     }
-    __device__ __forceinline__ float t(float x) const {
-        return __builtin_fmaf(x, c, -refc);
+    // (x - ref) c, whichever form the row takes
+    __device__ __forceinline__ float difference(float x) const {
+        return (x - ref) * c;
     }
-    __device__ __forceinline__ float e(float x) const {
-        return __builtin_amdgcn_exp2f(t(x));
+    // walk(t, each): a walk over the row with its form of t.
+    template <typename R, typename F>
+    __device__ __forceinline__ void with_t(R& row, F walk) const {
+        if (one_fma)
+            walk([this](float x) { return __builtin_fmaf(x, c, -refc); },
+                 [&row](auto f) { row.each(f); });
+        else
+            walk([this](float x) { return difference(x); },
+                 [&row](auto f) { row.template each<true>(f); });
     }
-    // log2 of sum 2^((x - ref) c), from s = the sum of e
+    // log2 of sum 2^((x - ref) c), from s = the sum of 2^t
     __device__ __forceinline__ float log2_sum(float s) const {
-        return __log2f(s) + __builtin_fmaf(-ref, c, refc);
+        return __log2f(s) + (one_fma ? __builtin_fmaf(-ref, c, refc) : 0.f);
     }
 };
 

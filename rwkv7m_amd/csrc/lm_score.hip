@@ -219,18 +219,21 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     }
     const RowSoftmax soft(largest, A.c);
     float s0 = 0.f, s1 = 0.f;
-    const auto add = [&](float x) {
-        // (held above -200, where e is 0 already: -inf adds 0, not 0 * -inf)
-        const float t = larger(soft.t(x), -200.f);
-        const float e = __builtin_amdgcn_exp2f(t);
-        s0 += e;
-        s1 = __builtin_fmaf(e, t, s1);
-    };
-    row.each([&](const Vec<E>& a, int) {
+    soft.with_t(row, [&](auto exponent, auto each) {
+        const auto add = [&](float x) {
+            // (held above -200, where e is 0 already: -inf adds 0, not
+            // 0 * -inf)
+            const float t = larger(exponent(x), -200.f);
+            const float e = __builtin_amdgcn_exp2f(t);
+            s0 += e;
+            s1 = __builtin_fmaf(e, t, s1);
+        };
+        each([&](const Vec<E>& a, int) {
 #pragma unroll
-        for (int j = 0; j < n; ++j) add(a.get(j));
+            for (int j = 0; j < n; ++j) add(a.get(j));
+        });
+        add(row.one);
     });
-    add(row.one);
     s0 = lanes_sum<64>(s0);
     s1 = lanes_sum<64>(s1);
     if (lane == 0) {

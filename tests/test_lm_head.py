@@ -770,3 +770,78 @@ def test_the_example_learns(hip_lib):
     assert float(losses[-1]) < 0.7 * float(losses[0])
     assert float(after.logprobs.mean()) > float(before.logprobs.mean())
     assert after.top_ids.shape == (4, 64, 3)
+
+
+# --- the softmax over every temperature and size of logit that is accepted --
+
+def _check_distill_range(lm, x, ids, top, w, T):
+    """As _check_distill, with the row losses' tolerance by their terms: q_k
+    is off by SUM of itself, log q_k and log p_k by SUM times max(1, |value|),
+    and what fp32 cannot hold (2^-149) is 0."""
+    leaf = x.cuda().requires_grad_()
+    r = lm.distill_loss(leaf, ids.cuda(), top.cuda(), w.cuda(), temperature=T)
+    d, = torch.autograd.grad(r.loss, leaf, retain_graph=True)
+    scaled, = torch.autograd.grad(-2.0 * r.loss, leaf)
+    loss, rows, want, scale = _distill64(x, ids, top, w, T)
+    logq = torch.log_softmax((top.double() / T).masked_fill(ids < 0, -INF), -1)
+    lp = torch.log_softmax(x.double() / T, -1).gather(-1, ids.clamp(min=0))
+    q = logq.exp()
+    size = sum(torch.where(q > 0, q * v.abs().clamp(min=1.0), 0.0).sum(-1)
+               for v in (logq, lp))
+    tol = 2 * SUM * T * T * size + 2.0 ** -149
+    off = (r.row_losses.double().cpu() - rows).abs()
+    assert bool((off <= tol).all()), (T, off, tol)
+    off = abs(float(r.loss) - float(loss))
+    assert off <= float((w.double() * tol).sum()) + 1e-7 * abs(float(loss)), (
+        T, off)
+    _close("gradient", d, want, scale, own=False)
+    _close("scaled gradient", scaled, -2 * want, 2 * scale, own=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [300, 5000, 40003])
+def test_softmax_at_every_temperature(lm, V, dtype):
+    """Down to greedy: the exponents go up to 1e32, past fp32's whole
+    numbers."""
+    g = _gen(V)
+    x = _logits(g, 6, V, dtype=dtype).clamp(max=19.0)
+    x[0, 7] = 30.25
+    x[1, V - 2] = 23.5
+    x[2, [3, V // 2, V - 1]] = 30.25       # three of the same
+    x[3, 11] = 20.0
+    x[4] = -x[4].abs() - 2.5               # the largest is negative
+    x[5, ::2] = -INF
+    tok = torch.tensor([7, V - 2, 3, 12, 0, 1])
+    ids, top = _teacher(g, torch.Size((6,)), V, 9)
+    ids[:, 0] = x.float().argmax(-1)
+    ids[5] = 1 + 2 * torch.arange(9)       # none of the masked
+    top[0, 3], top[1, 0], top[2, 1:3] = 30.25, 23.5, 20.0
+    w = torch.rand(6, generator=g) + 0.5
+    for e in (3, 1, *range(-3, -31, -1)):
+        T = 10.0 ** e
+        print("case: temperature", V, dtype, T, flush=True)
+        _check_score(lm, x.cuda(), tok.cuda(), 3 if V == 300 else 0, T)
+        _check_distill_range(lm, x, ids, top, w, T)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [300, 5000, 40003])
+def test_softmax_at_every_size_of_logits(lm, V, dtype):
+    """Rows of one value throughout (a mask's), a few beside it, and rows that
+    spread around it, student and teacher."""
+    g = _gen(V + 1)
+    for e in (3, 4, 5, 6, 7, 8, 9, 10, 12, 16, 20, 25, 29, 30, 31, 38):
+        print("case: size of logits", V, dtype, e, flush=True)
+        at = torch.tensor([-1.0, 1.0, -1.0, 1.0, -1.0, 1.0]) * 10.0 ** e
+        x = at[:, None].expand(6, V).clone()
+        x[2:4] += 3 * torch.randn(2, V, generator=g)
+        x[4:] *= 1 + 2.0 ** -7 * torch.rand(2, V, generator=g)
+        x[1, V // 3] *= 1.0 + 2.0 ** -6
+        x = x.to(DT[dtype])
+        ids, top = _teacher(g, torch.Size((6,)), V, 9)
+        top = top + (at * torch.tensor([1.0, 0, 1, 0, 0, -1]))[:, None]
+        top[0], top[1, :5] = at[0], -10.0 ** e
+        tok = ids[:, 0].clone()
+        w = torch.rand(6, generator=g) + 0.5
+        _check_score(lm, x.cuda(), tok.cuda(), 3 if V == 300 else 0)
+        _check_distill_range(lm, x, ids, top, w, 1.0)
