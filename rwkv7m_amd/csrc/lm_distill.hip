@@ -123,10 +123,12 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
         const float q = S.ids[k] == -1 ? 0.f : te / ts;
         float share = 0.f;
         if (q != 0.f) {
-            // log2 q - log2 p; a row of nothing but -inf has p = 0
-            const float lp = soft.difference(S.student[k]) -
-                             (s0 == 0.f ? inf : soft.log2_sum(s0));
-            share = q * (teacher.difference(t) - __log2f(ts) - lp);
+            // half of T (log q - log p), which fits where neither log does; a
+            // row of nothing but -inf has p = 0
+            const float ls = s0 == 0.f ? inf : soft.log2_sum(s0);
+            share = q * (teacher.half_difference(t) -
+                         soft.half_difference(S.student[k]) +
+                         0.5f * kLn2 * A.temperature * (ls - __log2f(ts)));
         }
         share = lanes_sum<64>(share);
         if (lane == 0) S.teacher[2][wave] = share;
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
     __syncthreads();
     const float kl = waves_sum<KW>(S.teacher[2]) + bad;
     if (threadIdx.x == 0 && A.row_losses)
-        A.row_losses[r] = kl * kLn2 * A.temperature * A.temperature;
+        A.row_losses[r] = kl * A.temperature * 2.f;
     if (!dx || k >= K || S.ids[k] < 0) return;
     float sum = 0.f;
     bool first = true;

@@ -344,6 +344,10 @@ struct RowSoftmax {
     __device__ __forceinline__ float difference(float x) const {
         return (x - ref) * c;
     }
+    // (x - ref) / 2, which does not overflow where x - ref does
+    __device__ __forceinline__ float half_difference(float x) const {
+        return __builtin_fmaf(x, 0.5f, -0.5f * ref);
+    }
     // walk(t, each): a walk over the row with its form of t.
     template <typename R, typename F>
     __device__ __forceinline__ void with_t(R& row, F walk) const {

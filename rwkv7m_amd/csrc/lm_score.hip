@@ -246,7 +246,9 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
     const bool empty = largest == -inf;
     const float ls = kLn2 * soft.log2_sum(s0);
     const auto logp = [&](float x) {
-        return empty ? -inf : __builtin_fmaf(x - soft.ref, inv_t, -ls);
+        return empty ? -inf
+                     : __builtin_fmaf(soft.half_difference(x), 2.f * inv_t,
+                                      -ls);
     };
     if (threadIdx.x == 0) {
         A.logprobs[r] = S.token < 0    ? 0.f

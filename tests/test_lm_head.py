@@ -845,3 +845,30 @@ def test_softmax_at_every_size_of_logits(lm, V, dtype):
         w = torch.rand(6, generator=g) + 0.5
         _check_score(lm, x.cuda(), tok.cuda(), 3 if V == 300 else 0)
         _check_distill_range(lm, x, ids, top, w, 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_results_that_fit_where_a_difference_does_not(lm, dtype):
+    """x - largest, or the loss before T^2, past fp32's range: the log
+    probability at a high temperature and the loss at a low one are within."""
+    V = 300
+    g = _gen(21)
+    x = _logits(g, 4, V, dtype="f32")
+    x[0, ::3], x[0, 1::3] = -3e38, 3e38
+    x[1] = -3.2e38
+    x[1, 5] = 3.2e38
+    x[2, 4], x[2, 9] = 1e30, -1e30
+    x[3, :9] *= 1e12
+    x = x.to(DT[dtype])
+    tok = torch.tensor([0, 0, 9, 3])
+    for T in (2.0, 3.7, 1e4, 1e20, 1e30):
+        print("case: differences past fp32, scored", dtype, T, flush=True)
+        _check_score(lm, x.cuda(), tok.cuda(), 64, T)
+    # the teacher sure of what the student all but excludes
+    ids = torch.tensor([[0, 1, 2], [0, 5, 7], [9, 4, 3], [3, 8, 100]])
+    top = torch.tensor([[3.0, 1.0, 0.0], [3e38, -3e38, -3e38],
+                        [1e30, -1e30, 0.0], [1e12, 0.0, 1e11]])
+    w = torch.rand(4, generator=g) + 0.5
+    for T in (0.1, 1e-3, 1e-8, 1e-30):
+        print("case: differences past fp32, distilled", dtype, T, flush=True)
+        _check_distill_range(lm, x, ids, top, w, T)
