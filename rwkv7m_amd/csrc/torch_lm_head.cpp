@@ -124,6 +124,15 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
+// A tangent of forward-mode differentiation, which needs no gradient to be
+// enabled, is refused and not dropped.
+void no_tangents(const char* fn, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_TYPE(!t->defined() || !t->_fw_grad(0).defined(), fn,
+                         " supports reverse-mode differentiation only; "
+                         "forward-mode autodiff (jvp) is not implemented");
+}
+
 at::TensorOptions f32(const Tensor& like) {
     return like.options().dtype(at::kFloat).requires_grad(false);
 }
@@ -197,6 +206,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list dys) {
+        no_tangents("layer_norm", {&dys[0]});
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &bias = saved[2], &stats = saved[3];
         const c10::DeviceGuard guard(x.device());
@@ -234,6 +244,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& weight,
                   const OptTensor& bias, double eps) {
     const Tensor w = or_undefined(weight), b = or_undefined(bias);
+    no_tangents("layer_norm", {&x, &w, &b});
     if (!wants_grad({&x, &w, &b}))
         return std::get<0>(norm_forward(x, w, b, eps, false));
     return LayerNorm::apply(x, weight, bias, eps);
@@ -310,6 +321,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     static variable_list backward(AutogradContext* ctx, variable_list d) {
         if (!d[0].defined() && !d[1].defined())
             return {Tensor(), Tensor(), Tensor(), Tensor()};
+        no_tangents("token_logprobs", {&d[0], &d[1]});
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &stats = saved[2], &ent = saved[3];
         const c10::DeviceGuard guard(logits.device());
@@ -333,6 +345,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(
     const Tensor& logits, const Tensor& tokens, int64_t top_k,
     double temperature) {
+    no_tangents("token_logprobs", {&logits});
     const auto out = wants_grad({&logits})
                          ? TokenLogprobs::apply(logits, tokens, top_k,
                                                 temperature)
@@ -423,6 +436,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         variable_list none(5);
         if (!g[0].defined()) return none;
+        no_tangents("distill_loss", {&g[0]});
         const auto saved = ctx->get_saved_variables();
         const Tensor& logits = saved[0];
         const Distill d(logits, saved[1], saved[2], saved[3]);
@@ -456,6 +470,7 @@ std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits,
                                         const OptTensor& weight,
                                         double temperature) {
     const Tensor w = or_undefined(weight);
+    no_tangents("distill_loss", {&logits, &teacher, &w});
     const auto out =
         wants_grad({&logits})
             ? DistillLoss::apply(logits, ids, teacher, weight, temperature)

@@ -13,8 +13,8 @@ The head's product between the first and the other two is a plain GEMM and
 stays the caller's (``x @ head.T``).  Each is one or two HIP kernels
 (``kernels/lm_head_hip.py``); tensors are on the GPU, activations and logits
 bf16 or fp32, and every sum is held in fp32 or more.  Gradients are first
-order: a second derivative raises.  ``examples/distill_and_score.py`` runs
-the three together.
+order and reverse mode: a second derivative or a forward-mode tangent raises.
+``examples/distill_and_score.py`` runs the three together.
 """
 
 from __future__ import annotations

@@ -185,3 +185,60 @@ def test_calls_on_the_gpu_refuse(hip_lib):
              lambda: distill_loss(x, t.long(), t, torch.ones(3)))):
         with pytest.raises(kind, match=words):
             call()
+
+
+def _with_tangents(x, i, t, w, c):
+    """(name, call on inputs of which one has a tangent)"""
+    dual = torch.autograd.forward_ad.make_dual
+
+    def d(v):
+        return dual(v, torch.ones_like(v))
+
+    yield "layer_norm", lambda: layer_norm(d(x), c, c)
+    yield "layer_norm", lambda: layer_norm(x, d(c), c)
+    yield "layer_norm", lambda: layer_norm(x, c, d(c))
+    yield "layer_norm", lambda: layer_norm(d(x))
+    yield "token_logprobs", lambda: token_logprobs(d(x), i, top_k=2)
+    yield "distill_loss", lambda: distill_loss(d(x), t.long(), t)
+    yield "distill_loss", lambda: distill_loss(x, t.long(), d(t))
+    yield "distill_loss", lambda: distill_loss(x, t.long(), t, d(w))
+
+
+def _refuses_tangents(device):
+    x, c = torch.zeros(3, 8, device=device), torch.ones(8, device=device)
+    i = torch.zeros(3, dtype=torch.int64, device=device)
+    t, w = torch.zeros(3, 4, device=device), torch.ones(3, device=device)
+    words = " supports reverse-mode differentiation only"
+    with torch.autograd.forward_ad.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            for name, call in _with_tangents(leaf, i, t, w, c):
+                for grad in (torch.enable_grad, torch.no_grad):
+                    with grad(), pytest.raises(TypeError, match=name + words):
+                        call()
+    for name, f in (
+            ("layer_norm", layer_norm),
+            ("token_logprobs", lambda v: token_logprobs(v, i).logprobs),
+            ("distill_loss", lambda v: distill_loss(v, t.long(), t).loss)):
+        with pytest.raises(TypeError, match=name + words):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+
+
+def test_forward_mode_is_refused():
+    _refuses_tangents("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_the_gpu(hip_lib):
+    print("case: tangents, also of a cotangent", flush=True)
+    _refuses_tangents("cuda")
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    i = torch.zeros(3, dtype=torch.int64, device="cuda")
+    t = torch.zeros(3, 4, device="cuda")
+    for name, out in (("layer_norm", layer_norm(x)),
+                      ("token_logprobs", token_logprobs(x, i).entropy),
+                      ("distill_loss", distill_loss(x, t.long(), t).loss)):
+        with torch.autograd.forward_ad.dual_level():
+            cot = torch.autograd.forward_ad.make_dual(
+                torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(TypeError, match=name):
+                torch.autograd.grad(out, x, cot)
