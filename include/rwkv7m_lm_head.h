@@ -16,7 +16,11 @@
  * no byte with an input.  Calls only enqueue work on `stream`, never allocate
  * and never synchronise, so they may be captured in a HIP graph.  Results do
  * not depend on the order in which workgroups run, nor a row's on how many
- * others there are.
+ * others there are.  A row of logits is summed in an order that goes by its
+ * address modulo 16 bytes and, up to 8192 bytes, by whether more than 40
+ * alternatives are asked for or a teacher gives more than 64: between those
+ * its values agree to rounding, not to the last bit.  (Rows of a batch whose
+ * length is no multiple of 16 bytes lie at different such addresses.)
  */
 #ifndef RWKV7M_LM_HEAD_H
 #define RWKV7M_LM_HEAD_H

@@ -872,3 +872,86 @@ def test_results_that_fit_where_a_difference_does_not(lm, dtype):
     for T in (0.1, 1e-3, 1e-8, 1e-30):
         print("case: differences past fp32, distilled", dtype, T, flush=True)
         _check_distill_range(lm, x, ids, top, w, T)
+
+
+# --- what a row's bits depend on ------------------------------------------
+
+def _placed(row, past, dtype):
+    """A copy of the row whose address is `past` elements above a multiple of
+    16 bytes."""
+    buf = torch.zeros(row.numel() + 64, dtype=dtype, device="cuda")
+    first = -buf.data_ptr() % 16 // buf.element_size()
+    out = buf[first + past:first + past + row.numel()]
+    assert out.data_ptr() % 16 == past * buf.element_size()
+    return out.copy_(row)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [61, 1001, 5003, 20011, 65529, 140007])
+def test_bits_of_a_row_by_its_alignment(lm, V, dtype):
+    """The rows of a batch of odd length against each alone: equal bits at
+    the same address modulo 16, else equal ids and values to rounding."""
+    print("case: alignment of rows", V, dtype, flush=True)
+    g = _gen(V)
+    dt = DT[dtype]
+    n = 16 // torch.empty((), dtype=dt).element_size()
+    x = _logits(g, n + 1, V, dtype=dtype).cuda()
+    assert x.data_ptr() % 16 == 0
+    tok = torch.randint(0, V, (n + 1,), generator=g).cuda()
+    ids, top = (t.cuda() for t in _teacher(g, torch.Size((n + 1,)), V, 5))
+    w = torch.ones(n + 1, device="cuda")
+
+    def scored(x, s):
+        x = x.detach().requires_grad_()
+        r = lm.token_logprobs(x, tok[s], top_k=5)
+        d, = torch.autograd.grad((r.logprobs.sum(), r.entropy.sum()), x)
+        k = lm.distill_loss(x, ids[s], top[s], w[s])
+        dk, = torch.autograd.grad(k.loss, x)
+        return [*r, k.row_losses, d, dk]
+
+    every = scored(x, slice(None))
+    for r in (0, 1, n // 2, n - 1, n):
+        s, past = slice(r, r + 1), r * V % n
+        same = scored(_placed(x[r], past, dt)[None], s)
+        for a, b in zip(every, same):
+            assert torch.equal(a[s], b)
+        other = scored(_placed(x[r], (past + 1) % n, dt)[None], s)
+        assert torch.equal(every[2][s], other[2])
+        for i in (0, 1, 3, 4):
+            _close("value", other[i], every[i][s].double())
+        for i in (5, 6):  # (two roundings to bf16 may fall a step apart)
+            a, b = other[i].double(), every[i][s].double()
+            step = 2.0 ** -7 * b.abs() if dtype == "bf16" else 0.0
+            assert bool(((a - b).abs() <= 14 * SUM + step).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [500, 2048, 20000])
+def test_bits_of_a_row_by_its_alternatives(lm, V, dtype):
+    """Equal for 0 to 40 alternatives and 0 to 64 of the teacher's, for any
+    number in rows of more than 512 vectors of 16 bytes."""
+    print("case: number of alternatives", V, dtype, flush=True)
+    g = _gen(V)
+    x = _logits(g, 3, V, dtype=dtype).cuda()
+    tok = torch.randint(0, V, (3,), generator=g).cuda()
+    ids, top = (t.cuda() for t in _teacher(g, torch.Size((3,)), V, 4))
+    long = V * x.element_size() > 512 * 16
+    base = lm.token_logprobs(x, tok)
+    for k in (1, 5, 40, 41, 64):
+        r = lm.token_logprobs(x, tok, top_k=k)
+        if k <= 40 or long:
+            assert torch.equal(r.logprobs, base.logprobs)
+            assert torch.equal(r.entropy, base.entropy)
+        else:
+            _close("logprobs", r.logprobs, base.logprobs.double())
+            _close("entropy", r.entropy, base.entropy.double())
+    base = lm.distill_loss(x, ids, top).row_losses
+    for k in (5, 64, 65, 256):
+        more = torch.full((3, k - 4), -1, device="cuda")
+        got = lm.distill_loss(
+            x, torch.cat([ids, more], -1),
+            torch.cat([top, more.float()], -1)).row_losses
+        if k <= 64 or long:
+            assert torch.equal(got, base)
+        else:
+            _close("row losses", got, base.double())
