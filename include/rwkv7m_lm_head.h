@@ -69,10 +69,10 @@ int rwkv7m_layer_norm_backward(int dtype, int param_dtype, int64_t outer,
  *   logprobs[r] = log p[tokens[r]];  entropy[r] = -sum p log p;
  *   top_ids[r], top_logprobs[r]: the top_k largest logits, equal ones in the
  *   order of their ids, and their log p ([rows][top_k]; NULL with top_k 0).
- * tokens int64: one below 0 is not scored (logprob 0), one >= V gives NaN.
- * An element of -inf has p = 0 and adds nothing; in a row of nothing else
- * every log p is -inf and the entropy 0.  A row that holds NaN or +inf has
- * NaN in place of all these; NaN ranks above +inf.  0 <= top_k <=
+ * tokens int64: one below 0 is not scored (logprob 0 whatever its row holds),
+ * one >= V gives NaN.  An element of -inf has p = 0 and adds nothing; in a row
+ * of nothing else every log p is -inf and the entropy 0.  A row that holds NaN
+ * or +inf has NaN in place of the others; NaN ranks above +inf.  0 <= top_k <=
  * min(V, RWKV7M_MAX_TOP_K).  `stats` [rows][2] is what the backward takes (NULL
  * where there is none). */
 int rwkv7m_token_logprobs(int dtype, int64_t outer, int64_t inner, int64_t V,
@@ -104,6 +104,10 @@ int rwkv7m_token_logprobs_backward(
  * >= V gives NaN; an alternative of -inf has q = 0 and adds nothing.  weight
  * [rows] fp32, or NULL: 1 / rows each.  A row with weight 0, or without an
  * alternative above -inf, has loss and gradient 0 whatever its logits hold.
+ * In the other rows NaN or +inf among the logits makes loss and gradient NaN,
+ * among the present teacher's the loss and the gradient at its ids; a logit of
+ * -inf has p = 0, and the loss is +inf where q > 0 there (the gradient stays
+ * finite: -weight T q).
  * row_losses [rows] fp32; dlogits [rows][V] of `dtype`, or NULL: the losses
  * alone. */
 int rwkv7m_distill_loss(int dtype, int teacher_dtype, int64_t outer,

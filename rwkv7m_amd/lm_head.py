@@ -53,12 +53,13 @@ def token_logprobs(logits, tokens, top_k: int = 0,
     entropy, and the ``top_k`` (at most 64) likeliest ids with their log
     probabilities, equal ones in the order of their ids.
 
-    A token below 0 (padding, -100) is not scored: its logprob is 0 and it
-    has no gradient.  A token of V or more gives NaN.  Logits of -inf are
-    masked: probability 0, nothing added to the entropy.  Differentiable in
-    ``logits`` through ``logprobs`` and ``entropy``; the alternatives are a
-    report and carry no gradient.  A position whose cotangents are zero has a
-    zero gradient whatever its logits hold."""
+    A token below 0 (padding, -100) is not scored: its logprob is 0, whatever
+    its position's logits hold, and it has no gradient.  A token of V or more
+    gives NaN.  Logits of -inf are masked: probability 0, nothing added to the
+    entropy.  Differentiable in ``logits`` through ``logprobs`` and
+    ``entropy``; the alternatives are a report and carry no gradient.  A
+    position whose cotangents are zero has a zero gradient whatever its logits
+    hold."""
     return TokenLogprobs(*load_binding().token_logprobs(logits, tokens, top_k,
                                                         temperature))
 

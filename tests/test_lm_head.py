@@ -955,3 +955,39 @@ def test_bits_of_a_row_by_its_alternatives(lm, V, dtype):
             assert torch.equal(got, base)
         else:
             _close("row losses", got, base.double())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_unscored_tokens_of_rows_without_a_distribution(lm, dtype):
+    """A token below 0 has logprob 0 whatever its row holds; the entropy and
+    the alternatives are the row's."""
+    print("case: unscored tokens of NaN rows", dtype, flush=True)
+    V = 900
+    x = _logits(_gen(6), 4, V, dtype=dtype)
+    x[0, 5], x[1, 6], x[2] = float("nan"), INF, -INF
+    tok = torch.full((4,), -100).cuda()
+    leaf = x.cuda().requires_grad_()
+    r = lm.token_logprobs(leaf, tok, top_k=3)
+    assert not r.logprobs.any() and r.entropy[:2].isnan().all()
+    assert r.entropy[2] == 0 and r.top_logprobs[:2].isnan().all()
+    assert torch.equal(r.top_ids.cpu(), _top64(x.float(), 3))
+    d, = torch.autograd.grad(r.logprobs, leaf, torch.ones(4).cuda())
+    assert not d.any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_distill_non_finite_teachers_and_students(lm, dtype):
+    print("case: distill, NaN and +inf on either side", dtype, flush=True)
+    V = 900
+    x = _logits(_gen(7), 5, V, dtype=dtype)
+    ids, top = _teacher(_gen(8), torch.Size((5,)), V, 6)
+    x[0, 5], x[1, 6] = INF, float("nan")
+    top[2, 1], top[3, 4] = INF, float("nan")
+    top[4, 3], ids[4, 3] = float("nan"), -1     # absent: not looked at
+    leaf = x.cuda().requires_grad_()
+    r = lm.distill_loss(leaf, ids.cuda(), top.cuda())
+    d, = torch.autograd.grad(r.loss, leaf)
+    assert r.row_losses[:4].isnan().all() and r.row_losses[4].isfinite()
+    assert d[:2].isnan().all() and d[4].isfinite().all()
+    at = torch.zeros(2, V, dtype=torch.bool).scatter_(1, ids[2:4], True)
+    assert torch.equal(d[2:4].isnan().cpu(), at)
