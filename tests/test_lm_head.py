@@ -991,3 +991,51 @@ def test_distill_non_finite_teachers_and_students(lm, dtype):
     assert d[:2].isnan().all() and d[4].isfinite().all()
     at = torch.zeros(2, V, dtype=torch.bool).scatter_(1, ids[2:4], True)
     assert torch.equal(d[2:4].isnan().cpu(), at)
+
+
+# --- gradients where a workgroup takes more than one turn -------------------
+
+@pytest.mark.parametrize("dtype,rows,C", [
+    ("bf16", 40001, 40), ("f32", 40001, 40),       # 16 threads a row
+    ("bf16", 9001, 320), ("f32", 9001, 500),       # a wave, one and two vectors
+    ("bf16", 9001, 1000),
+    ("bf16", 2731, 1536), ("f32", 2731, 1001),     # 4 waves
+    ("bf16", 2600, 4096), ("f32", 2600, 2048),
+    ("bf16", 600, 8191), ("f32", 600, 4093),       # 16 waves
+    ("bf16", 517, 16384), ("f32", 517, 8192),
+    ("bf16", 600, 5), ("f32", 600, 3),             # element by element
+    ("bf16", 300, 20000), ("f32", 300, 20000)])
+def test_layer_norm_gradients_of_many_rows(lm, dtype, rows, C):
+    """Two turns and a rest of the backward's workgroups."""
+    print("case: layer norm, many rows", rows, C, dtype, flush=True)
+    g = _gen(rows + C)
+    x = (torch.randn(rows, C, generator=g) * 2 + torch.randn(C, generator=g)
+         ).to(DT[dtype]).cuda()
+    w = (1 + 0.2 * torch.randn(C, generator=g)).cuda()
+    b = torch.randn(C, generator=g).cuda()
+    dy = torch.randn(rows, C, generator=g).to(DT[dtype]).cuda()
+    _check_norm(lm, x, w, b, dy)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_token_logprobs_gradients_of_many_rows(lm, dtype):
+    """More tiles of a row than the gradient's grid has workgroups."""
+    rows, V = (1 << 20) + 1003, 9
+    print("case: token logprobs, many rows", rows, dtype, flush=True)
+    g = _gen(17)
+    x = _logits(g, rows, V, dtype=dtype).cuda()
+    tok = torch.randint(-1, V, (rows,), generator=g)
+    _check_score(lm, x, tok.cuda(), 0, 1.3)
+
+
+def test_top_alternatives_far_from_zero(lm):
+    """Distinct fp32 logits that share an offset: their order is in the low
+    bits of their values."""
+    for V in (300, 20011, 65536):
+        x = 2 * torch.randn(3, V, generator=_gen(V))
+        x[1] += 1000.0
+        x[2] -= 4000.0
+        tok = torch.zeros(3, dtype=torch.int64).cuda()
+        for k in (1, 5, 64):
+            print("case: far from zero", V, k, flush=True)
+            _check_score(lm, x.cuda(), tok, k, grads=False)
