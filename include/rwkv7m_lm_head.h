@@ -94,9 +94,9 @@ int rwkv7m_token_logprobs_backward(
     const float *d_logprobs, const float *d_entropy, void *dlogits,
     void *stream);
 
-/* Distillation from a teacher's top K logits (K <= RWKV7M_MAX_TEACHER_K).  With q
- * = softmax(teacher_logits / T) over the row's present alternatives (id >= 0)
- * and p = softmax(logits / T) over V:
+/* Distillation from a teacher's top K logits (K <= RWKV7M_MAX_TEACHER_K).
+ * With q = softmax(teacher_logits / T) over the row's present alternatives
+ * (id >= 0) and p = softmax(logits / T) over V:
  *   row_losses[r] = T^2 * sum_k q_k (log q_k - log p[id_k]),
  *   loss[0] = sum_r weight[r] * row_losses[r],
  *   dlogits[r][j] = weight[r] * T * (p_j - sum over k with id_k = j of q_k).

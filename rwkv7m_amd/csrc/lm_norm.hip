@@ -10,8 +10,8 @@
 // many rows, with the parameters, and in the backward their gradients' sums,
 // in registers; each workgroup writes one partial row of those sums and a
 // second kernel adds the partial rows in a fixed order.
-// [32768, 2048] bf16 with fp32 parameters: forward 44 us (6.1 TB/s), backward
-// 80 + 4 us (5.0 TB/s).
+// [32768, 2048] bf16 with fp32 parameters, medians under a profiler: forward
+// 44 us (6.1 TB/s), backward 82 + 5 us (4.9 TB/s without the second kernel).
 //
 // A row whose length is no multiple of the vector ends in a vector moved back
 // to end with it (its first `dup` elements are the vector before's): every
@@ -211,8 +211,8 @@ __global__ __launch_bounds__(kBwdThreads) void norm_bwd_kernel(LmNormArgs A) {
     constexpr int RPB = kBwdThreads / TPR, n = Vec<E>::n;
     constexpr int kCols = RPB > 1 ? TPR * NV * n : 1;
     // A thread with one vector a row asks for the next row's while it works
-    // on this one's ([32768, 2048] bf16: 84 against 87 us); with two the
-    // waves have enough in flight without ([16384, 4096]: 83 against 81).
+    // on this one's ([32768, 2048] bf16: 3 % less time); with two the waves
+    // have enough in flight without ([16384, 4096]: 2 % more).
     constexpr bool kAhead = NV == 1;
     __shared__ float s[2][2][kBwdThreads / 64];
     __shared__ float part[RPB][2][kCols];
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(LmNormArgs A,
 // Vectors a thread of a group below the widest holds.  The backward has four
 // arrays of them in fp32 and one workgroup of 16 waves a CU: two, or too few
 // waves have room ([32768, 2048] bf16 by waves of 4 vectors, in workgroups of
-// 4, 94 us; by groups of 4 waves with one vector each 84).
+// 4, takes 12 % longer than by groups of 4 waves with one vector each).
 constexpr int64_t kFwdVectors = 4, kBwdVectors = 2;
 constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 256;
 

@@ -162,10 +162,10 @@ __device__ __forceinline__ float waves_larger(const float* s) {
 
 // Waves a SIMD that a kernel with a Row of NV vectors a thread leaves room for,
 // of the 512 registers a lane has there: 8 of 64 (4 NV <= 32 hold the row),
-// 6 of 80 for three workgroups of 512 threads a CU and for single waves (LDS
-// has no room for 8 of those), 4 of 128 where the row takes 64.
+// 6 of 80 for three workgroups of 512 threads a CU, 4 of 128 where the row
+// takes 64.
 template <int NT, int NV>
-constexpr int kRowWaves = NT == 64 || NT == 512 ? 6 : NV <= 8 ? 8 : 4;
+constexpr int kRowWaves = NT == 512 ? 6 : NV <= 8 ? 8 : 4;
 
 // An offset that is the same in every lane, in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t x) {

@@ -5,23 +5,27 @@
 // workgroup holds a row in its registers as it came (65536 bf16 logits: 512
 // threads of 64 registers), so that the largest logit, the sums and the
 // alternatives are three walks over registers and not over memory.  [4088,
-// 65536] bf16 is read in 91 us (5.9 TB/s), with 10 alternatives in 99 (5.4):
+// 65536] bf16 is read in 90 us (6.0 TB/s), with 10 alternatives in 98 (5.5):
 // what those add is mostly latency, a search of the bound, two passes over LDS
 // and three barriers in which the row's registers wait.  Rows of more than
 // 65536 bf16 leave room for one workgroup a CU, whose loads nothing overlaps:
-// 4.1 TB/s at 131072.
+// 4.0 TB/s at 131072.
 //
 // The alternatives.  Each thread's largest logit is known from the first
 // walk; the k-th largest over g = 256 groups of threads (64 threads in a wave
 // of its own) is a lower bound T of the row's k-th largest logit, and for
 // logits in no particular order not many more than k of them lie at or above
-// it (-g log(1 - k / g) on average).
+// it (-g log(1 - k / g) on average, as long as the bound's 16 high bits tell
+// the largest apart).
 // The vectors that hold one go to LDS, their elements at or above T to a list
 // there, and each of those finds its rank by counting the ones before it.
-// Where they are more than LDS has room for (many equal logits, or large ones
-// at the same few threads), or NaN are among them, the list's bound is found
-// exactly, by counting and bisection over the order of the values and then of
-// the ids: 0.40 ms for [4088, 65536] of nothing but equal logits.
+// Where they are more than LDS has room for (many equal logits, large ones at
+// the same few threads, a mask that leaves fewer than k groups anything, fp32
+// logits whose offset is some hundred times their spread and that agree in
+// their high bits), or NaN are among them, the list's bound is found exactly,
+// by counting and bisection over the order of the values and then of the ids:
+// 0.40 ms for [4088, 65536] of nothing but equal logits, 1.0 ms for [1022,
+// 65536] fp32 around 1000 with a spread of 2 (61 us around 0).
 
 #include "lm_rows.h"
 
@@ -312,7 +316,8 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
 // dlogits: a workgroup a tile of kTile vectors a thread of one row (a wave's
 // where a row is no longer than that); the first tile's also takes the
 // elements before and behind the row's vectors.  Bound by memory: 12
-// operations and 4 bytes an element in bf16, 5.8 TB/s at [4088, 65536].
+// operations and 4 bytes an element in bf16, 5.1 TB/s at [4088, 65536] behind
+// the forward (209 us, the shortest of 20 168).
 constexpr int kTile = 4;
 
 template <typename E, int NT>

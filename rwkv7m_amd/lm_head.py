@@ -80,8 +80,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, weight=None,
 
     Where a gradient is wanted the call forms it (for a cotangent of 1 on
     the loss) while it reads the logits; scaling the loss afterwards costs a
-    second pass in the backward, scaling ``weight`` nothing.  No gradient
-    flows to the teacher or the weight."""
+    second pass in the backward, scaling ``weight`` nothing.  Until the
+    backward the gradient is held beside the saved logits, out of reach of
+    saved-tensor hooks.  No gradient flows to the teacher or the weight."""
     return DistillLoss(*load_binding().distill_loss(
         logits, teacher_ids, teacher_logits, weight, temperature))
 
