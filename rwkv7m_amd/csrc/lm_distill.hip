@@ -151,9 +151,9 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
             if (row.has_one()) store_f(dx + row.one_id(), grad(row.one));
         });
     __syncthreads();
-    const float kl = waves_sum<KW>(S.teacher[2]) + bad;
+    const float half = waves_sum<KW>(S.teacher[2]) + bad;
     if (threadIdx.x == 0 && A.row_losses)
-        A.row_losses[r] = kl * A.temperature * 2.f;
+        A.row_losses[r] = half * A.temperature * 2.f;
     if (!dx || k >= K || S.ids[k] < 0) return;
     float sum = 0.f;
     bool first = true;
@@ -164,8 +164,10 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void distill_kernel(
     }
     if (!first) return;
     soft.with_t(row, [&](auto t, auto) {
+        // (p by a division: 1 where it is, so that p - q is 0)
         const float e = __builtin_amdgcn_exp2f(t(S.student[k]));
-        store_f(dx + S.ids[k], __builtin_fmaf(e, wp, -sum * wt));
+        const float p = (s0 == 0.f ? 0.f : e / s0) + bad;
+        store_f(dx + S.ids[k], (p - sum) * wt);
     });
 }
 

@@ -358,9 +358,16 @@ struct RowSoftmax {
             walk([this](float x) { return difference(x); },
                  [&row](auto f) { row.template each<true>(f); });
     }
-    // log2 of sum 2^((x - ref) c), from s = the sum of 2^t
+    // The largest's t: what the form moves every t by.
+    __device__ __forceinline__ float largest_t() const {
+        return one_fma ? __builtin_fmaf(ref, c, -refc) : 0.f;
+    }
+    // log2 of sum 2^((x - ref) c), from s = the sum of 2^t: 0 or more, and
+    // exactly 0 where none counts beside the largest.
     __device__ __forceinline__ float log2_sum(float s) const {
-        return __log2f(s) + (one_fma ? __builtin_fmaf(-ref, c, refc) : 0.f);
+        const float t = largest_t();
+        return s == __builtin_amdgcn_exp2f(t) ? 0.f
+                                              : larger(__log2f(s) - t, 0.f);
     }
 };
 

@@ -245,27 +245,9 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
         S.sums[1][wave] = s1;
     }
     __syncthreads();
-    s0 = waves_sum<W>(S.sums[0]);
-    s1 = waves_sum<W>(S.sums[1]);
-    const bool empty = largest == -inf;
-    const float ls = kLn2 * soft.log2_sum(s0);
-    const auto logp = [&](float x) {
-        return empty ? -inf
-                     : __builtin_fmaf(soft.half_difference(x), 2.f * inv_t,
-                                      -ls);
-    };
-    if (threadIdx.x == 0) {
-        A.logprobs[r] = S.token < 0    ? 0.f
-                        : S.token >= V ? __builtin_nanf("")
-                                       : logp(S.at_token);
-        A.entropy[r] = empty ? 0.f : kLn2 * (__log2f(s0) - s1 / s0);
-        if (A.stats) {
-            A.stats[2 * r] = soft.ref;
-            A.stats[2 * r + 1] = empty ? inf : ls;
-        }
-    }
-    if (!K) return;
-    const uint32_t bound = S.bound;
+    s0 = uniform(waves_sum<W>(S.sums[0]));
+    s1 = uniform(waves_sum<W>(S.sums[1]));
+    const uint32_t bound = K ? S.bound : 0u;
     // (below the key of -inf: the groups that hold anything are fewer
     // than k)
     const float least = bound < 0x00800000u ? -inf : key_value(bound);
@@ -274,21 +256,48 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
         if (at < kList<NT>)
             S.list[at] = uint64_t(key) << 32 | (0xffffffffu - uint32_t(id));
     };
-    if (mine >= least)
-        row.each([&](const Vec<E>& a, int k) {
-            float most = a.get(0);
+    if (K) {
+        if (mine >= least)
+            row.each([&](const Vec<E>& a, int k) {
+                float most = a.get(0);
 #pragma unroll
-            for (int j = 1; j < n; ++j) most = larger(most, a.get(j));
-            if (!(most >= least) || k >= row.cut.whole) return;
-            const int at = atomicAdd(&S.vectors, 1);
-            if (at >= kVectors<NT>) return;
-            S.first[at] = row.cut.lead + k * n;
+                for (int j = 1; j < n; ++j) most = larger(most, a.get(j));
+                if (!(most >= least) || k >= row.cut.whole) return;
+                const int at = atomicAdd(&S.vectors, 1);
+                if (at >= kVectors<NT>) return;
+                S.first[at] = row.cut.lead + k * n;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) S.raw[at][w] = a.raw[w];
-        });
-    if (row.has_one() && row.one >= least)
-        put(order_key(row.one), row.one_id());
-    __syncthreads();
+                for (int w = 0; w < 4; ++w) S.raw[at][w] = a.raw[w];
+            });
+        if (row.has_one() && row.one >= least)
+            put(order_key(row.one), row.one_id());
+        __syncthreads();
+    }
+    // (after the last walk: the row's registers are free for the divisions)
+    const bool empty = largest == -inf;
+    const float log2_s = soft.log2_sum(s0), ls = kLn2 * log2_s;
+    const auto logp = [&](float x) {
+        return empty ? -inf
+                     : __builtin_fmaf(soft.half_difference(x), 2.f * inv_t,
+                                      -ls);
+    };
+    // (a thread of the last wave, which seldom has alternatives to rank)
+    if (threadIdx.x == NT - 64) {
+        A.logprobs[r] = S.token < 0    ? 0.f
+                        : S.token >= V ? __builtin_nanf("")
+                                       : logp(S.at_token);
+        // s1 with every t moved back by the largest's, whose own term goes
+        // first: exactly 0 where no other counts
+        const float t = soft.largest_t(), e = __builtin_amdgcn_exp2f(t);
+        const float own = __builtin_fmaf(e, t, 0.f);
+        s1 = __builtin_fmaf(-t, s0 - e, s1 - own);
+        A.entropy[r] = empty ? 0.f : kLn2 * (log2_s - s1 / s0);
+        if (A.stats) {
+            A.stats[2 * r] = soft.ref;
+            A.stats[2 * r + 1] = empty ? inf : ls;
+        }
+    }
+    if (!K) return;
     const int vectors = S.vectors;
     for (int i = threadIdx.x; i < vectors * n && vectors <= kVectors<NT>;
          i += NT) {

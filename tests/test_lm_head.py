@@ -1039,3 +1039,37 @@ def test_top_alternatives_far_from_zero(lm):
         for k in (1, 5, 64):
             print("case: far from zero", V, k, flush=True)
             _check_score(lm, x.cuda(), tok, k, grads=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [40, 700, 5003, 65536])
+def test_certain_rows_are_certain(lm, V, dtype):
+    """One token allowed, or one far above the rest: its log probability, the
+    entropy, the loss of a teacher as sure and its gradients are exactly 0,
+    and no log probability is above 0."""
+    print("case: certain rows", V, dtype, flush=True)
+    g = _gen(V)
+    at = torch.randint(0, V, (64,), generator=g)
+    size = (20 * torch.randn(64, 1, generator=g)).to(DT[dtype])
+    x = torch.full((64, V), -INF).scatter_(1, at[:, None], size.float())
+    x[32:][x[32:] == -INF] = -30000.0
+    x = x.to(DT[dtype])
+    for T in (1.0, 0.7, 1.3):
+        leaf = x.cuda().requires_grad_()
+        r = lm.token_logprobs(leaf, at.cuda(), top_k=3, temperature=T)
+        assert not r.logprobs.any() and not r.entropy.any()
+        assert torch.equal(r.top_ids[:, 0].cpu(), at)
+        assert not r.top_logprobs[:, 0].any()
+        d, = torch.autograd.grad((r.logprobs, r.entropy), leaf,
+                                 [torch.ones(64).cuda()] * 2)
+        assert not d.any()
+        k = lm.distill_loss(leaf, at[:, None].cuda(), size.cuda(),
+                            temperature=T)
+        d, = torch.autograd.grad(k.loss, leaf)
+        assert not k.loss.any() and not k.row_losses.any() and not d.any()
+        y = (4 * torch.randn(64, V, generator=g)).to(DT[dtype])
+        y[:, 0] += 16.0
+        r = lm.token_logprobs(y.cuda(), torch.zeros_like(at).cuda(), top_k=3,
+                              temperature=T)
+        assert (r.logprobs <= 0).all() and (r.top_logprobs <= 0).all()
+        assert (r.entropy >= 0).all()
