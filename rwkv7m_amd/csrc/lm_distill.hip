@@ -8,7 +8,7 @@
 // exponentials, and for the gradient weight T p, with each exponential
 // computed again rather than kept (the row would take twice the registers).
 // [4088, 65536] bf16 takes 209 us (5.1 TB/s) by itself; between backward
-// passes, under a profiler, 210 to 224.  The teacher's alternatives are one to
+// passes, under a profiler, 210 to 228.  The teacher's alternatives are one to
 // a thread of the first 4 waves and stay in LDS; after the gradient's row is
 // out, each writes its entry again with its q taken off, the first of equal
 // ids with all their q, summed in the order of the alternatives.

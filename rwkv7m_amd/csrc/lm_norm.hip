@@ -11,7 +11,7 @@
 // in registers; each workgroup writes one partial row of those sums and a
 // second kernel adds the partial rows in a fixed order.
 // [32768, 2048] bf16 with fp32 parameters, medians under a profiler: forward
-// 44 us (6.1 TB/s), backward 82 + 5 us (4.9 TB/s without the second kernel).
+// 44 us (6.0 TB/s), backward 82 + 5 us (4.9 TB/s without the second kernel).
 //
 // A row whose length is no multiple of the vector ends in a vector moved back
 // to end with it (its first `dup` elements are the vector before's): every

@@ -5,11 +5,11 @@
 // workgroup holds a row in its registers as it came (65536 bf16 logits: 512
 // threads of 64 registers), so that the largest logit, the sums and the
 // alternatives are three walks over registers and not over memory.  [4088,
-// 65536] bf16 is read in 90 us (6.0 TB/s), with 10 alternatives in 98 (5.5):
-// what those add is mostly latency, a search of the bound, two passes over LDS
-// and three barriers in which the row's registers wait.  Rows of more than
-// 65536 bf16 leave room for one workgroup a CU, whose loads nothing overlaps:
-// 4.0 TB/s at 131072.
+// 65536] bf16 is read in 90 to 93 us (5.9 TB/s), with 10 alternatives in 98
+// (5.5): what those add is mostly latency, a search of the bound, two passes
+// over LDS and three barriers in which the row's registers wait.  Rows of more
+// than 65536 bf16 leave room for one workgroup a CU, whose loads nothing
+// overlaps: 3.8 TB/s at 131072.
 //
 // The alternatives.  Each thread's largest logit is known from the first
 // walk; the k-th largest over g = 256 groups of threads (64 threads in a wave
@@ -325,8 +325,8 @@ __global__ __launch_bounds__(NT, (kRowWaves<NT, NV>)) void score_kernel(
 // dlogits: a workgroup a tile of kTile vectors a thread of one row (a wave's
 // where a row is no longer than that); the first tile's also takes the
 // elements before and behind the row's vectors.  Bound by memory: 12
-// operations and 4 bytes an element in bf16, 5.1 TB/s at [4088, 65536] behind
-// the forward (209 us, the shortest of 20 168).
+// operations and 4 bytes an element in bf16, 5.2 TB/s at [4088, 65536] behind
+// the forward (207 us, the shortest of 20 175).
 constexpr int kTile = 4;
 
 template <typename E, int NT>
