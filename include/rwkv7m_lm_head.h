@@ -41,7 +41,8 @@ extern "C" {
 /* y = (x - mean) * rstd * weight + bias over the C elements of each row, with
  * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  x and y of `dtype`; weight and
  * bias (C elements each of `param_dtype`) may be NULL (1 and 0).  mean and
- * rstd [rows] fp32 are what the backward takes; NULL where there is none. */
+ * rstd [rows] fp32 are what the backward takes; NULL where there is none.  A
+ * row's sum and the sum of its squared deviations have to fit fp32. */
 int rwkv7m_layer_norm(int dtype, int param_dtype, int64_t outer, int64_t inner,
                       int64_t C, int64_t outer_stride, int64_t inner_stride,
                       const void *x, const void *weight, const void *bias,
@@ -73,8 +74,8 @@ int rwkv7m_layer_norm_backward(int dtype, int param_dtype, int64_t outer,
  * one >= V gives NaN.  An element of -inf has p = 0 and adds nothing; in a row
  * of nothing else every log p is -inf and the entropy 0.  A row that holds NaN
  * or +inf has NaN in place of the others; NaN ranks above +inf.  0 <= top_k <=
- * min(V, RWKV7M_MAX_TOP_K).  `stats` [rows][2] is what the backward takes (NULL
- * where there is none). */
+ * min(V, RWKV7M_MAX_TOP_K), 1e-30 <= temperature <= 1e30.  `stats` [rows][2]
+ * is what the backward takes (NULL where there is none). */
 int rwkv7m_token_logprobs(int dtype, int64_t outer, int64_t inner, int64_t V,
                           int64_t outer_stride, int64_t inner_stride,
                           const void *logits, const int64_t *tokens,
@@ -108,8 +109,9 @@ int rwkv7m_token_logprobs_backward(
  * among the present teacher's the loss and the gradient at its ids; a logit of
  * -inf has p = 0, and the loss is +inf where q > 0 there (the gradient stays
  * finite: -weight T q).
- * row_losses [rows] fp32; dlogits [rows][V] of `dtype`, or NULL: the losses
- * alone. */
+ * row_losses [rows] fp32, off by fp32's rounding of T^2 max(1, |log p|);
+ * dlogits [rows][V] of `dtype`, or NULL: the losses alone.  1e-30 <=
+ * temperature <= 1e30. */
 int rwkv7m_distill_loss(int dtype, int teacher_dtype, int64_t outer,
                         int64_t inner, int64_t V, int64_t outer_stride,
                         int64_t inner_stride, int64_t K, const void *logits,

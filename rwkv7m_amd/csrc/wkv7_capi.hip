@@ -863,7 +863,7 @@ int lm_temperature(const char* fn, double t) {
     if (!(t >= 1e-30 && t <= 1e30))
         return fail(RWKV7M_ERR_INVALID_ARGUMENT,
                     std::string(fn) +
-                        ": temperature must be positive and finite");
+                        ": temperature must be within 1e-30 and 1e30");
     return RWKV7M_OK;
 }
 

@@ -49,8 +49,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
 def token_logprobs(logits, tokens, top_k: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
     """Log probability of ``tokens`` (``[...]`` int64 or int32) under
-    ``softmax(logits / temperature)`` (``[..., V]``), the distribution's
-    entropy, and the ``top_k`` (at most 64) likeliest ids with their log
+    ``softmax(logits / temperature)`` (``[..., V]``; temperatures from 1e-30 to
+    1e30), the distribution's entropy, and the ``top_k`` (at most 64) likeliest ids with their log
     probabilities, equal ones in the order of their ids.
 
     A token below 0 (padding, -100) is not scored: its logprob is 0, whatever

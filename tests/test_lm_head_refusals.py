@@ -242,3 +242,19 @@ def test_forward_mode_is_refused_on_the_gpu(hip_lib):
                 torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(TypeError, match=name):
                 torch.autograd.grad(out, x, cot)
+
+
+def test_temperatures_outside_the_range_are_refused(lib):
+    P = 4096  # nothing is read before every check has passed
+    for temp in (0.0, 9e-31, 1.1e30, float("inf"), float("nan")):
+        for rc in (
+                lib.rwkv7m_token_logprobs(1, 1, 3, 50, 0, 50, P, P, 2, temp,
+                                          P, P, P, P, None, None),
+                lib.rwkv7m_token_logprobs_backward(
+                    1, 1, 3, 50, 0, 50, P, P, temp, P, P, P, P, P, None),
+                lib.rwkv7m_distill_loss(1, 0, 1, 3, 50, 0, 50, 4, P, P, P,
+                                        None, temp, P, P, P, None),
+                lib.rwkv7m_distill_loss_backward(
+                    1, 0, 1, 3, 50, 0, 50, 4, P, P, P, None, temp, P, 0, P,
+                    None)):
+            _refused(lib, rc, 1, "temperature must be within 1e-30 and 1e30")
