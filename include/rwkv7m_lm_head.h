@@ -37,6 +37,9 @@ extern "C" {
  * that a teacher gives rwkv7m_distill_loss. */
 #define RWKV7M_MAX_TOP_K 64
 #define RWKV7M_MAX_TEACHER_K 256
+/* Largest number of drafted tokens a sequence that rwkv7m_verify_drafts
+ * takes. */
+#define RWKV7M_MAX_DRAFTS 64
 
 /* y = (x - mean) * rstd * weight + bias over the C elements of each row, with
  * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  x and y of `dtype`; weight and
@@ -130,6 +133,40 @@ int rwkv7m_distill_loss_backward(
     const int64_t *teacher_ids, const void *teacher_logits,
     const float *weight, double temperature, const float *scale,
     int holds_unit, void *dlogits, void *stream);
+
+/* Verification of drafted tokens.  With p_i = softmax(target row i /
+ * temperature) and q_i = softmax(draft row i / temperature), or, where draft is
+ * NULL, q_i = 1 at the drafted token: the drafts x_i = tokens[b][i] of sequence
+ * b, i < n = draft_lengths[b] (NULL, or more than K: K), are taken from the
+ * first on while accept[b][i] q_i(x_i) < p_i(x_i).  accepted[b] = m is their
+ * number.  Behind them one token is drawn: from max(p_m - q_m, 0) if m < n,
+ * from p_n otherwise, the first whose running sum over the vocabulary passes
+ * sample[b] times the whole.  out[b] holds the m drafts, that token, and -1
+ * behind; chances[b][i] = min(1, p_i(x_i) / q_i(x_i)) for i < n, 0 behind.
+ *
+ * temperature 0: a draft is taken where it is the likeliest token (the lowest
+ * id of equal ones), which is also the one drawn; draft, accept and sample may
+ * be NULL and are not read.  Otherwise 1e-30 <= temperature <= 1e30, and the
+ * random numbers, from 0 to below 1, decide in float64.
+ *
+ * target has rows [B][K + 1] of V logits (outer = B, inner = K + 1), draft
+ * [B][K], one dtype; rows past n are not read.  A logit of -inf has p = 0.  A
+ * drafted token outside the vocabulary is never taken.  Where the row that is
+ * drawn from, or the draft's, holds NaN or +inf, or nothing above -inf, the
+ * token drawn is -1 (and no draft is taken against such a row).  The workspace
+ * is rwkv7m_verify_drafts_workspace_bytes, 16-byte aligned (-1 for invalid
+ * sizes); free again once the call's work is done. */
+int64_t rwkv7m_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
+int rwkv7m_verify_drafts(int dtype, int64_t B, int64_t K, int64_t V,
+                         int64_t target_outer_stride,
+                         int64_t target_inner_stride, const void *target,
+                         int64_t draft_outer_stride,
+                         int64_t draft_inner_stride, const void *draft,
+                         const int64_t *tokens, const float *accept,
+                         const float *sample, const int64_t *draft_lengths,
+                         double temperature, int64_t *out, int64_t *accepted,
+                         float *chances, void *workspace,
+                         int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,9 +1,9 @@
 """Build librwkv7m_wkv.so in-tree with hipcc for gfx950, and the torch binding
-of the language model head's operators beside it.
+of the language model head's operators and the gated delta rule beside it.
 
 The library is plain ``extern "C"`` (include/*.h) with no torch or Python
-types in its signatures; Python reaches it through ctypes, and for the head's
-operators through ``_lm_head_torch.so`` (csrc/torch_lm_head.cpp, host code).
+types in its signatures; Python reaches it through ctypes, and for those
+operators through ``_lm_head_torch.so`` (csrc/torch_*.cpp, host code).
 """
 
 from __future__ import annotations
@@ -68,13 +68,14 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
     hipcc = _hipcc()
     os.makedirs(BUILD_DIR, exist_ok=True)
     objs = []
-    binding = os.path.join(CSRC, "torch_lm_head.cpp")
+    bindings = [os.path.join(CSRC, f)
+                for f in ("torch_lm_head.cpp", "torch_gated_delta.cpp")]
     torch_compile, torch_link = _torch_flags()
 
     def compile_one(src: str) -> str:
         obj = os.path.join(BUILD_DIR,
                            os.path.splitext(os.path.basename(src))[0] + ".o")
-        flags = torch_compile if src == binding else HIPCC_FLAGS
+        flags = torch_compile if src in bindings else HIPCC_FLAGS
         cmd = [hipcc, *flags, "-c", src, "-o", obj]
         res = subprocess.run(cmd, capture_output=True, text=True)
         msg = "\n".join(line for line in (res.stdout + res.stderr).splitlines()
@@ -86,8 +87,9 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
         return obj
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
-        # (the binding takes longest: first)
-        binding_obj, *objs = pool.map(compile_one, [binding, *sources()])
+        # (the bindings take longest: first)
+        objs = list(pool.map(compile_one, [*bindings, *sources()]))
+    binding_objs, objs = objs[:len(bindings)], objs[len(bindings):]
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs,
            "-o", tmp]
@@ -96,7 +98,7 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
         raise RuntimeError(f"link failed:\n{res.stdout}{res.stderr}")
     os.replace(tmp, LIB_PATH)
     tmp = TORCH_LIB_PATH + ".tmp"
-    cmd = [hipcc, "-shared", "-fPIC", "-no-hip-rt", binding_obj,
+    cmd = [hipcc, "-shared", "-fPIC", "-no-hip-rt", *binding_objs,
            "-L" + PKG_DIR, "-l:" + LIB_NAME, *torch_link, "-o", tmp]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

@@ -1,0 +1,324 @@
+// Pieces shared by the gated delta rule's chunk kernels (gdr_prepare.hip,
+// gdr_forward.hip, gdr_backward.hip, gdr_gradients.hip).
+//
+// A chunk is 64 tokens.  Within it, with G the running sum of the log decays
+// (in base 2, float64: E is formed from differences of sums that far tokens
+// make long), S0 the state before it, [Dv][Dk]:
+//
+//   E_ts = 2^(G_t - G_s),  A = tril(beta_t E_ts k_t.k_s, -1),  T = (I + A)^-1
+//   R = beta (V - 2^G (K S0^T)),  X = T R
+//   O = scale (2^G (Q S0^T) + P X),  P = tril(E_ts q_t.k_s)
+//   S_L = 2^G_L S0 + (2^(G_L - G) X)^T K
+//
+// Operands.  All products run on v_mfma_f32_16x16x32_bf16 with fp32 sums.  A
+// number of more bits is a sum of bf16 planes, and a product the sum of the
+// planes' products that count: bf16 q, k and v are one plane (exact), what is
+// computed from them two, the state among it (2^-18 left out); fp32 vectors
+// and what follows from them three (2^-27).  One plane for all would halve the
+// products, and leave the state, an fp32 output that every later chunk reads,
+// 1e-3 off.
+//
+// Register layouts (lane l, r = l % 16, q = l / 16).  An accumulator tile D(X)
+// holds X[4q + e][r], e = 0..3.  An operand of 32 places along the contracted
+// axis holds, in eight slots, X[r][..]: places 4q + e (slots 0..3) and 16 + 4q
+// + e (slots 4..7) of two adjoining tiles, so that the two accumulator tiles
+// D(X^T) are it without a move ("natural"); or 8q + i ("dense": 16 bytes of
+// a row of memory), where both sides of a product are read that way.  The
+// same registers are X as the left operand and X^T as the right one.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "wkv7_common.h"
+#include "wkv7_launch.h"
+
+namespace rwkv7m {
+namespace gdr {
+
+constexpr int C = kGdrChunk;
+constexpr int NT = 256;  // threads of the chunk kernels: 4 waves
+constexpr double kLog2e = 1.4426950408889634;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+
+template <typename E>
+constexpr int kIn = sizeof(E) == 2 ? 1 : 3;  // planes of an input
+template <typename E>
+constexpr int kMade = sizeof(E) == 2 ? 2 : 3;  // planes of a computed number
+
+template <int N>
+struct Frag {
+    u32x4_t p[N];
+};
+
+__device__ __forceinline__ f32x4_t zero4() { return f32x4_t{0.f, 0.f, 0.f, 0.f}; }
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t f = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+}
+
+// Two floats to N planes, a packed pair each.  (A plane that is not finite
+// leaves NaN in the next: such numbers make NaN of their products.)
+template <int N>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&out)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        out[n] = pack2(a, b);
+        if (n + 1 < N) {
+            a -= __uint_as_float(out[n] << 16);
+            b -= __uint_as_float(out[n] & 0xffff0000u);
+        }
+    }
+}
+
+// Slots 0..3 from a, 4..7 from b.
+template <int N>
+__device__ __forceinline__ Frag<N> split8(const f32x4_t& a, const f32x4_t& b) {
+    Frag<N> f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t u[N];
+        if (i < 2)
+            split2<N>(a[2 * i], a[2 * i + 1], u);
+        else
+            split2<N>(b[2 * i - 4], b[2 * i - 3], u);
+#pragma unroll
+        for (int n = 0; n < N; ++n) f.p[n][i] = u[n];
+    }
+    return f;
+}
+
+// acc += a b over 32 places, the small planes' products first.
+template <int NA, int NB>
+__device__ __forceinline__ void mul(f32x4_t& acc, const Frag<NA>& a,
+                                    const Frag<NB>& b) {
+    constexpr int most = NA > NB ? NA : NB;
+#pragma unroll
+    for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = s - i;
+            if (j < 0 || j >= NB) continue;
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, a.p[i]),
+                __builtin_bit_cast(bf16x8_t, b.p[j]), acc, 0, 0, 0);
+        }
+}
+
+__device__ __forceinline__ float exp2_of(double x) {
+    return __builtin_amdgcn_exp2f(float(x));
+}
+
+// --- memory -----------------------------------------------------------------
+
+// Eight adjoining elements of a row as they are held in memory, at 16-byte
+// aligned addresses (a row's places past Dk or Dv, and rows past T, are 0).
+template <typename E>
+struct Eight;
+template <>
+struct Eight<bf16_t> {
+    u32x4_t a;
+    __device__ __forceinline__ void load(const bf16_t* p) {
+        a = *reinterpret_cast<const u32x4_t*>(p);
+    }
+    __device__ __forceinline__ void clear() { a = u32x4_t{0, 0, 0, 0}; }
+    __device__ __forceinline__ Frag<1> planes() const { return {{a}}; }
+    __device__ __forceinline__ float get(int i) const {
+        return __uint_as_float(i & 1 ? a[i >> 1] & 0xffff0000u : a[i >> 1] << 16);
+    }
+};
+template <>
+struct Eight<float> {
+    f32x4_t a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = *reinterpret_cast<const f32x4_t*>(p);
+        b = *reinterpret_cast<const f32x4_t*>(p + 4);
+    }
+    __device__ __forceinline__ void clear() { a = b = zero4(); }
+    __device__ __forceinline__ Frag<3> planes() const { return split8<3>(a, b); }
+    __device__ __forceinline__ float get(int i) const {
+        return i < 4 ? a[i] : b[i - 4];
+    }
+};
+
+// A chunk's 64 rows of DKP = 32 KT places in LDS, NP planes.  The pitch puts
+// 16 rows' 8-byte pieces on 64 different banks.
+template <int NP, int KT>
+struct Rows64 {
+    static constexpr int pitch = 32 * KT + 8;
+    bf16_t x[NP][C][pitch];
+
+    // Left operand of rows 16 tb .., places 32 p .. (natural).
+    __device__ __forceinline__ Frag<NP> rows(int tb, int p, int lane) const {
+        const int r = lane & 15, q = lane >> 4;
+        Frag<NP> f;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const uint2 lo = *reinterpret_cast<const uint2*>(
+                &x[n][16 * tb + r][32 * p + 4 * q]);
+            const uint2 hi = *reinterpret_cast<const uint2*>(
+                &x[n][16 * tb + r][32 * p + 16 + 4 * q]);
+            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        }
+        return f;
+    }
+    // X[4q + e][16 jb + r] of the rows at `row`, by a transposing read.
+    __device__ __forceinline__ uint2 column(int n, int row, int jb,
+                                            int lane) const {
+        const int s = lane & 15, q = lane >> 4;
+        const bf16_t* p = &x[n][row + 4 * q + (s >> 2)][16 * jb + 4 * (s & 3)];
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                             (lds_i16x4_t*)(p)));
+    }
+    // Left operand of rows 16 jb .. of the transpose (columns of x), over the
+    // 32 rows of pair p (natural); as the right operand, x itself.
+    __device__ __forceinline__ Frag<NP> columns(int jb, int p, int lane) const {
+        Frag<NP> f;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const uint2 lo = column(n, 32 * p, jb, lane);
+            const uint2 hi = column(n, 32 * p + 16, jb, lane);
+            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        }
+        return f;
+    }
+    // The same over rows 32 p + 8q + i (dense).
+    __device__ __forceinline__ Frag<NP> columns_dense(int jb, int p,
+                                                      int lane) const {
+        const int s = lane & 15, q = lane >> 4;
+        Frag<NP> f;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const bf16_t* at =
+                &x[n][32 * p + 8 * q + (s >> 2)][16 * jb + 4 * (s & 3)];
+            const uint2 lo = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (lds_i16x4_t*)(at)));
+            const uint2 hi = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (lds_i16x4_t*)(at + 4 * pitch)));
+            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        }
+        return f;
+    }
+    // X[row + 4q + e][16 jb + r] as floats.
+    __device__ __forceinline__ f32x4_t values(int row, int jb, int lane) const {
+        f32x4_t v = zero4();
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) {
+            const uint2 u = column(n, row, jb, lane);
+            v[0] += __uint_as_float(u.x << 16);
+            v[1] += __uint_as_float(u.x & 0xffff0000u);
+            v[2] += __uint_as_float(u.y << 16);
+            v[3] += __uint_as_float(u.y & 0xffff0000u);
+        }
+        return v;
+    }
+};
+
+// A thread's share of a chunk's rows on their way to LDS.
+template <typename E, int KT>
+struct Staged {
+    static constexpr int per_row = 4 * KT, n = C * per_row / NT;
+    Eight<E> v[n];
+
+    // Rows 0 .. valid - 1 of `base`, `dim` places each.
+    __device__ __forceinline__ void load(const E* base, int64_t stride,
+                                         int valid, int dim) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int u = i * NT + int(threadIdx.x);
+            const int row = u / per_row, col = 8 * (u % per_row);
+            if (row < valid && col < dim)
+                v[i].load(base + row * stride + col);
+            else
+                v[i].clear();
+        }
+    }
+    __device__ __forceinline__ void store(Rows64<kIn<E>, KT>& to) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int u = i * NT + int(threadIdx.x);
+            const int row = u / per_row, col = 8 * (u % per_row);
+            const auto f = v[i].planes();
+#pragma unroll
+            for (int m = 0; m < kIn<E>; ++m)
+                *reinterpret_cast<u32x4_t*>(&to.x[m][row][col]) = f.p[m];
+        }
+    }
+};
+
+// --- what gdr_prepare.hip leaves for a chunk of a head ------------------------
+
+// Lower triangular 64 x 64 matrices as operands: of the left operand's row
+// block tb and pair p of 32 places only those that hold anything, six.
+// Transposed ones hold row blocks of the transpose.
+__device__ __forceinline__ constexpr bool image_has(bool transposed, int tb,
+                                                    int p) {
+    return transposed ? 2 * p + 1 >= tb : 2 * p <= tb;
+}
+__device__ __forceinline__ constexpr int image_at(bool transposed, int tb,
+                                                  int p) {
+    int at = 0;
+    for (int t = 0; t < 4; ++t)
+        for (int u = 0; u < 2; ++u) {
+            if (t == tb && u == p) return at;
+            at += image_has(transposed, t, u);
+        }
+    return at;
+}
+
+template <int NC>
+struct Prepared {
+    u32x4_t t[6][NC][64], p[6][NC][64];  // T and P (or their transposes)
+    double G[C];                          // base 2
+    float first[C], last[C], beta[C];     // 2^G, 2^(G_L - G)
+};
+
+template <int NC>
+__device__ __forceinline__ Frag<NC> image(const u32x4_t (&m)[6][NC][64], int at,
+                                          int lane) {
+    Frag<NC> f;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) f.p[n] = m[at][n][lane];
+    return f;
+}
+
+__device__ __forceinline__ f32x4_t four(const float* p) {
+    return *reinterpret_cast<const f32x4_t*>(p);
+}
+
+// Sum over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ float sum16(float x) { return group_sum<16>(x); }
+
+// A head's workgroups on one of the 8 XCDs (consecutive workgroups go to
+// different ones), so that they share its L2: workgroup `id` of head and part.
+struct Place {
+    int64_t head;
+    int part;
+};
+__device__ __forceinline__ Place place(unsigned id, unsigned parts) {
+    const unsigned xcd = id % 8, slot = id / 8;
+    return {int64_t(slot / parts) * 8 + xcd, int(slot % parts)};
+}
+inline unsigned places(int64_t heads, int64_t parts) {
+    return unsigned((heads + 7) / 8 * 8 * parts);
+}
+
+template <typename E>
+__device__ __forceinline__ const E* at(const GdrTensor& t, int64_t b, int64_t h,
+                                       int64_t token) {
+    return static_cast<const E*>(t.p) + b * t.sb + h * t.sh + token * t.st;
+}
+
+}  // namespace gdr
+}  // namespace rwkv7m

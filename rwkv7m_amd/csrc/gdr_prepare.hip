@@ -1,0 +1,248 @@
+// The gated delta rule's chunk matrices (gdr_common.h has the formulas): T =
+// (I + A)^-1 and P, as operands of the recurrences' products, and the gates.
+//
+// One workgroup a chunk and value head, all of them independent.  T's diagonal
+// blocks of 16 are substituted forward, a lane a column: with keys that
+// resemble each other the powers of A in a product form of the inverse grow to
+// 1e3 and cancel, which would cost fp32 three of its digits.  The blocks
+// below follow by fp32 matrix products, T_ij = -T_ii sum_m A_im T_mj.
+#include "gdr_common.h"
+
+namespace rwkv7m {
+namespace {
+
+using namespace gdr;
+
+constexpr int PITCH = C + 4;
+
+struct Shared {
+    alignas(16) float a[C][PITCH], t[C][PITCH];
+    double G[C];
+    float beta[C];
+};
+
+__device__ __forceinline__ float gate(const GdrTensor& t, bool bf16, int64_t b,
+                                      int64_t h, int64_t token) {
+    return bf16 ? load_f(at<bf16_t>(t, b, h, token))
+                : load_f(at<float>(t, b, h, token));
+}
+
+// D(M Y) + c from D(M^T) and D(Y) in fp32.
+__device__ __forceinline__ f32x4_t mm32(const f32x4_t& mt, const f32x4_t& y,
+                                        f32x4_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(mt[e], y[e], c, 0, 0, 0);
+    return c;
+}
+
+template <typename E, int KT, bool BWD>
+__global__ void __launch_bounds__(NT)
+gdr_prepare_kernel(const GdrArgs A) {
+    constexpr int NI = kIn<E>, NC = kMade<E>;
+    __shared__ Shared S;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const int64_t chunks = (A.T + C - 1) / C;
+    const int64_t id = blockIdx.x, head = id / chunks, c = id % chunks;
+    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    const int64_t t0 = c * C;
+    const int valid = int(A.T - t0 < C ? A.T - t0 : C);
+    auto* out = static_cast<Prepared<NC>*>(A.prepared) + id;
+
+    if (wave == 0) {
+        // the running sum of the log decays: a decay of 0 (-inf) is held to
+        // e^-1000, 0 in any result, so that later differences stay finite
+        double G = 0.0;
+        float beta = 0.f;
+        if (lane < valid) {
+            const float g = gate(A.g, A.g_bf16, b, h, t0 + lane);
+            G = kLog2e * double(g < -1000.f ? -1000.f : g);
+            beta = gate(A.beta, A.beta_bf16, b, h, t0 + lane);
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const double x = __shfl_up(G, m);
+            if (lane >= m) G += x;
+        }
+        S.G[lane] = G;
+        S.beta[lane] = beta;
+        out->G[lane] = G;
+        out->first[lane] = exp2_of(G);
+        out->last[lane] = exp2_of(__shfl(G, 63) - G);
+        out->beta[lane] = beta;
+    }
+    // rows of k and q: places 32 p + 8q + i of token 16 tb + r
+    const auto rows = [&](const GdrTensor& x, int tb, Frag<NI> (&f)[KT]) {
+        const int t = 16 * tb + r;
+        const E* p = at<E>(x, b, hk, t0 + t);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+            Eight<E> v;
+            const int col = 32 * i + 8 * q;
+            if (t < valid && col < A.Dk)
+                v.load(p + col);
+            else
+                v.clear();
+            f[i] = v.planes();
+        }
+    };
+    Frag<NI> kw[KT], qw[KT];
+    rows(A.k, wave, kw);
+    rows(A.q, wave, qw);
+    __syncthreads();
+    f32x4_t pt[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pt[j] = zero4();
+    const double Gw = S.G[16 * wave + r];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        Frag<NI> kj[KT], qj[KT];
+        if (BWD ? j >= wave : j <= wave) {
+            if constexpr (BWD) rows(A.q, j, qj);
+            if constexpr (!BWD) rows(A.k, j, kj);
+#pragma unroll
+            for (int p = 0; p < KT; ++p) {
+                if constexpr (BWD)
+                    mul(pt[j], qj[p], kw[p]);  // D(P): t = 4q + e, s = r
+                else
+                    mul(pt[j], kj[p], qw[p]);  // D(P^T): s = 4q + e, t = r
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // (i: the tile's row of its accumulator, in block j)
+                const int i = 16 * j + 4 * q + e, w = 16 * wave + r;
+                const int t = BWD ? i : w, s = BWD ? w : i;
+                const double Gi = S.G[i];
+                pt[j][e] = s <= t ? pt[j][e] * exp2_of(BWD ? Gi - Gw : Gw - Gi)
+                                  : 0.f;
+            }
+        }
+        if (j <= wave) {
+            if constexpr (BWD) rows(A.k, j, kj);
+            f32x4_t a = zero4();  // D(A): t = 4q + e, s = r
+#pragma unroll
+            for (int p = 0; p < KT; ++p) mul(a, kw[p], kj[p]);
+            const double Gs = S.G[16 * j + r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = 16 * wave + 4 * q + e, s = 16 * j + r;
+                S.a[t][s] = s < t ? a[e] * S.beta[t] * exp2_of(S.G[t] - Gs)
+                                  : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        // (row block and pair of P's operand: the wave's and tiles 2p, 2p + 1)
+        const Frag<NC> f = split8<NC>(pt[2 * p], pt[2 * p + 1]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            if (w == wave && image_has(BWD, w, p))
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+                    out->p[image_at(BWD, w, p)][n][lane] = f.p[n];
+    }
+    __syncthreads();
+    if (wave == 0) {
+        // block q's column r of the inverse
+        float x[16];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            float sum = t == r ? 1.f : 0.f;
+#pragma unroll
+            for (int s = 0; s < t; s += 4) {
+                const f32x4_t a = four(&S.a[16 * q + t][16 * q + s]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (s + i < t) sum -= a[i] * x[s + i];
+            }
+            x[t] = sum;
+            S.t[16 * q + t][16 * q + r] = sum;
+        }
+    }
+    __syncthreads();
+    if (wave < 3) {
+        // column block `wave`, downwards
+        f32x4_t y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            y[0][e] = S.t[16 * wave + 4 * q + e][16 * wave + r];
+#pragma unroll
+        for (int d = 1; d < 4; ++d) {
+            const int i = wave + d;
+            if (i > 3) break;
+            f32x4_t sum = zero4();
+#pragma unroll
+            for (int m = 0; m < d; ++m)
+                sum = mm32(four(&S.a[16 * i + r][16 * (wave + m) + 4 * q]),
+                           y[m], sum);
+            y[d] = mm32(four(&S.t[16 * i + r][16 * i + 4 * q]), sum, zero4());
+            y[d] = -y[d];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                S.t[16 * i + 4 * q + e][16 * wave + r] = y[d][e];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w != wave) continue;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            if (!image_has(BWD, w, p)) continue;
+            f32x4_t x[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int block = 2 * p + u;
+                x[u] = zero4();
+                if (BWD && block >= w) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[u][e] = S.t[16 * block + 4 * q + e][16 * w + r];
+                } else if (!BWD && block <= w) {
+                    x[u] = four(&S.t[16 * w + r][16 * block + 4 * q]);
+                }
+            }
+            const Frag<NC> f = split8<NC>(x[0], x[1]);
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+                out->t[image_at(BWD, w, p)][n][lane] = f.p[n];
+        }
+    }
+}
+
+}  // namespace
+
+int gdr_dkp(int Dk) { return Dk <= 64 ? 64 : 128; }
+int gdr_dvp(int Dv) { return (Dv + 31) / 32 * 32; }
+
+int64_t gdr_prepared_bytes(bool bf16) {
+    return bf16 ? int64_t(sizeof(Prepared<kMade<bf16_t>>))
+                : int64_t(sizeof(Prepared<kMade<float>>));
+}
+
+hipError_t launch_gdr_prepare(bool bf16, bool backward, const GdrArgs& A,
+                              hipStream_t stream) {
+    const int64_t grid = A.B * A.Hv * ((A.T + C - 1) / C);
+    const bool wide = gdr_dkp(A.Dk) == 128;
+#define RWKV7M_GDR(E, KT, BWD)                                             \
+    hipLaunchKernelGGL((gdr_prepare_kernel<E, KT, BWD>),                   \
+                       dim3(unsigned(grid)), dim3(NT), 0, stream, A)
+#define RWKV7M_GDR2(E)                                                     \
+    do {                                                                   \
+        if (wide && backward) RWKV7M_GDR(E, 4, true);                      \
+        else if (wide) RWKV7M_GDR(E, 4, false);                            \
+        else if (backward) RWKV7M_GDR(E, 2, true);                         \
+        else RWKV7M_GDR(E, 2, false);                                      \
+    } while (0)
+    if (bf16)
+        RWKV7M_GDR2(bf16_t);
+    else
+        RWKV7M_GDR2(float);
+#undef RWKV7M_GDR2
+#undef RWKV7M_GDR
+    return hipGetLastError();
+}
+
+}  // namespace rwkv7m

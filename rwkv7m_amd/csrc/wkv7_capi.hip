@@ -15,6 +15,7 @@
 #include <mutex>
 #include <string>
 
+#include "../../include/rwkv7m_gated_delta.h"
 #include "../../include/rwkv7m_lm_head.h"
 #include "../../include/rwkv7m_screening.h"
 #include "../../include/rwkv7m_timemix.h"
@@ -876,6 +877,138 @@ int lm_guard(F body) {
     } catch (...) {
         return RWKV7M_ERR_HIP;
     }
+}
+
+// ---------------------------------------------------------------------------
+// Gated delta rule (include/rwkv7m_gated_delta.h)
+// ---------------------------------------------------------------------------
+
+struct GdrSizes {
+    int64_t chunks, heads, states, x, prepared;  // (the last in bytes)
+};
+
+// The sizes and types alone (pointers and strides are not looked at).
+int gdr_sizes(const char* fn, const rwkv7m_gated_delta_inputs* in,
+              GdrSizes* s) {
+    const std::string f(fn);
+    if (in == nullptr)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": inputs is NULL");
+    RWKV7M_TRY(lm_dtype(fn, "q, k and v", in->dtype));
+    RWKV7M_TRY(lm_dtype(fn, "g", in->g_dtype));
+    RWKV7M_TRY(lm_dtype(fn, "beta", in->beta_dtype));
+    if (in->B < 0 || in->T < 0 || in->Hk < 0 || in->Hv < 0)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": negative dimension");
+    if (in->Hk < 1 || in->Hv < 1 || in->Hv % in->Hk)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    f + ": Hv=" + std::to_string(in->Hv) +
+                        " must be a multiple of Hk=" + std::to_string(in->Hk) +
+                        ", at least 1");
+    if (in->Dk < 8 || in->Dk > 128 || in->Dk % 8 || in->Dv < 8 ||
+        in->Dv > 256 || in->Dv % 8)
+        return fail(RWKV7M_ERR_UNSUPPORTED,
+                    f + ": head sizes Dk=" + std::to_string(in->Dk) +
+                        ", Dv=" + std::to_string(in->Dv) +
+                        " are not supported (multiples of 8, Dk up to 128, "
+                        "Dv up to 256)");
+    if (!std::isfinite(in->scale))
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": scale is not finite");
+    // (launches have fewer than 2^32 threads along an axis, chunk kernels 256
+    // a chunk, and a few workgroups a head)
+    const int64_t C = rwkv7m::kGdrChunk, most = (int64_t(1) << 24) - 1;
+    if (in->B > most || in->Hv > most || in->T > (int64_t(1) << 40))
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": sizes too large");
+    s->chunks = (in->T + C - 1) / C;
+    s->heads = in->B * in->Hv;
+    if (s->heads > most / 8 || (s->heads > 0 && s->chunks > most / s->heads))
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": sizes too large");
+    const int64_t dkp = rwkv7m::gdr_dkp(int(in->Dk)),
+                  dvp = rwkv7m::gdr_dvp(int(in->Dv));
+    s->states = s->heads * s->chunks * dvp * dkp;
+    s->x = s->heads * s->chunks * C * dvp;
+    s->prepared = s->heads * s->chunks *
+                  rwkv7m::gdr_prepared_bytes(in->dtype == RWKV7M_DTYPE_BF16);
+    return RWKV7M_OK;
+}
+
+int64_t gdr_workspace(const rwkv7m_gated_delta_inputs* in, const GdrSizes& s,
+                      bool backward) {
+    int64_t bytes = s.prepared;
+    if (backward) {
+        bytes += 4 * (s.states + s.x);
+        if (in->Hv > in->Hk) bytes += 2 * 4 * in->B * in->T * in->Hv * in->Dk;
+    }
+    return bytes;
+}
+
+// A vector's or gate's place, its strides checked against its extents.
+int gdr_tensor(const char* fn, const char* name, const void* p,
+               const int64_t* stride, const rwkv7m_gated_delta_inputs* in,
+               int64_t heads, int64_t unit, int64_t align,
+               rwkv7m::GdrTensor* out) {
+    const std::string f = std::string(fn) + ": " + name;
+    RWKV7M_TRY(lm_need(fn, align, {{name, p}}));
+    const int64_t bytes = int64_t(1) << 46;
+    const int64_t extent[3] = {in->B, in->T, heads};
+    for (int i = 0; i < 3; ++i) {
+        if (stride[i] < 0)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": negative stride");
+        if (extent[i] > 1 && stride[i] > bytes / (extent[i] - 1))
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": sizes too large");
+        if (extent[i] > 1 && (stride[i] * unit) % align)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        f + ": rows are not " + std::to_string(align) +
+                            "-byte aligned");
+    }
+    *out = {p, stride[0], stride[1], stride[2]};
+    return RWKV7M_OK;
+}
+
+int gdr_inputs(const char* fn, const rwkv7m_gated_delta_inputs* in,
+               int64_t v_align, rwkv7m::GdrTensor (&t)[5]) {
+    const int64_t unit = lm_size(in->dtype);
+    const int64_t gu = lm_size(in->g_dtype), bu = lm_size(in->beta_dtype);
+    RWKV7M_TRY(gdr_tensor(fn, "q", in->q, in->q_stride, in, in->Hk, unit, 16,
+                          &t[0]));
+    RWKV7M_TRY(gdr_tensor(fn, "k", in->k, in->k_stride, in, in->Hk, unit, 16,
+                          &t[1]));
+    RWKV7M_TRY(gdr_tensor(fn, "v", in->v, in->v_stride, in, in->Hv, unit,
+                          v_align, &t[2]));
+    RWKV7M_TRY(gdr_tensor(fn, "g", in->g, in->g_stride, in, in->Hv, gu, gu,
+                          &t[3]));
+    return gdr_tensor(fn, "beta", in->beta, in->beta_stride, in, in->Hv, bu,
+                      bu, &t[4]);
+}
+
+int gdr_args(const char* fn, const rwkv7m_gated_delta_inputs* in,
+             rwkv7m::GdrArgs* A) {
+    rwkv7m::GdrTensor t[5];
+    RWKV7M_TRY(gdr_inputs(fn, in, 16, t));
+    A->B = in->B;
+    A->T = in->T;
+    A->Hk = in->Hk;
+    A->Hv = in->Hv;
+    A->Dk = int(in->Dk);
+    A->Dv = int(in->Dv);
+    A->q = t[0];
+    A->k = t[1];
+    A->v = t[2];
+    A->g = t[3];
+    A->beta = t[4];
+    A->g_bf16 = in->g_dtype == RWKV7M_DTYPE_BF16;
+    A->beta_bf16 = in->beta_dtype == RWKV7M_DTYPE_BF16;
+    A->scale = float(in->scale);
+    return RWKV7M_OK;
+}
+
+int gdr_workspace_holds(const char* fn, void* workspace, int64_t bytes,
+                        int64_t need_) {
+    if (bytes < need_)
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    std::string(fn) + ": workspace holds " +
+                        std::to_string(bytes) + " bytes, needs " +
+                        std::to_string(need_));
+    if (need_ > 0) return lm_need(fn, 16, {{"workspace", workspace}});
+    return RWKV7M_OK;
 }
 
 int lm_distill_args(const char* fn, int dtype, int teacher_dtype,
@@ -1934,6 +2067,262 @@ int rwkv7m_distill_loss_backward(
         A.holds_unit = holds_unit != 0;
         return hip_status("distillation gradient launch",
                           rwkv7m::launch_lm_distill(
+                              dtype == RWKV7M_DTYPE_BF16, A,
+                              static_cast<hipStream_t>(stream)));
+    });
+}
+
+int64_t rwkv7m_gated_delta_workspace_bytes(const rwkv7m_gated_delta_inputs* in,
+                                           int backward) {
+    GdrSizes s;
+    if (lm_guard([&]() -> int {
+            return gdr_sizes("rwkv7m_gated_delta_workspace_bytes", in, &s);
+        }) != RWKV7M_OK)
+        return -1;
+    return gdr_workspace(in, s, backward != 0);
+}
+
+int64_t rwkv7m_gated_delta_saved_floats(const rwkv7m_gated_delta_inputs* in) {
+    GdrSizes s;
+    if (lm_guard([&]() -> int {
+            return gdr_sizes("rwkv7m_gated_delta_saved_floats", in, &s);
+        }) != RWKV7M_OK)
+        return -1;
+    return s.states + s.x;
+}
+
+int rwkv7m_gated_delta_rule(const rwkv7m_gated_delta_inputs* in,
+                            const float* initial_state, void* o,
+                            float* final_state, float* saved, void* workspace,
+                            int64_t workspace_bytes, void* stream_) {
+    const char* fn = "rwkv7m_gated_delta_rule";
+    return lm_guard([&]() -> int {
+        GdrSizes s;
+        RWKV7M_TRY(gdr_sizes(fn, in, &s));
+        RWKV7M_TRY(lm_may(fn, 16, {{"initial_state", initial_state},
+                                   {"final_state", final_state},
+                                   {"saved", saved}}));
+        const auto stream = static_cast<hipStream_t>(stream_);
+        if (in->B == 0) return RWKV7M_OK;
+        if (in->T == 0)
+            return final_state
+                       ? copy_or_clear(final_state, initial_state,
+                                       s.heads * in->Dk * in->Dv, stream)
+                       : RWKV7M_OK;
+        rwkv7m::GdrArgs A{};
+        RWKV7M_TRY(gdr_args(fn, in, &A));
+        RWKV7M_TRY(lm_need(fn, 16, {{"o", o}}));
+        RWKV7M_TRY(gdr_workspace_holds(fn, workspace, workspace_bytes,
+                                       gdr_workspace(in, s, false)));
+        A.s0 = initial_state;
+        A.o = o;
+        A.s_t = final_state;
+        A.states = saved;
+        A.x = saved ? saved + s.states : nullptr;
+        A.prepared = workspace;
+        const bool bf16 = in->dtype == RWKV7M_DTYPE_BF16;
+        RWKV7M_TRY(hip_status("gated delta rule launch",
+                              rwkv7m::launch_gdr_prepare(bf16, false, A,
+                                                         stream)));
+        return hip_status("gated delta rule launch",
+                          rwkv7m::launch_gdr_forward(bf16, A, stream));
+    });
+}
+
+int rwkv7m_gated_delta_rule_backward(
+    const rwkv7m_gated_delta_inputs* in, const void* d_o,
+    const int64_t* d_o_stride, const float* d_final_state, const float* saved,
+    void* dq, void* dk, void* dv, void* dg, void* dbeta,
+    float* d_initial_state, void* workspace, int64_t workspace_bytes,
+    void* stream_) {
+    const char* fn = "rwkv7m_gated_delta_rule_backward";
+    return lm_guard([&]() -> int {
+        GdrSizes s;
+        RWKV7M_TRY(gdr_sizes(fn, in, &s));
+        RWKV7M_TRY(lm_may(fn, 16, {{"d_final_state", d_final_state},
+                                   {"d_initial_state", d_initial_state}}));
+        const auto stream = static_cast<hipStream_t>(stream_);
+        if (in->B == 0) return RWKV7M_OK;
+        if (in->T == 0)
+            return d_initial_state
+                       ? copy_or_clear(d_initial_state, d_final_state,
+                                       s.heads * in->Dk * in->Dv, stream)
+                       : RWKV7M_OK;
+        rwkv7m::GdrArgs A{};
+        RWKV7M_TRY(gdr_args(fn, in, &A));
+        if (d_o_stride == nullptr)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": d_o_stride is NULL");
+        RWKV7M_TRY(gdr_tensor(fn, "d_o", d_o, d_o_stride, in, in->Hv,
+                              lm_size(in->dtype), 16, &A.dout));
+        RWKV7M_TRY(lm_need(fn, 16, {{"saved", saved}, {"dq", dq}, {"dk", dk},
+                                    {"dv", dv}}));
+        RWKV7M_TRY(lm_need(fn, lm_size(in->g_dtype), {{"dg", dg}}));
+        RWKV7M_TRY(lm_need(fn, lm_size(in->beta_dtype), {{"dbeta", dbeta}}));
+        RWKV7M_TRY(gdr_workspace_holds(fn, workspace, workspace_bytes,
+                                       gdr_workspace(in, s, true)));
+        A.states = const_cast<float*>(saved);
+        A.x = A.states + s.states;
+        A.ds_t = d_final_state;
+        A.ds0 = d_initial_state;
+        A.dq = dq;
+        A.dk = dk;
+        A.dv = dv;
+        A.dg = dg;
+        A.dbeta = dbeta;
+        char* at = static_cast<char*>(workspace);
+        A.prepared = at;
+        at += s.prepared;
+        A.dstates = reinterpret_cast<float*>(at);
+        A.dr = A.dstates + s.states;
+        if (in->Hv > in->Hk) {
+            A.dq_part = A.dr + s.x;
+            A.dk_part = A.dq_part + in->B * in->T * in->Hv * in->Dk;
+        }
+        const bool bf16 = in->dtype == RWKV7M_DTYPE_BF16;
+        RWKV7M_TRY(hip_status(
+            "gated delta rule backward launch",
+            rwkv7m::launch_gdr_prepare(bf16, true, A, stream)));
+        RWKV7M_TRY(hip_status("gated delta rule backward launch",
+                              rwkv7m::launch_gdr_backward(bf16, A, stream)));
+        return hip_status("gated delta rule gradients launch",
+                          rwkv7m::launch_gdr_gradients(bf16, A, stream));
+    });
+}
+
+int rwkv7m_gated_delta_step(const rwkv7m_gated_delta_inputs* in, int64_t pool,
+                            float* state, const int64_t* slots,
+                            const int64_t* lengths, int update, void* o,
+                            void* stream) {
+    const char* fn = "rwkv7m_gated_delta_step";
+    return lm_guard([&]() -> int {
+        GdrSizes s;
+        RWKV7M_TRY(gdr_sizes(fn, in, &s));
+        if (pool < 0 || (!slots && pool < in->B))
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": a pool of " +
+                            std::to_string(pool) + " states for B=" +
+                            std::to_string(in->B));
+        if (pool > (int64_t(1) << 46) / (in->Hv * in->Dk * in->Dv))
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": sizes too large");
+        RWKV7M_TRY(lm_may(fn, 8, {{"slots", slots}, {"lengths", lengths}}));
+        if (in->B == 0 || in->T == 0) return RWKV7M_OK;
+        rwkv7m::GdrTensor t[5];
+        const bool bf16 = in->dtype == RWKV7M_DTYPE_BF16;
+        RWKV7M_TRY(gdr_inputs(fn, in, bf16 ? 8 : 16, t));
+        RWKV7M_TRY(lm_need(fn, 16, {{"o", o}}));
+        if (pool > 0) RWKV7M_TRY(lm_need(fn, 16, {{"state", state}}));
+        rwkv7m::GdrStepArgs A{};
+        A.B = in->B;
+        A.T = in->T;
+        A.Hk = in->Hk;
+        A.Hv = in->Hv;
+        A.pool = pool;
+        A.Dk = int(in->Dk);
+        A.Dv = int(in->Dv);
+        A.q = t[0];
+        A.k = t[1];
+        A.v = t[2];
+        A.g = t[3];
+        A.beta = t[4];
+        A.g_bf16 = in->g_dtype == RWKV7M_DTYPE_BF16;
+        A.beta_bf16 = in->beta_dtype == RWKV7M_DTYPE_BF16;
+        A.update = update != 0;
+        A.scale = float(in->scale);
+        A.state = state;
+        A.slots = slots;
+        A.lengths = lengths;
+        A.o = o;
+        return hip_status("gated delta step launch",
+                          rwkv7m::launch_gdr_step(
+                              bf16, A, static_cast<hipStream_t>(stream)));
+    });
+}
+
+int64_t rwkv7m_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V) {
+    if (B < 0 || B > (int64_t(1) << 24) || K < 0 || K > RWKV7M_MAX_DRAFTS ||
+        V < 1 || V > (int64_t(1) << 30))
+        return -1;
+    const int64_t parts = (V + rwkv7m::kVerifyPart - 1) / rwkv7m::kVerifyPart;
+    return B * ((2 * K + 1) * parts * int64_t(sizeof(rwkv7m::LmVerifyStats)) +
+                2 * parts * 8 + 4);
+}
+
+int rwkv7m_verify_drafts(int dtype, int64_t B, int64_t K, int64_t V,
+                         int64_t target_outer_stride,
+                         int64_t target_inner_stride, const void* target,
+                         int64_t draft_outer_stride,
+                         int64_t draft_inner_stride, const void* draft,
+                         const int64_t* tokens, const float* accept,
+                         const float* sample, const int64_t* draft_lengths,
+                         double temperature, int64_t* out, int64_t* accepted,
+                         float* chances, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+    const char* fn = "rwkv7m_verify_drafts";
+    return lm_guard([&]() -> int {
+        rwkv7m::LmVerifyArgs A{};
+        int64_t rows;
+        const bool greedy = temperature == 0.0;
+        if (K < 0 || K > RWKV7M_MAX_DRAFTS)
+            return fail(K < 0 ? RWKV7M_ERR_INVALID_ARGUMENT
+                              : RWKV7M_ERR_UNSUPPORTED,
+                        std::string(fn) + ": K=" + std::to_string(K) +
+                            " drafts are not supported (0 to " +
+                            std::to_string(RWKV7M_MAX_DRAFTS) + ")");
+        RWKV7M_TRY(lm_rows(fn, "logits", dtype, B, K + 1, V,
+                           target_outer_stride, target_inner_stride, &rows,
+                           &A.tr));
+        if (greedy) draft = nullptr;
+        if (draft)
+            RWKV7M_TRY(lm_rows(fn, "draft logits", dtype, B, K, V,
+                               draft_outer_stride, draft_inner_stride, &rows,
+                               &A.dr));
+        if (!greedy) RWKV7M_TRY(lm_temperature(fn, temperature));
+        const int64_t need_ = rwkv7m_verify_drafts_workspace_bytes(B, K, V);
+        if (need_ < 0 || B * (2 * K + 1) > (int64_t(1) << 40) /
+                                 ((V + rwkv7m::kVerifyPart - 1) /
+                                  rwkv7m::kVerifyPart) / 256)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": sizes too large");
+        if (B == 0) return RWKV7M_OK;
+        RWKV7M_TRY(lm_need(fn, lm_size(dtype), {{"logits", target}}));
+        RWKV7M_TRY(lm_may(fn, lm_size(dtype), {{"draft logits", draft}}));
+        RWKV7M_TRY(lm_may(fn, 8, {{"draft_lengths", draft_lengths}}));
+        if (K > 0) {
+            RWKV7M_TRY(lm_need(fn, 8, {{"tokens", tokens}}));
+            RWKV7M_TRY(lm_need(fn, 4, {{"chances", chances}}));
+            if (!greedy) RWKV7M_TRY(lm_need(fn, 4, {{"accept", accept}}));
+        }
+        if (!greedy) RWKV7M_TRY(lm_need(fn, 4, {{"sample", sample}}));
+        RWKV7M_TRY(lm_need(fn, 8, {{"out", out}, {"accepted", accepted}}));
+        if (workspace_bytes < need_)
+            return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                        std::string(fn) + ": workspace holds " +
+                            std::to_string(workspace_bytes) +
+                            " bytes, needs " + std::to_string(need_));
+        RWKV7M_TRY(lm_need(fn, 16, {{"workspace", workspace}}));
+        A.B = B;
+        A.V = V;
+        A.K = int(K);
+        A.parts = int((V + rwkv7m::kVerifyPart - 1) / rwkv7m::kVerifyPart);
+        A.target = target;
+        A.draft = K > 0 ? draft : nullptr;
+        A.tokens = tokens;
+        A.lengths = draft_lengths;
+        A.accept = accept;
+        A.sample = sample;
+        A.c = greedy ? 1.0 : 1.4426950408889634 / temperature;
+        A.greedy = greedy;
+        A.out = out;
+        A.taken = accepted;
+        A.chance = chances;
+        A.stats = static_cast<rwkv7m::LmVerifyStats*>(workspace);
+        A.masses = reinterpret_cast<double*>(A.stats + B * (2 * K + 1) *
+                                                           A.parts);
+        A.arrived = reinterpret_cast<int*>(A.masses + B * 2 * A.parts);
+        return hip_status("verification of drafts launch",
+                          rwkv7m::launch_lm_verify(
                               dtype == RWKV7M_DTYPE_BF16, A,
                               static_cast<hipStream_t>(stream)));
     });

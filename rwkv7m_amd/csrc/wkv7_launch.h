@@ -348,6 +348,32 @@ struct LmDistillArgs {
     const float* scale;        // may be 0: 1
     int holds_unit;
 };
+// Verification of drafted tokens (lm_verify.hip): rows b * (K + 1) + i of the
+// target's logits, b * K + i of the draft's.
+constexpr int kVerifyPart = 8192;  // logits of a row a workgroup reads
+constexpr int kVerifyMostDrafts = 64;
+struct LmVerifyStats {
+    double sum;
+    float largest;
+    int id;
+};
+struct LmVerifyArgs {
+    int64_t B, V;
+    int K, parts;  // parts = ceil(V / kVerifyPart)
+    LmRows tr, dr;
+    const void *target, *draft;  // draft may be 0 (certain drafts)
+    const int64_t *tokens, *lengths;  // [B][K]; [B], may be 0 (K)
+    const float *accept, *sample;     // [B][K], [B]; greedy: may be 0
+    double c;                         // log2(e) / temperature
+    bool greedy;
+    int64_t *out, *taken;  // [B][K + 1], [B]
+    float* chance;         // [B][K]
+    LmVerifyStats* stats;  // workspaces: [B][rows][parts],
+    double* masses;        // [B][2][parts],
+    int* arrived;          // [B]
+};
+hipError_t launch_lm_verify(bool bf16, const LmVerifyArgs& A,
+                            hipStream_t stream);
 int64_t lm_norm_workspace_floats(int64_t rows, int64_t C);
 hipError_t launch_lm_norm(bool bf16, const LmNormArgs& A, hipStream_t stream);
 hipError_t launch_lm_norm_backward(bool bf16, const LmNormArgs& A,
@@ -358,6 +384,57 @@ hipError_t launch_lm_score_backward(bool bf16, const LmScoreArgs& A,
                                     hipStream_t stream);
 hipError_t launch_lm_distill(bool bf16, const LmDistillArgs& A,
                              hipStream_t stream);
+
+// Gated delta rule (gdr_*.hip).  Element (b, t, h, j) of a vector sits at b *
+// sb + t * st + h * sh + j, of a gate at b * sb + t * st + h * sh.
+constexpr int kGdrChunk = 64;  // tokens
+struct GdrTensor {
+    const void* p;
+    int64_t sb, st, sh;
+};
+struct GdrArgs {
+    int64_t B, T, Hk, Hv;
+    int Dk, Dv;
+    GdrTensor q, k, v, g, beta, dout;
+    bool g_bf16, beta_bf16;
+    float scale;
+    const float* s0;     // [B][Hv][Dv][Dk]; may be 0 (zeros)
+    void* o;             // [B][T][Hv][Dv]
+    float* s_t;          // may be 0
+    // Training: the state before each chunk, [B * Hv][chunks][DVP][DKP], and
+    // X, [B * Hv][chunks][64][DVP] (DKP and DVP: Dk and Dv rounded up, zeros
+    // behind); forward: may be 0.
+    float *states, *x;
+    const float* ds_t;   // backward: may be 0
+    float *dstates, *dr;  // workspaces of the shapes of states and x
+    float *dq_part, *dk_part;  // workspaces [B][T][Hv][Dk] where Hv > Hk
+    void *dq, *dk, *dv, *dg, *dbeta;  // contiguous
+    float* ds0;          // may be 0
+    void* prepared;      // gdr_prepared_bytes for each head and chunk
+};
+int gdr_dkp(int Dk);
+int gdr_dvp(int Dv);
+int64_t gdr_prepared_bytes(bool bf16);
+hipError_t launch_gdr_prepare(bool bf16, bool backward, const GdrArgs& A,
+                              hipStream_t stream);
+hipError_t launch_gdr_forward(bool bf16, const GdrArgs& A, hipStream_t stream);
+hipError_t launch_gdr_backward(bool bf16, const GdrArgs& A,
+                               hipStream_t stream);
+hipError_t launch_gdr_gradients(bool bf16, const GdrArgs& A,
+                                hipStream_t stream);
+// T tokens at a time on a pool of states, updated in place.
+struct GdrStepArgs {
+    int64_t B, T, Hk, Hv, pool;
+    int Dk, Dv;
+    GdrTensor q, k, v, g, beta;
+    bool g_bf16, beta_bf16, update;
+    float scale;
+    float* state;            // [pool][Hv][Dv][Dk]
+    const int64_t *slots, *lengths;  // [B]; may be 0
+    void* o;
+};
+hipError_t launch_gdr_step(bool bf16, const GdrStepArgs& A,
+                           hipStream_t stream);
 
 // One token (T = 1) for N = 64 without checkpoints; s_t may alias s0.
 hipError_t launch_decode(const SeqFwdArgs& p, hipStream_t stream);

@@ -95,6 +95,13 @@ EXPORTED_SYMBOLS = (
     "rwkv7m_token_logprobs_backward",
     "rwkv7m_distill_loss",
     "rwkv7m_distill_loss_backward",
+    "rwkv7m_verify_drafts_workspace_bytes",
+    "rwkv7m_verify_drafts",
+    "rwkv7m_gated_delta_workspace_bytes",
+    "rwkv7m_gated_delta_saved_floats",
+    "rwkv7m_gated_delta_rule",
+    "rwkv7m_gated_delta_rule_backward",
+    "rwkv7m_gated_delta_step",
 )
 
 LAYOUTS = ("tbhn", "bthn")
@@ -219,10 +226,22 @@ def load_library(path: str | None = None):
                 ("distill_loss", [i32] * 2 + [i64] * 6 + [vp] * 4 + [f64] +
                  [vp] * 4),
                 ("distill_loss_backward", [i32] * 2 + [i64] * 6 + [vp] * 4 +
-                 [f64, vp, i32, vp, vp])):
+                 [f64, vp, i32, vp, vp]),
+                ("verify_drafts", [i32] + [i64] * 5 + [vp] + [i64] * 2 +
+                 [vp] * 5 + [f64] + [vp] * 4 + [i64, vp]),
+                ("gated_delta_rule", [vp] * 6 + [i64, vp]),
+                ("gated_delta_rule_backward", [vp] * 12 + [i64, vp]),
+                ("gated_delta_step", [vp, i64] + [vp] * 3 + [i32] +
+                 [vp] * 2)):
             fn = getattr(lib, "rwkv7m_" + name)
             fn.restype = i32
             fn.argtypes = args
+        lib.rwkv7m_verify_drafts_workspace_bytes.restype = i64
+        lib.rwkv7m_verify_drafts_workspace_bytes.argtypes = [i64] * 3
+        lib.rwkv7m_gated_delta_workspace_bytes.restype = i64
+        lib.rwkv7m_gated_delta_workspace_bytes.argtypes = [vp, i32]
+        lib.rwkv7m_gated_delta_saved_floats.restype = i64
+        lib.rwkv7m_gated_delta_saved_floats.argtypes = [vp]
         if path is None:
             _lib = lib
         return lib

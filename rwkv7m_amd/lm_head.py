@@ -7,14 +7,16 @@ The end of the model and what is made of its logits:
   alternatives, for scoring, for a decode step's report and, being
   differentiable, for training on them;
 * ``distill_loss``: the distillation loss from a teacher's top logits, whose
-  gradient is formed in the same pass over the logits.
+  gradient is formed in the same pass over the logits;
+* ``verify_drafts``: which of a sequence's drafted tokens the model takes, and
+  the token behind them, from given random numbers.
 
-The head's product between the first and the other two is a plain GEMM and
+The head's product between the first and the others is a plain GEMM and
 stays the caller's (``x @ head.T``).  Each is one or two HIP kernels
 (``kernels/lm_head_hip.py``); tensors are on the GPU, activations and logits
 bf16 or fp32, and every sum is held in fp32 or more.  Gradients are first
 order and reverse mode: a second derivative or a forward-mode tangent raises.
-``examples/distill_and_score.py`` runs the three together.
+``examples/distill_and_score.py`` runs the first three together.
 """
 
 from __future__ import annotations
@@ -36,6 +38,12 @@ class TokenLogprobs(NamedTuple):
 class DistillLoss(NamedTuple):
     loss: torch.Tensor        # fp32 scalar, differentiable in the logits
     row_losses: torch.Tensor  # [...] fp32, each position's, no gradient
+
+
+class VerifiedDrafts(NamedTuple):
+    tokens: torch.Tensor    # [B, K + 1] int64: the drafts taken, one more, -1
+    accepted: torch.Tensor  # [B] int64, how many drafts were taken
+    chances: torch.Tensor   # [B, K] fp32, each draft's chance to be taken
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
@@ -87,5 +95,39 @@ def distill_loss(logits, teacher_ids, teacher_logits, weight=None,
         logits, teacher_ids, teacher_logits, weight, temperature))
 
 
-__all__ = ["DistillLoss", "TokenLogprobs", "distill_loss", "layer_norm",
-           "token_logprobs"]
+def verify_drafts(logits, draft_tokens, draft_logits=None,
+                  accept_uniforms=None, sample_uniforms=None,
+                  draft_lengths=None,
+                  temperature: float = 1.0) -> VerifiedDrafts:
+    """Verify drafted tokens (``draft_tokens`` ``[B, K]`` int64 or int32, K at
+    most 64) against a model's ``logits`` ``[B, K + 1, V]``, row i those that
+    follow the first i drafts, so that what is emitted is distributed as the
+    model's own samples are.
+
+    With ``p = softmax(logits / temperature)`` and ``q = softmax(draft_logits
+    / temperature)`` (``[B, K, V]``, the dtype of ``logits``; None where the
+    drafts are certain, found by lookup, not drawn), draft x of a position is
+    taken while ``accept_uniforms * q(x) < p(x)``; behind the ``accepted``
+    ones a token is drawn from ``max(p - q, 0)`` of the first position not
+    taken, or from the last row's ``p`` where all were, by ``sample_uniforms``
+    along the running sum over the vocabulary.  ``accept_uniforms`` ``[B,
+    K]`` and ``sample_uniforms`` ``[B]`` are fp32, from 0 to below 1; they are
+    compared in float64.  ``draft_lengths`` ``[B]`` (int64 or int32) gives
+    sequences with fewer drafts than K; rows past them are not read.
+
+    ``temperature=0.0`` is greedy: a draft is taken where it is the likeliest
+    token (the lowest id of equal ones), which is also the one emitted behind
+    them; ``draft_logits`` and the random numbers are not looked at.
+
+    ``tokens`` holds the drafts taken, the token drawn, then -1.  ``accepted +
+    1`` is the number of tokens by which the sequence goes on: the
+    ``lengths`` of ``gated_delta_step``.  A token is -1 where its row has no
+    distribution (it, or the draft's, holds NaN or +inf, or nothing above
+    -inf); chances of such rows are NaN.  Nothing here has a gradient."""
+    return VerifiedDrafts(*load_binding().verify_drafts(
+        logits, draft_tokens, draft_logits, accept_uniforms, sample_uniforms,
+        draft_lengths, temperature))
+
+
+__all__ = ["DistillLoss", "TokenLogprobs", "VerifiedDrafts", "distill_loss",
+           "layer_norm", "token_logprobs", "verify_drafts"]
