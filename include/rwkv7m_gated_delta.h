@@ -62,7 +62,8 @@ int64_t rwkv7m_gated_delta_workspace_bytes(const rwkv7m_gated_delta_inputs *in,
 int64_t rwkv7m_gated_delta_saved_floats(const rwkv7m_gated_delta_inputs *in);
 
 /* o [B][T][Hv][Dv]; initial_state [B][Hv][Dv][Dk] or NULL (zeros); final_state
- * the same or NULL (not wanted); saved NULL, or what the backward takes. */
+ * the same or NULL (not wanted); saved NULL, or what the backward takes (the
+ * workspace is then not needed). */
 int rwkv7m_gated_delta_rule(const rwkv7m_gated_delta_inputs *in,
                             const float *initial_state, void *o,
                             float *final_state, float *saved, void *workspace,

@@ -1,13 +1,10 @@
-// The gated delta rule's recurrence backwards over chunks: the cotangent D of
-// the state after each chunk, and dR, from which gdr_gradients.hip forms the
-// gradients, chunk by chunk.
+// The gated delta rule's recurrence backwards over chunks (gdr_chain.h has the
+// division of work): the cotangent D of the state after each chunk, and dR,
+// from which gdr_gradients.hip forms the gradients, chunk by chunk.
 //
 //   dX = scale P^T dO + 2^(G_L - G) (K D^T),  dR = T^T dX
 //   D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K
-//
-// As in the forward a wave owns 16 rows of D for the whole sequence and needs
-// nothing from another one.
-#include "gdr_common.h"
+#include "gdr_chain.h"
 
 namespace rwkv7m {
 namespace {
@@ -15,74 +12,47 @@ namespace {
 using namespace gdr;
 
 template <typename E, int KT>
-struct BwdShared {
-    Rows64<kIn<E>, KT> k, q;
-};
-
-template <typename E, int KT>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(2 * BRING)
 gdr_backward_kernel(const GdrArgs A, int parts) {
     constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
     extern __shared__ char lds_raw[];
-    auto& L = *reinterpret_cast<BwdShared<E, KT>*>(lds_raw);
     const Place at_ = place(blockIdx.x, parts);
     const int64_t head = at_.head;
     if (head >= A.B * A.Hv) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    const int64_t b = head / A.Hv, h = head % A.Hv;
     const int64_t chunks = (A.T + C - 1) / C;
     const int DVP = (A.Dv + 31) / 32 * 32;
     const int v0 = 64 * at_.part + 16 * wave, v = v0 + r;  // the lane's row
     const bool has = v0 < DVP, on = v < A.Dv;
-    const auto* prepared =
-        static_cast<const Prepared<NC>*>(A.prepared) + head * chunks;
 
     f32x4_t D[2 * KT];  // D(D^T): k = 16 kb + 4q + e, v = r
 #pragma unroll
     for (int kb = 0; kb < 2 * KT; ++kb) {
         const int k = 16 * kb + 4 * q;
         D[kb] = zero4();
-        if (A.ds_t && on && k < A.Dk)
+        if (A.ds_t && wave < 4 && on && k < A.Dk)
             D[kb] = four(A.ds_t + (head * A.Dv + v) * A.Dk + k);
     }
-    const E* kp = at<E>(A.k, b, hk, 0);
-    const E* qp = at<E>(A.q, b, hk, 0);
-    const E* dop = at<E>(A.dout, b, h, 0) + v;
 
-    Staged<E, KT> ks, qs;
-    E dn[16], dcur[16];
-    const auto fetch = [&](int64_t c) {
-        const int64_t t0 = c * C;
-        const int valid = int(A.T - t0 < C ? A.T - t0 : C);
-        ks.load(kp + t0 * A.k.st, A.k.st, valid, A.Dk);
-        qs.load(qp + t0 * A.q.st, A.q.st, valid, A.Dk);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = 16 * (i >> 2) + 4 * q + (i & 3);
-            dn[i] = on && t < valid ? dop[(t0 + t) * A.dout.st] : E(0);
-        }
-    };
-    fetch(chunks - 1);
-    for (int64_t c = chunks - 1; c >= 0; --c) {
-        __syncthreads();
-        ks.store(L.k);
-        qs.store(L.q);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dcur[i] = dn[i];
-        __syncthreads();
-        if (c > 0) fetch(c - 1);
-        if (!has) continue;
-        const Prepared<NC>& M = prepared[c];
+    OwnColumn<E, KT> column(A, A.dout, b, h, v, wave < 4);
+    column.fetch(chunks - 1, lane);
 
+    chain<E, KT>(
+        A, A.dout,
+        static_cast<const Prepared<NC>*>(A.prepared) + head * chunks, head,
+        64 * at_.part, chunks - 1, -1, chunks,
+        reinterpret_cast<ChainChunk<E, KT>*>(lds_raw),
+        [&](const ChainChunk<E, KT>& L, int64_t c) {
+        if (!has) return;
         float* keep = A.dstates + ((head * chunks + c) * DVP + v) * DKP;
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb)
             *reinterpret_cast<f32x4_t*>(keep + 16 * kb + 4 * q) = D[kb];
 
         f32x4_t dO[4], dX[4], dR[4];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dO[i >> 2][i & 3] = load_f(&dcur[i]);
+        column.take(L, c - 1, wave, lane, dO);
         // dX: t = 4q + e, v = r
         {
             Frag<NI> f[2];
@@ -94,9 +64,8 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                 dX[tb] = zero4();
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
-                    if (image_has(true, tb, p))
-                        mul(dX[tb], image<NC>(M.p, image_at(true, tb, p), lane),
-                            f[p]);
+                    if (holds(true, tb, p))
+                        mul(dX[tb], L.p.columns(tb, p, lane), f[p]);
             }
         }
         {
@@ -111,7 +80,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                 for (int p = 0; p < KT; ++p)
                     mul(acc, L.k.rows(tb, p, lane), Df[p]);
                 dX[tb] = A.scale * dX[tb] +
-                         four(M.last + 16 * tb + 4 * q) * acc;
+                         four(L.last + 16 * tb + 4 * q) * acc;
             }
         }
         {
@@ -124,9 +93,8 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                 dR[tb] = zero4();
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
-                    if (image_has(true, tb, p))
-                        mul(dR[tb], image<NC>(M.t, image_at(true, tb, p), lane),
-                            f[p]);
+                    if (holds(true, tb, p))
+                        mul(dR[tb], L.t.columns(tb, p, lane), f[p]);
             }
         }
         float* to = A.dr + (head * chunks + c) * C * DVP + v;
@@ -134,13 +102,13 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
         for (int i = 0; i < 16; ++i)
             to[(16 * (i >> 2) + 4 * q + (i & 3)) * DVP] = dR[i >> 2][i & 3];
 
-        const float whole = M.first[C - 1];
+        const float whole = L.first[C - 1];
         Frag<NC> of[2], rf[2];
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
-            const f32x4_t first = four(M.first + 16 * tb + 4 * q);
+            const f32x4_t first = four(L.first + 16 * tb + 4 * q);
             dO[tb] *= A.scale * first;
-            dR[tb] *= -(first * four(M.beta + 16 * tb + 4 * q));
+            dR[tb] *= -(first * four(L.beta + 16 * tb + 4 * q));
         }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -156,8 +124,8 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                 mul(D[kb], L.k.columns(kb, p, lane), rf[p]);
             }
         }
-    }
-    if (A.ds0 && on) {
+    });
+    if (A.ds0 && wave < 4 && on) {
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb) {
             const int k = 16 * kb + 4 * q;
@@ -171,14 +139,14 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
 template <typename E, int KT>
 hipError_t launch(const GdrArgs& A, hipStream_t stream) {
     const auto kernel = gdr_backward_kernel<E, KT>;
-    const int lds = int(sizeof(BwdShared<E, KT>));
+    const int lds = int(kBuffers<E, KT> * sizeof(ChainChunk<E, KT>));
     const hipError_t e = hipFuncSetAttribute(
         reinterpret_cast<const void*>(kernel),
         hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     const int parts = (gdr_dvp(A.Dv) + 63) / 64;
-    hipLaunchKernelGGL(kernel, dim3(places(A.B * A.Hv, parts)), dim3(NT), lds,
-                       stream, A, parts);
+    hipLaunchKernelGGL(kernel, dim3(places(A.B * A.Hv, parts)),
+                       dim3(2 * BRING), lds, stream, A, parts);
     return hipGetLastError();
 }
 

@@ -1,0 +1,218 @@
+// What the gated delta rule's two recurrences over chunks share
+// (gdr_forward.hip, gdr_backward.hip).
+//
+// A recurrence acts on each row of the state by itself (row i uses only
+// element i of v or do), so a wave owns 16 rows, all of the state's columns,
+// in accumulator registers for the whole sequence, and needs nothing from
+// another wave.  Four such waves make a workgroup, with four more that bring
+// what a chunk needs (K, Q, T, P, the gates, V or dO) from memory through their
+// registers to LDS, one chunk ahead of its use and two ahead with their loads.
+// The owning waves then wait for no load at all: where they brought their own
+// operands, each wait for one was also a wait for every store before it, and a
+// chunk took 14 us.
+#pragma once
+
+#include <type_traits>
+
+#include "gdr_common.h"
+
+namespace rwkv7m {
+namespace gdr {
+
+constexpr int BRING = 256;  // threads that bring, as many as own rows
+
+// 64 columns of a chunk's V or dO.
+template <typename E>
+struct Columns;
+template <>
+struct Columns<bf16_t> {
+    Rows<1, 2> x;
+    // [16 tb + 4q + e][16 wave + r]
+    __device__ __forceinline__ f32x4_t values(int tb, int wave,
+                                              int lane) const {
+        return x.values(16 * tb, wave, lane);
+    }
+    __device__ __forceinline__ void put(int row, int col,
+                                        const Eight<bf16_t>& v) {
+        *reinterpret_cast<u32x4_t*>(&x.x[0][row][col]) = v.a;
+    }
+};
+template <>
+struct Columns<float> {
+    alignas(16) float x[C][68];
+    __device__ __forceinline__ f32x4_t values(int tb, int wave,
+                                              int lane) const {
+        const int r = lane & 15, q = lane >> 4;
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x[16 * tb + 4 * q + e][16 * wave + r];
+        return v;
+    }
+    __device__ __forceinline__ void put(int row, int col,
+                                        const Eight<float>& v) {
+        *reinterpret_cast<f32x4_t*>(&x[row][col]) = v.a;
+        *reinterpret_cast<f32x4_t*>(&x[row][col + 4]) = v.b;
+    }
+};
+
+struct NoColumns {};
+
+// (fp32 at 128 columns leaves no room for the 64 columns in LDS)
+template <typename E, int KT>
+constexpr bool kColumns = sizeof(E) == 2 || KT < 4;
+
+template <typename E, int KT>
+struct ChainChunk {
+    Rows<kIn<E>, KT> k, q;
+    Rows<kMade<E>, 2> t, p;
+    std::conditional_t<kColumns<E, KT>, Columns<E>, NoColumns> v;
+    alignas(16) float first[C], last[C], beta[C];
+};
+static_assert(sizeof(ChainChunk<float, 4>) <= 160 * 1024, "");
+// One chunk ahead in a second buffer where two fit.
+template <typename E, int KT>
+constexpr int kBuffers = 2 * sizeof(ChainChunk<E, KT>) <= 160 * 1024 ? 2 : 1;
+
+// The owning lane's column of V or dO: from LDS, or brought by itself, a chunk
+// ahead of its use.
+template <typename E, int KT>
+struct OwnColumn {
+    const E* base;  // (token 0)
+    int64_t stride, T;
+    bool on;
+    E next[16];
+
+    __device__ __forceinline__ OwnColumn(const GdrArgs& A, const GdrTensor& x,
+                                         int64_t b, int64_t h, int v, bool own)
+        : base(at<E>(x, b, h, 0) + v), stride(x.st), T(A.T),
+          on(own && v < A.Dv) {}
+    __device__ __forceinline__ void fetch(int64_t c, int lane) {
+        if constexpr (!kColumns<E, KT>)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int64_t t =
+                    c * C + 16 * (i >> 2) + 4 * (lane >> 4) + (i & 3);
+                next[i] = on && t >= 0 && t < T ? base[t * stride] : E(0);
+            }
+    }
+    // The chunk's values, with the loads of chunk `then`, if any, begun.
+    __device__ __forceinline__ void take(const ChainChunk<E, KT>& L, int64_t then,
+                                         int wave, int lane,
+                                         f32x4_t (&x)[4]) {
+        if constexpr (kColumns<E, KT>) {
+#pragma unroll
+            for (int tb = 0; tb < 4; ++tb) x[tb] = L.v.values(tb, wave, lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = load_f(&next[i]);
+            fetch(then, lane);
+        }
+    }
+};
+
+// A bringing thread's share of a chunk.
+template <typename E, int KT>
+struct Bring {
+    static constexpr int NC = kMade<E>;
+    Staged<E, KT, BRING> k, q;
+    u32x4_t t[2 * NC], p[2 * NC];
+    Eight<E> v[2];
+    float first, last, beta;
+
+    // (v0: the workgroup's first column; x: V or dO)
+    __device__ __forceinline__ void load(const GdrArgs& A, const GdrTensor& x,
+                                         const Prepared<NC>& M, int64_t b,
+                                         int64_t h, int64_t hk, int64_t c,
+                                         int v0, int thread) {
+        const int64_t t0 = c * C;
+        const int valid = int(A.T - t0 < C ? A.T - t0 : C);
+        k.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, thread);
+        q.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, thread);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
+            if constexpr (kColumns<E, KT>) {
+                v[i].clear();
+                if (row < valid && v0 + col < A.Dv)
+                    v[i].load(at<E>(x, b, h, t0 + row) + v0 + col);
+            }
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                t[i * NC + n] = u32x4_t{0, 0, 0, 0};
+                p[i * NC + n] = u32x4_t{0, 0, 0, 0};
+                if (row >= 32 || col < 32) {
+                    t[i * NC + n] =
+                        *reinterpret_cast<const u32x4_t*>(&M.t[n][row][col]);
+                    p[i * NC + n] =
+                        *reinterpret_cast<const u32x4_t*>(&M.p[n][row][col]);
+                }
+            }
+        }
+        first = M.first[thread & 63];
+        last = M.last[thread & 63];
+        beta = M.beta[thread & 63];
+    }
+    __device__ __forceinline__ void store(ChainChunk<E, KT>& L,
+                                          int thread) const {
+        k.store(L.k, thread);
+        q.store(L.q, thread);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
+            if constexpr (kColumns<E, KT>) L.v.put(row, col, v[i]);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                *reinterpret_cast<u32x4_t*>(&L.t.x[n][row][col]) =
+                    t[i * NC + n];
+                *reinterpret_cast<u32x4_t*>(&L.p.x[n][row][col]) =
+                    p[i * NC + n];
+            }
+        }
+        if (thread < C) {
+            L.first[thread] = first;
+            L.last[thread] = last;
+            L.beta[thread] = beta;
+        }
+    }
+};
+
+// The loop of both: chunks first, first + step, .. (n of them).  own(L, c) by
+// the threads that own rows, with the chunk in L.
+template <typename E, int KT, typename F>
+__device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
+                                      const Prepared<kMade<E>>* M, int64_t head,
+                                      int v0, int64_t first, int64_t step,
+                                      int64_t n, ChainChunk<E, KT>* L, F own) {
+    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    constexpr int NB = kBuffers<E, KT>;
+    if (threadIdx.x >= BRING) {
+        const int thread = threadIdx.x - BRING;
+        Bring<E, KT> s;
+        s.load(A, x, M[first], b, h, hk, first, v0, thread);
+        s.store(L[0], thread);
+        const auto ahead = [&](int64_t i) {
+            const int64_t c = first + step * i;
+            if (i < n) s.load(A, x, M[c], b, h, hk, c, v0, thread);
+        };
+        ahead(1);
+        __syncthreads();
+        for (int64_t i = 0; i < n; ++i) {
+            if constexpr (NB == 1) __syncthreads();
+            if (i + 1 < n) {
+                s.store(L[NB == 2 ? (i + 1) & 1 : 0], thread);
+                ahead(i + 2);
+            }
+            __syncthreads();
+        }
+    } else {
+        __syncthreads();
+        for (int64_t i = 0; i < n; ++i) {
+            own(L[NB == 2 ? i & 1 : 0], first + step * i);
+            if constexpr (NB == 1) __syncthreads();
+            __syncthreads();
+        }
+    }
+}
+
+}  // namespace gdr
+}  // namespace rwkv7m

@@ -37,7 +37,6 @@ namespace rwkv7m {
 namespace gdr {
 
 constexpr int C = kGdrChunk;
-constexpr int NT = 256;  // threads of the chunk kernels: 4 waves
 constexpr double kLog2e = 1.4426950408889634;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -150,12 +149,12 @@ struct Eight<float> {
     }
 };
 
-// A chunk's 64 rows of DKP = 32 KT places in LDS, NP planes.  The pitch puts
-// 16 rows' 8-byte pieces on 64 different banks.
-template <int NP, int KT>
-struct Rows64 {
+// R rows of 32 KT places in LDS, NP planes.  The pitch puts 16 rows' 8-byte
+// pieces on 64 different banks.
+template <int NP, int KT, int R = C>
+struct Rows {
     static constexpr int pitch = 32 * KT + 8;
-    bf16_t x[NP][C][pitch];
+    bf16_t x[NP][R][pitch];
 
     // Left operand of rows 16 tb .., places 32 p .. (natural).
     __device__ __forceinline__ Frag<NP> rows(int tb, int p, int lane) const {
@@ -225,18 +224,31 @@ struct Rows64 {
     }
 };
 
-// A thread's share of a chunk's rows on their way to LDS.
-template <typename E, int KT>
+// Four floats as planes at four adjoining places.
+template <int NP, int KT, int R>
+__device__ __forceinline__ void put4(Rows<NP, KT, R>& to, int row, int col,
+                                     const f32x4_t& x) {
+    uint32_t lo[NP], hi[NP];
+    split2<NP>(x[0], x[1], lo);
+    split2<NP>(x[2], x[3], hi);
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+        *reinterpret_cast<uint2*>(&to.x[n][row][col]) =
+            make_uint2(lo[n], hi[n]);
+}
+
+// The share of a chunk's rows of one of `T` threads, on its way to LDS.
+template <typename E, int KT, int T>
 struct Staged {
-    static constexpr int per_row = 4 * KT, n = C * per_row / NT;
+    static constexpr int per_row = 4 * KT, n = C * per_row / T;
     Eight<E> v[n];
 
     // Rows 0 .. valid - 1 of `base`, `dim` places each.
     __device__ __forceinline__ void load(const E* base, int64_t stride,
-                                         int valid, int dim) {
+                                         int valid, int dim, int thread) {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int u = i * NT + int(threadIdx.x);
+            const int u = i * T + thread;
             const int row = u / per_row, col = 8 * (u % per_row);
             if (row < valid && col < dim)
                 v[i].load(base + row * stride + col);
@@ -244,10 +256,11 @@ struct Staged {
                 v[i].clear();
         }
     }
-    __device__ __forceinline__ void store(Rows64<kIn<E>, KT>& to) const {
+    __device__ __forceinline__ void store(Rows<kIn<E>, KT>& to,
+                                          int thread) const {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int u = i * NT + int(threadIdx.x);
+            const int u = i * T + thread;
             const int row = u / per_row, col = 8 * (u % per_row);
             const auto f = v[i].planes();
 #pragma unroll
@@ -259,38 +272,20 @@ struct Staged {
 
 // --- what gdr_prepare.hip leaves for a chunk of a head ------------------------
 
-// Lower triangular 64 x 64 matrices as operands: of the left operand's row
-// block tb and pair p of 32 places only those that hold anything, six.
-// Transposed ones hold row blocks of the transpose.
-__device__ __forceinline__ constexpr bool image_has(bool transposed, int tb,
-                                                    int p) {
-    return transposed ? 2 * p + 1 >= tb : 2 * p <= tb;
-}
-__device__ __forceinline__ constexpr int image_at(bool transposed, int tb,
-                                                  int p) {
-    int at = 0;
-    for (int t = 0; t < 4; ++t)
-        for (int u = 0; u < 2; ++u) {
-            if (t == tb && u == p) return at;
-            at += image_has(transposed, t, u);
-        }
-    return at;
-}
-
+// T and P in planes, row by row, and the gates.  The upper right quarters are
+// zeros that nothing reads.
 template <int NC>
 struct Prepared {
-    u32x4_t t[6][NC][64], p[6][NC][64];  // T and P (or their transposes)
+    bf16_t t[NC][C][C], p[NC][C][C];
     double G[C];                          // base 2
     float first[C], last[C], beta[C];     // 2^G, 2^(G_L - G)
 };
 
-template <int NC>
-__device__ __forceinline__ Frag<NC> image(const u32x4_t (&m)[6][NC][64], int at,
-                                          int lane) {
-    Frag<NC> f;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) f.p[n] = m[at][n][lane];
-    return f;
+// Does row block tb of such a matrix (or of its transpose) hold anything in
+// the 32 places of pair p?
+__device__ __forceinline__ constexpr bool holds(bool transposed, int tb,
+                                                int p) {
+    return transposed ? 2 * p + 1 >= tb : 2 * p <= tb;
 }
 
 __device__ __forceinline__ f32x4_t four(const float* p) {

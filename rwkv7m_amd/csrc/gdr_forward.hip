@@ -1,95 +1,49 @@
 // The gated delta rule's recurrence over chunks (gdr_common.h has the
-// formulas): outputs, and the state before each chunk where a backward
-// follows.
-//
-// The recurrence acts on each row of the state by itself (row i uses only
-// element i of v, and yields only that of o), so a wave owns 16 rows, all of
-// S^T's columns, in accumulator registers for the whole sequence, and needs
-// nothing from another wave: K and Q of the chunk come to LDS for the four
-// waves of a workgroup, T and P as operands from memory.
-#include "gdr_common.h"
+// formulas, gdr_chain.h the division of work): outputs, and the state before
+// each chunk and X where a backward follows.
+#include "gdr_chain.h"
 
 namespace rwkv7m {
 namespace {
 
 using namespace gdr;
 
-template <typename E, int KT>
-struct FwdShared {
-    Rows64<kIn<E>, KT> k, q;
-};
-
-// V[16 tb + 4q + e][v] of a chunk, v = the lane's column.
-template <typename E>
-struct Column {
-    E x[16];
-    __device__ __forceinline__ void load(const E* base, int64_t stride,
-                                         int valid, bool on, int q) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = 16 * (i >> 2) + 4 * q + (i & 3);
-            x[i] = on && t < valid ? base[t * stride] : E(0);
-        }
-    }
-    __device__ __forceinline__ float get(int tb, int e) const {
-        return load_f(&x[4 * tb + e]);
-    }
-};
-
 template <typename E, int KT, bool TRAIN>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(2 * BRING)
 gdr_forward_kernel(const GdrArgs A, int parts) {
     constexpr int NC = kMade<E>, DKP = 32 * KT;
     extern __shared__ char lds_raw[];
-    auto& L = *reinterpret_cast<FwdShared<E, KT>*>(lds_raw);
     const Place at_ = place(blockIdx.x, parts);
     const int64_t head = at_.head;
     if (head >= A.B * A.Hv) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    const int64_t b = head / A.Hv, h = head % A.Hv;
     const int64_t chunks = (A.T + C - 1) / C;
     const int DVP = (A.Dv + 31) / 32 * 32;
     const int v0 = 64 * at_.part + 16 * wave, v = v0 + r;  // the lane's row
     const bool has = v0 < DVP, on = v < A.Dv;
-    const auto* prepared =
-        static_cast<const Prepared<NC>*>(A.prepared) + head * chunks;
 
     f32x4_t S[2 * KT];  // D(S^T): k = 16 kb + 4q + e, v = r
 #pragma unroll
     for (int kb = 0; kb < 2 * KT; ++kb) {
         const int k = 16 * kb + 4 * q;
         S[kb] = zero4();
-        if (A.s0 && on && k < A.Dk)
+        if (A.s0 && wave < 4 && on && k < A.Dk)
             S[kb] = four(A.s0 + (head * A.Dv + v) * A.Dk + k);
     }
-    const E* kp = at<E>(A.k, b, hk, 0);
-    const E* qp = at<E>(A.q, b, hk, 0);
-    const E* vp = at<E>(A.v, b, h, 0) + v;
     E* op = static_cast<E*>(A.o) + (b * A.T * A.Hv + h) * A.Dv;
+    OwnColumn<E, KT> column(A, A.v, b, h, v, wave < 4);
+    column.fetch(0, lane);
 
-    Staged<E, KT> ks, qs;
-    Column<E> vs, vn;
-    const auto fetch = [&](int64_t c) {
+    chain<E, KT>(
+        A, A.v, static_cast<const Prepared<NC>*>(A.prepared) + head * chunks,
+        head, 64 * at_.part, 0, 1, chunks,
+        reinterpret_cast<ChainChunk<E, KT>*>(lds_raw),
+        [&](const ChainChunk<E, KT>& L, int64_t c) {
+        if (!has) return;
         const int64_t t0 = c * C;
         const int valid = int(A.T - t0 < C ? A.T - t0 : C);
-        ks.load(kp + t0 * A.k.st, A.k.st, valid, A.Dk);
-        qs.load(qp + t0 * A.q.st, A.q.st, valid, A.Dk);
-        vn.load(vp + t0 * A.v.st, A.v.st, valid, on, q);
-    };
-    fetch(0);
-    for (int64_t c = 0; c < chunks; ++c) {
-        const int64_t t0 = c * C;
-        const int valid = int(A.T - t0 < C ? A.T - t0 : C);
-        __syncthreads();
-        ks.store(L.k);
-        qs.store(L.q);
-        vs = vn;
-        __syncthreads();
-        if (c + 1 < chunks) fetch(c + 1);
-        if (!has) continue;
-        const Prepared<NC>& M = prepared[c];
-
         Frag<NC> Sf[KT];
 #pragma unroll
         for (int p = 0; p < KT; ++p) Sf[p] = split8<NC>(S[2 * p], S[2 * p + 1]);
@@ -100,20 +54,20 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                 *reinterpret_cast<f32x4_t*>(to + 16 * kb + 4 * q) = S[kb];
         }
         // R = beta (V - 2^G (K S^T)), t = 4q + e, v = r
-        f32x4_t R[4], X[4];
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-            f32x4_t acc = zero4();
-#pragma unroll
-            for (int p = 0; p < KT; ++p) mul(acc, L.k.rows(tb, p, lane), Sf[p]);
-            const f32x4_t first = four(M.first + 16 * tb + 4 * q);
-            const f32x4_t beta = four(M.beta + 16 * tb + 4 * q);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                R[tb][e] = beta[e] * (vs.get(tb, e) - first[e] * acc[e]);
-        }
-        // X = T R
+        f32x4_t X[4];
         {
+            f32x4_t R[4], V[4];
+            column.take(L, c + 1, wave, lane, V);
+#pragma unroll
+            for (int tb = 0; tb < 4; ++tb) {
+                f32x4_t acc = zero4();
+#pragma unroll
+                for (int p = 0; p < KT; ++p)
+                    mul(acc, L.k.rows(tb, p, lane), Sf[p]);
+                R[tb] = four(L.beta + 16 * tb + 4 * q) *
+                        (V[tb] - four(L.first + 16 * tb + 4 * q) * acc);
+            }
+            // X = T R
             Frag<NC> Rf[2];
 #pragma unroll
             for (int p = 0; p < 2; ++p) Rf[p] = split8<NC>(R[2 * p], R[2 * p + 1]);
@@ -122,9 +76,8 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                 X[tb] = zero4();
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
-                    if (image_has(false, tb, p))
-                        mul(X[tb], image<NC>(M.t, image_at(false, tb, p), lane),
-                            Rf[p]);
+                    if (holds(false, tb, p))
+                        mul(X[tb], L.t.rows(tb, p, lane), Rf[p]);
             }
         }
         if constexpr (TRAIN) {
@@ -144,12 +97,11 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
                 for (int p = 0; p < KT; ++p)
                     mul(acc, Sf[p], L.q.rows(tb, p, lane));
-                acc *= M.first[16 * tb + r];
+                acc *= L.first[16 * tb + r];
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
-                    if (image_has(false, tb, p))
-                        mul(acc, Xf[p],
-                            image<NC>(M.p, image_at(false, tb, p), lane));
+                    if (holds(false, tb, p))
+                        mul(acc, Xf[p], L.p.rows(tb, p, lane));
                 const int t = 16 * tb + r, col = v0 + 4 * q;
                 if (t < valid && col < A.Dv) {
                     E* to = op + (t0 + t) * A.Hv * A.Dv + col;
@@ -164,10 +116,10 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             }
         }
         // S^T = 2^G_L S^T + K^T (2^(G_L - G) X)
-        const float whole = M.first[C - 1];
+        const float whole = L.first[C - 1];
         Frag<NC> Xf[2];
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) X[tb] *= four(M.last + 16 * tb + 4 * q);
+        for (int tb = 0; tb < 4; ++tb) X[tb] *= four(L.last + 16 * tb + 4 * q);
 #pragma unroll
         for (int p = 0; p < 2; ++p) Xf[p] = split8<NC>(X[2 * p], X[2 * p + 1]);
 #pragma unroll
@@ -177,8 +129,8 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             for (int p = 0; p < 2; ++p)
                 mul(S[kb], L.k.columns(kb, p, lane), Xf[p]);
         }
-    }
-    if (A.s_t && on) {
+    });
+    if (A.s_t && wave < 4 && on) {
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb) {
             const int k = 16 * kb + 4 * q;
@@ -192,14 +144,14 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
 template <typename E, int KT, bool TRAIN>
 hipError_t launch(const GdrArgs& A, hipStream_t stream) {
     const auto kernel = gdr_forward_kernel<E, KT, TRAIN>;
-    const int lds = int(sizeof(FwdShared<E, KT>));
+    const int lds = int(kBuffers<E, KT> * sizeof(ChainChunk<E, KT>));
     const hipError_t e = hipFuncSetAttribute(
         reinterpret_cast<const void*>(kernel),
         hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     const int parts = (gdr_dvp(A.Dv) + 63) / 64;
-    hipLaunchKernelGGL(kernel, dim3(places(A.B * A.Hv, parts)), dim3(NT), lds,
-                       stream, A, parts);
+    hipLaunchKernelGGL(kernel, dim3(places(A.B * A.Hv, parts)),
+                       dim3(2 * BRING), lds, stream, A, parts);
     return hipGetLastError();
 }
 

@@ -11,10 +11,12 @@
 //   dg = the sum of dG from the token on,
 //   <D, S_L> = 2^G_L <D, S0> + sum_t k_t.(2^(G_L - G) X D)_t
 //
-// One workgroup a chunk and value head, all of them independent; a wave owns
-// 16 tokens.  S0 and D pass through LDS in blocks of 64 rows, whose columns are
-// operands by transposing reads; N and dP are formed in both orientations
-// (rows of the wave's tokens, and columns), so that no wave needs another's.
+// One workgroup a chunk and value head, all of them independent.  A wave owns
+// 32 tokens and a quarter of the columns of dq, left and right.  S0 and D pass
+// through LDS in blocks of 32 rows, whose columns are operands by transposing
+// reads; each operand so read serves two blocks of tokens.  The ten lower
+// blocks of N and dP are divided among the waves and meet in LDS, whose rows
+// are operands for dq and left, whose columns for right.
 #include "gdr_common.h"
 
 namespace rwkv7m {
@@ -22,24 +24,33 @@ namespace {
 
 using namespace gdr;
 
+constexpr int KQ = 4, NT = 2 * KQ * 64;  // shares of the columns; threads
+
 template <typename E, int KT>
 struct GradShared {
-    Rows64<kIn<E>, KT> k, q;
-    Rows64<kMade<E>, KT> s;  // 64 rows of S0, then of D
+    union {
+        struct {
+            Rows<kIn<E>, KT> k, q;
+        };
+        E out[2][C][32 * KT + 8];  // dq and dk, once k and q are done with
+    };
+    union {
+        struct {
+            Rows<kMade<E>, KT, 32> s, d;  // 32 rows of S0 and of D
+        };
+        struct {
+            Rows<kMade<E>, 2> n;  // N, then -beta N
+            union {
+                Rows<kMade<E>, 2> p;  // dP
+                // of q.dq, k.left, k.right, k.(first of right), behind it
+                float dots[KQ][4][C];
+            };
+        };
+    };
     double G[C];
-    float dG[C], rv[C], sums[4];
+    float first[C], last[C], beta[C], rv[C];
+    float sums[2 * KQ];
 };
-
-// Eight places 32 p + 8q + i of a row of X or dR, in planes.
-template <int NC>
-__device__ __forceinline__ Frag<NC> row8(const float* p, bool on) {
-    Eight<float> v;
-    if (on)
-        v.load(p);
-    else
-        v.clear();
-    return split8<NC>(v.a, v.b);
-}
 
 __device__ __forceinline__ void store_gate(void* p, bool bf16, int64_t i,
                                            float x) {
@@ -57,6 +68,8 @@ gdr_gradients_kernel(const GdrArgs A) {
     auto& L = *reinterpret_cast<GradShared<E, KT>*>(lds_raw);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
+    const int th = wave / KQ, kh = wave % KQ;  // tokens 32 th .., share kh
+    constexpr int KW = 2 * KT / KQ;  // the wave's tiles of 16 columns
     const int64_t chunks = (A.T + C - 1) / C;
     const int64_t id = blockIdx.x, head = id / chunks, c = id % chunks;
     const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
@@ -66,97 +79,102 @@ gdr_gradients_kernel(const GdrArgs A) {
     const Prepared<NC>& M =
         static_cast<const Prepared<NC>*>(A.prepared)[head * chunks + c];
 
-    Staged<E, KT> ks, qs;
-    ks.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk);
-    qs.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk);
-    if (threadIdx.x < C) L.G[threadIdx.x] = M.G[threadIdx.x];
-    ks.store(L.k);
-    qs.store(L.q);
-
-    f32x4_t dq[2 * KT], left[2 * KT], right[2 * KT];
-#pragma unroll
-    for (int j = 0; j < 2 * KT; ++j) dq[j] = left[j] = right[j] = zero4();
-    // (rows: token block `wave` against block j <= wave, t = r, s = 4q + e;
-    // columns: block j >= wave against `wave`, t = 4q + e, s = r)
-    f32x4_t dp_row[4], n_row[4], dp_col[4], n_col[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        dp_row[j] = n_row[j] = dp_col[j] = n_col[j] = zero4();
-    float rv = 0.f, ds = 0.f;  // dR.v of token 16 wave + r; <D, S0>
-
     const E* dop = at<E>(A.dout, b, h, t0);
     const E* vp = at<E>(A.v, b, h, t0);
     const float* x0 = A.x + (head * chunks + c) * C * DVP;
     const float* r0 = A.dr + (head * chunks + c) * C * DVP;
     const float* s0 = A.states + (head * chunks + c) * DVP * DKP;
     const float* d0 = A.dstates + (head * chunks + c) * DVP * DKP;
-    const int own = 16 * wave + r;  // the lane's token
-    E* dvp = static_cast<E*>(A.dv) + ((b * A.T + t0 + own) * A.Hv + h) * A.Dv;
-    const float beta_own = M.beta[own];
 
-    for (int v0 = 0; v0 < DVP; v0 += 64) {
-        // the block's rows of S0 and D, 8 places a thread and turn
-        constexpr int per_row = DKP / 4, turns = 64 * per_row / NT;
-        f32x4_t sv[turns], dv[turns];
+    // 32 rows of S0 and D on their way to LDS
+    constexpr int turns = 32 * DKP / 4 / NT;
+    f32x4_t sv[turns], dv[turns];
+    const auto fetch = [&](int v0) {
 #pragma unroll
         for (int i = 0; i < turns; ++i) {
-            const int u = i * NT + int(threadIdx.x);
-            const int row = v0 + u / per_row, col = 4 * (u % per_row);
-            sv[i] = dv[i] = zero4();
-            if (row < DVP) {
-                sv[i] = four(s0 + row * DKP + col);
-                dv[i] = four(d0 + row * DKP + col);
-            }
+            const int u = 4 * (i * NT + int(threadIdx.x));
+            sv[i] = four(s0 + v0 * DKP + u);
+            dv[i] = four(d0 + v0 * DKP + u);
         }
+    };
+    // places v0 + 8q + i of a row of dO, X or dR
+    const auto dout = [&](int tb, int v0) {
+        const int t = 16 * tb + r, col = v0 + 8 * q;
+        Eight<E> e;
+        e.clear();
+        if (t < valid && col < A.Dv) e.load(dop + t * A.dout.st + col);
+        return e;
+    };
+    const auto made = [&](const float* from, int tb, int v0) {
+        Eight<float> e;
+        e.load(from + (16 * tb + r) * DVP + v0 + 8 * q);
+        return e;
+    };
+    const auto planes = [&](const Eight<float>& e) {
+        return split8<NC>(e.a, e.b);
+    };
+
+    fetch(0);
+    {
+        Staged<E, KT, NT> ks, qs;
+        ks.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, threadIdx.x);
+        qs.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, threadIdx.x);
+        if (threadIdx.x < C) {
+            L.G[threadIdx.x] = M.G[threadIdx.x];
+            L.first[threadIdx.x] = M.first[threadIdx.x];
+            L.last[threadIdx.x] = M.last[threadIdx.x];
+            L.beta[threadIdx.x] = M.beta[threadIdx.x];
+        }
+        ks.store(L.k, threadIdx.x);
+        qs.store(L.q, threadIdx.x);
+    }
+
+    f32x4_t dq[2][KW], left[2][KW], right[2][KW];
 #pragma unroll
-        for (int i = 0; i < turns; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) ds += sv[i][e] * dv[i][e];
-        const auto put = [&](const f32x4_t (&x)[turns]) {
-            __syncthreads();
+        for (int j = 0; j < KW; ++j)
+            dq[i][j] = left[i][j] = right[i][j] = zero4();
+    // Blocks (tb, sb) of N and dP, t = 4q + e, s = r: with kh 0, 1, 2 one of
+    // the wave's own tokens, (0, 0), (1, 0), (1, 1) from 2 th on; with kh 3
+    // (2 + th, 0) and (2 + th, 1).
+    f32x4_t dp[2], nn[2];
 #pragma unroll
-            for (int i = 0; i < turns; ++i) {
-                const int u = i * NT + int(threadIdx.x);
-                const int row = u / per_row, col = 4 * (u % per_row);
-                uint32_t lo[NC], hi[NC];
-                split2<NC>(x[i][0], x[i][1], lo);
-                split2<NC>(x[i][2], x[i][3], hi);
-#pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    *reinterpret_cast<uint2*>(&L.s.x[n][row][col]) =
-                        make_uint2(lo[n], hi[n]);
-            }
-            __syncthreads();
-        };
-        // operands of the wave's own tokens (left or right alike)
+    for (int i = 0; i < 2; ++i) dp[i] = nn[i] = zero4();
+    float rv = 0.f, ds = 0.f;  // dR.v of token 16 (2 th + kh) + r; <D, S0>
+    const int mine = 16 * (2 * th + (kh & 1)) + r;
+    E* dvp = static_cast<E*>(A.dv) + ((b * A.T + t0 + mine) * A.Hv + h) * A.Dv;
+    const float beta_mine = M.beta[mine];
+
+    for (int v0 = 0; v0 < DVP; v0 += 32) {
+        // operands of the wave's tokens (left or right alike)
         Frag<NI> of[2];
         Frag<NC> xf[2], rf[2];
-        const auto dout = [&](int tb, int p) {
-            const int t = 16 * tb + r, col = v0 + 32 * p + 8 * q;
-            Eight<E> e;
-            if (t < valid && col < A.Dv)
-                e.load(dop + t * A.dout.st + col);
-            else
-                e.clear();
-            return e.planes();
-        };
+        {
+            Eight<E> o8[2], v8;
+            Eight<float> x8[2], r8[2];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const int col = v0 + 32 * p + 8 * q;
-            of[p] = dout(wave, p);
-            xf[p] = row8<NC>(x0 + own * DVP + col, col < DVP);
-            // dv and dR.v
-            Eight<float> dr;
-            dr.clear();
-            if (col < DVP) dr.load(r0 + own * DVP + col);
-            rf[p] = split8<NC>(dr.a, dr.b);
-            if (own < valid && col < A.Dv) {
-                Eight<E> vv;
-                vv.load(vp + own * A.v.st + col);
+            for (int i = 0; i < 2; ++i) {
+                o8[i] = dout(2 * th + i, v0);
+                x8[i] = made(x0, 2 * th + i, v0);
+                r8[i] = made(r0, 2 * th + i, v0);
+            }
+            const int col = v0 + 8 * q;
+            const bool on = kh < 2 && mine < valid && col < A.Dv;
+            v8.clear();
+            if (on) v8.load(vp + mine * A.v.st + col);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) rv += dr.get(i) * vv.get(i);
-                dr.a *= beta_own;
-                dr.b *= beta_own;
+            for (int i = 0; i < 2; ++i) {
+                of[i] = o8[i].planes();
+                xf[i] = planes(x8[i]);
+                rf[i] = planes(r8[i]);
+            }
+            Eight<float> dr = kh ? r8[1] : r8[0];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rv += dr.get(i) * v8.get(i);
+            dr.a *= beta_mine;
+            dr.b *= beta_mine;
+            if (on) {
                 if constexpr (sizeof(E) == 4) {
                     *reinterpret_cast<f32x4_t*>(dvp + col) = dr.a;
                     *reinterpret_cast<f32x4_t*>(dvp + col + 4) = dr.b;
@@ -169,178 +187,270 @@ gdr_gradients_kernel(const GdrArgs A) {
                 }
             }
         }
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j <= wave) {
+        for (int i = 0; i < turns; ++i) {
+            const int u = i * NT + int(threadIdx.x);
+            const int row = u / (DKP / 4), col = 4 * (u % (DKP / 4));
+            put4(L.s, row, col, sv[i]);
+            put4(L.d, row, col, dv[i]);
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const int col = v0 + 32 * p + 8 * q;
-                    const Frag<NC> xj =
-                        row8<NC>(x0 + (16 * j + r) * DVP + col, col < DVP);
-                    mul(dp_row[j], xj, of[p]);
-                    mul(n_row[j], xj, rf[p]);
-                }
-            }
-            if (j >= wave) {
+            for (int e = 0; e < 4; ++e) ds += sv[i][e] * dv[i][e];
+        }
+        __syncthreads();
+        if (v0 + 32 < DVP) fetch(v0 + 32);
+        if (kh == 0) {
+            mul(dp[0], of[0], xf[0]);
+            mul(nn[0], rf[0], xf[0]);
+        } else if (kh == 1) {
+            mul(dp[0], of[1], xf[0]);
+            mul(nn[0], rf[1], xf[0]);
+        } else if (kh == 2) {
+            mul(dp[0], of[1], xf[1]);
+            mul(nn[0], rf[1], xf[1]);
+        } else if (th == 0) {
+            const Frag<NI> o = dout(2, v0).planes();
+            const Frag<NC> g = planes(made(r0, 2, v0));
+            mul(dp[0], o, xf[0]);
+            mul(dp[1], o, xf[1]);
+            mul(nn[0], g, xf[0]);
+            mul(nn[1], g, xf[1]);
+        } else {
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const int col = v0 + 32 * p + 8 * q;
-                    mul(dp_col[j], dout(j, p), xf[p]);
-                    mul(n_col[j],
-                        row8<NC>(r0 + (16 * j + r) * DVP + col, col < DVP),
-                        xf[p]);
-                }
+            for (int i = 0; i < 2; ++i) {
+                const Frag<NC> x = planes(made(x0, i, v0));
+                mul(dp[i], of[1], x);
+                mul(nn[i], rf[1], x);
             }
         }
-        put(sv);
 #pragma unroll
-        for (int jb = 0; jb < 2 * KT; ++jb)
+        for (int j = 0; j < KW; ++j) {
+            const Frag<NC> f = L.s.columns_dense(kh * KW + j, 0, lane);
+            const Frag<NC> g = L.d.columns_dense(kh * KW + j, 0, lane);
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const Frag<NC> f = L.s.columns_dense(jb, p, lane);
-                mul(dq[jb], of[p], f);
-                mul(left[jb], rf[p], f);
+            for (int i = 0; i < 2; ++i) {
+                mul(dq[i][j], of[i], f);
+                mul(left[i][j], rf[i], f);
+                mul(right[i][j], xf[i], g);
             }
-        put(dv);
-#pragma unroll
-        for (int jb = 0; jb < 2 * KT; ++jb)
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-                mul(right[jb], xf[p], L.s.columns_dense(jb, p, lane));
+        }
     }
-
-    // rows' factors, t = 16 wave + 4q + e
-    const int row = 16 * wave + 4 * q;
-    const f32x4_t first = four(M.first + row), last = four(M.last + row),
-                  beta = four(M.beta + row);
-    f32x4_t klast = zero4();
+    __syncthreads();
+    // N and dP with their decays, to LDS
+    const auto place_tiles = [&](bool again) {
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j) {
-        dq[j] *= first;
-        left[j] *= first;
-        right[j] *= last;
-        klast += L.k.values(16 * wave, j, lane) * right[j];
-    }
-    // E and the masks
-    const double Gw = L.G[own];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j <= wave) {
+        for (int i = 0; i < 2; ++i) {
+            if (kh < 3 && i == 1) break;
+            const int tb = kh == 3 ? 2 + th : 2 * th + (kh > 0),
+                      sb = kh == 3 ? i : 2 * th + (kh > 1);
+            const int s = 16 * sb + r;
+            const double Gs = L.G[s];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int s = 16 * j + 4 * q + e;
-                const float E_ = s <= own ? exp2_of(Gw - L.G[s]) : 0.f;
-                dp_row[j][e] = s <= own ? dp_row[j][e] * (A.scale * E_) : 0.f;
-                n_row[j][e] = s < own ? n_row[j][e] * E_ : 0.f;
+                const int t = 16 * tb + 4 * q + e;
+                uint32_t u[NC];
+                if (!again) {
+                    const float E_ = s <= t ? exp2_of(L.G[t] - Gs) : 0.f;
+                    nn[i][e] = s < t ? nn[i][e] * E_ : 0.f;
+                    split2<NC>(nn[i][e],
+                               s <= t ? dp[i][e] * (A.scale * E_) : 0.f, u);
+                } else {
+                    split2<NC>(-L.beta[t] * nn[i][e], 0.f, u);
+                }
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    L.n.x[n][t][s] = bf16_t(u[n]);
+                    if (!again) L.p.x[n][t][s] = bf16_t(u[n] >> 16);
+                }
             }
         }
-        if (j >= wave) {
+    };
+    place_tiles(false);
+    // (the blocks right of the diagonal that share a pair with it)
+    if (kh == 0) {
+        const int t = 32 * th + r, s = 32 * th + 16 + 4 * q;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = 16 * j + 4 * q + e;
-                const float E_ = own <= t ? exp2_of(L.G[t] - Gw) : 0.f;
-                dp_col[j][e] = own <= t ? dp_col[j][e] * (A.scale * E_) : 0.f;
-                n_col[j][e] =
-                    own < t ? n_col[j][e] * (-M.beta[t] * E_) : 0.f;
-            }
+        for (int n = 0; n < NC; ++n)
+            *reinterpret_cast<uint2*>(&L.n.x[n][t][s]) =
+                *reinterpret_cast<uint2*>(&L.p.x[n][t][s]) = make_uint2(0, 0);
+    }
+    // the rows' factors, t = 16 (2 th + i) + 4q + e
+    f32x4_t kfirst[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = 16 * (2 * th + i) + 4 * q;
+        const f32x4_t first = four(L.first + row), last = four(L.last + row);
+        kfirst[i] = zero4();
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            dq[i][j] *= A.scale * first;
+            left[i][j] *= first;
+            right[i][j] *= last;
+            kfirst[i] += L.k.values(16 * (2 * th + i), kh * KW + j, lane) *
+                         right[i][j];
         }
     }
-    // dq so far is without the scale; left with the other sign
-#pragma unroll
-    for (int j = 0; j < 2 * KT; ++j) dq[j] *= A.scale;
+    __syncthreads();
+    // left, with the other sign, and dP^T Q; (beta N)^T K after them, since
+    // beta belongs to the rows of N, which it contracts
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-        if (2 * p <= wave) {
-            const Frag<NC> a = split8<NC>(dp_row[2 * p], dp_row[2 * p + 1]);
-            const Frag<NC> n = split8<NC>(n_row[2 * p], n_row[2 * p + 1]);
+        if (p <= th) {
+            Frag<NC> a[2], n[2];
 #pragma unroll
-            for (int j = 0; j < 2 * KT; ++j) {
-                const Frag<NI> f = L.k.columns(j, p, lane);
-                mul(dq[j], a, f);
-                mul(left[j], n, f);
+            for (int i = 0; i < 2; ++i) {
+                a[i] = L.p.rows(2 * th + i, p, lane);
+                n[i] = L.n.rows(2 * th + i, p, lane);
+            }
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                const Frag<NI> f = L.k.columns(kh * KW + j, p, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    mul(dq[i][j], a[i], f);
+                    mul(left[i][j], n[i], f);
+                }
             }
         }
-        if (2 * p + 1 >= wave) {
-            const Frag<NC> a = split8<NC>(dp_col[2 * p], dp_col[2 * p + 1]);
-            const Frag<NC> n = split8<NC>(n_col[2 * p], n_col[2 * p + 1]);
+        if (p >= th) {
+            Frag<NC> a[2];
 #pragma unroll
-            for (int j = 0; j < 2 * KT; ++j) {
-                mul(right[j], a, L.q.columns(j, p, lane));
-                mul(right[j], n, L.k.columns(j, p, lane));
+            for (int i = 0; i < 2; ++i) a[i] = L.p.columns(2 * th + i, p, lane);
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                const Frag<NI> f = L.q.columns(kh * KW + j, p, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mul(right[i][j], a[i], f);
             }
         }
     }
-    f32x4_t qdq = zero4(), kleft = zero4(), kright = zero4();
+    __syncthreads();
+    place_tiles(true);
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j) {
-        const f32x4_t kv = L.k.values(16 * wave, j, lane);
-        left[j] = -left[j];
-        qdq += L.q.values(16 * wave, j, lane) * dq[j];
-        kleft += kv * left[j];
-        kright += kv * right[j];
+    for (int p = 0; p < 2; ++p) {
+        if (p < th) continue;
+        Frag<NC> n[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) n[i] = L.n.columns(2 * th + i, p, lane);
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            const Frag<NI> f = L.k.columns(kh * KW + j, p, lane);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mul(right[i][j], n[i], f);
+        }
+    }
+    // the gates' gradients
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f32x4_t qdq = zero4(), kleft = zero4(), kright = zero4();
+        const int row = 16 * (2 * th + i);
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            const f32x4_t kv = L.k.values(row, kh * KW + j, lane);
+            left[i][j] = -left[i][j];
+            qdq += L.q.values(row, kh * KW + j, lane) * dq[i][j];
+            kleft += kv * left[i][j];
+            kright += kv * right[i][j];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x[4] = {sum16(qdq[e]), sum16(kleft[e]),
+                                sum16(kright[e]), sum16(kfirst[i][e])};
+            if (r < 4)
+                L.dots[kh][r][row + 4 * q + e] = r == 0   ? x[0]
+                                                 : r == 1 ? x[1]
+                                                 : r == 2 ? x[2]
+                                                          : x[3];
+        }
     }
     rv += __shfl_xor(rv, 16);
     rv += __shfl_xor(rv, 32);
-    if (q == 0) L.rv[own] = rv;
+    if (kh < 2 && q == 0) L.rv[mine] = rv;
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) ds += __shfl_xor(ds, m);
-    float kl = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        qdq[e] = sum16(qdq[e]);
-        kleft[e] = sum16(kleft[e]);
-        kright[e] = sum16(kright[e]);
-        kl += sum16(klast[e]);
-    }
-    kl += __shfl_xor(kl, 16);
-    kl += __shfl_xor(kl, 32);
-    if (lane == 0) L.sums[wave] = kl + ds * M.first[C - 1];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (r == e) L.dG[row + e] = qdq[e] + beta[e] * kleft[e] - kright[e];
+    if (lane == 0) L.sums[wave] = ds;
     __syncthreads();
-    if (r < 4) {
-        const int t = row + r;
-        float kt = r == 0 ? kleft[0] : r == 1 ? kleft[1] : r == 2 ? kleft[2]
-                                                                  : kleft[3];
-        if (t < valid)
-            store_gate(A.dbeta, A.beta_bf16, (b * A.T + t0 + t) * A.Hv + h,
-                       kt + L.rv[t]);
-    }
     if (wave == 0) {
-        double x = L.dG[lane];
-        if (lane == 63)
-            x += double(L.sums[0]) + double(L.sums[1]) + double(L.sums[2]) +
-                 double(L.sums[3]);
+        const auto dot = [&](int i) {
+            float sum = L.dots[0][i][lane];
+#pragma unroll
+            for (int k = 1; k < KQ; ++k) sum += L.dots[k][i][lane];
+            return sum;
+        };
+        const float kleft = dot(1);
+        double x = double(dot(0)) + double(L.beta[lane] * kleft) -
+                   double(dot(2));
+        // <D, S_L> at the chunk's last token
+        double end = dot(3);
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) end += __shfl_xor(end, m);
+        double sums = 0.0;
+#pragma unroll
+        for (int w = 0; w < 2 * KQ; ++w) sums += L.sums[w];
+        end += L.first[C - 1] * sums;
+        if (lane == 63) x += end;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
             const double y = __shfl_down(x, m);
             if (lane + m < 64) x += y;
         }
-        if (lane < valid)
-            store_gate(A.dg, A.g_bf16, (b * A.T + t0 + lane) * A.Hv + h,
-                       float(x));
+        if (lane < valid) {
+            const int64_t at = (b * A.T + t0 + lane) * A.Hv + h;
+            store_gate(A.dg, A.g_bf16, at, float(x));
+            store_gate(A.dbeta, A.beta_bf16, at, kleft + L.rv[lane]);
+        }
     }
+    if (A.dq_part) {
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j) {
-        const int col = 16 * j + r;
-        if (col >= A.Dk) continue;
+        for (int i = 0; i < 2; ++i) {
+            const int row = 16 * (2 * th + i) + 4 * q;
+            const f32x4_t beta = four(L.beta + row);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int t = row + e;
-            if (t >= valid) continue;
-            const float dk = beta[e] * left[j][e] + right[j][e];
-            if (A.dq_part) {
-                const int64_t i =
-                    ((b * A.T + t0 + t) * A.Hv + h) * A.Dk + col;
-                A.dq_part[i] = dq[j][e];
-                A.dk_part[i] = dk;
-            } else {
-                const int64_t i =
-                    ((b * A.T + t0 + t) * A.Hk + hk) * A.Dk + col;
-                store_f(static_cast<E*>(A.dq) + i, dq[j][e]);
-                store_f(static_cast<E*>(A.dk) + i, dk);
+            for (int j = 0; j < KW; ++j) {
+                const int col = 16 * (kh * KW + j) + r;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (row + e >= valid || col >= A.Dk) continue;
+                    const int64_t at =
+                        ((b * A.T + t0 + row + e) * A.Hv + h) * A.Dk + col;
+                    A.dq_part[at] = dq[i][j][e];
+                    A.dk_part[at] = beta[e] * left[i][j][e] + right[i][j][e];
+                }
             }
+        }
+        return;
+    }
+    // dq and dk through LDS to whole rows (k and q are done with: the barrier
+    // above is behind their last reads)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = 16 * (2 * th + i) + 4 * q;
+        const f32x4_t beta = four(L.beta + row);
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            const int col = 16 * (kh * KW + j) + r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                store_f(&L.out[0][row + e][col], dq[i][j][e]);
+                store_f(&L.out[1][row + e][col],
+                        beta[e] * left[i][j][e] + right[i][j][e]);
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int per16 = 16 / sizeof(E), per_row = DKP / per16;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        E* to = static_cast<E*>(m ? A.dk : A.dq) +
+                ((b * A.T + t0) * A.Hk + hk) * A.Dk;
+#pragma unroll
+        for (int i = 0; i < C * per_row / NT; ++i) {
+            const int u = i * NT + int(threadIdx.x);
+            const int row = u / per_row, col = per16 * (u % per_row);
+            if (row < valid && col < A.Dk)
+                *reinterpret_cast<u32x4_t*>(to + row * A.Hk * A.Dk + col) =
+                    *reinterpret_cast<const u32x4_t*>(&L.out[m][row][col]);
         }
     }
 }

@@ -1,5 +1,5 @@
 // The gated delta rule's chunk matrices (gdr_common.h has the formulas): T =
-// (I + A)^-1 and P, as operands of the recurrences' products, and the gates.
+// (I + A)^-1 and P in planes, and the gates.
 //
 // One workgroup a chunk and value head, all of them independent.  T's diagonal
 // blocks of 16 are substituted forward, a lane a column: with keys that
@@ -13,7 +13,7 @@ namespace {
 
 using namespace gdr;
 
-constexpr int PITCH = C + 4;
+constexpr int NT = 256, PITCH = C + 4;
 
 struct Shared {
     alignas(16) float a[C][PITCH], t[C][PITCH];
@@ -36,7 +36,7 @@ __device__ __forceinline__ f32x4_t mm32(const f32x4_t& mt, const f32x4_t& y,
     return c;
 }
 
-template <typename E, int KT, bool BWD>
+template <typename E, int KT>
 __global__ void __launch_bounds__(NT)
 gdr_prepare_kernel(const GdrArgs A) {
     constexpr int NI = kIn<E>, NC = kMade<E>;
@@ -50,6 +50,25 @@ gdr_prepare_kernel(const GdrArgs A) {
     const int valid = int(A.T - t0 < C ? A.T - t0 : C);
     auto* out = static_cast<Prepared<NC>*>(A.prepared) + id;
 
+    // rows of k and q: places 32 p + 8q + i of token 16 tb + r, all loads
+    // before the first is waited for
+    const auto rows = [&](const GdrTensor& x, int tb, Eight<E> (&f)[KT]) {
+        const int t = 16 * tb + r;
+        const E* p = at<E>(x, b, hk, t0 + t);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+            const int col = 32 * i + 8 * q;
+            if (t < valid && col < A.Dk)
+                f[i].load(p + col);
+            else
+                f[i].clear();
+        }
+    };
+    Eight<E> qw[KT], kj[4][KT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j <= wave) rows(A.k, j, kj[j]);
+    rows(A.q, wave, qw);
     if (wave == 0) {
         // the running sum of the log decays: a decay of 0 (-inf) is held to
         // e^-1000, 0 in any result, so that later differences stay finite
@@ -72,76 +91,53 @@ gdr_prepare_kernel(const GdrArgs A) {
         out->last[lane] = exp2_of(__shfl(G, 63) - G);
         out->beta[lane] = beta;
     }
-    // rows of k and q: places 32 p + 8q + i of token 16 tb + r
-    const auto rows = [&](const GdrTensor& x, int tb, Frag<NI> (&f)[KT]) {
-        const int t = 16 * tb + r;
-        const E* p = at<E>(x, b, hk, t0 + t);
-#pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            Eight<E> v;
-            const int col = 32 * i + 8 * q;
-            if (t < valid && col < A.Dk)
-                v.load(p + col);
-            else
-                v.clear();
-            f[i] = v.planes();
-        }
-    };
-    Frag<NI> kw[KT], qw[KT];
-    rows(A.k, wave, kw);
-    rows(A.q, wave, qw);
     __syncthreads();
-    f32x4_t pt[4];
+    Frag<NI> qf[KT], kf[KT];  // the wave's own token block
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pt[j] = zero4();
-    const double Gw = S.G[16 * wave + r];
+    for (int p = 0; p < KT; ++p) {
+        qf[p] = qw[p].planes();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j == wave) kf[p] = kj[j][p].planes();
+    }
+    const int own = 16 * wave + r;
+    const double Gw = S.G[own];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        Frag<NI> kj[KT], qj[KT];
-        if (BWD ? j >= wave : j <= wave) {
-            if constexpr (BWD) rows(A.q, j, qj);
-            if constexpr (!BWD) rows(A.k, j, kj);
+        if (j > wave) break;
+        f32x4_t a = zero4(), pt = zero4();
 #pragma unroll
-            for (int p = 0; p < KT; ++p) {
-                if constexpr (BWD)
-                    mul(pt[j], qj[p], kw[p]);  // D(P): t = 4q + e, s = r
-                else
-                    mul(pt[j], kj[p], qw[p]);  // D(P^T): s = 4q + e, t = r
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                // (i: the tile's row of its accumulator, in block j)
-                const int i = 16 * j + 4 * q + e, w = 16 * wave + r;
-                const int t = BWD ? i : w, s = BWD ? w : i;
-                const double Gi = S.G[i];
-                pt[j][e] = s <= t ? pt[j][e] * exp2_of(BWD ? Gi - Gw : Gw - Gi)
-                                  : 0.f;
-            }
+        for (int p = 0; p < KT; ++p) {
+            const Frag<NI> f = kj[j][p].planes();
+            mul(a, f, kf[p]);   // D(A^T): s = 4q + e, t = r
+            mul(pt, f, qf[p]);  // D(P^T)
         }
-        if (j <= wave) {
-            if constexpr (BWD) rows(A.k, j, kj);
-            f32x4_t a = zero4();  // D(A): t = 4q + e, s = r
+        uint32_t lo[NC], hi[NC];
+        const float beta = S.beta[own];
+        f32x4_t at_;
 #pragma unroll
-            for (int p = 0; p < KT; ++p) mul(a, kw[p], kj[p]);
-            const double Gs = S.G[16 * j + r];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = 16 * wave + 4 * q + e, s = 16 * j + r;
-                S.a[t][s] = s < t ? a[e] * S.beta[t] * exp2_of(S.G[t] - Gs)
-                                  : 0.f;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int s = 16 * j + 4 * q + e;
+            const float E_ = s <= own ? exp2_of(Gw - S.G[s]) : 0.f;
+            at_[e] = s < own ? a[e] * (beta * E_) : 0.f;
+            pt[e] = s <= own ? pt[e] * E_ : 0.f;
         }
+        *reinterpret_cast<f32x4_t*>(&S.a[own][16 * j + 4 * q]) = at_;
+        split2<NC>(pt[0], pt[1], lo);
+        split2<NC>(pt[2], pt[3], hi);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+            *reinterpret_cast<uint2*>(&out->p[n][own][16 * j + 4 * q]) =
+                make_uint2(lo[n], hi[n]);
     }
+    if ((wave & 1) == 0) {
+        // (the block right of the diagonal that shares a pair with it)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        // (row block and pair of P's operand: the wave's and tiles 2p, 2p + 1)
-        const Frag<NC> f = split8<NC>(pt[2 * p], pt[2 * p + 1]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-            if (w == wave && image_has(BWD, w, p))
-#pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    out->p[image_at(BWD, w, p)][n][lane] = f.p[n];
+        for (int n = 0; n < NC; ++n)
+            *reinterpret_cast<uint2*>(
+                &out->p[n][own][16 * (wave + 1) + 4 * q]) = make_uint2(0, 0);
+        *reinterpret_cast<f32x4_t*>(&S.t[own][16 * (wave + 1) + 4 * q]) =
+            zero4();
     }
     __syncthreads();
     if (wave == 0) {
@@ -186,29 +182,14 @@ gdr_prepare_kernel(const GdrArgs A) {
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w != wave) continue;
+    for (int i = 0; i < 2; ++i) {
+        const int u = i * NT + int(threadIdx.x), row = u / 8, col = 8 * (u % 8);
+        if (row < 32 && col >= 32) continue;
+        const Frag<NC> f =
+            split8<NC>(four(&S.t[row][col]), four(&S.t[row][col + 4]));
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            if (!image_has(BWD, w, p)) continue;
-            f32x4_t x[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int block = 2 * p + u;
-                x[u] = zero4();
-                if (BWD && block >= w) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[u][e] = S.t[16 * block + 4 * q + e][16 * w + r];
-                } else if (!BWD && block <= w) {
-                    x[u] = four(&S.t[16 * w + r][16 * block + 4 * q]);
-                }
-            }
-            const Frag<NC> f = split8<NC>(x[0], x[1]);
-#pragma unroll
-            for (int n = 0; n < NC; ++n)
-                out->t[image_at(BWD, w, p)][n][lane] = f.p[n];
-        }
+        for (int n = 0; n < NC; ++n)
+            *reinterpret_cast<u32x4_t*>(&out->t[n][row][col]) = f.p[n];
     }
 }
 
@@ -222,25 +203,21 @@ int64_t gdr_prepared_bytes(bool bf16) {
                 : int64_t(sizeof(Prepared<kMade<float>>));
 }
 
-hipError_t launch_gdr_prepare(bool bf16, bool backward, const GdrArgs& A,
+hipError_t launch_gdr_prepare(bool bf16, const GdrArgs& A,
                               hipStream_t stream) {
-    const int64_t grid = A.B * A.Hv * ((A.T + C - 1) / C);
+    const dim3 grid(unsigned(A.B * A.Hv * ((A.T + C - 1) / C)));
     const bool wide = gdr_dkp(A.Dk) == 128;
-#define RWKV7M_GDR(E, KT, BWD)                                             \
-    hipLaunchKernelGGL((gdr_prepare_kernel<E, KT, BWD>),                   \
-                       dim3(unsigned(grid)), dim3(NT), 0, stream, A)
-#define RWKV7M_GDR2(E)                                                     \
-    do {                                                                   \
-        if (wide && backward) RWKV7M_GDR(E, 4, true);                      \
-        else if (wide) RWKV7M_GDR(E, 4, false);                            \
-        else if (backward) RWKV7M_GDR(E, 2, true);                         \
-        else RWKV7M_GDR(E, 2, false);                                      \
-    } while (0)
-    if (bf16)
-        RWKV7M_GDR2(bf16_t);
+#define RWKV7M_GDR(E, KT)                                                \
+    hipLaunchKernelGGL((gdr_prepare_kernel<E, KT>), grid, dim3(NT), 0,   \
+                       stream, A)
+    if (bf16 && wide)
+        RWKV7M_GDR(bf16_t, 4);
+    else if (bf16)
+        RWKV7M_GDR(bf16_t, 2);
+    else if (wide)
+        RWKV7M_GDR(float, 4);
     else
-        RWKV7M_GDR2(float);
-#undef RWKV7M_GDR2
+        RWKV7M_GDR(float, 2);
 #undef RWKV7M_GDR
     return hipGetLastError();
 }

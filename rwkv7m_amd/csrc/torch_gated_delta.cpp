@@ -133,7 +133,8 @@ variable_list rule_forward(Inputs& x, const Tensor& initial, bool train) {
         const int64_t n = rwkv7m_gated_delta_saved_floats(&x.in);
         saved = at::empty({n > 0 ? n : 1}, f32(x.q));
     }
-    const int64_t bytes = rwkv7m_gated_delta_workspace_bytes(&x.in, 0);
+    const int64_t bytes =
+        train ? 0 : rwkv7m_gated_delta_workspace_bytes(&x.in, 0);
     const Tensor ws = workspace(x.q, bytes);
     check("rwkv7m_gated_delta_rule",
           rwkv7m_gated_delta_rule(&x.in, ptr<float>(s0), ptr(o),

@@ -930,14 +930,12 @@ int gdr_sizes(const char* fn, const rwkv7m_gated_delta_inputs* in,
     return RWKV7M_OK;
 }
 
+// (a forward that keeps something for a backward keeps the chunk matrices too)
 int64_t gdr_workspace(const rwkv7m_gated_delta_inputs* in, const GdrSizes& s,
                       bool backward) {
-    int64_t bytes = s.prepared;
-    if (backward) {
-        bytes += 4 * (s.states + s.x);
-        if (in->Hv > in->Hk) bytes += 2 * 4 * in->B * in->T * in->Hv * in->Dk;
-    }
-    return bytes;
+    if (!backward) return s.prepared;
+    return 4 * (s.states + s.x) +
+           (in->Hv > in->Hk ? 2 * 4 * in->B * in->T * in->Hv * in->Dk : 0);
 }
 
 // A vector's or gate's place, its strides checked against its extents.
@@ -2088,7 +2086,7 @@ int64_t rwkv7m_gated_delta_saved_floats(const rwkv7m_gated_delta_inputs* in) {
             return gdr_sizes("rwkv7m_gated_delta_saved_floats", in, &s);
         }) != RWKV7M_OK)
         return -1;
-    return s.states + s.x;
+    return s.states + s.x + s.prepared / 4;
 }
 
 int rwkv7m_gated_delta_rule(const rwkv7m_gated_delta_inputs* in,
@@ -2112,18 +2110,18 @@ int rwkv7m_gated_delta_rule(const rwkv7m_gated_delta_inputs* in,
         rwkv7m::GdrArgs A{};
         RWKV7M_TRY(gdr_args(fn, in, &A));
         RWKV7M_TRY(lm_need(fn, 16, {{"o", o}}));
-        RWKV7M_TRY(gdr_workspace_holds(fn, workspace, workspace_bytes,
-                                       gdr_workspace(in, s, false)));
+        if (!saved)
+            RWKV7M_TRY(gdr_workspace_holds(fn, workspace, workspace_bytes,
+                                           gdr_workspace(in, s, false)));
         A.s0 = initial_state;
         A.o = o;
         A.s_t = final_state;
         A.states = saved;
         A.x = saved ? saved + s.states : nullptr;
-        A.prepared = workspace;
+        A.prepared = saved ? static_cast<void*>(A.x + s.x) : workspace;
         const bool bf16 = in->dtype == RWKV7M_DTYPE_BF16;
         RWKV7M_TRY(hip_status("gated delta rule launch",
-                              rwkv7m::launch_gdr_prepare(bf16, false, A,
-                                                         stream)));
+                              rwkv7m::launch_gdr_prepare(bf16, A, stream)));
         return hip_status("gated delta rule launch",
                           rwkv7m::launch_gdr_forward(bf16, A, stream));
     });
@@ -2170,19 +2168,14 @@ int rwkv7m_gated_delta_rule_backward(
         A.dv = dv;
         A.dg = dg;
         A.dbeta = dbeta;
-        char* at = static_cast<char*>(workspace);
-        A.prepared = at;
-        at += s.prepared;
-        A.dstates = reinterpret_cast<float*>(at);
+        A.prepared = A.x + s.x;
+        A.dstates = static_cast<float*>(workspace);
         A.dr = A.dstates + s.states;
         if (in->Hv > in->Hk) {
             A.dq_part = A.dr + s.x;
             A.dk_part = A.dq_part + in->B * in->T * in->Hv * in->Dk;
         }
         const bool bf16 = in->dtype == RWKV7M_DTYPE_BF16;
-        RWKV7M_TRY(hip_status(
-            "gated delta rule backward launch",
-            rwkv7m::launch_gdr_prepare(bf16, true, A, stream)));
         RWKV7M_TRY(hip_status("gated delta rule backward launch",
                               rwkv7m::launch_gdr_backward(bf16, A, stream)));
         return hip_status("gated delta rule gradients launch",

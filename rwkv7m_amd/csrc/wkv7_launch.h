@@ -415,7 +415,7 @@ struct GdrArgs {
 int gdr_dkp(int Dk);
 int gdr_dvp(int Dv);
 int64_t gdr_prepared_bytes(bool bf16);
-hipError_t launch_gdr_prepare(bool bf16, bool backward, const GdrArgs& A,
+hipError_t launch_gdr_prepare(bool bf16, const GdrArgs& A,
                               hipStream_t stream);
 hipError_t launch_gdr_forward(bool bf16, const GdrArgs& A, hipStream_t stream);
 hipError_t launch_gdr_backward(bool bf16, const GdrArgs& A,
