@@ -170,6 +170,15 @@ struct Rows {
         }
         return f;
     }
+    // The same of the 32 places of one pair, dense.
+    __device__ __forceinline__ Frag<NP> rows_dense(int tb, int lane) const {
+        Frag<NP> f;
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            f.p[n] = *reinterpret_cast<const u32x4_t*>(
+                &x[n][16 * tb + (lane & 15)][8 * (lane >> 4)]);
+        return f;
+    }
     // X[4q + e][16 jb + r] of the rows at `row`, by a transposing read.
     __device__ __forceinline__ uint2 column(int n, int row, int jb,
                                             int lane) const {

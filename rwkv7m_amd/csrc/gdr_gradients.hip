@@ -29,16 +29,18 @@ constexpr int KQ = 4, NT = 2 * KQ * 64;  // shares of the columns; threads
 template <typename E, int KT>
 struct GradShared {
     union {
-        struct {
-            Rows<kIn<E>, KT> k, q;
+        struct {  // a block of 32 columns of v
+            Rows<kMade<E>, KT, 32> s, d;  // S0's and D's rows
+            Rows<kMade<E>, 1> x, r;       // X, dR
+            Rows<kIn<E>, 1> o;            // dO
         };
-        E out[2][C][32 * KT + 8];  // dq and dk, once k and q are done with
-    };
-    union {
-        struct {
-            Rows<kMade<E>, KT, 32> s, d;  // 32 rows of S0 and of D
-        };
-        struct {
+        struct {  // what is made of them
+            union {
+                struct {
+                    Rows<kIn<E>, KT> k, q;
+                };
+                E out[2][C][32 * KT + 8];  // dq and dk, behind them
+            };
             Rows<kMade<E>, 2> n;  // N, then -beta N
             union {
                 Rows<kMade<E>, 2> p;  // dP
@@ -51,6 +53,44 @@ struct GradShared {
     float first[C], last[C], beta[C], rv[C];
     float sums[2 * KQ];
 };
+
+// Four adjoining elements of a row.
+template <typename E>
+struct Four;
+template <>
+struct Four<bf16_t> {
+    uint2 a;
+    __device__ __forceinline__ void load(const bf16_t* p) {
+        a = *reinterpret_cast<const uint2*>(p);
+    }
+    __device__ __forceinline__ void clear() { a = make_uint2(0, 0); }
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t u = i < 2 ? a.x : a.y;
+        return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+    }
+    __device__ __forceinline__ void put(Rows<1, 1>& to, int row,
+                                        int col) const {
+        *reinterpret_cast<uint2*>(&to.x[0][row][col]) = a;
+    }
+};
+template <>
+struct Four<float> {
+    f32x4_t a;
+    __device__ __forceinline__ void load(const float* p) { a = four(p); }
+    __device__ __forceinline__ void clear() { a = zero4(); }
+    __device__ __forceinline__ float get(int i) const { return a[i]; }
+    __device__ __forceinline__ void put(Rows<3, 1>& to, int row,
+                                        int col) const {
+        put4(to, row, col, a);
+    }
+};
+__device__ __forceinline__ void store4(float* p, const f32x4_t& x) {
+    *reinterpret_cast<f32x4_t*>(p) = x;
+}
+__device__ __forceinline__ void store4(bf16_t* p, const f32x4_t& x) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x[0], x[1]),
+                                              pack2(x[2], x[3]));
+}
 
 __device__ __forceinline__ void store_gate(void* p, bool bf16, int64_t i,
                                            float x) {
@@ -86,9 +126,13 @@ gdr_gradients_kernel(const GdrArgs A) {
     const float* s0 = A.states + (head * chunks + c) * DVP * DKP;
     const float* d0 = A.dstates + (head * chunks + c) * DVP * DKP;
 
-    // 32 rows of S0 and D on their way to LDS
+    // A block of 32 columns of v on its way to LDS: rows of S0 and D, places of
+    // X, dR, dO and v, a thread's share of each.
     constexpr int turns = 32 * DKP / 4 / NT;
-    f32x4_t sv[turns], dv[turns];
+    static_assert(NT == 8 * C, "a thread takes four places of X, dR, dO and v");
+    f32x4_t sv[turns], dv[turns], xv, rv4;
+    Four<E> ov, vv;
+    const int trow = threadIdx.x / 8, tcol = 4 * (threadIdx.x % 8);
     const auto fetch = [&](int v0) {
 #pragma unroll
         for (int i = 0; i < turns; ++i) {
@@ -96,37 +140,23 @@ gdr_gradients_kernel(const GdrArgs A) {
             sv[i] = four(s0 + v0 * DKP + u);
             dv[i] = four(d0 + v0 * DKP + u);
         }
-    };
-    // places v0 + 8q + i of a row of dO, X or dR
-    const auto dout = [&](int tb, int v0) {
-        const int t = 16 * tb + r, col = v0 + 8 * q;
-        Eight<E> e;
-        e.clear();
-        if (t < valid && col < A.Dv) e.load(dop + t * A.dout.st + col);
-        return e;
-    };
-    const auto made = [&](const float* from, int tb, int v0) {
-        Eight<float> e;
-        e.load(from + (16 * tb + r) * DVP + v0 + 8 * q);
-        return e;
-    };
-    const auto planes = [&](const Eight<float>& e) {
-        return split8<NC>(e.a, e.b);
+        xv = four(x0 + trow * DVP + v0 + tcol);
+        rv4 = four(r0 + trow * DVP + v0 + tcol);
+        ov.clear();
+        vv.clear();
+        if (trow < valid && v0 + tcol < A.Dv) {
+            ov.load(dop + trow * A.dout.st + v0 + tcol);
+            vv.load(vp + trow * A.v.st + v0 + tcol);
+        }
     };
 
     fetch(0);
-    {
-        Staged<E, KT, NT> ks, qs;
-        ks.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, threadIdx.x);
-        qs.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, threadIdx.x);
-        if (threadIdx.x < C) {
-            L.G[threadIdx.x] = M.G[threadIdx.x];
-            L.first[threadIdx.x] = M.first[threadIdx.x];
-            L.last[threadIdx.x] = M.last[threadIdx.x];
-            L.beta[threadIdx.x] = M.beta[threadIdx.x];
-        }
-        ks.store(L.k, threadIdx.x);
-        qs.store(L.q, threadIdx.x);
+    Staged<E, KT, NT> ks, qs;
+    if (threadIdx.x < C) {
+        L.G[threadIdx.x] = M.G[threadIdx.x];
+        L.first[threadIdx.x] = M.first[threadIdx.x];
+        L.last[threadIdx.x] = M.last[threadIdx.x];
+        L.beta[threadIdx.x] = M.beta[threadIdx.x];
     }
 
     f32x4_t dq[2][KW], left[2][KW], right[2][KW];
@@ -141,52 +171,12 @@ gdr_gradients_kernel(const GdrArgs A) {
     f32x4_t dp[2], nn[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) dp[i] = nn[i] = zero4();
-    float rv = 0.f, ds = 0.f;  // dR.v of token 16 (2 th + kh) + r; <D, S0>
-    const int mine = 16 * (2 * th + (kh & 1)) + r;
-    E* dvp = static_cast<E*>(A.dv) + ((b * A.T + t0 + mine) * A.Hv + h) * A.Dv;
-    const float beta_mine = M.beta[mine];
+    float rv = 0.f, ds = 0.f;  // dR.v of token trow; <D, S0>
+    E* dvp = static_cast<E*>(A.dv) + ((b * A.T + t0 + trow) * A.Hv + h) * A.Dv +
+             tcol;
+    const float beta_own = M.beta[trow];
 
     for (int v0 = 0; v0 < DVP; v0 += 32) {
-        // operands of the wave's tokens (left or right alike)
-        Frag<NI> of[2];
-        Frag<NC> xf[2], rf[2];
-        {
-            Eight<E> o8[2], v8;
-            Eight<float> x8[2], r8[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                o8[i] = dout(2 * th + i, v0);
-                x8[i] = made(x0, 2 * th + i, v0);
-                r8[i] = made(r0, 2 * th + i, v0);
-            }
-            const int col = v0 + 8 * q;
-            const bool on = kh < 2 && mine < valid && col < A.Dv;
-            v8.clear();
-            if (on) v8.load(vp + mine * A.v.st + col);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                of[i] = o8[i].planes();
-                xf[i] = planes(x8[i]);
-                rf[i] = planes(r8[i]);
-            }
-            Eight<float> dr = kh ? r8[1] : r8[0];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rv += dr.get(i) * v8.get(i);
-            dr.a *= beta_mine;
-            dr.b *= beta_mine;
-            if (on) {
-                if constexpr (sizeof(E) == 4) {
-                    *reinterpret_cast<f32x4_t*>(dvp + col) = dr.a;
-                    *reinterpret_cast<f32x4_t*>(dvp + col + 4) = dr.b;
-                } else {
-                    *reinterpret_cast<uint4*>(dvp + col) =
-                        make_uint4(pack2(dr.a[0], dr.a[1]),
-                                   pack2(dr.a[2], dr.a[3]),
-                                   pack2(dr.b[0], dr.b[1]),
-                                   pack2(dr.b[2], dr.b[3]));
-                }
-            }
-        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < turns; ++i) {
@@ -197,8 +187,29 @@ gdr_gradients_kernel(const GdrArgs A) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) ds += sv[i][e] * dv[i][e];
         }
+        put4(L.x, trow, tcol, xv);
+        put4(L.r, trow, tcol, rv4);
+        ov.put(L.o, trow, tcol);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rv += rv4[e] * vv.get(e);
+        if (trow < valid && v0 + tcol < A.Dv)
+            store4(dvp + v0, beta_own * rv4);
         __syncthreads();
-        if (v0 + 32 < DVP) fetch(v0 + 32);
+        if (v0 + 32 < DVP) {
+            fetch(v0 + 32);
+        } else {
+            ks.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, threadIdx.x);
+            qs.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, threadIdx.x);
+        }
+        // operands of the wave's tokens (left or right alike)
+        Frag<NI> of[2];
+        Frag<NC> xf[2], rf[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            of[i] = L.o.rows_dense(2 * th + i, lane);
+            xf[i] = L.x.rows_dense(2 * th + i, lane);
+            rf[i] = L.r.rows_dense(2 * th + i, lane);
+        }
         if (kh == 0) {
             mul(dp[0], of[0], xf[0]);
             mul(nn[0], rf[0], xf[0]);
@@ -208,19 +219,14 @@ gdr_gradients_kernel(const GdrArgs A) {
         } else if (kh == 2) {
             mul(dp[0], of[1], xf[1]);
             mul(nn[0], rf[1], xf[1]);
-        } else if (th == 0) {
-            const Frag<NI> o = dout(2, v0).planes();
-            const Frag<NC> g = planes(made(r0, 2, v0));
-            mul(dp[0], o, xf[0]);
-            mul(dp[1], o, xf[1]);
-            mul(nn[0], g, xf[0]);
-            mul(nn[1], g, xf[1]);
         } else {
+            const Frag<NI> o = L.o.rows_dense(2 + th, lane);
+            const Frag<NC> g = L.r.rows_dense(2 + th, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const Frag<NC> x = planes(made(x0, i, v0));
-                mul(dp[i], of[1], x);
-                mul(nn[i], rf[1], x);
+                const Frag<NC> x = L.x.rows_dense(i, lane);
+                mul(dp[i], o, x);
+                mul(nn[i], g, x);
             }
         }
 #pragma unroll
@@ -236,6 +242,8 @@ gdr_gradients_kernel(const GdrArgs A) {
         }
     }
     __syncthreads();
+    ks.store(L.k, threadIdx.x);
+    qs.store(L.q, threadIdx.x);
     // N and dP with their decays, to LDS
     const auto place_tiles = [&](bool again) {
 #pragma unroll
@@ -274,6 +282,7 @@ gdr_gradients_kernel(const GdrArgs A) {
             *reinterpret_cast<uint2*>(&L.n.x[n][t][s]) =
                 *reinterpret_cast<uint2*>(&L.p.x[n][t][s]) = make_uint2(0, 0);
     }
+    __syncthreads();
     // the rows' factors, t = 16 (2 th + i) + 4q + e
     f32x4_t kfirst[2];
 #pragma unroll
@@ -290,7 +299,6 @@ gdr_gradients_kernel(const GdrArgs A) {
                          right[i][j];
         }
     }
-    __syncthreads();
     // left, with the other sign, and dP^T Q; (beta N)^T K after them, since
     // beta belongs to the rows of N, which it contracts
 #pragma unroll
@@ -364,9 +372,8 @@ gdr_gradients_kernel(const GdrArgs A) {
                                                           : x[3];
         }
     }
-    rv += __shfl_xor(rv, 16);
-    rv += __shfl_xor(rv, 32);
-    if (kh < 2 && q == 0) L.rv[mine] = rv;
+    rv = group_sum<8>(rv);
+    if (threadIdx.x % 8 == 0) L.rv[trow] = rv;
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) ds += __shfl_xor(ds, m);
     if (lane == 0) L.sums[wave] = ds;
