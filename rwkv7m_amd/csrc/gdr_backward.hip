@@ -21,8 +21,8 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
     if (head >= A.B * A.Hv) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int64_t b = head / A.Hv, h = head % A.Hv;
-    const int64_t chunks = (A.T + C - 1) / C;
+    const Head at_head(A, at_.head);
+    const int64_t b = at_head.b, h = at_head.h, chunks = chunk_count(A);
     const int DVP = (A.Dv + 31) / 32 * 32;
     const int v0 = 64 * at_.part + 16 * wave, v = v0 + r;  // the lane's row
     const bool has = v0 < DVP, on = v < A.Dv;

@@ -183,7 +183,8 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
                                       const Prepared<kMade<E>>* M, int64_t head,
                                       int v0, int64_t first, int64_t step,
                                       int64_t n, ChainChunk<E, KT>* L, F own) {
-    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    const Head at_head(A, uint32_t(head));
+    const int64_t b = at_head.b, h = at_head.h, hk = at_head.hk;
     constexpr int NB = kBuffers<E, KT>;
     if (threadIdx.x >= BRING) {
         const int thread = threadIdx.x - BRING;

@@ -307,15 +307,27 @@ __device__ __forceinline__ float sum16(float x) { return group_sum<16>(x); }
 // A head's workgroups on one of the 8 XCDs (consecutive workgroups go to
 // different ones), so that they share its L2: workgroup `id` of head and part.
 struct Place {
-    int64_t head;
+    uint32_t head;
     int part;
 };
-__device__ __forceinline__ Place place(unsigned id, unsigned parts) {
-    const unsigned xcd = id % 8, slot = id / 8;
-    return {int64_t(slot / parts) * 8 + xcd, int(slot % parts)};
+__device__ __forceinline__ Place place(uint32_t id, uint32_t parts) {
+    const uint32_t xcd = id % 8, slot = id / 8;
+    return {slot / parts * 8 + xcd, int(slot % parts)};
 }
 inline unsigned places(int64_t heads, int64_t parts) {
     return unsigned((heads + 7) / 8 * 8 * parts);
+}
+
+// Batch row, value head and key head of head `id` of B * Hv (fewer than 2^24:
+// a 64-bit division is 130 instructions).
+struct Head {
+    uint32_t b, h, hk;
+    __device__ __forceinline__ Head(const GdrArgs& A, uint32_t id)
+        : b(id / uint32_t(A.Hv)), h(id % uint32_t(A.Hv)),
+          hk(h / (uint32_t(A.Hv) / uint32_t(A.Hk))) {}
+};
+__device__ __forceinline__ uint32_t chunk_count(const GdrArgs& A) {
+    return uint32_t((A.T + C - 1) / C);
 }
 
 template <typename E>

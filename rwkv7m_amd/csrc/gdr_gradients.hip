@@ -12,7 +12,7 @@
 //   <D, S_L> = 2^G_L <D, S0> + sum_t k_t.(2^(G_L - G) X D)_t
 //
 // One workgroup a chunk and value head, all of them independent.  A wave owns
-// 32 tokens and a quarter of the columns of dq, left and right.  S0 and D pass
+// 32 tokens and a share of the columns of dq, left and right.  S0 and D pass
 // through LDS in blocks of 32 rows, whose columns are operands by transposing
 // reads; each operand so read serves two blocks of tokens.  The ten lower
 // blocks of N and dP are divided among the waves and meet in LDS, whose rows
@@ -24,7 +24,13 @@ namespace {
 
 using namespace gdr;
 
-constexpr int KQ = 4, NT = 2 * KQ * 64;  // shares of the columns; threads
+// Shares of the columns a workgroup's waves are divided over (two rows of
+// waves).  bf16 up to 64 columns: 2, and two workgroups a CU (train_0185b 32
+// us, with 4 and one workgroup 38).  At 128 the sums of half the columns leave
+// no room for a second workgroup's registers: 4, and the next block's loads
+// begun ahead (train_1b 732 us; with 2 890).
+template <typename E, int KT>
+constexpr int kShares = sizeof(E) == 2 && KT == 4 ? 4 : 2;
 
 template <typename E, int KT>
 struct GradShared {
@@ -44,14 +50,13 @@ struct GradShared {
             Rows<kMade<E>, 2> n;  // N, then -beta N
             union {
                 Rows<kMade<E>, 2> p;  // dP
-                // of q.dq, k.left, k.right, k.(first of right), behind it
-                float dots[KQ][4][C];
+                float dots[kShares<E, KT>][2][C];  // of dG, k.left, behind it
             };
         };
     };
     double G[C];
     float first[C], last[C], beta[C], rv[C];
-    float sums[2 * KQ];
+    float sums[2 * kShares<E, KT>];
 };
 
 // Four adjoining elements of a row.
@@ -101,18 +106,21 @@ __device__ __forceinline__ void store_gate(void* p, bool bf16, int64_t i,
 }
 
 template <typename E, int KT>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__((128 * kShares<E, KT>), sizeof(E) == 2 ? 2 : 1)
 gdr_gradients_kernel(const GdrArgs A) {
     constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
+    constexpr int KQ = kShares<E, KT>, NT = 128 * KQ;
+    constexpr bool AHEAD = KQ == 4;
     extern __shared__ char lds_raw[];
     auto& L = *reinterpret_cast<GradShared<E, KT>*>(lds_raw);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
     const int th = wave / KQ, kh = wave % KQ;  // tokens 32 th .., share kh
     constexpr int KW = 2 * KT / KQ;  // the wave's tiles of 16 columns
-    const int64_t chunks = (A.T + C - 1) / C;
-    const int64_t id = blockIdx.x, head = id / chunks, c = id % chunks;
-    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    const uint32_t chunks = chunk_count(A), id = blockIdx.x;
+    const int64_t head = id / chunks, c = id % chunks;
+    const Head at_head(A, uint32_t(head));
+    const int64_t b = at_head.b, h = at_head.h, hk = at_head.hk;
     const int64_t t0 = c * C;
     const int valid = int(A.T - t0 < C ? A.T - t0 : C);
     const int DVP = (A.Dv + 31) / 32 * 32;
@@ -126,32 +134,12 @@ gdr_gradients_kernel(const GdrArgs A) {
     const float* s0 = A.states + (head * chunks + c) * DVP * DKP;
     const float* d0 = A.dstates + (head * chunks + c) * DVP * DKP;
 
-    // A block of 32 columns of v on its way to LDS: rows of S0 and D, places of
-    // X, dR, dO and v, a thread's share of each.
-    constexpr int turns = 32 * DKP / 4 / NT;
-    static_assert(NT == 8 * C, "a thread takes four places of X, dR, dO and v");
-    f32x4_t sv[turns], dv[turns], xv, rv4;
-    Four<E> ov, vv;
-    const int trow = threadIdx.x / 8, tcol = 4 * (threadIdx.x % 8);
-    const auto fetch = [&](int v0) {
-#pragma unroll
-        for (int i = 0; i < turns; ++i) {
-            const int u = 4 * (i * NT + int(threadIdx.x));
-            sv[i] = four(s0 + v0 * DKP + u);
-            dv[i] = four(d0 + v0 * DKP + u);
-        }
-        xv = four(x0 + trow * DVP + v0 + tcol);
-        rv4 = four(r0 + trow * DVP + v0 + tcol);
-        ov.clear();
-        vv.clear();
-        if (trow < valid && v0 + tcol < A.Dv) {
-            ov.load(dop + trow * A.dout.st + v0 + tcol);
-            vv.load(vp + trow * A.v.st + v0 + tcol);
-        }
-    };
-
-    fetch(0);
     Staged<E, KT, NT> ks, qs;
+    const auto bring = [&]() {
+        ks.load(gdr::at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, threadIdx.x);
+        qs.load(gdr::at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, threadIdx.x);
+    };
+    if constexpr (AHEAD) bring();
     if (threadIdx.x < C) {
         L.G[threadIdx.x] = M.G[threadIdx.x];
         L.first[threadIdx.x] = M.first[threadIdx.x];
@@ -165,18 +153,54 @@ gdr_gradients_kernel(const GdrArgs A) {
 #pragma unroll
         for (int j = 0; j < KW; ++j)
             dq[i][j] = left[i][j] = right[i][j] = zero4();
-    // Blocks (tb, sb) of N and dP, t = 4q + e, s = r: with kh 0, 1, 2 one of
-    // the wave's own tokens, (0, 0), (1, 0), (1, 1) from 2 th on; with kh 3
-    // (2 + th, 0) and (2 + th, 1).
-    f32x4_t dp[2], nn[2];
+    // Blocks (tb, sb) of N and dP, t = 4q + e, s = r.  The last share's waves
+    // have (2 + th, 0) and (2 + th, 1), the others those of the wave's own
+    // tokens, (0, 0), (1, 0), (1, 1) from 2 th on: all three, or one each.
+    constexpr int OWN = KQ == 2 ? 3 : 1, TILES = KQ == 2 ? 3 : 2;
+    const bool last_share = kh == KQ - 1;
+    f32x4_t dp[TILES], nn[TILES];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) dp[i] = nn[i] = zero4();
-    float rv = 0.f, ds = 0.f;  // dR.v of token trow; <D, S0>
-    E* dvp = static_cast<E*>(A.dv) + ((b * A.T + t0 + trow) * A.Hv + h) * A.Dv +
-             tcol;
-    const float beta_own = M.beta[trow];
+    for (int i = 0; i < TILES; ++i) dp[i] = nn[i] = zero4();
+    float ds = 0.f;  // <D, S0>
+    // Four places of X, dR, dO and v a thread and turn, of rows trow[i]; dR.v
+    constexpr int rows = 8 * C / NT, step = C / rows;
+    const int trow = threadIdx.x / 8, tcol = 4 * (threadIdx.x % 8);
+    float rv[rows], beta_own[rows];
+#pragma unroll
+    for (int i = 0; i < rows; ++i) {
+        rv[i] = 0.f;
+        beta_own[i] = M.beta[trow + i * step];
+    }
+    E* dvp = static_cast<E*>(A.dv) + ((b * A.T + t0) * A.Hv + h) * A.Dv + tcol;
 
+    // 32 columns of v on their way to LDS: rows of S0 and D, places of X, dR,
+    // dO and v
+    constexpr int turns = 32 * DKP / 4 / NT;
+    f32x4_t sv[turns], dv[turns], xv[rows], r4[rows];
+    Four<E> ov[rows], vv[rows];
+    const auto fetch = [&](int v0) {
+#pragma unroll
+        for (int i = 0; i < turns; ++i) {
+            const int u = 4 * (i * NT + int(threadIdx.x));
+            sv[i] = four(s0 + v0 * DKP + u);
+            dv[i] = four(d0 + v0 * DKP + u);
+        }
+#pragma unroll
+        for (int i = 0; i < rows; ++i) {
+            const int t = trow + i * step;
+            xv[i] = four(x0 + t * DVP + v0 + tcol);
+            r4[i] = four(r0 + t * DVP + v0 + tcol);
+            ov[i].clear();
+            vv[i].clear();
+            if (t < valid && v0 + tcol < A.Dv) {
+                ov[i].load(dop + t * A.dout.st + v0 + tcol);
+                vv[i].load(vp + t * A.v.st + v0 + tcol);
+            }
+        }
+    };
+    if constexpr (AHEAD) fetch(0);
     for (int v0 = 0; v0 < DVP; v0 += 32) {
+        if constexpr (!AHEAD) fetch(v0);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < turns; ++i) {
@@ -187,20 +211,20 @@ gdr_gradients_kernel(const GdrArgs A) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) ds += sv[i][e] * dv[i][e];
         }
-        put4(L.x, trow, tcol, xv);
-        put4(L.r, trow, tcol, rv4);
-        ov.put(L.o, trow, tcol);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) rv += rv4[e] * vv.get(e);
-        if (trow < valid && v0 + tcol < A.Dv)
-            store4(dvp + v0, beta_own * rv4);
-        __syncthreads();
-        if (v0 + 32 < DVP) {
-            fetch(v0 + 32);
-        } else {
-            ks.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, threadIdx.x);
-            qs.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, threadIdx.x);
+        for (int i = 0; i < rows; ++i) {
+            const int t = trow + i * step;
+            put4(L.x, t, tcol, xv[i]);
+            put4(L.r, t, tcol, r4[i]);
+            ov[i].put(L.o, t, tcol);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rv[i] += r4[i][e] * vv[i].get(e);
+            if (t < valid && v0 + tcol < A.Dv)
+                store4(dvp + t * A.Hv * A.Dv + v0, beta_own[i] * r4[i]);
         }
+        __syncthreads();
+        if constexpr (AHEAD)
+            if (v0 + 32 < DVP) fetch(v0 + 32);
         // operands of the wave's tokens (left or right alike)
         Frag<NI> of[2];
         Frag<NC> xf[2], rf[2];
@@ -210,15 +234,21 @@ gdr_gradients_kernel(const GdrArgs A) {
             xf[i] = L.x.rows_dense(2 * th + i, lane);
             rf[i] = L.r.rows_dense(2 * th + i, lane);
         }
-        if (kh == 0) {
-            mul(dp[0], of[0], xf[0]);
-            mul(nn[0], rf[0], xf[0]);
-        } else if (kh == 1) {
-            mul(dp[0], of[1], xf[0]);
-            mul(nn[0], rf[1], xf[0]);
-        } else if (kh == 2) {
-            mul(dp[0], of[1], xf[1]);
-            mul(nn[0], rf[1], xf[1]);
+        if (!last_share) {
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const int at = KQ == 2 ? i : kh;
+                if (at == 0) {
+                    mul(dp[i], of[0], xf[0]);
+                    mul(nn[i], rf[0], xf[0]);
+                } else if (at == 1) {
+                    mul(dp[i], of[1], xf[0]);
+                    mul(nn[i], rf[1], xf[0]);
+                } else {
+                    mul(dp[i], of[1], xf[1]);
+                    mul(nn[i], rf[1], xf[1]);
+                }
+            }
         } else {
             const Frag<NI> o = L.o.rows_dense(2 + th, lane);
             const Frag<NC> g = L.r.rows_dense(2 + th, lane);
@@ -242,15 +272,17 @@ gdr_gradients_kernel(const GdrArgs A) {
         }
     }
     __syncthreads();
+    if constexpr (!AHEAD) bring();
     ks.store(L.k, threadIdx.x);
     qs.store(L.q, threadIdx.x);
     // N and dP with their decays, to LDS
     const auto place_tiles = [&](bool again) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (kh < 3 && i == 1) break;
-            const int tb = kh == 3 ? 2 + th : 2 * th + (kh > 0),
-                      sb = kh == 3 ? i : 2 * th + (kh > 1);
+        for (int i = 0; i < TILES; ++i) {
+            if (i >= (last_share ? 2 : OWN)) break;
+            const int at = KQ == 2 ? i : kh;
+            const int tb = last_share ? 2 + th : 2 * th + (at > 0),
+                      sb = last_share ? i : 2 * th + (at > 1);
             const int s = 16 * sb + r;
             const double Gs = L.G[s];
 #pragma unroll
@@ -284,19 +316,19 @@ gdr_gradients_kernel(const GdrArgs A) {
     }
     __syncthreads();
     // the rows' factors, t = 16 (2 th + i) + 4q + e
-    f32x4_t kfirst[2];
+    float kfirst = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int row = 16 * (2 * th + i) + 4 * q;
         const f32x4_t first = four(L.first + row), last = four(L.last + row);
-        kfirst[i] = zero4();
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
             dq[i][j] *= A.scale * first;
             left[i][j] *= first;
             right[i][j] *= last;
-            kfirst[i] += L.k.values(16 * (2 * th + i), kh * KW + j, lane) *
-                         right[i][j];
+            const f32x4_t x = L.k.values(16 * (2 * th + i), kh * KW + j, lane) *
+                              right[i][j];
+            kfirst += (x[0] + x[1]) + (x[2] + x[3]);
         }
     }
     // left, with the other sign, and dP^T Q; (beta N)^T K after them, since
@@ -351,32 +383,34 @@ gdr_gradients_kernel(const GdrArgs A) {
     // the gates' gradients
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        f32x4_t qdq = zero4(), kleft = zero4(), kright = zero4();
+        f32x4_t kleft = zero4(), dg = zero4();
         const int row = 16 * (2 * th + i);
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
             const f32x4_t kv = L.k.values(row, kh * KW + j, lane);
             left[i][j] = -left[i][j];
-            qdq += L.q.values(row, kh * KW + j, lane) * dq[i][j];
+            dg += L.q.values(row, kh * KW + j, lane) * dq[i][j] -
+                  kv * right[i][j];
             kleft += kv * left[i][j];
-            kright += kv * right[i][j];
         }
+        dg += four(L.beta + row + 4 * q) * kleft;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x[4] = {sum16(qdq[e]), sum16(kleft[e]),
-                                sum16(kright[e]), sum16(kfirst[i][e])};
-            if (r < 4)
-                L.dots[kh][r][row + 4 * q + e] = r == 0   ? x[0]
-                                                 : r == 1 ? x[1]
-                                                 : r == 2 ? x[2]
-                                                          : x[3];
+            const float x = sum16(dg[e]), y = sum16(kleft[e]);
+            if (r < 2) L.dots[kh][r][row + 4 * q + e] = r ? y : x;
         }
     }
-    rv = group_sum<8>(rv);
-    if (threadIdx.x % 8 == 0) L.rv[trow] = rv;
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) ds += __shfl_xor(ds, m);
-    if (lane == 0) L.sums[wave] = ds;
+    for (int i = 0; i < rows; ++i) {
+        rv[i] = group_sum<8>(rv[i]);
+        if (threadIdx.x % 8 == 0) L.rv[trow + i * step] = rv[i];
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        ds += __shfl_xor(ds, m);
+        kfirst += __shfl_xor(kfirst, m);
+    }
+    if (lane == 0) L.sums[wave] = L.first[C - 1] * ds + kfirst;
     __syncthreads();
     if (wave == 0) {
         const auto dot = [&](int i) {
@@ -385,17 +419,9 @@ gdr_gradients_kernel(const GdrArgs A) {
             for (int k = 1; k < KQ; ++k) sum += L.dots[k][i][lane];
             return sum;
         };
-        const float kleft = dot(1);
-        double x = double(dot(0)) + double(L.beta[lane] * kleft) -
-                   double(dot(2));
-        // <D, S_L> at the chunk's last token
-        double end = dot(3);
+        double x = dot(0), end = 0.0;  // <D, S_L> at the chunk's last token
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) end += __shfl_xor(end, m);
-        double sums = 0.0;
-#pragma unroll
-        for (int w = 0; w < 2 * KQ; ++w) sums += L.sums[w];
-        end += L.first[C - 1] * sums;
+        for (int w = 0; w < 2 * KQ; ++w) end += L.sums[w];
         if (lane == 63) x += end;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
@@ -405,7 +431,7 @@ gdr_gradients_kernel(const GdrArgs A) {
         if (lane < valid) {
             const int64_t at = (b * A.T + t0 + lane) * A.Hv + h;
             store_gate(A.dg, A.g_bf16, at, float(x));
-            store_gate(A.dbeta, A.beta_bf16, at, kleft + L.rv[lane]);
+            store_gate(A.dbeta, A.beta_bf16, at, dot(1) + L.rv[lane]);
         }
     }
     if (A.dq_part) {
@@ -464,13 +490,15 @@ gdr_gradients_kernel(const GdrArgs A) {
 
 // The shares of the value heads that read one key head, added up in their
 // order: four places a thread.
+constexpr int GROUP = 256;  // threads
+
 template <typename E>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(GROUP)
 gdr_group_kernel(const GdrArgs A, int64_t n) {
     const int per = int(A.Hv / A.Hk);
     const int64_t quads = A.Dk / 4;
-    for (int64_t i = int64_t(blockIdx.x) * NT + threadIdx.x; i < n;
-         i += int64_t(gridDim.x) * NT) {
+    for (int64_t i = int64_t(blockIdx.x) * GROUP + threadIdx.x; i < n;
+         i += int64_t(gridDim.x) * GROUP) {
         const int64_t row = i / quads, col = 4 * (i % quads);
         // (row: token and key head; its value heads are adjoining)
         const float* from[2] = {A.dq_part, A.dk_part};
@@ -499,13 +527,14 @@ hipError_t launch(const GdrArgs& A, hipStream_t stream) {
         hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     const int64_t grid = A.B * A.Hv * ((A.T + C - 1) / C);
-    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(NT), lds, stream, A);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)),
+                       dim3(128 * kShares<E, KT>), lds, stream, A);
     e = hipGetLastError();
     if (e != hipSuccess || !A.dq_part) return e;
     const int64_t n = A.B * A.T * A.Hk * (A.Dk / 4);
-    int64_t blocks = (n + NT - 1) / NT;
+    int64_t blocks = (n + GROUP - 1) / GROUP;
     if (blocks > 8192) blocks = 8192;
-    hipLaunchKernelGGL(gdr_group_kernel<E>, dim3(unsigned(blocks)), dim3(NT),
+    hipLaunchKernelGGL(gdr_group_kernel<E>, dim3(unsigned(blocks)), dim3(GROUP),
                        0, stream, A, n);
     return hipGetLastError();
 }

@@ -43,9 +43,10 @@ gdr_prepare_kernel(const GdrArgs A) {
     __shared__ Shared S;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int64_t chunks = (A.T + C - 1) / C;
-    const int64_t id = blockIdx.x, head = id / chunks, c = id % chunks;
-    const int64_t b = head / A.Hv, h = head % A.Hv, hk = h / (A.Hv / A.Hk);
+    const uint32_t chunks = chunk_count(A), id = blockIdx.x;
+    const int64_t head = id / chunks, c = id % chunks;
+    const Head at_head(A, uint32_t(head));
+    const int64_t b = at_head.b, h = at_head.h, hk = at_head.hk;
     const int64_t t0 = c * C;
     const int valid = int(A.T - t0 < C ? A.T - t0 : C);
     auto* out = static_cast<Prepared<NC>*>(A.prepared) + id;

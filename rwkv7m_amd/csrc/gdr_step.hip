@@ -54,12 +54,14 @@ __device__ __forceinline__ float dot(const f32x4_t& a, const f32x4_t& b) {
 // KQ: 16-lane groups of 4 places a row (Dk up to 64 KQ).
 template <typename E, int KQ>
 __global__ void __launch_bounds__(NT)
-gdr_step_kernel(const GdrStepArgs A, int parts) {
+gdr_step_kernel(const GdrStepArgs A, uint32_t parts) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15;
-    const int64_t id = blockIdx.x, bh = id / parts;
-    const int64_t b = bh / A.Hv, h = bh % A.Hv, hk = h / (A.Hv / A.Hk);
-    const int row = int(id % parts) * ROWS + wave * 16 + (lane >> 4) * 4;
+    // (32 bits: a 64-bit division is 130 instructions)
+    const uint32_t bh = blockIdx.x / parts, Hv = uint32_t(A.Hv);
+    const int64_t b = bh / Hv, h = bh % Hv,
+                  hk = uint32_t(h) / (Hv / uint32_t(A.Hk));
+    const int row = int(blockIdx.x % parts) * ROWS + wave * 16 + (lane >> 4) * 4;
     const bool on = row < A.Dv;  // (Dv is a multiple of 8)
 
     const int64_t slot = A.slots ? A.slots[b] : b;
@@ -143,7 +145,7 @@ gdr_step_kernel(const GdrStepArgs A, int parts) {
 
 hipError_t launch_gdr_step(bool bf16, const GdrStepArgs& A,
                            hipStream_t stream) {
-    const int parts = (A.Dv + ROWS - 1) / ROWS;
+    const uint32_t parts = uint32_t(A.Dv + ROWS - 1) / ROWS;
     const dim3 grid(unsigned(A.B * A.Hv * parts));
 #define RWKV7M_GDR(E, KQ)                                                   \
     hipLaunchKernelGGL((gdr_step_kernel<E, KQ>), grid, dim3(NT), 0, stream, \
