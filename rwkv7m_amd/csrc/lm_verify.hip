@@ -6,14 +6,16 @@
 // Two launches.  The first reads every row once, in parts of 8192 logits, and
 // leaves each part's largest logit and sum; the second decides and draws: the
 // workgroups of a sequence, one a part of the vocabulary, each find the number
-// taken (a few sums), add up their part of the one row that is drawn from, and
-// the last of them to finish finds the token within its part.  Which one is
-// last changes nothing: the parts' sums are added in their order.
+// taken (a few sums), add up their part of the one row that is drawn from in
+// segments of 64 vectors, and the last of them to finish finds the token within
+// its segment.  Which one is last changes nothing: the segments' sums are added
+// in their order.
 //
 // What is drawn lies next to a border of a sum over 65536 numbers, one sample
-// in 500 within fp32's rounding of it: exponentials and sums are float64 (a
-// wave takes float64 multiply-adds at fp32's rate; 11 of them an exponential).
-// The rows' bytes stay what bounds the call.
+// in 500 within fp32's rounding of it: exponentials and sums are float64, which
+// costs the first launch as much as its bytes (a wave takes float64
+// multiply-adds at fp32's rate, 16 operations a logit).  An exponential off by
+// 1e-12 moves one sample in ten million.
 
 #include "lm_rows.h"
 
@@ -23,24 +25,27 @@ namespace {
 constexpr int NT = 256;
 constexpr int PART = kVerifyPart;
 
-// 2^t for t <= 0: 2^round(t) times the exponential series of the rest, |rest|
-// ln 2 <= 0.347, off by 0.347^12 / 12! = 6e-15.
+// 2^t for t <= 0: 2^round(t) times the polynomial that meets 2^x at the nine
+// Chebyshev nodes of [-1/2, 1/2], off by 1.1e-12.  The rounding and the power
+// are additions (1.5 2^52 leaves the whole number in the low bits; it is added
+// to the exponent), since float64's rounding, conversion and scaling
+// instructions run at a fraction of its additions' rate.  Below -1000 2^-1000.
 __device__ __forceinline__ double exp2_64(double t) {
-    t = __builtin_fmax(t, -1100.0);
-    const double n = __builtin_rint(t), y = (t - n) * 0.6931471805599453094;
-    double s = 1.0 / 39916800.0;
-    s = __builtin_fma(s, y, 1.0 / 3628800.0);
-    s = __builtin_fma(s, y, 1.0 / 362880.0);
-    s = __builtin_fma(s, y, 1.0 / 40320.0);
-    s = __builtin_fma(s, y, 1.0 / 5040.0);
-    s = __builtin_fma(s, y, 1.0 / 720.0);
-    s = __builtin_fma(s, y, 1.0 / 120.0);
-    s = __builtin_fma(s, y, 1.0 / 24.0);
-    s = __builtin_fma(s, y, 1.0 / 6.0);
-    s = __builtin_fma(s, y, 0.5);
-    s = __builtin_fma(s, y, 1.0);
-    s = __builtin_fma(s, y, 1.0);
-    return __builtin_amdgcn_ldexp(s, int(n));
+    t = t > -1000.0 ? t : -1000.0;
+    const double big = 6755399441055744.0, n = t + big, x = t - (n - big);
+    double s = 1.325522488583589e-06;
+    s = __builtin_fma(s, x, 1.5310079402360393e-05);
+    s = __builtin_fma(s, x, 0.00015403455852412883);
+    s = __builtin_fma(s, x, 0.0013333450568000116);
+    s = __builtin_fma(s, x, 0.009618129159402631);
+    s = __builtin_fma(s, x, 0.055504109412059334);
+    s = __builtin_fma(s, x, 0.2402265069581299);
+    s = __builtin_fma(s, x, 0.6931471805459335);
+    s = __builtin_fma(s, x, 1.0);
+    const uint64_t u = __builtin_bit_cast(uint64_t, s);
+    const uint32_t k = uint32_t(__builtin_bit_cast(uint64_t, n));
+    return __builtin_bit_cast(
+        double, u + (uint64_t(k << 20) << 32));
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -122,6 +127,13 @@ verify_stats_kernel(const LmVerifyArgs A) {
     if (target ? i > n : i - A.K - 1 >= n) return;
     const E* x = target ? row_of<E>(A.target, A.tr, b * (A.K + 1) + i)
                         : row_of<E>(A.draft, A.dr, b * A.K + i - A.K - 1);
+    // (the row's drafted token, for the second launch to have at hand)
+    const int which = target ? i : i - A.K - 1;
+    if (part == 0 && threadIdx.x == 0 && which < n) {
+        const int64_t word = A.tokens[b * A.K + which];
+        A.picked[row] = word >= 0 && word < A.V ? load_f(x + word)
+                                                : -__builtin_inff();
+    }
     const Part<E> P(x, int64_t(part) * PART, A.V);
     float m = -__builtin_inff();
 #pragma unroll
@@ -171,21 +183,38 @@ struct RowSums {
     int id;
     double inv;
 };
+// By 16 lanes, the same in each.
 __device__ __forceinline__ RowSums join(const LmVerifyStats* s, int parts,
                                         double c) {
+    const int l = threadIdx.x % 16;
     float m = -__builtin_inff();
-    int id = -1;
-    for (int i = 0; i < parts; ++i) {
-        const float x = s[i].largest;
-        if (x > m) id = s[i].id;
-        m = larger(m, x);
+    int id = 0x7fffffff;
+    double sum = 0.0;
+    for (int i = l; i < parts; i += 16) {
+        const LmVerifyStats a = s[i];
+        if (a.largest > m || a.largest != a.largest) {
+            // (what came before, next to the new largest)
+            sum = m > -__builtin_inff()
+                      ? sum * exp2_64((double(m) - double(a.largest)) * c)
+                      : 0.0;
+            sum += a.sum;
+            m = larger(m, a.largest);
+            id = a.id;
+        } else if (a.largest > -__builtin_inff()) {
+            sum += a.sum * exp2_64((double(a.largest) - double(m)) * c);
+        }
     }
+    const float own = m;
+    m = lanes_larger<16>(m);
+    id = lanes_fold<16>(own == m ? id : 0x7fffffff,
+                        [](int a, int b) { return a < b ? a : b; });
     if (!(m > -__builtin_inff() && m < __builtin_inff()))
         return {__builtin_nanf(""), -1, __builtin_nan("")};
-    double sum = 0.0;
-    for (int i = 0; i < parts; ++i)
-        if (s[i].largest > -__builtin_inff())
-            sum += s[i].sum * exp2_64((double(s[i].largest) - double(m)) * c);
+    sum = own > -__builtin_inff()
+              ? sum * exp2_64((double(own) - double(m)) * c)
+              : 0.0;
+#pragma unroll
+    for (int k = 8; k >= 1; k >>= 1) sum += __shfl_xor(sum, k);
     return {m, id, 1.0 / sum};
 }
 __device__ __forceinline__ double prob(const RowSums& r, float x, double c) {
@@ -194,10 +223,35 @@ __device__ __forceinline__ double prob(const RowSums& r, float x, double c) {
 
 struct DrawShared {
     RowSums rows[2 * kVerifyMostDrafts + 1];
+    float picked[2 * kVerifyMostDrafts + 1];
     int taken, last;
     double waves[2][NT / 64];
-    int found[NT / 64], positive[NT / 64];
+    int found[NT / 64], positive[NT / 64], segment;
+    double before;
 };
+
+// The sum over the workgroup, and over the threads before the calling one.
+__device__ __forceinline__ double block_scan(double x, double* s,
+                                             double* before) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    double upto = x;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const double z = __shfl_up(upto, k);
+        if (lane >= k) upto += z;
+    }
+    __syncthreads();
+    if (lane == 63) s[wave] = upto;
+    __syncthreads();
+    double ahead = 0.0, all = 0.0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w == wave) ahead = all;
+        all += s[w];
+    }
+    *before = ahead + (upto - x);
+    return all;
+}
 
 template <typename E>
 __global__ void __launch_bounds__(NT)
@@ -212,11 +266,14 @@ verify_draw_kernel(const LmVerifyArgs A) {
     const int n = drafted(A, b), rows = A.draft ? 2 * A.K + 1 : A.K + 1;
     const int64_t* drafts = A.tokens + b * A.K;
     const LmVerifyStats* stats = A.stats + b * rows * A.parts;
-    // (rows 0 .. n of the target, then those of the draft)
-    for (int i = t; i < n + 1 + (A.draft ? n : 0); i += NT) {
-        const int row = i <= n ? i : A.K + 1 + i - (n + 1);
-        S.rows[i] = join(stats + int64_t(row) * A.parts, A.parts, A.c);
+    // (also those past n, which hold anything and are not used: the loads do
+    // not wait for n)
+    for (int i = t / 16; i < (rows + 15) / 16 * 16; i += NT / 16) {
+        const int row = i < rows ? i : rows - 1;
+        const RowSums r = join(stats + int64_t(row) * A.parts, A.parts, A.c);
+        if (t % 16 == 0 && i < rows) S.rows[i] = r;
     }
+    if (t < rows) S.picked[t] = A.picked[b * rows + t];
     __syncthreads();
     if (wave == 0) {
         // draft `lane` of each 64
@@ -230,7 +287,7 @@ verify_draw_kernel(const LmVerifyArgs A) {
                 if (i < n) {
                     const int64_t x = drafts[i];
                     const bool word = x >= 0 && x < A.V;
-                    const RowSums &r = S.rows[i];
+                    const RowSums& r = S.rows[i];
                     if (A.greedy) {
                         p = word && x == r.id ? 1.0 : 0.0;
                         q = 1.0;
@@ -238,14 +295,10 @@ verify_draw_kernel(const LmVerifyArgs A) {
                     } else {
                         q = 1.0;
                         if (word) {
-                            p = prob(r, load_f(row_of<E>(A.target, A.tr,
-                                                         b * (A.K + 1) + i) + x),
-                                     A.c);
+                            p = prob(r, S.picked[i], A.c);
                             if (A.draft)
-                                q = prob(S.rows[n + 1 + i],
-                                         load_f(row_of<E>(A.draft, A.dr,
-                                                          b * A.K + i) + x),
-                                         A.c);
+                                q = prob(S.rows[A.K + 1 + i],
+                                         S.picked[A.K + 1 + i], A.c);
                         }
                         stop = !(double(A.accept[b * A.K + i]) * q < p);
                     }
@@ -263,16 +316,16 @@ verify_draw_kernel(const LmVerifyArgs A) {
     const RowSums P = S.rows[m];
     const bool residual = m < n;
     const bool with_q = residual && A.draft;
-    const RowSums Q = with_q ? S.rows[n + 1 + m] : RowSums{0.f, 0, 0.0};
+    const RowSums Q = with_q ? S.rows[A.K + 1 + m] : RowSums{0.f, 0, 0.0};
     const bool none = !(P.largest == P.largest) || !(Q.largest == Q.largest);
     int64_t* out = A.out + b * (A.K + 1);
     const auto finish = [&](int64_t token) {
-        for (int i = 0; i <= A.K; ++i)
-            out[i] = i < m ? drafts[i] : i == m ? token : -1;
-        A.taken[b] = m;
+        static_assert(2 * kVerifyMostDrafts + 1 < NT, "a thread a token");
+        if (t <= A.K) out[t] = t < m ? drafts[t] : t == m ? token : -1;
+        if (t == 0) A.taken[b] = m;
     };
     if (A.greedy || none) {
-        if (part == 0 && t == 0) finish(none ? -1 : P.id);
+        if (part == 0) finish(none ? -1 : P.id);
         return;
     }
     const int64_t without = residual && !A.draft ? drafts[m] : -1;
@@ -283,115 +336,128 @@ verify_draw_kernel(const LmVerifyArgs A) {
         if (with_q) return __builtin_fmax(p - prob(Q, yv, A.c), 0.0);
         return j == without ? 0.0 : p;
     };
-    double sum = 0.0, whole = 0.0;
+    // segments of the vocabulary: a wave's vectors i of its part, in their
+    // order
+    constexpr int nv = Part<E>::nv, per_part = nv * (NT / 64),
+                  width = PART / per_part;
+    double* masses = A.masses + b * 2 * A.parts * kVerifySegments;
+    const int64_t segments = int64_t(A.parts) * per_part;
     {
         const Part<E> a(x, int64_t(part) * PART, A.V);
         const Part<E> d(y, int64_t(part) * PART, A.V);
 #pragma unroll
-        for (int i = 0; i < a.nv; ++i)
+        for (int i = 0; i < nv; ++i) {
+            double sum = 0.0, whole = 0.0;
 #pragma unroll
             for (int u = 0; u < a.n; ++u) {
                 double p;
                 sum += mass(a.v[i].get(u), d.v[i].get(u), a.id(i, u), p);
                 whole += p;
             }
-    }
-    sum = wave_sum(sum);
-    whole = wave_sum(whole);
-    if (lane == 0) {
-        S.waves[0][wave] = sum;
-        S.waves[1][wave] = whole;
-    }
-    __syncthreads();
-    double* masses = A.masses + b * 2 * A.parts;
-    if (t == 0) {
-        for (int w = 1; w < NT / 64; ++w) {
-            sum += S.waves[0][w];
-            whole += S.waves[1][w];
-        }
-        __hip_atomic_store(masses + part, sum, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(masses + A.parts + part, whole, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-        S.last = __hip_atomic_fetch_add(A.arrived + b, 1, __ATOMIC_ACQ_REL,
-                                        __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
-    }
-    __syncthreads();
-    if (!S.last) return;
-    // the sequence's last workgroup: the part that the draw falls into
-    const auto mass_of = [&](int which, int i) {
-        return __hip_atomic_load(masses + which * A.parts + i, __ATOMIC_RELAXED,
-                                 __HIP_MEMORY_SCOPE_AGENT);
-    };
-    double total = 0.0;
-    for (int i = 0; i < parts; ++i) total += mass_of(0, i);
-    // p where nothing is left of it (p = q, to rounding)
-    const bool plain = !(total > 0.0);
-    if (plain) {
-        total = 0.0;
-        for (int i = 0; i < parts; ++i) total += mass_of(1, i);
-    }
-    const float u_ = A.sample[b];
-    const double u = total * double(u_ > 0.f ? u_ : 0.f);
-    double before = 0.0;
-    int at = -1;
-    for (int i = 0; i < parts; ++i) {
-        const double w = mass_of(plain, i);
-        if (w > 0.0) at = i;  // (the last that holds anything, if none crosses)
-        if (before + w > u) break;
-        if (i + 1 < parts) before += w;
-    }
-    // its tokens in their order, PART / NT adjoining ones a thread
-    constexpr int per = PART / NT;
-    const int64_t j0 = int64_t(at) * PART + t * per;
-    double mine = 0.0;
-    const auto weight = [&](int64_t j) {
-        if (j >= A.V) return 0.0;
-        double p;
-        const double w = mass(load_f(x + j), load_f(y + j), j, p);
-        return plain ? p : w;
-    };
-#pragma unroll 4
-    for (int i = 0; i < per; ++i) mine += weight(j0 + i);
-    double upto = mine;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const double z = __shfl_up(upto, s);
-        if (lane >= s) upto += z;
-    }
-    __syncthreads();
-    if (lane == 63) S.waves[0][wave] = upto;
-    __syncthreads();
-    double ahead = 0.0;
-    for (int i = 0; i < at; ++i) ahead += mass_of(plain, i);
-    for (int w = 0; w < wave; ++w) ahead += S.waves[0][w];
-    // the first token whose sum passes u, and the last that has any mass
-    int found = 0x7fffffff, positive = -1;
-    if (mine > 0.0) {
-        double run = ahead + (upto - mine);
-        for (int i = 0; i < per; ++i) {
-            const double w = weight(j0 + i);
-            run += w;
-            if (w > 0.0) {
-                positive = int(j0 + i);
-                if (run > u && found == 0x7fffffff) found = int(j0 + i);
+            sum = wave_sum(sum);
+            whole = wave_sum(whole);
+            const int64_t at = int64_t(part) * per_part + i * (NT / 64) + wave;
+            if (lane == 0) {
+                __hip_atomic_store(masses + at, sum, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(masses + segments + at, whole,
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
     }
+    // Each wave's sums are out before the workgroup is counted.  They are
+    // written and read past the L2s (device-scope atomics), so that waiting for
+    // the writes is all it takes: a device-scope release would write the whole
+    // L2 back as well, a workgroup at a time (96 sequences: 73 us for 22).
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0)
+        S.last = __hip_atomic_fetch_add(A.arrived + b, 1, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    __syncthreads();
+    if (!S.last) return;
+    // the sequence's last workgroup: the segment that the draw falls into
+    const auto mass_of = [&](int which, int64_t i) {
+        return i < segments
+                   ? __hip_atomic_load(masses + which * segments + i,
+                                       __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT)
+                   : 0.0;
+    };
+    double total = 0.0, whole = 0.0, before;
+    const double first[2] = {mass_of(0, t), mass_of(1, t)};
+    const float u_ = A.sample[b];
+    for (int64_t i = 0; i < segments; i += NT) {
+        const double a = i ? mass_of(0, i + t) : first[0];
+        const double p = i ? mass_of(1, i + t) : first[1];
+        total += block_scan(a, S.waves[0], &before);
+        whole += block_scan(p, S.waves[1], &before);
+    }
+    // p where nothing is left of it (p = q, to rounding)
+    const bool plain = !(total > 0.0);
+    const double u = (plain ? whole : total) * double(u_ > 0.f ? u_ : 0.f);
+    if (t == 0) {
+        S.segment = 0x7fffffff;
+        S.last = -1;
+        S.before = 0.0;
+    }
+    double run = 0.0;
+    for (int64_t i = 0; i < segments; i += NT) {
+        const double w = i ? mass_of(plain, i + t) : plain ? first[1] : first[0];
+        // (the barriers in here order the words of S set above)
+        const double all = block_scan(w, S.waves[0], &before);
+        if (w > 0.0) {
+            if (run + before + w > u) atomicMin(&S.segment, int(i + t));
+            atomicMax(&S.last, int(i + t));
+        }
+        __syncthreads();
+        if (S.segment == int(i + t)) S.before = run + before;
+        run += all;
+        if (S.segment != 0x7fffffff) break;
+    }
+    __syncthreads();
+    // (the last that holds anything, if rounding lets none cross)
+    const int segment = S.segment != 0x7fffffff ? S.segment : S.last;
+    // its tokens in their order, the first whose sum passes u, and the last
+    // that has any mass
+    constexpr int per = (width + NT - 1) / NT;
+    int found = 0x7fffffff, positive = -1;
+    double w[per], mine = 0.0;
+    const int64_t j0 = int64_t(segment) * width + t * per;
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+        const int64_t j = j0 + i;
+        w[i] = 0.0;
+        if (t * per + i < width && j < A.V) {
+            double p;
+            const double r = mass(load_f(x + j), load_f(y + j), j, p);
+            w[i] = plain ? p : r;
+        }
+        mine += w[i];
+    }
+    block_scan(mine, S.waves[0], &before);
+    before += S.before;
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+        before += w[i];
+        if (w[i] > 0.0) {
+            positive = int(j0 + i);
+            if (before > u && found == 0x7fffffff) found = int(j0 + i);
+        }
+    }
     found = lanes_fold<64>(found, [](int a, int c) { return a < c ? a : c; });
-    positive = lanes_fold<64>(positive, [](int a, int c) { return a > c ? a : c; });
+    positive = lanes_fold<64>(positive,
+                              [](int a, int c) { return a > c ? a : c; });
     if (lane == 0) {
         S.found[wave] = found;
         S.positive[wave] = positive;
     }
     __syncthreads();
-    if (t == 0) {
-        for (int w = 1; w < NT / 64; ++w) {
-            found = S.found[w] < found ? S.found[w] : found;
-            positive = S.positive[w] > positive ? S.positive[w] : positive;
-        }
-        finish(found != 0x7fffffff ? found : positive);
+    for (int k = 0; k < NT / 64; ++k) {
+        found = S.found[k] < found ? S.found[k] : found;
+        positive = S.positive[k] > positive ? S.positive[k] : positive;
     }
+    finish(found != 0x7fffffff ? found : positive);
 }
 
 template <typename E>

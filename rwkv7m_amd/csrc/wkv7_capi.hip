@@ -2239,7 +2239,7 @@ int64_t rwkv7m_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V) {
         return -1;
     const int64_t parts = (V + rwkv7m::kVerifyPart - 1) / rwkv7m::kVerifyPart;
     return B * ((2 * K + 1) * parts * int64_t(sizeof(rwkv7m::LmVerifyStats)) +
-                2 * parts * 8 + 4);
+                2 * parts * rwkv7m::kVerifySegments * 8 + (2 * K + 1) * 4 + 4);
 }
 
 int rwkv7m_verify_drafts(int dtype, int64_t B, int64_t K, int64_t V,
@@ -2313,7 +2313,9 @@ int rwkv7m_verify_drafts(int dtype, int64_t B, int64_t K, int64_t V,
         A.stats = static_cast<rwkv7m::LmVerifyStats*>(workspace);
         A.masses = reinterpret_cast<double*>(A.stats + B * (2 * K + 1) *
                                                            A.parts);
-        A.arrived = reinterpret_cast<int*>(A.masses + B * 2 * A.parts);
+        A.picked = reinterpret_cast<float*>(
+            A.masses + B * 2 * A.parts * rwkv7m::kVerifySegments);
+        A.arrived = reinterpret_cast<int*>(A.picked + B * (2 * K + 1));
         return hip_status("verification of drafts launch",
                           rwkv7m::launch_lm_verify(
                               dtype == RWKV7M_DTYPE_BF16, A,

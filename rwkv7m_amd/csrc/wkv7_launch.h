@@ -351,6 +351,7 @@ struct LmDistillArgs {
 // Verification of drafted tokens (lm_verify.hip): rows b * (K + 1) + i of the
 // target's logits, b * K + i of the draft's.
 constexpr int kVerifyPart = 8192;  // logits of a row a workgroup reads
+constexpr int kVerifySegments = 32;  // sums of a part, at most
 constexpr int kVerifyMostDrafts = 64;
 struct LmVerifyStats {
     double sum;
@@ -369,7 +370,8 @@ struct LmVerifyArgs {
     int64_t *out, *taken;  // [B][K + 1], [B]
     float* chance;         // [B][K]
     LmVerifyStats* stats;  // workspaces: [B][rows][parts],
-    double* masses;        // [B][2][parts],
+    double* masses;        // [B][2][parts][kVerifySegments],
+    float* picked;         // [B][rows],
     int* arrived;          // [B]
 };
 hipError_t launch_lm_verify(bool bf16, const LmVerifyArgs& A,
