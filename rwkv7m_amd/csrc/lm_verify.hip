@@ -22,7 +22,7 @@
 namespace rwkv7m {
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 256, DRAW = 512;  // threads
 constexpr int PART = kVerifyPart;
 
 // 2^t for t <= 0: 2^round(t) times the polynomial that meets 2^x at the nine
@@ -48,10 +48,45 @@ __device__ __forceinline__ double exp2_64(double t) {
         double, u + (uint64_t(k << 20) << 32));
 }
 
+// x of another lane by a DPP control (0 where there is none), as two words.
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double x) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    i32x2 u = __builtin_bit_cast(i32x2, x);
+    u[0] = __builtin_amdgcn_update_dpp(0, u[0], CTRL, 0xf, 0xf, true);
+    u[1] = __builtin_amdgcn_update_dpp(0, u[1], CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, u);
+}
+__device__ __forceinline__ double lane64(double x, int lane) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    i32x2 u = __builtin_bit_cast(i32x2, x);
+    u[0] = __builtin_amdgcn_readlane(u[0], lane);
+    u[1] = __builtin_amdgcn_readlane(u[1], lane);
+    return __builtin_bit_cast(double, u);
+}
+// Sums over a wave without LDS: a shuffle of a double is two round trips
+// through it, and there are twelve in a sum's way (they were a third of a
+// single sequence's time).
+__device__ __forceinline__ double row_sum(double x) {  // rows of 16 lanes
+    x += dpp64<0x128>(x);
+    x += dpp64<0x124>(x);
+    x += dpp64<0x122>(x);
+    return x + dpp64<0x121>(x);
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-    return x;
+    x = row_sum(x);
+    return (lane64(x, 0) + lane64(x, 16)) + (lane64(x, 32) + lane64(x, 48));
+}
+// The sum over the lanes up to and with the calling one; `all`: over all.
+__device__ __forceinline__ double wave_scan(double x, double* all) {
+    x += dpp64<0x111>(x);
+    x += dpp64<0x112>(x);
+    x += dpp64<0x114>(x);
+    x += dpp64<0x118>(x);
+    const int row = threadIdx.x % 64 / 16;
+    const double a = lane64(x, 15), b = lane64(x, 31), c = lane64(x, 47);
+    *all = (a + b) + (c + lane64(x, 63));
+    return x + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? a + b : (a + b) + c);
 }
 
 // Drafts of sequence b: 0 .. K.
@@ -63,7 +98,7 @@ __device__ __forceinline__ int drafted(const LmVerifyArgs& A, int64_t b) {
 
 // A part of a row in registers: vectors i * NT + thread of 16 bytes, -inf
 // behind the row's end.
-template <typename E>
+template <typename E, int NT>
 struct Part {
     static constexpr int n = Vec<E>::n, nv = PART / n / NT;
     Vec<E> v[nv];
@@ -134,7 +169,7 @@ verify_stats_kernel(const LmVerifyArgs A) {
         A.picked[row] = word >= 0 && word < A.V ? load_f(x + word)
                                                 : -__builtin_inff();
     }
-    const Part<E> P(x, int64_t(part) * PART, A.V);
+    const Part<E, NT> P(x, int64_t(part) * PART, A.V);
     float m = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < P.nv; ++j)
@@ -213,9 +248,7 @@ __device__ __forceinline__ RowSums join(const LmVerifyStats* s, int parts,
     sum = own > -__builtin_inff()
               ? sum * exp2_64((double(own) - double(m)) * c)
               : 0.0;
-#pragma unroll
-    for (int k = 8; k >= 1; k >>= 1) sum += __shfl_xor(sum, k);
-    return {m, id, 1.0 / sum};
+    return {m, id, 1.0 / row_sum(sum)};
 }
 __device__ __forceinline__ double prob(const RowSums& r, float x, double c) {
     return exp2_64((double(x) - double(r.largest)) * c) * r.inv;
@@ -225,36 +258,11 @@ struct DrawShared {
     RowSums rows[2 * kVerifyMostDrafts + 1];
     float picked[2 * kVerifyMostDrafts + 1];
     int taken, last;
-    double waves[2][NT / 64];
-    int found[NT / 64], positive[NT / 64], segment;
-    double before;
 };
 
-// The sum over the workgroup, and over the threads before the calling one.
-__device__ __forceinline__ double block_scan(double x, double* s,
-                                             double* before) {
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    double upto = x;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const double z = __shfl_up(upto, k);
-        if (lane >= k) upto += z;
-    }
-    __syncthreads();
-    if (lane == 63) s[wave] = upto;
-    __syncthreads();
-    double ahead = 0.0, all = 0.0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
-        if (w == wave) ahead = all;
-        all += s[w];
-    }
-    *before = ahead + (upto - x);
-    return all;
-}
 
 template <typename E>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(DRAW)
 verify_draw_kernel(const LmVerifyArgs A) {
     __shared__ DrawShared S;
     const int64_t id = grid_row();
@@ -268,11 +276,12 @@ verify_draw_kernel(const LmVerifyArgs A) {
     const LmVerifyStats* stats = A.stats + b * rows * A.parts;
     // (also those past n, which hold anything and are not used: the loads do
     // not wait for n)
-    for (int i = t / 16; i < (rows + 15) / 16 * 16; i += NT / 16) {
+    for (int i = t / 16; i < (rows + 15) / 16 * 16; i += DRAW / 16) {
         const int row = i < rows ? i : rows - 1;
         const RowSums r = join(stats + int64_t(row) * A.parts, A.parts, A.c);
         if (t % 16 == 0 && i < rows) S.rows[i] = r;
     }
+    static_assert(2 * kVerifyMostDrafts + 1 <= DRAW, "");
     if (t < rows) S.picked[t] = A.picked[b * rows + t];
     __syncthreads();
     if (wave == 0) {
@@ -320,8 +329,9 @@ verify_draw_kernel(const LmVerifyArgs A) {
     const bool none = !(P.largest == P.largest) || !(Q.largest == Q.largest);
     int64_t* out = A.out + b * (A.K + 1);
     const auto finish = [&](int64_t token) {
-        static_assert(2 * kVerifyMostDrafts + 1 < NT, "a thread a token");
-        if (t <= A.K) out[t] = t < m ? drafts[t] : t == m ? token : -1;
+        if (wave == 0)
+            for (int i = t; i <= A.K; i += 64)
+                out[i] = i < m ? drafts[i] : i == m ? token : -1;
         if (t == 0) A.taken[b] = m;
     };
     if (A.greedy || none) {
@@ -338,13 +348,14 @@ verify_draw_kernel(const LmVerifyArgs A) {
     };
     // segments of the vocabulary: a wave's vectors i of its part, in their
     // order
-    constexpr int nv = Part<E>::nv, per_part = nv * (NT / 64),
-                  width = PART / per_part;
+    constexpr int nv = Part<E, DRAW>::nv, per_part = nv * (DRAW / 64),
+                  width = PART / per_part, per = width / 64;
+    static_assert(per_part <= kVerifySegments && per == Vec<E>::n, "");
     double* masses = A.masses + b * 2 * A.parts * kVerifySegments;
     const int64_t segments = int64_t(A.parts) * per_part;
     {
-        const Part<E> a(x, int64_t(part) * PART, A.V);
-        const Part<E> d(y, int64_t(part) * PART, A.V);
+        const Part<E, DRAW> a(x, int64_t(part) * PART, A.V);
+        const Part<E, DRAW> d(y, int64_t(part) * PART, A.V);
 #pragma unroll
         for (int i = 0; i < nv; ++i) {
             double sum = 0.0, whole = 0.0;
@@ -356,7 +367,7 @@ verify_draw_kernel(const LmVerifyArgs A) {
             }
             sum = wave_sum(sum);
             whole = wave_sum(whole);
-            const int64_t at = int64_t(part) * per_part + i * (NT / 64) + wave;
+            const int64_t at = int64_t(part) * per_part + i * (DRAW / 64) + wave;
             if (lane == 0) {
                 __hip_atomic_store(masses + at, sum, __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
@@ -376,67 +387,87 @@ verify_draw_kernel(const LmVerifyArgs A) {
                                         __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
     __syncthreads();
     if (!S.last) return;
-    // the sequence's last workgroup: the segment that the draw falls into
-    const auto mass_of = [&](int which, int64_t i) {
-        return i < segments
-                   ? __hip_atomic_load(masses + which * segments + i,
-                                       __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT)
-                   : 0.0;
+    // The sequence's last workgroup, one wave of it: the segment that the draw
+    // falls into, four a lane and turn.
+    if (wave) return;
+    const auto four_masses = [&](int which, int64_t i, double (&w)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            w[k] = i + k < segments
+                       ? __hip_atomic_load(masses + which * segments + i + k,
+                                           __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT)
+                       : 0.0;
     };
-    double total = 0.0, whole = 0.0, before;
-    const double first[2] = {mass_of(0, t), mass_of(1, t)};
     const float u_ = A.sample[b];
-    for (int64_t i = 0; i < segments; i += NT) {
-        const double a = i ? mass_of(0, i + t) : first[0];
-        const double p = i ? mass_of(1, i + t) : first[1];
-        total += block_scan(a, S.waves[0], &before);
-        whole += block_scan(p, S.waves[1], &before);
+    double w0[2][4], total = 0.0, whole = 0.0;
+    four_masses(0, 4 * lane, w0[0]);
+    four_masses(1, 4 * lane, w0[1]);
+    for (int64_t i = 0; i < segments; i += 256) {
+        double w[2][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            w[0][k] = w0[0][k];
+            w[1][k] = w0[1][k];
+        }
+        if (i) {
+            four_masses(0, i + 4 * lane, w[0]);
+            four_masses(1, i + 4 * lane, w[1]);
+        }
+        total += wave_sum((w[0][0] + w[0][1]) + (w[0][2] + w[0][3]));
+        whole += wave_sum((w[1][0] + w[1][1]) + (w[1][2] + w[1][3]));
     }
     // p where nothing is left of it (p = q, to rounding)
     const bool plain = !(total > 0.0);
     const double u = (plain ? whole : total) * double(u_ > 0.f ? u_ : 0.f);
-    if (t == 0) {
-        S.segment = 0x7fffffff;
-        S.last = -1;
-        S.before = 0.0;
-    }
-    double run = 0.0;
-    for (int64_t i = 0; i < segments; i += NT) {
-        const double w = i ? mass_of(plain, i + t) : plain ? first[1] : first[0];
-        // (the barriers in here order the words of S set above)
-        const double all = block_scan(w, S.waves[0], &before);
-        if (w > 0.0) {
-            if (run + before + w > u) atomicMin(&S.segment, int(i + t));
-            atomicMax(&S.last, int(i + t));
+    // the first whose running sum passes u; the last that holds anything, if
+    // rounding lets none pass
+    double run = 0.0, before = 0.0;
+    int segment = -1, last = -1;
+    for (int64_t i = 0; i < segments && segment < 0; i += 256) {
+        double w[4], all;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = plain ? w0[1][k] : w0[0][k];
+        if (i) four_masses(plain, i + 4 * lane, w);
+        const double sum = (w[0] + w[1]) + (w[2] + w[3]);
+        double ahead = run + wave_scan(sum, &all) - sum;
+        int mine = -1;
+        double at = 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (mine < 0 && w[k] > 0.0 && ahead + w[k] > u) {
+                mine = int(i) + 4 * lane + k;
+                at = ahead;
+            }
+            ahead += w[k];
+            if (w[k] > 0.0) last = int(i) + 4 * lane + k;
         }
-        __syncthreads();
-        if (S.segment == int(i + t)) S.before = run + before;
+        const uint64_t passed = __builtin_amdgcn_ballot_w64(mine >= 0);
+        if (passed) {
+            const int l = __builtin_ctzll(passed);
+            segment = __builtin_amdgcn_readlane(mine, l);
+            before = lane64(at, l);
+        }
         run += all;
-        if (S.segment != 0x7fffffff) break;
     }
-    __syncthreads();
-    // (the last that holds anything, if rounding lets none cross)
-    const int segment = S.segment != 0x7fffffff ? S.segment : S.last;
-    // its tokens in their order, the first whose sum passes u, and the last
-    // that has any mass
-    constexpr int per = (width + NT - 1) / NT;
-    int found = 0x7fffffff, positive = -1;
-    double w[per], mine = 0.0;
-    const int64_t j0 = int64_t(segment) * width + t * per;
+    if (segment < 0)
+        segment = lanes_fold<64>(last, [](int a, int c) { return a > c ? a : c; });
+    // its tokens in their order, adjoining ones a lane
+    const int64_t j0 = int64_t(segment) * width + lane * per;
+    double w[per], mine = 0.0, all;
 #pragma unroll
     for (int i = 0; i < per; ++i) {
         const int64_t j = j0 + i;
         w[i] = 0.0;
-        if (t * per + i < width && j < A.V) {
+        if (j < A.V) {
             double p;
             const double r = mass(load_f(x + j), load_f(y + j), j, p);
             w[i] = plain ? p : r;
         }
         mine += w[i];
     }
-    block_scan(mine, S.waves[0], &before);
-    before += S.before;
+    before += wave_scan(mine, &all) - mine;
+    int found = 0x7fffffff, positive = -1;
 #pragma unroll
     for (int i = 0; i < per; ++i) {
         before += w[i];
@@ -448,15 +479,6 @@ verify_draw_kernel(const LmVerifyArgs A) {
     found = lanes_fold<64>(found, [](int a, int c) { return a < c ? a : c; });
     positive = lanes_fold<64>(positive,
                               [](int a, int c) { return a > c ? a : c; });
-    if (lane == 0) {
-        S.found[wave] = found;
-        S.positive[wave] = positive;
-    }
-    __syncthreads();
-    for (int k = 0; k < NT / 64; ++k) {
-        found = S.found[k] < found ? S.found[k] : found;
-        positive = S.positive[k] > positive ? S.positive[k] : positive;
-    }
     finish(found != 0x7fffffff ? found : positive);
 }
 
@@ -468,7 +490,7 @@ hipError_t launch(const LmVerifyArgs& A, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(verify_draw_kernel<E>,
-                       row_grid(A.B * (A.greedy ? 1 : A.parts)), dim3(NT), 0,
+                       row_grid(A.B * (A.greedy ? 1 : A.parts)), dim3(DRAW), 0,
                        stream, A);
     return hipGetLastError();
 }
