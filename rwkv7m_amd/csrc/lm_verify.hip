@@ -31,7 +31,7 @@ constexpr int PART = kVerifyPart;
 // to the exponent), since float64's rounding, conversion and scaling
 // instructions run at a fraction of its additions' rate.  Below -1000 2^-1000.
 __device__ __forceinline__ double exp2_64(double t) {
-    t = t > -1000.0 ? t : -1000.0;
+    t = __builtin_fmax(t, -1000.0);
     const double big = 6755399441055744.0, n = t + big, x = t - (n - big);
     double s = 1.325522488583589e-06;
     s = __builtin_fma(s, x, 1.5310079402360393e-05);
@@ -153,9 +153,11 @@ verify_stats_kernel(const LmVerifyArgs A) {
     const int rows = A.draft ? 2 * A.K + 1 : A.K + 1;
     const int64_t id = grid_row();
     if (id >= A.B * rows * A.parts) return;
-    const int part = int(id % A.parts);
-    const int64_t row = id / A.parts, b = row / rows;
-    const int i = int(row % rows);
+    // (32 bits, which hold every id: a 64-bit division is 130 instructions)
+    const uint32_t row32 = uint32_t(id) / uint32_t(A.parts);
+    const int part = int(uint32_t(id) % uint32_t(A.parts));
+    const int64_t row = row32, b = row32 / uint32_t(rows);
+    const int i = int(row32 % uint32_t(rows));
     if (i == 0 && part == 0 && threadIdx.x == 0) A.arrived[b] = 0;
     const int n = drafted(A, b);
     const bool target = i <= A.K;
@@ -268,8 +270,8 @@ verify_draw_kernel(const LmVerifyArgs A) {
     const int64_t id = grid_row();
     const int parts = A.greedy ? 1 : A.parts;
     if (id >= A.B * parts) return;
-    const int64_t b = id / parts;
-    const int part = int(id % parts), t = threadIdx.x;
+    const int64_t b = uint32_t(id) / uint32_t(parts);
+    const int part = int(uint32_t(id) % uint32_t(parts)), t = threadIdx.x;
     const int lane = t % 64, wave = t / 64;
     const int n = drafted(A, b), rows = A.draft ? 2 * A.K + 1 : A.K + 1;
     const int64_t* drafts = A.tokens + b * A.K;

@@ -2273,9 +2273,9 @@ int rwkv7m_verify_drafts(int dtype, int64_t B, int64_t K, int64_t V,
                                &A.dr));
         if (!greedy) RWKV7M_TRY(lm_temperature(fn, temperature));
         const int64_t need_ = rwkv7m_verify_drafts_workspace_bytes(B, K, V);
-        if (need_ < 0 || B * (2 * K + 1) > (int64_t(1) << 40) /
+        if (need_ < 0 || B * (2 * K + 1) > (int64_t(1) << 31) /
                                  ((V + rwkv7m::kVerifyPart - 1) /
-                                  rwkv7m::kVerifyPart) / 256)
+                                  rwkv7m::kVerifyPart))
             return fail(RWKV7M_ERR_INVALID_ARGUMENT,
                         std::string(fn) + ": sizes too large");
         if (B == 0) return RWKV7M_OK;
