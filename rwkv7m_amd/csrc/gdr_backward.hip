@@ -36,7 +36,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
             D[kb] = four(A.ds_t + (head * A.Dv + v) * A.Dk + k);
     }
 
-    OwnColumn<E, KT> column(A, A.dout, b, h, v, wave < 4);
+    OwnColumn<E, KT> column(A, A.dout, b, h, v);
     column.fetch(chunks - 1, lane);
 
     chain<E, KT>(
@@ -52,7 +52,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
             *reinterpret_cast<f32x4_t*>(keep + 16 * kb + 4 * q) = D[kb];
 
         f32x4_t dO[4], dX[4], dR[4];
-        column.take(L, c - 1, wave, lane, dO);
+        column.take(L, c, c - 1, wave, lane, dO);
         // dX: t = 4q + e, v = r
         {
             Frag<NI> f[2];

@@ -83,28 +83,33 @@ struct OwnColumn {
     E next[16];
 
     __device__ __forceinline__ OwnColumn(const GdrArgs& A, const GdrTensor& x,
-                                         int64_t b, int64_t h, int v, bool own)
-        : base(at<E>(x, b, h, 0) + v), stride(x.st), T(A.T),
-          on(own && v < A.Dv) {}
+                                         int64_t b, int64_t h, int v)
+        : base(at<E>(x, b, h, 0) + near(v, A.Dv - 1)), stride(x.st), T(A.T),
+          on(v < A.Dv) {}
+    static __device__ __forceinline__ int64_t token(int64_t c, int i,
+                                                    int lane) {
+        return c * C + 16 * (i >> 2) + 4 * (lane >> 4) + (i & 3);
+    }
     __device__ __forceinline__ void fetch(int64_t c, int lane) {
         if constexpr (!kColumns<E, KT>)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int64_t t =
-                    c * C + 16 * (i >> 2) + 4 * (lane >> 4) + (i & 3);
-                next[i] = on && t >= 0 && t < T ? base[t * stride] : E(0);
+                const int64_t t = token(c, i, lane);
+                next[i] = base[(t < 0 ? 0 : t < T ? t : T - 1) * stride];
             }
     }
     // The chunk's values, with the loads of chunk `then`, if any, begun.
-    __device__ __forceinline__ void take(const ChainChunk<E, KT>& L, int64_t then,
-                                         int wave, int lane,
+    __device__ __forceinline__ void take(const ChainChunk<E, KT>& L, int64_t c,
+                                         int64_t then, int wave, int lane,
                                          f32x4_t (&x)[4]) {
         if constexpr (kColumns<E, KT>) {
 #pragma unroll
             for (int tb = 0; tb < 4; ++tb) x[tb] = L.v.values(tb, wave, lane);
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = load_f(&next[i]);
+            for (int i = 0; i < 16; ++i)
+                x[i >> 2][i & 3] =
+                    on && token(c, i, lane) < T ? load_f(&next[i]) : 0.f;
             fetch(then, lane);
         }
     }
@@ -131,35 +136,38 @@ struct Bring {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
-            if constexpr (kColumns<E, KT>) {
-                v[i].clear();
-                if (row < valid && v0 + col < A.Dv)
-                    v[i].load(at<E>(x, b, h, t0 + row) + v0 + col);
-            }
+            if constexpr (kColumns<E, KT>)
+                v[i].load(at<E>(x, b, h, t0 + near(row, valid - 1)) +
+                          near(v0 + col, A.Dv - 8));
+            // (the upper right quarters, which nothing reads, hold the lower
+            // left ones' first columns again)
+            const int at_col = row < 32 ? col % 32 : col;
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                t[i * NC + n] = u32x4_t{0, 0, 0, 0};
-                p[i * NC + n] = u32x4_t{0, 0, 0, 0};
-                if (row >= 32 || col < 32) {
-                    t[i * NC + n] =
-                        *reinterpret_cast<const u32x4_t*>(&M.t[n][row][col]);
-                    p[i * NC + n] =
-                        *reinterpret_cast<const u32x4_t*>(&M.p[n][row][col]);
-                }
+                t[i * NC + n] =
+                    *reinterpret_cast<const u32x4_t*>(&M.t[n][row][at_col]);
+                p[i * NC + n] =
+                    *reinterpret_cast<const u32x4_t*>(&M.p[n][row][at_col]);
             }
         }
         first = M.first[thread & 63];
         last = M.last[thread & 63];
         beta = M.beta[thread & 63];
     }
-    __device__ __forceinline__ void store(ChainChunk<E, KT>& L,
+    __device__ __forceinline__ void store(const GdrArgs& A, ChainChunk<E, KT>& L,
+                                          int64_t c, int v0,
                                           int thread) const {
-        k.store(L.k, thread);
-        q.store(L.q, thread);
+        const int valid = int(A.T - c * C < C ? A.T - c * C : C);
+        k.store(L.k, valid, A.Dk, thread);
+        q.store(L.q, valid, A.Dk, thread);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
-            if constexpr (kColumns<E, KT>) L.v.put(row, col, v[i]);
+            if constexpr (kColumns<E, KT>) {
+                Eight<E> x = v[i];
+                x.keep(row < valid && v0 + col < A.Dv);
+                L.v.put(row, col, x);
+            }
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 *reinterpret_cast<u32x4_t*>(&L.t.x[n][row][col]) =
@@ -176,6 +184,79 @@ struct Bring {
     }
 };
 
+// The six operands of T or P (or of their transposes) that hold anything, in
+// the order (0, 0) .. (3, 0), (2, 1), (3, 1); transposed (0, 0), (1, 0), (0, 1)
+// .. (3, 1).
+template <bool TRANSPOSED, int NC>
+__device__ __forceinline__ void triangle(const Rows<NC, 2>& x, int lane,
+                                         Frag<NC> (&f)[6]) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        const int tb = TRANSPOSED ? i < 2 ? i : i - 2 : i < 4 ? i : i - 2;
+        const int p = TRANSPOSED ? i >= 2 : i >= 4;
+        f[i] = TRANSPOSED ? x.columns(tb, p, lane) : x.rows(tb, p, lane);
+    }
+}
+// acc[tb] += (that matrix) f, f[p] the operand of pair p.
+template <bool TRANSPOSED, int NC, int NB>
+__device__ __forceinline__ void mul_triangle(f32x4_t (&acc)[4],
+                                             const Frag<NC> (&m)[6],
+                                             const Frag<NB> (&f)[2]) {
+    constexpr int most = NC > NB ? NC : NB;
+#pragma unroll
+    for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int j = s - i;
+            if (j < 0 || j >= NB) continue;
+#pragma unroll
+            for (int n = 0; n < 6; ++n) {
+                const int tb = TRANSPOSED ? n < 2 ? n : n - 2 : n < 4 ? n : n - 2;
+                const int p = TRANSPOSED ? n >= 2 : n >= 4;
+                acc[tb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, m[n].p[i]),
+                    __builtin_bit_cast(bf16x8_t, f[p].p[j]), acc[tb], 0, 0, 0);
+            }
+        }
+}
+// acc[tb] += f (that matrix)^T, f[p] the left operand.
+template <int NC, int NA>
+__device__ __forceinline__ void mul_by_triangle(f32x4_t (&acc)[4],
+                                                const Frag<NA> (&f)[2],
+                                                const Frag<NC> (&m)[6]) {
+    constexpr int most = NC > NA ? NC : NA;
+#pragma unroll
+    for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = s - i;
+            if (j < 0 || j >= NC) continue;
+#pragma unroll
+            for (int n = 0; n < 6; ++n) {
+                const int tb = n < 4 ? n : n - 2, p = n >= 4;
+                acc[tb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, f[p].p[i]),
+                    __builtin_bit_cast(bf16x8_t, m[n].p[j]), acc[tb], 0, 0, 0);
+            }
+        }
+}
+
+// The four token blocks' operands of pair p.
+template <int NI, int KT>
+__device__ __forceinline__ void blocks(const Rows<NI, KT>& x, int p, int lane,
+                                       Frag<NI> (&f)[4]) {
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb) f[tb] = x.rows(tb, p, lane);
+}
+// The operands of four column blocks from 4 n on, of pair p of tokens.
+template <int NI, int KT>
+__device__ __forceinline__ void column_blocks(const Rows<NI, KT>& x, int n,
+                                              int p, int lane,
+                                              Frag<NI> (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = x.columns(4 * n + i, p, lane);
+}
+
 // The loop of both: chunks first, first + step, .. (n of them).  own(L, c) by
 // the threads that own rows, with the chunk in L.
 template <typename E, int KT, typename F>
@@ -190,7 +271,7 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
         const int thread = threadIdx.x - BRING;
         Bring<E, KT> s;
         s.load(A, x, M[first], b, h, hk, first, v0, thread);
-        s.store(L[0], thread);
+        s.store(A, L[0], first, v0, thread);
         const auto ahead = [&](int64_t i) {
             const int64_t c = first + step * i;
             if (i < n) s.load(A, x, M[c], b, h, hk, c, v0, thread);
@@ -200,7 +281,8 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
         for (int64_t i = 0; i < n; ++i) {
             if constexpr (NB == 1) __syncthreads();
             if (i + 1 < n) {
-                s.store(L[NB == 2 ? (i + 1) & 1 : 0], thread);
+                s.store(A, L[NB == 2 ? (i + 1) & 1 : 0],
+                        first + step * (i + 1), v0, thread);
                 ahead(i + 2);
             }
             __syncthreads();

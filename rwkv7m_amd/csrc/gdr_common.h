@@ -113,6 +113,48 @@ __device__ __forceinline__ void mul(f32x4_t& acc, const Frag<NA>& a,
         }
 }
 
+// acc[m] += a[m] b for M independent sums in turn, so that none waits for the
+// product before it.
+template <int M, int NA, int NB>
+__device__ __forceinline__ void mul_each(f32x4_t (&acc)[M],
+                                         const Frag<NA> (&a)[M],
+                                         const Frag<NB>& b) {
+    constexpr int most = NA > NB ? NA : NB;
+#pragma unroll
+    for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = s - i;
+            if (j < 0 || j >= NB) continue;
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, a[m].p[i]),
+                    __builtin_bit_cast(bf16x8_t, b.p[j]), acc[m], 0, 0, 0);
+        }
+}
+// The same with the sums' operand on the right.
+template <int M, int NA, int NB>
+__device__ __forceinline__ void mul_each(f32x4_t (&acc)[M], const Frag<NA>& a,
+                                         const Frag<NB> (&b)[M]) {
+    constexpr int most = NA > NB ? NA : NB;
+#pragma unroll
+    for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = s - i;
+            if (j < 0 || j >= NB) continue;
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, a.p[i]),
+                    __builtin_bit_cast(bf16x8_t, b[m].p[j]), acc[m], 0, 0, 0);
+        }
+}
+// Nothing is moved over this place: operands are read from LDS where they are
+// written to be, ahead of the products that hide their way.
+__device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0); }
+
 __device__ __forceinline__ float exp2_of(double x) {
     return __builtin_amdgcn_exp2f(float(x));
 }
@@ -120,7 +162,10 @@ __device__ __forceinline__ float exp2_of(double x) {
 // --- memory -----------------------------------------------------------------
 
 // Eight adjoining elements of a row as they are held in memory, at 16-byte
-// aligned addresses (a row's places past Dk or Dv, and rows past T, are 0).
+// aligned addresses.  A row's places past Dk or Dv, and rows past T, are 0:
+// they are loaded from the nearest place that there is and cleared when the
+// value is used (keep).  A load under a condition has its register merged with
+// the zeros behind the branch, and is waited for there and then.
 template <typename E>
 struct Eight;
 template <>
@@ -129,7 +174,10 @@ struct Eight<bf16_t> {
     __device__ __forceinline__ void load(const bf16_t* p) {
         a = *reinterpret_cast<const u32x4_t*>(p);
     }
-    __device__ __forceinline__ void clear() { a = u32x4_t{0, 0, 0, 0}; }
+    __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = on ? a[i] : 0u;
+    }
     __device__ __forceinline__ Frag<1> planes() const { return {{a}}; }
     __device__ __forceinline__ float get(int i) const {
         return __uint_as_float(i & 1 ? a[i >> 1] & 0xffff0000u : a[i >> 1] << 16);
@@ -142,7 +190,13 @@ struct Eight<float> {
         a = *reinterpret_cast<const f32x4_t*>(p);
         b = *reinterpret_cast<const f32x4_t*>(p + 4);
     }
-    __device__ __forceinline__ void clear() { a = b = zero4(); }
+    __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = on ? a[i] : 0.f;
+            b[i] = on ? b[i] : 0.f;
+        }
+    }
     __device__ __forceinline__ Frag<3> planes() const { return split8<3>(a, b); }
     __device__ __forceinline__ float get(int i) const {
         return i < 4 ? a[i] : b[i - 4];
@@ -246,6 +300,10 @@ __device__ __forceinline__ void put4(Rows<NP, KT, R>& to, int row, int col,
             make_uint2(lo[n], hi[n]);
 }
 
+__device__ __forceinline__ int near(int i, int most) {
+    return i < most ? i : most;
+}
+
 // The share of a chunk's rows of one of `T` threads, on its way to LDS.
 template <typename E, int KT, int T>
 struct Staged {
@@ -258,20 +316,19 @@ struct Staged {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
             const int u = i * T + thread;
-            const int row = u / per_row, col = 8 * (u % per_row);
-            if (row < valid && col < dim)
-                v[i].load(base + row * stride + col);
-            else
-                v[i].clear();
+            v[i].load(base + near(u / per_row, valid - 1) * stride +
+                      near(8 * (u % per_row), dim - 8));
         }
     }
-    __device__ __forceinline__ void store(Rows<kIn<E>, KT>& to,
-                                          int thread) const {
+    __device__ __forceinline__ void store(Rows<kIn<E>, KT>& to, int valid,
+                                          int dim, int thread) const {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
             const int u = i * T + thread;
             const int row = u / per_row, col = 8 * (u % per_row);
-            const auto f = v[i].planes();
+            Eight<E> x = v[i];
+            x.keep(row < valid && col < dim);
+            const auto f = x.planes();
 #pragma unroll
             for (int m = 0; m < kIn<E>; ++m)
                 *reinterpret_cast<u32x4_t*>(&to.x[m][row][col]) = f.p[m];

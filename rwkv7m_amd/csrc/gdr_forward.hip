@@ -10,8 +10,9 @@ using namespace gdr;
 
 template <typename E, int KT, bool TRAIN>
 __global__ void __launch_bounds__(2 * BRING)
+__attribute__((amdgpu_waves_per_eu(2, 2)))
 gdr_forward_kernel(const GdrArgs A, int parts) {
-    constexpr int NC = kMade<E>, DKP = 32 * KT;
+    constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
     extern __shared__ char lds_raw[];
     const Place at_ = place(blockIdx.x, parts);
     const int64_t head = at_.head;
@@ -33,7 +34,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             S[kb] = four(A.s0 + (head * A.Dv + v) * A.Dk + k);
     }
     E* op = static_cast<E*>(A.o) + (b * A.T * A.Hv + h) * A.Dv;
-    OwnColumn<E, KT> column(A, A.v, b, h, v, wave < 4);
+    OwnColumn<E, KT> column(A, A.v, b, h, v);
     column.fetch(0, lane);
 
     chain<E, KT>(
@@ -44,7 +45,22 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         if (!has) return;
         const int64_t t0 = c * C;
         const int valid = int(A.T - t0 < C ? A.T - t0 : C);
-        Frag<NC> Sf[KT];
+        // What follows is in the order in which it is issued: each step's
+        // operands are on their way from LDS during the step before.  (bf16:
+        // fp32's three planes leave no registers for it.)
+        constexpr bool DEEP = NI == 1;
+        constexpr int TWO = DEEP ? 2 : 1;
+        Frag<NI> kf[TWO][4], qf[TWO][4];
+        Frag<NC> Tf[6], Pf[6], Sf[KT], Rf[2], Xf[2];
+        f32x4_t V[4], first[4], beta[4], B0[4], O[4], X[4];
+        if (DEEP) blocks(L.k, 0, lane, kf[0]);
+        column.take(L, c, c + 1, wave, lane, V);
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) {
+            first[tb] = four(L.first + 16 * tb + 4 * q);
+            beta[tb] = four(L.beta + 16 * tb + 4 * q);
+            B0[tb] = O[tb] = X[tb] = zero4();
+        }
 #pragma unroll
         for (int p = 0; p < KT; ++p) Sf[p] = split8<NC>(S[2 * p], S[2 * p + 1]);
         if constexpr (TRAIN) {
@@ -53,32 +69,33 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             for (int kb = 0; kb < 2 * KT; ++kb)
                 *reinterpret_cast<f32x4_t*>(to + 16 * kb + 4 * q) = S[kb];
         }
-        // R = beta (V - 2^G (K S^T)), t = 4q + e, v = r
-        f32x4_t X[4];
-        {
-            f32x4_t R[4], V[4];
-            column.take(L, c + 1, wave, lane, V);
+        // K S^T, t = 4q + e, v = r
 #pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                f32x4_t acc = zero4();
+        for (int p = 0; p < KT; ++p) {
+            if (!DEEP) blocks(L.k, p, lane, kf[0]);
+            else if (p + 1 < KT) blocks(L.k, p + 1, lane, kf[(p + 1) % TWO]);
+            else triangle<false>(L.t, lane, Tf);
+            hold();
+            mul_each(B0, kf[p % TWO], Sf[p]);
+        }
+        // R = beta (V - 2^G (K S^T)), X = T R
+        if (DEEP) blocks(L.q, 0, lane, qf[0]);
 #pragma unroll
-                for (int p = 0; p < KT; ++p)
-                    mul(acc, L.k.rows(tb, p, lane), Sf[p]);
-                R[tb] = four(L.beta + 16 * tb + 4 * q) *
-                        (V[tb] - four(L.first + 16 * tb + 4 * q) * acc);
-            }
-            // X = T R
-            Frag<NC> Rf[2];
+        for (int tb = 0; tb < 4; ++tb)
+            V[tb] = beta[tb] * (V[tb] - first[tb] * B0[tb]);
 #pragma unroll
-            for (int p = 0; p < 2; ++p) Rf[p] = split8<NC>(R[2 * p], R[2 * p + 1]);
+        for (int p = 0; p < 2; ++p) Rf[p] = split8<NC>(V[2 * p], V[2 * p + 1]);
+        if (!DEEP) triangle<false>(L.t, lane, Tf);
+        hold();
+        mul_triangle<false>(X, Tf, Rf);
+        // S Q^T, v = 4q + e, t = r
 #pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                X[tb] = zero4();
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    if (holds(false, tb, p))
-                        mul(X[tb], L.t.rows(tb, p, lane), Rf[p]);
-            }
+        for (int p = 0; p < KT; ++p) {
+            if (!DEEP) blocks(L.q, p, lane, qf[0]);
+            else if (p + 1 < KT) blocks(L.q, p + 1, lane, qf[(p + 1) % TWO]);
+            else column_blocks(L.k, 0, 0, lane, kf[0]);
+            hold();
+            mul_each(O, Sf[p], qf[p % TWO]);
         }
         if constexpr (TRAIN) {
             float* to = A.x + (head * chunks + c) * C * DVP + v;
@@ -86,48 +103,57 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             for (int i = 0; i < 16; ++i)
                 to[(16 * (i >> 2) + 4 * q + (i & 3)) * DVP] = X[i >> 2][i & 3];
         }
-        // O^T: v = 4q + e, t = r
-        {
-            Frag<NC> Xf[2];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) Xf[p] = split8<NC>(X[2 * p], X[2 * p + 1]);
-#pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                f32x4_t acc = zero4();
-#pragma unroll
-                for (int p = 0; p < KT; ++p)
-                    mul(acc, Sf[p], L.q.rows(tb, p, lane));
-                acc *= L.first[16 * tb + r];
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    if (holds(false, tb, p))
-                        mul(acc, Xf[p], L.p.rows(tb, p, lane));
-                const int t = 16 * tb + r, col = v0 + 4 * q;
-                if (t < valid && col < A.Dv) {
-                    E* to = op + (t0 + t) * A.Hv * A.Dv + col;
-                    acc *= A.scale;
-                    if constexpr (sizeof(E) == 4)
-                        *reinterpret_cast<f32x4_t*>(to) = acc;
-                    else
-                        *reinterpret_cast<uint2*>(to) =
-                            make_uint2(pack2(acc[0], acc[1]),
-                                       pack2(acc[2], acc[3]));
-                }
-            }
-        }
         // S^T = 2^G_L S^T + K^T (2^(G_L - G) X)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            Xf[p] = split8<NC>(X[2 * p], X[2 * p + 1]);
+            Rf[p] = split8<NC>(
+                X[2 * p] * four(L.last + 32 * p + 4 * q),
+                X[2 * p + 1] * four(L.last + 32 * p + 16 + 4 * q));
+        }
         const float whole = L.first[C - 1];
-        Frag<NC> Xf[2];
+        float own_first[4];
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) X[tb] *= four(L.last + 16 * tb + 4 * q);
+        for (int tb = 0; tb < 4; ++tb) own_first[tb] = L.first[16 * tb + r];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) Xf[p] = split8<NC>(X[2 * p], X[2 * p + 1]);
+        for (int n = 0; n < KT / 2; ++n) {
+            f32x4_t sum[4];
 #pragma unroll
-        for (int kb = 0; kb < 2 * KT; ++kb) {
-            S[kb] *= whole;
+            for (int i = 0; i < 4; ++i) sum[i] = S[4 * n + i] * whole;
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-                mul(S[kb], L.k.columns(kb, p, lane), Xf[p]);
+            for (int p = 0; p < 2; ++p) {
+                const int at = 2 * n + p;
+                if (!DEEP)
+                    column_blocks(L.k, n, p, lane, kf[0]);
+                else if (at + 1 < KT)
+                    column_blocks(L.k, (at + 1) / 2, (at + 1) & 1, lane,
+                                  kf[(at + 1) % TWO]);
+                else
+                    triangle<false>(L.p, lane, Pf);
+                hold();
+                mul_each(sum, kf[at % TWO], Rf[p]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[4 * n + i] = sum[i];
+        }
+        // O^T = scale (2^G (S Q^T) + X^T P^T)
+        if (!DEEP) triangle<false>(L.p, lane, Pf);
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) O[tb] *= own_first[tb];
+        mul_by_triangle(O, Xf, Pf);
+        E* to = op + t0 * A.Hv * A.Dv + v0 + 4 * q;
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) {
+            const int t = 16 * tb + r;
+            if (t < valid && v0 + 4 * q < A.Dv) {
+                O[tb] *= A.scale;
+                if constexpr (sizeof(E) == 4)
+                    *reinterpret_cast<f32x4_t*>(to + t * A.Hv * A.Dv) = O[tb];
+                else
+                    *reinterpret_cast<uint2*>(to + t * A.Hv * A.Dv) =
+                        make_uint2(pack2(O[tb][0], O[tb][1]),
+                                   pack2(O[tb][2], O[tb][3]));
+            }
         }
     });
     if (A.s_t && wave < 4 && on) {

@@ -68,7 +68,10 @@ struct Four<bf16_t> {
     __device__ __forceinline__ void load(const bf16_t* p) {
         a = *reinterpret_cast<const uint2*>(p);
     }
-    __device__ __forceinline__ void clear() { a = make_uint2(0, 0); }
+    __device__ __forceinline__ void keep(bool on) {
+        a.x = on ? a.x : 0u;
+        a.y = on ? a.y : 0u;
+    }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t u = i < 2 ? a.x : a.y;
         return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
@@ -82,7 +85,10 @@ template <>
 struct Four<float> {
     f32x4_t a;
     __device__ __forceinline__ void load(const float* p) { a = four(p); }
-    __device__ __forceinline__ void clear() { a = zero4(); }
+    __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = on ? a[i] : 0.f;
+    }
     __device__ __forceinline__ float get(int i) const { return a[i]; }
     __device__ __forceinline__ void put(Rows<3, 1>& to, int row,
                                         int col) const {
@@ -190,12 +196,9 @@ gdr_gradients_kernel(const GdrArgs A) {
             const int t = trow + i * step;
             xv[i] = four(x0 + t * DVP + v0 + tcol);
             r4[i] = four(r0 + t * DVP + v0 + tcol);
-            ov[i].clear();
-            vv[i].clear();
-            if (t < valid && v0 + tcol < A.Dv) {
-                ov[i].load(dop + t * A.dout.st + v0 + tcol);
-                vv[i].load(vp + t * A.v.st + v0 + tcol);
-            }
+            const int col = near(v0 + tcol, A.Dv - 4);
+            ov[i].load(dop + near(t, valid - 1) * A.dout.st + col);
+            vv[i].load(vp + near(t, valid - 1) * A.v.st + col);
         }
     };
     if constexpr (AHEAD) fetch(0);
@@ -214,12 +217,15 @@ gdr_gradients_kernel(const GdrArgs A) {
 #pragma unroll
         for (int i = 0; i < rows; ++i) {
             const int t = trow + i * step;
+            const bool on = t < valid && v0 + tcol < A.Dv;
+            ov[i].keep(on);
+            vv[i].keep(on);
             put4(L.x, t, tcol, xv[i]);
             put4(L.r, t, tcol, r4[i]);
             ov[i].put(L.o, t, tcol);
 #pragma unroll
             for (int e = 0; e < 4; ++e) rv[i] += r4[i][e] * vv[i].get(e);
-            if (t < valid && v0 + tcol < A.Dv)
+            if (on)
                 store4(dvp + t * A.Hv * A.Dv + v0, beta_own[i] * r4[i]);
         }
         __syncthreads();
@@ -273,8 +279,8 @@ gdr_gradients_kernel(const GdrArgs A) {
     }
     __syncthreads();
     if constexpr (!AHEAD) bring();
-    ks.store(L.k, threadIdx.x);
-    qs.store(L.q, threadIdx.x);
+    ks.store(L.k, valid, A.Dk, threadIdx.x);
+    qs.store(L.q, valid, A.Dk, threadIdx.x);
     // N and dP with their decays, to LDS
     const auto place_tiles = [&](bool again) {
 #pragma unroll

@@ -54,16 +54,14 @@ gdr_prepare_kernel(const GdrArgs A) {
     // rows of k and q: places 32 p + 8q + i of token 16 tb + r, all loads
     // before the first is waited for
     const auto rows = [&](const GdrTensor& x, int tb, Eight<E> (&f)[KT]) {
-        const int t = 16 * tb + r;
-        const E* p = at<E>(x, b, hk, t0 + t);
+        const E* p = at<E>(x, b, hk, t0 + near(16 * tb + r, valid - 1));
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            const int col = 32 * i + 8 * q;
-            if (t < valid && col < A.Dk)
-                f[i].load(p + col);
-            else
-                f[i].clear();
-        }
+        for (int i = 0; i < KT; ++i)
+            f[i].load(p + near(32 * i + 8 * q, A.Dk - 8));
+    };
+    const auto planes = [&](Eight<E> x, int tb, int i) {
+        x.keep(16 * tb + r < valid && 32 * i + 8 * q < A.Dk);
+        return x.planes();
     };
     Eight<E> qw[KT], kj[4][KT];
 #pragma unroll
@@ -96,10 +94,10 @@ gdr_prepare_kernel(const GdrArgs A) {
     Frag<NI> qf[KT], kf[KT];  // the wave's own token block
 #pragma unroll
     for (int p = 0; p < KT; ++p) {
-        qf[p] = qw[p].planes();
+        qf[p] = planes(qw[p], wave, p);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j == wave) kf[p] = kj[j][p].planes();
+            if (j == wave) kf[p] = planes(kj[j][p], j, p);
     }
     const int own = 16 * wave + r;
     const double Gw = S.G[own];
@@ -109,7 +107,7 @@ gdr_prepare_kernel(const GdrArgs A) {
         f32x4_t a = zero4(), pt = zero4();
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
-            const Frag<NI> f = kj[j][p].planes();
+            const Frag<NI> f = planes(kj[j][p], j, p);
             mul(a, f, kf[p]);   // D(A^T): s = 4q + e, t = r
             mul(pt, f, qf[p]);  // D(P^T)
         }
