@@ -13,6 +13,7 @@ using namespace gdr;
 
 template <typename E, int KT>
 __global__ void __launch_bounds__(2 * BRING)
+__attribute__((amdgpu_waves_per_eu(2, 2)))
 gdr_backward_kernel(const GdrArgs A, int parts) {
     constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
     extern __shared__ char lds_raw[];
@@ -27,10 +28,10 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
     const int v0 = 64 * at_.part + 16 * wave, v = v0 + r;  // the lane's row
     const bool has = v0 < DVP, on = v < A.Dv;
 
-    f32x4_t D[2 * KT];  // D(D^T): k = 16 kb + 4q + e, v = r
+    f32x4_t D[2 * KT];  // D(D^T): k = spread(kb, 4q + e), v = r
 #pragma unroll
     for (int kb = 0; kb < 2 * KT; ++kb) {
-        const int k = 16 * kb + 4 * q;
+        const int k = spread(kb, 4 * q);
         D[kb] = zero4();
         if (A.ds_t && wave < 4 && on && k < A.Dk)
             D[kb] = four(A.ds_t + (head * A.Dv + v) * A.Dk + k);
@@ -49,86 +50,110 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
         float* keep = A.dstates + ((head * chunks + c) * DVP + v) * DKP;
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb)
-            *reinterpret_cast<f32x4_t*>(keep + 16 * kb + 4 * q) = D[kb];
+            *reinterpret_cast<f32x4_t*>(keep + spread(kb, 4 * q)) = D[kb];
 
-        f32x4_t dO[4], dX[4], dR[4];
+        // (the order of issue, as in the forward)
+        constexpr bool DEEP = NI == 1;
+        constexpr int TWO = DEEP ? 2 : 1;
+        Frag<NI> kf[TWO][4], of[2];
+        Frag<NC> Tf[6], Pf[6], Df[KT], xf[2], rf[2], sf[2];
+        f32x4_t dO[4], dX[4], dR[4], KD[4], first[4], last[4], beta[4];
         column.take(L, c, c - 1, wave, lane, dO);
-        // dX: t = 4q + e, v = r
-        {
-            Frag<NI> f[2];
+        if (DEEP) triangle<true>(L.p, lane, Pf);
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-                f[p] = split8<NI>(dO[2 * p], dO[2 * p + 1]);
-#pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                dX[tb] = zero4();
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    if (holds(true, tb, p))
-                        mul(dX[tb], L.p.columns(tb, p, lane), f[p]);
-            }
+        for (int tb = 0; tb < 4; ++tb) {
+            first[tb] = four(L.first + spread(tb, 4 * q));
+            last[tb] = four(L.last + spread(tb, 4 * q));
+            beta[tb] = four(L.beta + spread(tb, 4 * q));
+            dX[tb] = dR[tb] = KD[tb] = zero4();
         }
-        {
-            Frag<NC> Df[KT];
+        if (DEEP) blocks(L.k, 0, lane, kf[0]);
 #pragma unroll
-            for (int p = 0; p < KT; ++p)
-                Df[p] = split8<NC>(D[2 * p], D[2 * p + 1]);
-#pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                f32x4_t acc = zero4();
-#pragma unroll
-                for (int p = 0; p < KT; ++p)
-                    mul(acc, L.k.rows(tb, p, lane), Df[p]);
-                dX[tb] = A.scale * dX[tb] +
-                         four(L.last + 16 * tb + 4 * q) * acc;
-            }
+        for (int p = 0; p < 2; ++p) {
+            of[p] = split8<NI>(dO[2 * p], dO[2 * p + 1]);
+            sf[p] = split8<NC>(A.scale * first[2 * p] * dO[2 * p],
+                               A.scale * first[2 * p + 1] * dO[2 * p + 1]);
         }
-        {
-            Frag<NC> f[2];
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-                f[p] = split8<NC>(dX[2 * p], dX[2 * p + 1]);
+        for (int p = 0; p < KT; ++p) Df[p] = split8<NC>(D[2 * p], D[2 * p + 1]);
+        // P^T dO and K D^T, t = spread(tb, 4q + e), v = r
+        if (!DEEP) triangle<true>(L.p, lane, Pf);
+        hold();
+        mul_triangle<true>(dX, Pf, of);
 #pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                dR[tb] = zero4();
+        for (int p = 0; p < KT; ++p) {
+            if (!DEEP) blocks(L.k, p, lane, kf[0]);
+            else if (p + 1 < KT) blocks(L.k, p + 1, lane, kf[(p + 1) % TWO]);
+            else triangle<true>(L.t, lane, Tf);
+            hold();
+            mul_each(KD, kf[p % TWO], Df[p]);
+        }
+        // D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K: the first
+        // product while dX is made
+        const float whole = L.first[C - 1];
+        if (DEEP) column_blocks(L.q, 0, 0, lane, kf[0]);
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    if (holds(true, tb, p))
-                        mul(dR[tb], L.t.columns(tb, p, lane), f[p]);
+        for (int tb = 0; tb < 4; ++tb)
+            dX[tb] = A.scale * dX[tb] + last[tb] * KD[tb];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) xf[p] = split8<NC>(dX[2 * p], dX[2 * p + 1]);
+        if (!DEEP) triangle<true>(L.t, lane, Tf);
+        hold();
+        mul_triangle<true>(dR, Tf, xf);
+#pragma unroll
+        for (int n = 0; n < KT / 2; ++n) {
+            f32x4_t sum[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i] * whole;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int at = 2 * n + p;
+                if (!DEEP)
+                    column_blocks(L.q, n, p, lane, kf[0]);
+                else if (at + 1 < KT)
+                    column_blocks(L.q, (at + 1) / 2, (at + 1) & 1, lane,
+                                  kf[(at + 1) % TWO]);
+                else
+                    column_blocks(L.k, 0, 0, lane, kf[(at + 1) % TWO]);
+                hold();
+                mul_each(sum, kf[at % TWO], sf[p]);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
         }
         float* to = A.dr + (head * chunks + c) * C * DVP + v;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            to[(16 * (i >> 2) + 4 * q + (i & 3)) * DVP] = dR[i >> 2][i & 3];
-
-        const float whole = L.first[C - 1];
-        Frag<NC> of[2], rf[2];
+            to[spread(i >> 2, 4 * q + (i & 3)) * DVP] = dR[i >> 2][i & 3];
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-            const f32x4_t first = four(L.first + 16 * tb + 4 * q);
-            dO[tb] *= A.scale * first;
-            dR[tb] *= -(first * four(L.beta + 16 * tb + 4 * q));
-        }
+        for (int p = 0; p < 2; ++p)
+            rf[p] = split8<NC>(
+                -(first[2 * p] * beta[2 * p]) * dR[2 * p],
+                -(first[2 * p + 1] * beta[2 * p + 1]) * dR[2 * p + 1]);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            of[p] = split8<NC>(dO[2 * p], dO[2 * p + 1]);
-            rf[p] = split8<NC>(dR[2 * p], dR[2 * p + 1]);
-        }
+        for (int n = 0; n < KT / 2; ++n) {
+            f32x4_t sum[4];
 #pragma unroll
-        for (int kb = 0; kb < 2 * KT; ++kb) {
-            D[kb] *= whole;
+            for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                mul(D[kb], L.q.columns(kb, p, lane), of[p]);
-                mul(D[kb], L.k.columns(kb, p, lane), rf[p]);
+                const int at = 2 * n + p;
+                if (!DEEP)
+                    column_blocks(L.k, n, p, lane, kf[0]);
+                else if (at + 1 < KT)
+                    column_blocks(L.k, (at + 1) / 2, (at + 1) & 1, lane,
+                                  kf[(at + 1) % TWO]);
+                hold();
+                mul_each(sum, kf[at % TWO], rf[p]);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
         }
     });
     if (A.ds0 && wave < 4 && on) {
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb) {
-            const int k = 16 * kb + 4 * q;
+            const int k = spread(kb, 4 * q);
             if (k < A.Dk)
                 *reinterpret_cast<f32x4_t*>(
                     A.ds0 + (head * A.Dv + v) * A.Dk + k) = D[kb];

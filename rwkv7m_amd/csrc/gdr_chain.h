@@ -27,10 +27,10 @@ struct Columns;
 template <>
 struct Columns<bf16_t> {
     Rows<1, 2> x;
-    // [16 tb + 4q + e][16 wave + r]
+    // [spread(tb, 4q + e)][16 wave + r]
     __device__ __forceinline__ f32x4_t values(int tb, int wave,
                                               int lane) const {
-        return x.values(16 * tb, wave, lane);
+        return x.values(spread(tb, 4 * (lane >> 4)), wave, lane);
     }
     __device__ __forceinline__ void put(int row, int col,
                                         const Eight<bf16_t>& v) {
@@ -45,7 +45,8 @@ struct Columns<float> {
         const int r = lane & 15, q = lane >> 4;
         f32x4_t v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = x[16 * tb + 4 * q + e][16 * wave + r];
+        for (int e = 0; e < 4; ++e)
+            v[e] = x[spread(tb, 4 * q + e)][16 * wave + r];
         return v;
     }
     __device__ __forceinline__ void put(int row, int col,
@@ -88,7 +89,7 @@ struct OwnColumn {
           on(v < A.Dv) {}
     static __device__ __forceinline__ int64_t token(int64_t c, int i,
                                                     int lane) {
-        return c * C + 16 * (i >> 2) + 4 * (lane >> 4) + (i & 3);
+        return c * C + spread(i >> 2, 4 * (lane >> 4) + (i & 3));
     }
     __device__ __forceinline__ void fetch(int64_t c, int lane) {
         if constexpr (!kColumns<E, KT>)

@@ -20,11 +20,13 @@
 //
 // Register layouts (lane l, r = l % 16, q = l / 16).  An accumulator tile D(X)
 // holds X[4q + e][r], e = 0..3.  An operand of 32 places along the contracted
-// axis holds, in eight slots, X[r][..]: places 4q + e (slots 0..3) and 16 + 4q
-// + e (slots 4..7) of two adjoining tiles, so that the two accumulator tiles
-// D(X^T) are it without a move ("natural"); or 8q + i ("dense": 16 bytes of
-// a row of memory), where both sides of a product are read that way.  The
-// same registers are X as the left operand and X^T as the right one.
+// axis holds X[r][32 p + 8q + i] in its slots i = 0..7, 16 bytes of a row of
+// memory; the same registers are X as the left operand and X^T as the right
+// one.  So that two accumulator tiles are such an operand without a move, the
+// tiles of a pair share its 32 places: row (or column) m of tile 2p + u is
+// place 32 p + 8 (m / 4) + 4 u + m % 4 (spread()).  Taken in their natural
+// order they would be read from LDS in pairs of 8 bytes, at a quarter of the
+// rate (8.1 cycles of the LDS each, where 16 bytes take 4.2).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -203,81 +205,72 @@ struct Eight<float> {
     }
 };
 
-// R rows of 32 KT places in LDS, NP planes.  The pitch puts 16 rows' 8-byte
-// pieces on 64 different banks.
+// Place of row m of tile t.
+__device__ __forceinline__ int spread(int t, int m) {
+    return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
+}
+
+// R rows of 32 KT places in LDS, NP planes.  With this pitch 16 rows' 16-byte
+// pieces lie on different banks.
 template <int NP, int KT, int R = C>
 struct Rows {
     static constexpr int pitch = 32 * KT + 8;
     bf16_t x[NP][R][pitch];
 
-    // Left operand of rows 16 tb .., places 32 p .. (natural).
-    __device__ __forceinline__ Frag<NP> rows(int tb, int p, int lane) const {
-        const int r = lane & 15, q = lane >> 4;
-        Frag<NP> f;
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const uint2 lo = *reinterpret_cast<const uint2*>(
-                &x[n][16 * tb + r][32 * p + 4 * q]);
-            const uint2 hi = *reinterpret_cast<const uint2*>(
-                &x[n][16 * tb + r][32 * p + 16 + 4 * q]);
-            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-        }
-        return f;
-    }
-    // The same of the 32 places of one pair, dense.
-    __device__ __forceinline__ Frag<NP> rows_dense(int tb, int lane) const {
+    // The operand of rows `row` (the lane's), places 32 p ...
+    __device__ __forceinline__ Frag<NP> at_row(int row, int p, int q) const {
         Frag<NP> f;
 #pragma unroll
         for (int n = 0; n < NP; ++n)
-            f.p[n] = *reinterpret_cast<const u32x4_t*>(
-                &x[n][16 * tb + (lane & 15)][8 * (lane >> 4)]);
+            f.p[n] =
+                *reinterpret_cast<const u32x4_t*>(&x[n][row][32 * p + 8 * q]);
         return f;
     }
-    // X[4q + e][16 jb + r] of the rows at `row`, by a transposing read.
-    __device__ __forceinline__ uint2 column(int n, int row, int jb,
+    // .. of tile tb's rows, spread or in their order
+    __device__ __forceinline__ Frag<NP> rows(int tb, int p, int lane) const {
+        return at_row(spread(tb, lane & 15), p, lane >> 4);
+    }
+    __device__ __forceinline__ Frag<NP> rows_in_order(int tb, int p,
+                                                      int lane) const {
+        return at_row(16 * tb + (lane & 15), p, lane >> 4);
+    }
+    // X[row + e][..] of the column that each lane's place in its group of 16
+    // gives: the lane reads four columns from `col` of row `row` + s / 4.
+    __device__ __forceinline__ uint2 turned(int n, int row, int col,
                                             int lane) const {
-        const int s = lane & 15, q = lane >> 4;
-        const bf16_t* p = &x[n][row + 4 * q + (s >> 2)][16 * jb + 4 * (s & 3)];
+        const bf16_t* p = &x[n][row + ((lane & 15) >> 2)][col];
         return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                              (lds_i16x4_t*)(p)));
     }
-    // Left operand of rows 16 jb .. of the transpose (columns of x), over the
-    // 32 rows of pair p (natural); as the right operand, x itself.
+    // The operand of columns `col`.. (as `turned`), over the 32 rows of pair p:
+    // left, rows of the transpose; right, x itself.
+    __device__ __forceinline__ Frag<NP> at_column(int col, int p,
+                                                  int lane) const {
+        const int row = 32 * p + 8 * (lane >> 4);
+        Frag<NP> f;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const uint2 lo = turned(n, row, col, lane);
+            const uint2 hi = turned(n, row + 4, col, lane);
+            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        }
+        return f;
+    }
+    // .. of tile jb's columns, spread or in their order
     __device__ __forceinline__ Frag<NP> columns(int jb, int p, int lane) const {
-        Frag<NP> f;
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const uint2 lo = column(n, 32 * p, jb, lane);
-            const uint2 hi = column(n, 32 * p + 16, jb, lane);
-            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-        }
-        return f;
+        return at_column(32 * (jb >> 1) + 8 * (lane & 3) + 4 * (jb & 1), p,
+                         lane);
     }
-    // The same over rows 32 p + 8q + i (dense).
-    __device__ __forceinline__ Frag<NP> columns_dense(int jb, int p,
-                                                      int lane) const {
-        const int s = lane & 15, q = lane >> 4;
-        Frag<NP> f;
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const bf16_t* at =
-                &x[n][32 * p + 8 * q + (s >> 2)][16 * jb + 4 * (s & 3)];
-            const uint2 lo = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (lds_i16x4_t*)(at)));
-            const uint2 hi = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (lds_i16x4_t*)(at + 4 * pitch)));
-            f.p[n] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-        }
-        return f;
+    __device__ __forceinline__ Frag<NP> columns_in_order(int jb, int p,
+                                                         int lane) const {
+        return at_column(16 * jb + 4 * (lane & 3), p, lane);
     }
-    // X[row + 4q + e][16 jb + r] as floats.
+    // X[row + e][16 jb + r] as floats (row: the lane's first of four).
     __device__ __forceinline__ f32x4_t values(int row, int jb, int lane) const {
         f32x4_t v = zero4();
 #pragma unroll
         for (int n = NP - 1; n >= 0; --n) {
-            const uint2 u = column(n, row, jb, lane);
+            const uint2 u = turned(n, row, 16 * jb + 4 * (lane & 3), lane);
             v[0] += __uint_as_float(u.x << 16);
             v[1] += __uint_as_float(u.x & 0xffff0000u);
             v[2] += __uint_as_float(u.y << 16);
@@ -346,13 +339,6 @@ struct Prepared {
     double G[C];                          // base 2
     float first[C], last[C], beta[C];     // 2^G, 2^(G_L - G)
 };
-
-// Does row block tb of such a matrix (or of its transpose) hold anything in
-// the 32 places of pair p?
-__device__ __forceinline__ constexpr bool holds(bool transposed, int tb,
-                                                int p) {
-    return transposed ? 2 * p + 1 >= tb : 2 * p <= tb;
-}
 
 __device__ __forceinline__ f32x4_t four(const float* p) {
     return *reinterpret_cast<const f32x4_t*>(p);

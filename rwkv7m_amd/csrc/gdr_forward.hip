@@ -25,10 +25,10 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
     const int v0 = 64 * at_.part + 16 * wave, v = v0 + r;  // the lane's row
     const bool has = v0 < DVP, on = v < A.Dv;
 
-    f32x4_t S[2 * KT];  // D(S^T): k = 16 kb + 4q + e, v = r
+    f32x4_t S[2 * KT];  // D(S^T): k = spread(kb, 4q + e), v = r
 #pragma unroll
     for (int kb = 0; kb < 2 * KT; ++kb) {
-        const int k = 16 * kb + 4 * q;
+        const int k = spread(kb, 4 * q);
         S[kb] = zero4();
         if (A.s0 && wave < 4 && on && k < A.Dk)
             S[kb] = four(A.s0 + (head * A.Dv + v) * A.Dk + k);
@@ -57,8 +57,8 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         column.take(L, c, c + 1, wave, lane, V);
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
-            first[tb] = four(L.first + 16 * tb + 4 * q);
-            beta[tb] = four(L.beta + 16 * tb + 4 * q);
+            first[tb] = four(L.first + spread(tb, 4 * q));
+            beta[tb] = four(L.beta + spread(tb, 4 * q));
             B0[tb] = O[tb] = X[tb] = zero4();
         }
 #pragma unroll
@@ -67,9 +67,9 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             float* to = A.states + ((head * chunks + c) * DVP + v) * DKP;
 #pragma unroll
             for (int kb = 0; kb < 2 * KT; ++kb)
-                *reinterpret_cast<f32x4_t*>(to + 16 * kb + 4 * q) = S[kb];
+                *reinterpret_cast<f32x4_t*>(to + spread(kb, 4 * q)) = S[kb];
         }
-        // K S^T, t = 4q + e, v = r
+        // K S^T, t = spread(tb, 4q + e), v = r
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
             if (!DEEP) blocks(L.k, p, lane, kf[0]);
@@ -88,7 +88,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         if (!DEEP) triangle<false>(L.t, lane, Tf);
         hold();
         mul_triangle<false>(X, Tf, Rf);
-        // S Q^T, v = 4q + e, t = r
+        // S Q^T, v = 4q + e, t = spread(tb, r)
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
             if (!DEEP) blocks(L.q, p, lane, qf[0]);
@@ -101,20 +101,20 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             float* to = A.x + (head * chunks + c) * C * DVP + v;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                to[(16 * (i >> 2) + 4 * q + (i & 3)) * DVP] = X[i >> 2][i & 3];
+                to[spread(i >> 2, 4 * q + (i & 3)) * DVP] = X[i >> 2][i & 3];
         }
         // S^T = 2^G_L S^T + K^T (2^(G_L - G) X)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             Xf[p] = split8<NC>(X[2 * p], X[2 * p + 1]);
             Rf[p] = split8<NC>(
-                X[2 * p] * four(L.last + 32 * p + 4 * q),
-                X[2 * p + 1] * four(L.last + 32 * p + 16 + 4 * q));
+                X[2 * p] * four(L.last + spread(2 * p, 4 * q)),
+                X[2 * p + 1] * four(L.last + spread(2 * p + 1, 4 * q)));
         }
         const float whole = L.first[C - 1];
         float own_first[4];
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) own_first[tb] = L.first[16 * tb + r];
+        for (int tb = 0; tb < 4; ++tb) own_first[tb] = L.first[spread(tb, r)];
 #pragma unroll
         for (int n = 0; n < KT / 2; ++n) {
             f32x4_t sum[4];
@@ -144,7 +144,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         E* to = op + t0 * A.Hv * A.Dv + v0 + 4 * q;
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
-            const int t = 16 * tb + r;
+            const int t = spread(tb, r);
             if (t < valid && v0 + 4 * q < A.Dv) {
                 O[tb] *= A.scale;
                 if constexpr (sizeof(E) == 4)
@@ -159,7 +159,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
     if (A.s_t && wave < 4 && on) {
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb) {
-            const int k = 16 * kb + 4 * q;
+            const int k = spread(kb, 4 * q);
             if (k < A.Dk)
                 *reinterpret_cast<f32x4_t*>(
                     A.s_t + (head * A.Dv + v) * A.Dk + k) = S[kb];

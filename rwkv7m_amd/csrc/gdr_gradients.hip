@@ -236,9 +236,9 @@ gdr_gradients_kernel(const GdrArgs A) {
         Frag<NC> xf[2], rf[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            of[i] = L.o.rows_dense(2 * th + i, lane);
-            xf[i] = L.x.rows_dense(2 * th + i, lane);
-            rf[i] = L.r.rows_dense(2 * th + i, lane);
+            of[i] = L.o.rows_in_order(2 * th + i, 0, lane);
+            xf[i] = L.x.rows_in_order(2 * th + i, 0, lane);
+            rf[i] = L.r.rows_in_order(2 * th + i, 0, lane);
         }
         if (!last_share) {
 #pragma unroll
@@ -256,19 +256,19 @@ gdr_gradients_kernel(const GdrArgs A) {
                 }
             }
         } else {
-            const Frag<NI> o = L.o.rows_dense(2 + th, lane);
-            const Frag<NC> g = L.r.rows_dense(2 + th, lane);
+            const Frag<NI> o = L.o.rows_in_order(2 + th, 0, lane);
+            const Frag<NC> g = L.r.rows_in_order(2 + th, 0, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const Frag<NC> x = L.x.rows_dense(i, lane);
+                const Frag<NC> x = L.x.rows_in_order(i, 0, lane);
                 mul(dp[i], o, x);
                 mul(nn[i], g, x);
             }
         }
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
-            const Frag<NC> f = L.s.columns_dense(kh * KW + j, 0, lane);
-            const Frag<NC> g = L.d.columns_dense(kh * KW + j, 0, lane);
+            const Frag<NC> f = L.s.columns_in_order(kh * KW + j, 0, lane);
+            const Frag<NC> g = L.d.columns_in_order(kh * KW + j, 0, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 mul(dq[i][j], of[i], f);
@@ -332,7 +332,7 @@ gdr_gradients_kernel(const GdrArgs A) {
             dq[i][j] *= A.scale * first;
             left[i][j] *= first;
             right[i][j] *= last;
-            const f32x4_t x = L.k.values(16 * (2 * th + i), kh * KW + j, lane) *
+            const f32x4_t x = L.k.values(16 * (2 * th + i) + 4 * q, kh * KW + j, lane) *
                               right[i][j];
             kfirst += (x[0] + x[1]) + (x[2] + x[3]);
         }
@@ -345,12 +345,12 @@ gdr_gradients_kernel(const GdrArgs A) {
             Frag<NC> a[2], n[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                a[i] = L.p.rows(2 * th + i, p, lane);
-                n[i] = L.n.rows(2 * th + i, p, lane);
+                a[i] = L.p.rows_in_order(2 * th + i, p, lane);
+                n[i] = L.n.rows_in_order(2 * th + i, p, lane);
             }
 #pragma unroll
             for (int j = 0; j < KW; ++j) {
-                const Frag<NI> f = L.k.columns(kh * KW + j, p, lane);
+                const Frag<NI> f = L.k.columns_in_order(kh * KW + j, p, lane);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     mul(dq[i][j], a[i], f);
@@ -361,10 +361,10 @@ gdr_gradients_kernel(const GdrArgs A) {
         if (p >= th) {
             Frag<NC> a[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) a[i] = L.p.columns(2 * th + i, p, lane);
+            for (int i = 0; i < 2; ++i) a[i] = L.p.columns_in_order(2 * th + i, p, lane);
 #pragma unroll
             for (int j = 0; j < KW; ++j) {
-                const Frag<NI> f = L.q.columns(kh * KW + j, p, lane);
+                const Frag<NI> f = L.q.columns_in_order(kh * KW + j, p, lane);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) mul(right[i][j], a[i], f);
             }
@@ -378,10 +378,10 @@ gdr_gradients_kernel(const GdrArgs A) {
         if (p < th) continue;
         Frag<NC> n[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) n[i] = L.n.columns(2 * th + i, p, lane);
+        for (int i = 0; i < 2; ++i) n[i] = L.n.columns_in_order(2 * th + i, p, lane);
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
-            const Frag<NI> f = L.k.columns(kh * KW + j, p, lane);
+            const Frag<NI> f = L.k.columns_in_order(kh * KW + j, p, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) mul(right[i][j], n[i], f);
         }
@@ -393,9 +393,9 @@ gdr_gradients_kernel(const GdrArgs A) {
         const int row = 16 * (2 * th + i);
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
-            const f32x4_t kv = L.k.values(row, kh * KW + j, lane);
+            const f32x4_t kv = L.k.values(row + 4 * q, kh * KW + j, lane);
             left[i][j] = -left[i][j];
-            dg += L.q.values(row, kh * KW + j, lane) * dq[i][j] -
+            dg += L.q.values(row + 4 * q, kh * KW + j, lane) * dq[i][j] -
                   kv * right[i][j];
             kleft += kv * left[i][j];
         }
