@@ -11,8 +11,8 @@ namespace {
 
 using namespace gdr;
 
-template <typename E, int KT>
-__global__ void __launch_bounds__(2 * BRING)
+template <typename E, int KT, int OW>
+__global__ void __launch_bounds__(64 * OW + BRING)
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 gdr_backward_kernel(const GdrArgs A, int parts) {
     constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
@@ -25,7 +25,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
     const Head at_head(A, at_.head);
     const int64_t b = at_head.b, h = at_head.h, chunks = chunk_count(A);
     const int DVP = (A.Dv + 31) / 32 * 32;
-    const int v0 = 64 * at_.part + 16 * wave, v = v0 + r;  // the lane's row
+    const int v0 = 16 * (OW * at_.part + wave), v = v0 + r;  // the lane's row
     const bool has = v0 < DVP, on = v < A.Dv;
 
     f32x4_t D[2 * KT];  // D(D^T): k = spread(kb, 4q + e), v = r
@@ -33,17 +33,17 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
     for (int kb = 0; kb < 2 * KT; ++kb) {
         const int k = spread(kb, 4 * q);
         D[kb] = zero4();
-        if (A.ds_t && wave < 4 && on && k < A.Dk)
+        if (A.ds_t && wave < OW && on && k < A.Dk)
             D[kb] = four(A.ds_t + (head * A.Dv + v) * A.Dk + k);
     }
 
     OwnColumn<E, KT> column(A, A.dout, b, h, v);
     column.fetch(chunks - 1, lane);
 
-    chain<E, KT>(
+    chain<E, KT, OW>(
         A, A.dout,
         static_cast<const Prepared<NC>*>(A.prepared) + head * chunks, head,
-        64 * at_.part, chunks - 1, -1, chunks,
+        16 * OW * at_.part, chunks - 1, -1, chunks,
         reinterpret_cast<ChainChunk<E, KT>*>(lds_raw),
         [&](const ChainChunk<E, KT>& L, int64_t c) {
         if (!has) return;
@@ -150,7 +150,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
             for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
         }
     });
-    if (A.ds0 && wave < 4 && on) {
+    if (A.ds0 && wave < OW && on) {
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb) {
             const int k = spread(kb, 4 * q);
@@ -161,18 +161,27 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
     }
 }
 
-template <typename E, int KT>
-hipError_t launch(const GdrArgs& A, hipStream_t stream) {
-    const auto kernel = gdr_backward_kernel<E, KT>;
+template <typename E, int KT, int OW>
+hipError_t launch_with(const GdrArgs& A, hipStream_t stream) {
+    const auto kernel = gdr_backward_kernel<E, KT, OW>;
     const int lds = int(kBuffers<E, KT> * sizeof(ChainChunk<E, KT>));
     const hipError_t e = hipFuncSetAttribute(
         reinterpret_cast<const void*>(kernel),
         hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    const int parts = (gdr_dvp(A.Dv) + 63) / 64;
+    const int parts = (gdr_dvp(A.Dv) + 16 * OW - 1) / (16 * OW);
     hipLaunchKernelGGL(kernel, dim3(places(A.B * A.Hv, parts)),
-                       dim3(2 * BRING), lds, stream, A, parts);
+                       dim3(64 * OW + BRING), lds, stream, A, parts);
     return hipGetLastError();
+}
+
+template <typename E, int KT>
+hipError_t launch(const GdrArgs& A, hipStream_t stream) {
+    switch (owning_waves(A.B * A.Hv, gdr_dvp(A.Dv))) {
+        case 1: return launch_with<E, KT, 1>(A, stream);
+        case 2: return launch_with<E, KT, 2>(A, stream);
+        default: return launch_with<E, KT, 4>(A, stream);
+    }
 }
 
 }  // namespace

@@ -4,12 +4,12 @@
 // A recurrence acts on each row of the state by itself (row i uses only
 // element i of v or do), so a wave owns 16 rows, all of the state's columns,
 // in accumulator registers for the whole sequence, and needs nothing from
-// another wave.  Four such waves make a workgroup, with four more that bring
-// what a chunk needs (K, Q, T, P, the gates, V or dO) from memory through their
-// registers to LDS, one chunk ahead of its use and two ahead with their loads.
-// The owning waves then wait for no load at all: where they brought their own
-// operands, each wait for one was also a wait for every store before it, and a
-// chunk took 14 us.
+// another wave.  One, two or four such waves make a workgroup, with four more
+// that bring what a chunk needs (K, Q, T, P, the gates, V or dO) from memory
+// through their registers to LDS, one chunk ahead of its use and two ahead with
+// their loads.  The owning waves then wait for no load at all: where they
+// brought their own operands, each wait for one was also a wait for every store
+// before it, and a chunk took 14 us.
 #pragma once
 
 #include <type_traits>
@@ -19,7 +19,7 @@
 namespace rwkv7m {
 namespace gdr {
 
-constexpr int BRING = 256;  // threads that bring, as many as own rows
+constexpr int BRING = 256;  // threads that bring
 
 // 64 columns of a chunk's V or dO.
 template <typename E>
@@ -116,13 +116,14 @@ struct OwnColumn {
     }
 };
 
-// A bringing thread's share of a chunk.
-template <typename E, int KT>
+// A bringing thread's share of a chunk, for OW owning waves.
+template <typename E, int KT, int OW>
 struct Bring {
     static constexpr int NC = kMade<E>;
     Staged<E, KT, BRING> k, q;
     u32x4_t t[2 * NC], p[2 * NC];
-    Eight<E> v[2];
+    static constexpr int per_row = 2 * OW, turns = (OW + 1) / 2;
+    Eight<E> v[turns];
     float first, last, beta;
 
     // (v0: the workgroup's first column; x: V or dO)
@@ -137,9 +138,6 @@ struct Bring {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
-            if constexpr (kColumns<E, KT>)
-                v[i].load(at<E>(x, b, h, t0 + near(row, valid - 1)) +
-                          near(v0 + col, A.Dv - 8));
             // (the upper right quarters, which nothing reads, hold the lower
             // left ones' first columns again)
             const int at_col = row < 32 ? col % 32 : col;
@@ -151,6 +149,13 @@ struct Bring {
                     *reinterpret_cast<const u32x4_t*>(&M.p[n][row][at_col]);
             }
         }
+        if constexpr (kColumns<E, KT>)
+#pragma unroll
+            for (int i = 0; i < turns; ++i) {
+                const int u = i * BRING + thread;
+                v[i].load(at<E>(x, b, h, t0 + near(u / per_row, valid - 1)) +
+                          near(v0 + 8 * (u % per_row), A.Dv - 8));
+            }
         first = M.first[thread & 63];
         last = M.last[thread & 63];
         beta = M.beta[thread & 63];
@@ -164,11 +169,6 @@ struct Bring {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
-            if constexpr (kColumns<E, KT>) {
-                Eight<E> x = v[i];
-                x.keep(row < valid && v0 + col < A.Dv);
-                L.v.put(row, col, x);
-            }
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 *reinterpret_cast<u32x4_t*>(&L.t.x[n][row][col]) =
@@ -177,6 +177,15 @@ struct Bring {
                     p[i * NC + n];
             }
         }
+        if constexpr (kColumns<E, KT>)
+#pragma unroll
+            for (int i = 0; i < turns; ++i) {
+                const int u = i * BRING + thread;
+                const int row = u / per_row, col = 8 * (u % per_row);
+                Eight<E> x = v[i];
+                x.keep(row < valid && v0 + col < A.Dv);
+                if (row < C) L.v.put(row, col, x);
+            }
         if (thread < C) {
             L.first[thread] = first;
             L.last[thread] = last;
@@ -260,7 +269,7 @@ __device__ __forceinline__ void column_blocks(const Rows<NI, KT>& x, int n,
 
 // The loop of both: chunks first, first + step, .. (n of them).  own(L, c) by
 // the threads that own rows, with the chunk in L.
-template <typename E, int KT, typename F>
+template <typename E, int KT, int OW, typename F>
 __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
                                       const Prepared<kMade<E>>* M, int64_t head,
                                       int v0, int64_t first, int64_t step,
@@ -268,9 +277,9 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
     const Head at_head(A, uint32_t(head));
     const int64_t b = at_head.b, h = at_head.h, hk = at_head.hk;
     constexpr int NB = kBuffers<E, KT>;
-    if (threadIdx.x >= BRING) {
-        const int thread = threadIdx.x - BRING;
-        Bring<E, KT> s;
+    if (threadIdx.x >= 64 * OW) {
+        const int thread = threadIdx.x - 64 * OW;
+        Bring<E, KT, OW> s;
         s.load(A, x, M[first], b, h, hk, first, v0, thread);
         s.store(A, L[0], first, v0, thread);
         const auto ahead = [&](int64_t i) {
@@ -289,6 +298,8 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
             __syncthreads();
         }
     } else {
+        // (the owning waves' step is what the others wait for)
+        __builtin_amdgcn_s_setprio(2);
         __syncthreads();
         for (int64_t i = 0; i < n; ++i) {
             own(L[NB == 2 ? i & 1 : 0], first + step * i);
@@ -296,6 +307,16 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
             __syncthreads();
         }
     }
+}
+
+// Owning waves of a workgroup: as many workgroups as there are CUs, where the
+// heads are few (a CU's waves share its LDS, whose reads are half of a chunk's
+// time: 32 heads of 1999 tokens take @@ us with one, @@ with two and @@ with
+// four), and as few as possible beyond, since each brings its own K and Q.
+inline int owning_waves(int64_t heads, int dvp) {
+    for (int w = 1; w < 4; w *= 2)
+        if (heads * ((dvp + 16 * w - 1) / (16 * w)) <= device_cus()) return w;
+    return 4;
 }
 
 }  // namespace gdr
