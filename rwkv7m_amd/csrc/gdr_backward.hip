@@ -54,98 +54,111 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
 
         // (the order of issue, as in the forward)
         constexpr bool DEEP = NI == 1;
-        constexpr int TWO = DEEP ? 2 : 1;
+        constexpr int TWO = DEEP ? 2 : 1, HALF = KT / 2;
         Frag<NI> kf[TWO][4], of[2];
         Frag<NC> Tf[6], Pf[6], Df[KT], xf[2], rf[2], sf[2];
         f32x4_t dO[4], dX[4], dR[4], KD[4], first[4], last[4], beta[4];
+        const float whole = L.first[C - 1];
         column.take(L, c, c - 1, wave, lane, dO);
-        if (DEEP) triangle<true>(L.p, lane, Pf);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-            first[tb] = four(L.first + spread(tb, 4 * q));
-            last[tb] = four(L.last + spread(tb, 4 * q));
-            beta[tb] = four(L.beta + spread(tb, 4 * q));
-            dX[tb] = dR[tb] = KD[tb] = zero4();
+        if (DEEP) {
+            triangle<true>(L.p, lane, Pf);
+            blocks(L.k, 0, lane, kf[0]);
         }
-        if (DEEP) blocks(L.k, 0, lane, kf[0]);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+        for (int tb = 0; tb < 4; ++tb) dX[tb] = dR[tb] = KD[tb] = zero4();
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
             of[p] = split8<NI>(dO[2 * p], dO[2 * p + 1]);
-            sf[p] = split8<NC>(A.scale * first[2 * p] * dO[2 * p],
-                               A.scale * first[2 * p + 1] * dO[2 * p + 1]);
-        }
-#pragma unroll
-        for (int p = 0; p < KT; ++p) Df[p] = split8<NC>(D[2 * p], D[2 * p + 1]);
         // P^T dO and K D^T, t = spread(tb, 4q + e), v = r
         if (!DEEP) triangle<true>(L.p, lane, Pf);
         hold();
         mul_triangle<true>(dX, Pf, of);
+        Df[0] = split8<NC>(D[0], D[1]);
+        if (DEEP) interleave<8, 3>();
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
             if (!DEEP) blocks(L.k, p, lane, kf[0]);
             else if (p + 1 < KT) blocks(L.k, p + 1, lane, kf[(p + 1) % TWO]);
-            else triangle<true>(L.t, lane, Tf);
+            else column_blocks(L.q, 0, 0, lane, kf[(p + 1) % TWO]);
+            if (p + 1 == KT)
+#pragma unroll
+                for (int tb = 0; tb < 4; ++tb) {
+                    first[tb] = four(L.first + spread(tb, 4 * q));
+                    last[tb] = four(L.last + spread(tb, 4 * q));
+                }
             hold();
             mul_each(KD, kf[p % TWO], Df[p]);
+            if (p + 1 < KT)
+                Df[p + 1] = split8<NC>(D[2 * p + 2], D[2 * p + 3]);
+            if (DEEP) interleave<8, 3>();
         }
-        // D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K: the first
-        // product while dX is made
-        const float whole = L.first[C - 1];
-        if (DEEP) column_blocks(L.q, 0, 0, lane, kf[0]);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb)
-            dX[tb] = A.scale * dX[tb] + last[tb] * KD[tb];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) xf[p] = split8<NC>(dX[2 * p], dX[2 * p + 1]);
-        if (!DEEP) triangle<true>(L.t, lane, Tf);
-        hold();
-        mul_triangle<true>(dR, Tf, xf);
-#pragma unroll
-        for (int n = 0; n < KT / 2; ++n) {
-            f32x4_t sum[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i] * whole;
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int at = 2 * n + p;
-                if (!DEEP)
-                    column_blocks(L.q, n, p, lane, kf[0]);
-                else if (at + 1 < KT)
-                    column_blocks(L.q, (at + 1) / 2, (at + 1) & 1, lane,
-                                  kf[(at + 1) % TWO]);
-                else
-                    column_blocks(L.k, 0, 0, lane, kf[(at + 1) % TWO]);
-                hold();
-                mul_each(sum, kf[at % TWO], sf[p]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
-        }
-        float* to = A.dr + (head * chunks + c) * C * DVP + v;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            to[spread(i >> 2, 4 * q + (i & 3)) * DVP] = dR[i >> 2][i & 3];
+        // D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K, half of the
+        // first product while dX is put together, half while dR is
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-            rf[p] = split8<NC>(
-                -(first[2 * p] * beta[2 * p]) * dR[2 * p],
-                -(first[2 * p + 1] * beta[2 * p + 1]) * dR[2 * p + 1]);
+            sf[p] = split8<NC>(A.scale * first[2 * p] * dO[2 * p],
+                               A.scale * first[2 * p + 1] * dO[2 * p + 1]);
 #pragma unroll
-        for (int n = 0; n < KT / 2; ++n) {
+        for (int kb = 0; kb < 2 * KT; ++kb) D[kb] *= whole;
+        const auto queries = [&](int at) {
+            const int n = at / 2, p = at & 1;
+            if (!DEEP)
+                column_blocks(L.q, n, p, lane, kf[0]);
+            else if (at + 1 < KT)
+                column_blocks(L.q, (at + 1) / 2, (at + 1) & 1, lane,
+                              kf[(at + 1) % TWO]);
+            else
+                column_blocks(L.k, 0, 0, lane, kf[(at + 1) % TWO]);
+            if (DEEP && at + 1 == HALF) triangle<true>(L.t, lane, Tf);
+            hold();
             f32x4_t sum[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i];
+            mul_each(sum, kf[at % TWO], sf[p]);
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int at = 2 * n + p;
-                if (!DEEP)
-                    column_blocks(L.k, n, p, lane, kf[0]);
-                else if (at + 1 < KT)
-                    column_blocks(L.k, (at + 1) / 2, (at + 1) & 1, lane,
-                                  kf[(at + 1) % TWO]);
-                hold();
-                mul_each(sum, kf[at % TWO], rf[p]);
-            }
+            for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
+        };
+#pragma unroll
+        for (int at = 0; at < HALF; ++at) {
+            queries(at);
+#pragma unroll
+            for (int i = 4 * at / HALF; i < 4 * (at + 1) / HALF; ++i)
+                dX[i] = A.scale * dX[i] + last[i] * KD[i];
+#pragma unroll
+            for (int i = 2 * at / HALF; i < 2 * (at + 1) / HALF; ++i)
+                xf[i] = split8<NC>(dX[2 * i], dX[2 * i + 1]);
+            if (DEEP) interleave<8, 6>();
+        }
+        if (!DEEP) triangle<true>(L.t, lane, Tf);
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) beta[tb] = four(L.beta + spread(tb, 4 * q));
+        hold();
+        mul_triangle<true>(dR, Tf, xf);
+#pragma unroll
+        for (int at = HALF; at < KT; ++at) {
+            queries(at);
+#pragma unroll
+            for (int i = 2 * (at - HALF) / HALF; i < 2 * (at - HALF + 1) / HALF;
+                 ++i)
+                rf[i] = split8<NC>(
+                    -(first[2 * i] * beta[2 * i]) * dR[2 * i],
+                    -(first[2 * i + 1] * beta[2 * i + 1]) * dR[2 * i + 1]);
+            if (DEEP) interleave<8, 6>();
+        }
+        put_column(A.dr + (head * chunks + c) * C * DVP, DVP, q, v, dR);
+#pragma unroll
+        for (int at = 0; at < KT; ++at) {
+            const int n = at / 2, p = at & 1;
+            if (!DEEP)
+                column_blocks(L.k, n, p, lane, kf[0]);
+            else if (at + 1 < KT)
+                column_blocks(L.k, (at + 1) / 2, (at + 1) & 1, lane,
+                              kf[(at + 1) % TWO]);
+            hold();
+            f32x4_t sum[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i];
+            mul_each(sum, kf[at % TWO], rf[p]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
         }

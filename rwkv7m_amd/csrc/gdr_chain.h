@@ -56,6 +56,16 @@ struct Columns<float> {
     }
 };
 
+// A chunk's X or dR of the lane's column, 64 rows of `pitch` floats: uniform
+// row addresses and one 32-bit lane offset.
+__device__ __forceinline__ void put_column(float* to, int pitch, int q, int v,
+                                           const f32x4_t (&x)[4]) {
+    const uint32_t lane = uint32_t(8 * q * pitch + v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        (to + spread(i >> 2, i & 3) * pitch)[lane] = x[i >> 2][i & 3];
+}
+
 struct NoColumns {};
 
 // (fp32 at 128 columns leaves no room for the 64 columns in LDS)

@@ -46,80 +46,104 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         const int64_t t0 = c * C;
         const int valid = int(A.T - t0 < C ? A.T - t0 : C);
         // What follows is in the order in which it is issued: each step's
-        // operands are on their way from LDS during the step before.  (bf16:
-        // fp32's three planes leave no registers for it.)
+        // operands are on their way from LDS during the step before, and what
+        // the vector ALU has to do runs between products that do not need it.
+        // (bf16: fp32's three planes leave no registers for it.)
         constexpr bool DEEP = NI == 1;
-        constexpr int TWO = DEEP ? 2 : 1;
+        constexpr int TWO = DEEP ? 2 : 1, HALF = KT / 2;
         Frag<NI> kf[TWO][4], qf[TWO][4];
         Frag<NC> Tf[6], Pf[6], Sf[KT], Rf[2], Xf[2];
         f32x4_t V[4], first[4], beta[4], B0[4], O[4], X[4];
+        const float whole = L.first[C - 1];
         if (DEEP) blocks(L.k, 0, lane, kf[0]);
         column.take(L, c, c + 1, wave, lane, V);
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-            first[tb] = four(L.first + spread(tb, 4 * q));
-            beta[tb] = four(L.beta + spread(tb, 4 * q));
-            B0[tb] = O[tb] = X[tb] = zero4();
-        }
-#pragma unroll
-        for (int p = 0; p < KT; ++p) Sf[p] = split8<NC>(S[2 * p], S[2 * p + 1]);
+        for (int tb = 0; tb < 4; ++tb) B0[tb] = O[tb] = X[tb] = zero4();
         if constexpr (TRAIN) {
             float* to = A.states + ((head * chunks + c) * DVP + v) * DKP;
 #pragma unroll
             for (int kb = 0; kb < 2 * KT; ++kb)
                 *reinterpret_cast<f32x4_t*>(to + spread(kb, 4 * q)) = S[kb];
         }
+        Sf[0] = split8<NC>(S[0], S[1]);
         // K S^T, t = spread(tb, 4q + e), v = r
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
-            if (!DEEP) blocks(L.k, p, lane, kf[0]);
-            else if (p + 1 < KT) blocks(L.k, p + 1, lane, kf[(p + 1) % TWO]);
-            else triangle<false>(L.t, lane, Tf);
+            if (!DEEP) {
+                blocks(L.k, p, lane, kf[0]);
+            } else if (p + 1 < KT) {
+                blocks(L.k, p + 1, lane, kf[(p + 1) % TWO]);
+            } else {
+                blocks(L.q, 0, lane, qf[0]);
+            }
+            if (p + 1 == KT)
+#pragma unroll
+                for (int tb = 0; tb < 4; ++tb) {
+                    first[tb] = four(L.first + spread(tb, 4 * q));
+                    beta[tb] = four(L.beta + spread(tb, 4 * q));
+                }
             hold();
             mul_each(B0, kf[p % TWO], Sf[p]);
+            if (p + 1 < KT)
+                Sf[p + 1] = split8<NC>(S[2 * p + 2], S[2 * p + 3]);
+            if (DEEP) interleave<8, 3>();
         }
-        // R = beta (V - 2^G (K S^T)), X = T R
-        if (DEEP) blocks(L.q, 0, lane, qf[0]);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb)
-            V[tb] = beta[tb] * (V[tb] - first[tb] * B0[tb]);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) Rf[p] = split8<NC>(V[2 * p], V[2 * p + 1]);
-        if (!DEEP) triangle<false>(L.t, lane, Tf);
-        hold();
-        mul_triangle<false>(X, Tf, Rf);
-        // S Q^T, v = 4q + e, t = spread(tb, r)
-#pragma unroll
-        for (int p = 0; p < KT; ++p) {
+        // S Q^T, v = 4q + e, t = spread(tb, r), and meanwhile
+        const auto queries = [&](int p) {
             if (!DEEP) blocks(L.q, p, lane, qf[0]);
             else if (p + 1 < KT) blocks(L.q, p + 1, lane, qf[(p + 1) % TWO]);
             else column_blocks(L.k, 0, 0, lane, kf[0]);
+            if (DEEP && p + 1 == HALF) triangle<false>(L.t, lane, Tf);
             hold();
             mul_each(O, Sf[p], qf[p % TWO]);
-        }
-        if constexpr (TRAIN) {
-            float* to = A.x + (head * chunks + c) * C * DVP + v;
+        };
+        // R = beta (V - 2^G (K S^T))
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                to[spread(i >> 2, 4 * q + (i & 3)) * DVP] = X[i >> 2][i & 3];
-        }
-        // S^T = 2^G_L S^T + K^T (2^(G_L - G) X)
+        for (int p = 0; p < HALF; ++p) {
+            queries(p);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            Xf[p] = split8<NC>(X[2 * p], X[2 * p + 1]);
-            Rf[p] = split8<NC>(
-                X[2 * p] * four(L.last + spread(2 * p, 4 * q)),
-                X[2 * p + 1] * four(L.last + spread(2 * p + 1, 4 * q)));
+            for (int i = 4 * p / HALF; i < 4 * (p + 1) / HALF; ++i)
+                V[i] = beta[i] * (V[i] - first[i] * B0[i]);
+#pragma unroll
+            for (int i = 2 * p / HALF; i < 2 * (p + 1) / HALF; ++i)
+                Rf[i] = split8<NC>(V[2 * i], V[2 * i + 1]);
+            if (DEEP) interleave<8, 6>();
         }
-        const float whole = L.first[C - 1];
+        // X = T R
+        if (!DEEP) triangle<false>(L.t, lane, Tf);
+        hold();
+        mul_triangle<false>(X, Tf, Rf);
+#pragma unroll
+        for (int kb = 0; kb < 2 * KT; ++kb) S[kb] *= whole;
+        if (DEEP) interleave<18, 2>();
+        f32x4_t last[4];
         float own_first[4];
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) own_first[tb] = L.first[spread(tb, r)];
+        for (int tb = 0; tb < 4; ++tb) {
+            last[tb] = four(L.last + spread(tb, 4 * q));
+            own_first[tb] = L.first[spread(tb, r)];
+        }
+#pragma unroll
+        for (int p = HALF; p < KT; ++p) {
+            queries(p);
+#pragma unroll
+            for (int i = 2 * (p - HALF) / HALF; i < 2 * (p - HALF + 1) / HALF;
+                 ++i) {
+                Rf[i] = split8<NC>(X[2 * i] * last[2 * i],
+                                   X[2 * i + 1] * last[2 * i + 1]);
+                Xf[i] = split8<NC>(X[2 * i], X[2 * i + 1]);
+            }
+            if (DEEP) interleave<8, 7>();
+        }
+        if constexpr (TRAIN) {
+            put_column(A.x + (head * chunks + c) * C * DVP, DVP, q, v, X);
+        }
+        // S^T = 2^G_L S^T + K^T (2^(G_L - G) X)
 #pragma unroll
         for (int n = 0; n < KT / 2; ++n) {
             f32x4_t sum[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = S[4 * n + i] * whole;
+            for (int i = 0; i < 4; ++i) sum[i] = S[4 * n + i];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int at = 2 * n + p;
@@ -132,25 +156,28 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                     triangle<false>(L.p, lane, Pf);
                 hold();
                 mul_each(sum, kf[at % TWO], Rf[p]);
+                if (at == 0)
+#pragma unroll
+                    for (int tb = 0; tb < 4; ++tb) O[tb] *= own_first[tb];
+                if (DEEP && at == 0) interleave<8, 2>();
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) S[4 * n + i] = sum[i];
         }
         // O^T = scale (2^G (S Q^T) + X^T P^T)
         if (!DEEP) triangle<false>(L.p, lane, Pf);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb) O[tb] *= own_first[tb];
         mul_by_triangle(O, Xf, Pf);
-        E* to = op + t0 * A.Hv * A.Dv + v0 + 4 * q;
+        E* to = op + t0 * A.Hv * A.Dv + int64_t(spread(0, r)) * A.Hv * A.Dv +
+                v0 + 4 * q;
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
-            const int t = spread(tb, r);
-            if (t < valid && v0 + 4 * q < A.Dv) {
+            E* at = to + int64_t(spread(tb, 0)) * A.Hv * A.Dv;
+            if (spread(tb, r) < valid && v0 + 4 * q < A.Dv) {
                 O[tb] *= A.scale;
                 if constexpr (sizeof(E) == 4)
-                    *reinterpret_cast<f32x4_t*>(to + t * A.Hv * A.Dv) = O[tb];
+                    *reinterpret_cast<f32x4_t*>(at) = O[tb];
                 else
-                    *reinterpret_cast<uint2*>(to + t * A.Hv * A.Dv) =
+                    *reinterpret_cast<uint2*>(at) =
                         make_uint2(pack2(O[tb][0], O[tb][1]),
                                    pack2(O[tb][2], O[tb][3]));
             }
