@@ -7,7 +7,8 @@
 //   left = -2^G (dR S0) - N K
 //   right = 2^(G_L - G) (X D) + dP^T Q - (beta N)^T K
 //   dk = beta left + right,  dv = beta dR,  dbeta = k.left + dR.v
-//   dG = q.dq + beta k.left - k.right, + <D, S_L> at the last token,
+//   dG = q.dq + beta k.left - k.right = q.dq - dv.v (both of the others are
+//   dR.X less or without dv.v), + <D, S_L> at the last token,
 //   dg = the sum of dG from the token on,
 //   <D, S_L> = 2^G_L <D, S0> + sum_t k_t.(2^(G_L - G) X D)_t
 //
@@ -50,7 +51,7 @@ struct GradShared {
             Rows<kMade<E>, 2> n;  // N, then -beta N
             union {
                 Rows<kMade<E>, 2> p;  // dP
-                float dots[kShares<E, KT>][2][C];  // of dG, k.left, behind it
+                float dots[kShares<E, KT>][2][C];  // q.dq, k.left, behind it
             };
         };
     };
@@ -389,20 +390,18 @@ gdr_gradients_kernel(const GdrArgs A) {
     // the gates' gradients
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        f32x4_t kleft = zero4(), dg = zero4();
+        f32x4_t kleft = zero4(), qdq = zero4();
         const int row = 16 * (2 * th + i);
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
             const f32x4_t kv = L.k.values(row + 4 * q, kh * KW + j, lane);
             left[i][j] = -left[i][j];
-            dg += L.q.values(row + 4 * q, kh * KW + j, lane) * dq[i][j] -
-                  kv * right[i][j];
+            qdq += L.q.values(row + 4 * q, kh * KW + j, lane) * dq[i][j];
             kleft += kv * left[i][j];
         }
-        dg += four(L.beta + row + 4 * q) * kleft;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x = sum16(dg[e]), y = sum16(kleft[e]);
+            const float x = sum16(qdq[e]), y = sum16(kleft[e]);
             if (r < 2) L.dots[kh][r][row + 4 * q + e] = r ? y : x;
         }
     }
@@ -425,7 +424,8 @@ gdr_gradients_kernel(const GdrArgs A) {
             for (int k = 1; k < KQ; ++k) sum += L.dots[k][i][lane];
             return sum;
         };
-        double x = dot(0), end = 0.0;  // <D, S_L> at the chunk's last token
+        double x = double(dot(0)) - double(L.beta[lane] * L.rv[lane]);
+        double end = 0.0;  // <D, S_L> at the chunk's last token
 #pragma unroll
         for (int w = 0; w < 2 * KQ; ++w) end += L.sums[w];
         if (lane == 63) x += end;

@@ -1,11 +1,11 @@
 // The gated delta rule's chunk matrices (gdr_common.h has the formulas): T =
 // (I + A)^-1 and P in planes, and the gates.
 //
-// One workgroup a chunk and value head, all of them independent.  T's diagonal
-// blocks of 16 are substituted forward, a lane a column: with keys that
-// resemble each other the powers of A in a product form of the inverse grow to
-// 1e3 and cancel, which would cost fp32 three of its digits.  The blocks
-// below follow by fp32 matrix products, T_ij = -T_ii sum_m A_im T_mj.
+// One workgroup a chunk and value head, all of them independent, a wave a block
+// of 16 tokens.  T's diagonal blocks are substituted forward, a lane a column:
+// with keys that resemble each other the powers of A in a product form of the
+// inverse grow to 1e3 and cancel, which would cost fp32 three of its digits.
+// The blocks below follow by fp32 matrix products, T_ij = -T_ii sum_m A_im T_mj.
 #include "gdr_common.h"
 
 namespace rwkv7m {
@@ -17,14 +17,41 @@ constexpr int NT = 256, PITCH = C + 4;
 
 struct Shared {
     alignas(16) float a[C][PITCH], t[C][PITCH];
-    double G[C];
-    float beta[C];
+    double G[4][C];  // each wave its own
 };
 
 __device__ __forceinline__ float gate(const GdrTensor& t, bool bf16, int64_t b,
                                       int64_t h, int64_t token) {
     return bf16 ? load_f(at<bf16_t>(t, b, h, token))
                 : load_f(at<float>(t, b, h, token));
+}
+
+// The sum over the lanes up to and with the calling one (lane rotations and
+// scalar row totals: a shuffle of a double is two round trips through LDS).
+__device__ __forceinline__ double wave_scan(double x, double* all) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+#define RWKV7M_STEP(ctrl)                                                   \
+    do {                                                                    \
+        i32x2 u = __builtin_bit_cast(i32x2, x);                             \
+        u[0] = __builtin_amdgcn_update_dpp(0, u[0], ctrl, 0xf, 0xf, true);  \
+        u[1] = __builtin_amdgcn_update_dpp(0, u[1], ctrl, 0xf, 0xf, true);  \
+        x += __builtin_bit_cast(double, u);                                 \
+    } while (0)
+    RWKV7M_STEP(0x111);  // row_shr:1
+    RWKV7M_STEP(0x112);
+    RWKV7M_STEP(0x114);
+    RWKV7M_STEP(0x118);
+#undef RWKV7M_STEP
+    const auto lane = [&](int l) {
+        i32x2 u = __builtin_bit_cast(i32x2, x);
+        u[0] = __builtin_amdgcn_readlane(u[0], l);
+        u[1] = __builtin_amdgcn_readlane(u[1], l);
+        return __builtin_bit_cast(double, u);
+    };
+    const int row = threadIdx.x % 64 / 16;
+    const double a = lane(15), b = a + lane(31), c = b + lane(47);
+    *all = c + lane(63);
+    return x + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
 }
 
 // D(M Y) + c from D(M^T) and D(Y) in fp32.
@@ -63,34 +90,29 @@ gdr_prepare_kernel(const GdrArgs A) {
         x.keep(16 * tb + r < valid && 32 * i + 8 * q < A.Dk);
         return x.planes();
     };
+    // Each wave has the gates of all tokens, lane a token.  The running sum of
+    // the log decays: a decay of 0 (-inf) is held to e^-1000, 0 in any result,
+    // so that later differences stay finite.
+    const int token = near(lane, valid - 1);
+    const float g = gate(A.g, A.g_bf16, b, h, t0 + token);
+    const float beta_ = gate(A.beta, A.beta_bf16, b, h, t0 + token);
     Eight<E> qw[KT], kj[4][KT];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (j <= wave) rows(A.k, j, kj[j]);
     rows(A.q, wave, qw);
+    const float beta = lane < valid ? beta_ : 0.f;
+    double all;
+    const double G = wave_scan(
+        lane < valid ? kLog2e * double(g < -1000.f ? -1000.f : g) : 0.0, &all);
+    S.G[wave][lane] = G;
     if (wave == 0) {
-        // the running sum of the log decays: a decay of 0 (-inf) is held to
-        // e^-1000, 0 in any result, so that later differences stay finite
-        double G = 0.0;
-        float beta = 0.f;
-        if (lane < valid) {
-            const float g = gate(A.g, A.g_bf16, b, h, t0 + lane);
-            G = kLog2e * double(g < -1000.f ? -1000.f : g);
-            beta = gate(A.beta, A.beta_bf16, b, h, t0 + lane);
-        }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const double x = __shfl_up(G, m);
-            if (lane >= m) G += x;
-        }
-        S.G[lane] = G;
-        S.beta[lane] = beta;
         out->G[lane] = G;
         out->first[lane] = exp2_of(G);
-        out->last[lane] = exp2_of(__shfl(G, 63) - G);
+        out->last[lane] = exp2_of(all - G);
         out->beta[lane] = beta;
     }
-    __syncthreads();
+    const float beta_own = __shfl(beta, 16 * wave + r);
     Frag<NI> qf[KT], kf[KT];  // the wave's own token block
 #pragma unroll
     for (int p = 0; p < KT; ++p) {
@@ -100,25 +122,24 @@ gdr_prepare_kernel(const GdrArgs A) {
             if (j == wave) kf[p] = planes(kj[j][p], j, p);
     }
     const int own = 16 * wave + r;
-    const double Gw = S.G[own];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j > wave) break;
+    const double* Gs = S.G[wave];
+    const double Gw = Gs[own];
+    // A's and P's block (wave, j)
+    const auto block = [&](int j, const Eight<E> (&kb)[KT]) {
         f32x4_t a = zero4(), pt = zero4();
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
-            const Frag<NI> f = planes(kj[j][p], j, p);
+            const Frag<NI> f = planes(kb[p], j, p);
             mul(a, f, kf[p]);   // D(A^T): s = 4q + e, t = r
             mul(pt, f, qf[p]);  // D(P^T)
         }
         uint32_t lo[NC], hi[NC];
-        const float beta = S.beta[own];
         f32x4_t at_;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int s = 16 * j + 4 * q + e;
-            const float E_ = s <= own ? exp2_of(Gw - S.G[s]) : 0.f;
-            at_[e] = s < own ? a[e] * (beta * E_) : 0.f;
+            const float E_ = s <= own ? exp2_of(Gw - Gs[s]) : 0.f;
+            at_[e] = s < own ? a[e] * (beta_own * E_) : 0.f;
             pt[e] = s <= own ? pt[e] * E_ : 0.f;
         }
         *reinterpret_cast<f32x4_t*>(&S.a[own][16 * j + 4 * q]) = at_;
@@ -128,6 +149,33 @@ gdr_prepare_kernel(const GdrArgs A) {
         for (int n = 0; n < NC; ++n)
             *reinterpret_cast<uint2*>(&out->p[n][own][16 * j + 4 * q]) =
                 make_uint2(lo[n], hi[n]);
+    };
+    // the diagonal blocks first: the first wave, which has no other, inverts
+    // them while the rest are made
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j == wave) block(j, kj[j]);
+    __syncthreads();
+    if (wave == 0) {
+        // block q's column r of the inverse
+        float x[16];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            float sum[4] = {t == r ? 1.f : 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < t; s += 4) {
+                const f32x4_t a = four(&S.a[16 * q + t][16 * q + s]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (s + i < t) sum[i] -= a[i] * x[s + i];
+            }
+            x[t] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            S.t[16 * q + t][16 * q + r] = x[t];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < wave) block(j, kj[j]);
     }
     if ((wave & 1) == 0) {
         // (the block right of the diagonal that shares a pair with it)
@@ -137,24 +185,6 @@ gdr_prepare_kernel(const GdrArgs A) {
                 &out->p[n][own][16 * (wave + 1) + 4 * q]) = make_uint2(0, 0);
         *reinterpret_cast<f32x4_t*>(&S.t[own][16 * (wave + 1) + 4 * q]) =
             zero4();
-    }
-    __syncthreads();
-    if (wave == 0) {
-        // block q's column r of the inverse
-        float x[16];
-#pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            float sum = t == r ? 1.f : 0.f;
-#pragma unroll
-            for (int s = 0; s < t; s += 4) {
-                const f32x4_t a = four(&S.a[16 * q + t][16 * q + s]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (s + i < t) sum -= a[i] * x[s + i];
-            }
-            x[t] = sum;
-            S.t[16 * q + t][16 * q + r] = sum;
-        }
     }
     __syncthreads();
     if (wave < 3) {

@@ -21,13 +21,6 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4_t load4(const float* p) {
     return *reinterpret_cast<const f32x4_t*>(p);
 }
-__device__ __forceinline__ f32x4_t load4(const bf16_t* p) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    return f32x4_t{__uint_as_float(u.x << 16),
-                   __uint_as_float(u.x & 0xffff0000u),
-                   __uint_as_float(u.y << 16),
-                   __uint_as_float(u.y & 0xffff0000u)};
-}
 __device__ __forceinline__ void store4(float* p, const f32x4_t& x) {
     *reinterpret_cast<f32x4_t*>(p) = x;
 }
@@ -51,6 +44,52 @@ __device__ __forceinline__ float dot(const f32x4_t& a, const f32x4_t& b) {
     return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
 }
 
+// Four elements as they lie in memory.
+template <typename E>
+struct Raw;
+template <>
+struct Raw<float> {
+    f32x4_t x;
+    __device__ __forceinline__ void load(const float* p) { x = load4(p); }
+    __device__ __forceinline__ f32x4_t get() const { return x; }
+};
+template <>
+struct Raw<bf16_t> {
+    uint2 u;
+    __device__ __forceinline__ void load(const bf16_t* p) {
+        u = *reinterpret_cast<const uint2*>(p);
+    }
+    __device__ __forceinline__ f32x4_t get() const {
+        return f32x4_t{__uint_as_float(u.x << 16),
+                       __uint_as_float(u.x & 0xffff0000u),
+                       __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xffff0000u)};
+    }
+};
+
+// What the lane needs of a token, loaded without conditions (its places past
+// Dk, and rows past Dv, from the last ones there are).
+template <typename E, int KQ>
+struct Token {
+    Raw<E> k[KQ], q[KQ], v;
+    float g, beta;
+    __device__ __forceinline__ void load(const GdrStepArgs& A, int64_t b,
+                                         int64_t h, int64_t hk, int64_t t,
+                                         int row, int r) {
+        const E* kp = at<E>(A.k, b, hk, t);
+        const E* qp = at<E>(A.q, b, hk, t);
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) {
+            const int col = 64 * j + 4 * r, c = col < A.Dk ? col : A.Dk - 4;
+            k[j].load(kp + c);
+            q[j].load(qp + c);
+        }
+        v.load(at<E>(A.v, b, h, t) + (row < A.Dv ? row : A.Dv - 4));
+        g = gate(A.g, A.g_bf16, b, h, t);
+        beta = gate(A.beta, A.beta_bf16, b, h, t);
+    }
+};
+
 // KQ: 16-lane groups of 4 places a row (Dk up to 64 KQ).
 template <typename E, int KQ>
 __global__ void __launch_bounds__(NT)
@@ -64,6 +103,10 @@ gdr_step_kernel(const GdrStepArgs A, uint32_t parts) {
     const int row = int(blockIdx.x % parts) * ROWS + wave * 16 + (lane >> 4) * 4;
     const bool on = row < A.Dv;  // (Dv is a multiple of 8)
 
+    // the first token on its way before the slot and the state are known, and
+    // each next one while the one before is worked on
+    Token<E, KQ> now, next;
+    now.load(A, b, h, hk, 0, row, r);
     const int64_t slot = A.slots ? A.slots[b] : b;
     int64_t len = A.lengths ? A.lengths[b] : A.T;
     len = len < 0 ? 0 : len > A.T ? A.T : len;
@@ -91,23 +134,23 @@ gdr_step_kernel(const GdrStepArgs A, uint32_t parts) {
     }
     E* o = static_cast<E*>(A.o) + (b * A.T * A.Hv + h) * A.Dv + row;
     for (int64_t t = 0; t < len; ++t) {
-        f32x4_t k[KQ], q[KQ], v = {0.f, 0.f, 0.f, 0.f};
+        next.load(A, b, h, hk, t + 1 < len ? t + 1 : t, row, r);
+        f32x4_t k[KQ], q[KQ];
         float kq = 0.f;
-        const E* kp = at<E>(A.k, b, hk, t);
-        const E* qp = at<E>(A.q, b, hk, t);
 #pragma unroll
         for (int j = 0; j < KQ; ++j) {
-            const int col = 64 * j + 4 * r;
-            k[j] = q[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (col < A.Dk) {
-                k[j] = load4(kp + col);
-                q[j] = load4(qp + col);
+            const bool in = 64 * j + 4 * r < A.Dk;
+            k[j] = now.k[j].get();
+            q[j] = now.q[j].get();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                k[j][e] = in ? k[j][e] : 0.f;
+                q[j][e] = in ? q[j][e] : 0.f;
             }
             kq += dot(k[j], q[j]);
         }
-        if (on) v = load4(at<E>(A.v, b, h, t) + row);
-        const float a = expf(gate(A.g, A.g_bf16, b, h, t));
-        const float beta = gate(A.beta, A.beta_bf16, b, h, t);
+        const f32x4_t v = now.v.get();
+        const float a = expf(now.g), beta = now.beta;
         kq = group_sum<16>(kq);
         f32x4_t out;
 #pragma unroll
@@ -127,6 +170,7 @@ gdr_step_kernel(const GdrStepArgs A, uint32_t parts) {
         }
         if (bad) out = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
         if (r == 0 && on) store4(o + t * A.Hv * A.Dv, out);
+        now = next;
     }
     if (r == 0 && on)
         for (int64_t t = len; t < A.T; ++t)
