@@ -74,9 +74,10 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
         hold();
         mul_triangle<true>(dX, Pf, of);
         Df[0] = split8<NC>(D[0], D[1]);
-        if (DEEP) interleave<8, 3>();
+        if (DEEP) interleave<8, 0, 3>();
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
+            if (DEEP) hold();
             if (!DEEP) blocks(L.k, p, lane, kf[0]);
             else if (p + 1 < KT) blocks(L.k, p + 1, lane, kf[(p + 1) % TWO]);
             else column_blocks(L.q, 0, 0, lane, kf[(p + 1) % TWO]);
@@ -86,11 +87,12 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                     first[tb] = four(L.first + spread(tb, 4 * q));
                     last[tb] = four(L.last + spread(tb, 4 * q));
                 }
-            hold();
+            if (!DEEP) hold();
             mul_each(KD, kf[p % TWO], Df[p]);
             if (p + 1 < KT)
                 Df[p + 1] = split8<NC>(D[2 * p + 2], D[2 * p + 3]);
-            if (DEEP) interleave<8, 3>();
+            if (DEEP && p + 1 < KT) interleave<8, 1, 3>();
+            if (DEEP && p + 1 == KT) interleave<8, 2, 0>();
         }
         // D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K, half of the
         // first product while dX is put together, half while dR is
@@ -102,6 +104,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
         for (int kb = 0; kb < 2 * KT; ++kb) D[kb] *= whole;
         const auto queries = [&](int at) {
             const int n = at / 2, p = at & 1;
+            if (DEEP) hold();
             if (!DEEP)
                 column_blocks(L.q, n, p, lane, kf[0]);
             else if (at + 1 < KT)
@@ -110,7 +113,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
             else
                 column_blocks(L.k, 0, 0, lane, kf[(at + 1) % TWO]);
             if (DEEP && at + 1 == HALF) triangle<true>(L.t, lane, Tf);
-            hold();
+            if (!DEEP) hold();
             f32x4_t sum[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i];
@@ -127,7 +130,8 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
             for (int i = 2 * at / HALF; i < 2 * (at + 1) / HALF; ++i)
                 xf[i] = split8<NC>(dX[2 * i], dX[2 * i + 1]);
-            if (DEEP) interleave<8, 6>();
+            if (DEEP && at + 1 < HALF) interleave<8, 1, 8>();
+            if (DEEP && at + 1 == HALF) interleave<8, 4, 8>();
         }
         if (!DEEP) triangle<true>(L.t, lane, Tf);
 #pragma unroll
@@ -143,22 +147,24 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                 rf[i] = split8<NC>(
                     -(first[2 * i] * beta[2 * i]) * dR[2 * i],
                     -(first[2 * i + 1] * beta[2 * i + 1]) * dR[2 * i + 1]);
-            if (DEEP) interleave<8, 6>();
+            if (DEEP) interleave<8, 1, 8>();
         }
         put_column(A.dr + (head * chunks + c) * C * DVP, DVP, q, v, dR);
 #pragma unroll
         for (int at = 0; at < KT; ++at) {
             const int n = at / 2, p = at & 1;
+            if (DEEP) hold();
             if (!DEEP)
                 column_blocks(L.k, n, p, lane, kf[0]);
             else if (at + 1 < KT)
                 column_blocks(L.k, (at + 1) / 2, (at + 1) & 1, lane,
                               kf[(at + 1) % TWO]);
-            hold();
+            if (!DEEP) hold();
             f32x4_t sum[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i];
             mul_each(sum, kf[at % TWO], rf[p]);
+            if (DEEP) interleave<8, 1, 0>();
 #pragma unroll
             for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
         }

@@ -157,15 +157,17 @@ __device__ __forceinline__ void mul_each(f32x4_t (&acc)[M], const Frag<NA>& a,
 // written to be, ahead of the products that hide their way.
 __device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0); }
 
-// Since the last hold(): N products, each followed by V other vector
-// instructions.  A wave issues in order, a product every 16 cycles: what stands
-// behind them all waits for the last one's turn.
-template <int N, int V>
+// Between two hold(): N products, each followed by D reads of LDS and V other
+// vector instructions, as far as there are any.  A wave issues in order, a
+// product every 16 cycles and a read of LDS no faster: what stands behind a
+// row of either waits for all of it.
+template <int N, int D, int V>
 __device__ __forceinline__ void interleave() {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+        if constexpr (D > 0) __builtin_amdgcn_sched_group_barrier(0x100, D, 0);
+        if constexpr (V > 0) __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
     }
 }
 

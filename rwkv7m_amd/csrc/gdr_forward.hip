@@ -46,8 +46,8 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         const int64_t t0 = c * C;
         const int valid = int(A.T - t0 < C ? A.T - t0 : C);
         // What follows is in the order in which it is issued: each step's
-        // operands are on their way from LDS during the step before, and what
-        // the vector ALU has to do runs between products that do not need it.
+        // operands are read from LDS between the products of the step before,
+        // and so is what the vector ALU has to do and they do not need.
         // (bf16: fp32's three planes leave no registers for it.)
         constexpr bool DEEP = NI == 1;
         constexpr int TWO = DEEP ? 2 : 1, HALF = KT / 2;
@@ -69,6 +69,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         // K S^T, t = spread(tb, 4q + e), v = r
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
+            if (DEEP) hold();
             if (!DEEP) {
                 blocks(L.k, p, lane, kf[0]);
             } else if (p + 1 < KT) {
@@ -82,19 +83,21 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                     first[tb] = four(L.first + spread(tb, 4 * q));
                     beta[tb] = four(L.beta + spread(tb, 4 * q));
                 }
-            hold();
+            if (!DEEP) hold();
             mul_each(B0, kf[p % TWO], Sf[p]);
             if (p + 1 < KT)
                 Sf[p + 1] = split8<NC>(S[2 * p + 2], S[2 * p + 3]);
-            if (DEEP) interleave<8, 3>();
+            if (DEEP && p + 1 < KT) interleave<8, 1, 3>();
+            if (DEEP && p + 1 == KT) interleave<8, 2, 0>();
         }
         // S Q^T, v = 4q + e, t = spread(tb, r), and meanwhile
         const auto queries = [&](int p) {
+            if (DEEP) hold();
             if (!DEEP) blocks(L.q, p, lane, qf[0]);
             else if (p + 1 < KT) blocks(L.q, p + 1, lane, qf[(p + 1) % TWO]);
             else column_blocks(L.k, 0, 0, lane, kf[0]);
             if (DEEP && p + 1 == HALF) triangle<false>(L.t, lane, Tf);
-            hold();
+            if (!DEEP) hold();
             mul_each(O, Sf[p], qf[p % TWO]);
         };
         // R = beta (V - 2^G (K S^T))
@@ -107,22 +110,23 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
             for (int i = 2 * p / HALF; i < 2 * (p + 1) / HALF; ++i)
                 Rf[i] = split8<NC>(V[2 * i], V[2 * i + 1]);
-            if (DEEP) interleave<8, 6>();
+            if (DEEP && p + 1 < HALF) interleave<8, 1, 6>();
+            if (DEEP && p + 1 == HALF) interleave<8, 2, 8>();
         }
         // X = T R
-        if (!DEEP) triangle<false>(L.t, lane, Tf);
-        hold();
-        mul_triangle<false>(X, Tf, Rf);
-#pragma unroll
-        for (int kb = 0; kb < 2 * KT; ++kb) S[kb] *= whole;
-        if (DEEP) interleave<18, 2>();
         f32x4_t last[4];
         float own_first[4];
+        if (!DEEP) triangle<false>(L.t, lane, Tf);
+        hold();
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
             last[tb] = four(L.last + spread(tb, 4 * q));
             own_first[tb] = L.first[spread(tb, r)];
         }
+        mul_triangle<false>(X, Tf, Rf);
+#pragma unroll
+        for (int kb = 0; kb < 2 * KT; ++kb) S[kb] *= whole;
+        if (DEEP) interleave<18, 1, 2>();
 #pragma unroll
         for (int p = HALF; p < KT; ++p) {
             queries(p);
@@ -133,7 +137,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                                    X[2 * i + 1] * last[2 * i + 1]);
                 Xf[i] = split8<NC>(X[2 * i], X[2 * i + 1]);
             }
-            if (DEEP) interleave<8, 7>();
+            if (DEEP) interleave<8, 1, 7>();
         }
         if constexpr (TRAIN) {
             put_column(A.x + (head * chunks + c) * C * DVP, DVP, q, v, X);
@@ -147,6 +151,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int at = 2 * n + p;
+                if (DEEP) hold();
                 if (!DEEP)
                     column_blocks(L.k, n, p, lane, kf[0]);
                 else if (at + 1 < KT)
@@ -154,18 +159,21 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                                   kf[(at + 1) % TWO]);
                 else
                     triangle<false>(L.p, lane, Pf);
-                hold();
+                if (!DEEP) hold();
                 mul_each(sum, kf[at % TWO], Rf[p]);
                 if (at == 0)
 #pragma unroll
                     for (int tb = 0; tb < 4; ++tb) O[tb] *= own_first[tb];
-                if (DEEP && at == 0) interleave<8, 2>();
+                if (DEEP && at == 0) interleave<8, 1, 2>();
+                if (DEEP && at > 0 && at + 1 < KT) interleave<8, 1, 0>();
+                if (DEEP && at + 1 == KT) interleave<8, 2, 0>();
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) S[4 * n + i] = sum[i];
         }
         // O^T = scale (2^G (S Q^T) + X^T P^T)
         if (!DEEP) triangle<false>(L.p, lane, Pf);
+        hold();
         mul_by_triangle(O, Xf, Pf);
         E* to = op + t0 * A.Hv * A.Dv + int64_t(spread(0, r)) * A.Hv * A.Dv +
                 v0 + 4 * q;
