@@ -150,7 +150,8 @@ int rwkv7m_distill_loss_backward(
  * random numbers, from 0 to below 1, decide in float64.
  *
  * target has rows [B][K + 1] of V logits (outer = B, inner = K + 1), draft
- * [B][K], one dtype; rows past n are not read.  A logit of -inf has p = 0.  A
+ * [B][K], one dtype; rows past n are not read.  A logit of -inf has p = 0, as
+ * has one whose p is less than 2^-1000 of the likeliest token's.  A
  * drafted token outside the vocabulary is never taken.  Where the row that is
  * drawn from, or the draft's, holds NaN or +inf, or nothing above -inf, the
  * token drawn is -1 (and no draft is taken against such a row).  The workspace

@@ -252,8 +252,11 @@ __device__ __forceinline__ RowSums join(const LmVerifyStats* s, int parts,
               : 0.0;
     return {m, id, 1.0 / row_sum(sum)};
 }
+// (0 where exp2_64 holds at 2^-1000, for a logit of -inf above all: nothing
+// masked may be drawn or taken, not by a random number of 0 either)
 __device__ __forceinline__ double prob(const RowSums& r, float x, double c) {
-    return exp2_64((double(x) - double(r.largest)) * c) * r.inv;
+    const double t = (double(x) - double(r.largest)) * c;
+    return t < -1000.0 ? 0.0 : exp2_64(t) * r.inv;
 }
 
 struct DrawShared {
@@ -261,7 +264,6 @@ struct DrawShared {
     float picked[2 * kVerifyMostDrafts + 1];
     int taken, last;
 };
-
 
 template <typename E>
 __global__ void __launch_bounds__(DRAW)
@@ -303,6 +305,7 @@ verify_draw_kernel(const LmVerifyArgs A) {
                         p = word && x == r.id ? 1.0 : 0.0;
                         q = 1.0;
                         stop = p == 0.0;
+                        if (r.largest != r.largest) p = r.inv;  // NaN
                     } else {
                         q = 1.0;
                         if (word) {
@@ -369,7 +372,8 @@ verify_draw_kernel(const LmVerifyArgs A) {
             }
             sum = wave_sum(sum);
             whole = wave_sum(whole);
-            const int64_t at = int64_t(part) * per_part + i * (DRAW / 64) + wave;
+            const int64_t at =
+                int64_t(part) * per_part + i * (DRAW / 64) + wave;
             if (lane == 0) {
                 __hip_atomic_store(masses + at, sum, __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
@@ -453,7 +457,8 @@ verify_draw_kernel(const LmVerifyArgs A) {
         run += all;
     }
     if (segment < 0)
-        segment = lanes_fold<64>(last, [](int a, int c) { return a > c ? a : c; });
+        segment =
+            lanes_fold<64>(last, [](int a, int c) { return a > c ? a : c; });
     // its tokens in their order, adjoining ones a lane
     const int64_t j0 = int64_t(segment) * width + lane * per;
     double w[per], mine = 0.0, all;

@@ -142,3 +142,236 @@ def test_ragged_and_temperatures(lm, temp, dtype):
     check(lm, x, tok, y, u, s, n, temp)
     check(lm, x, tok.int(), y, u, s, n.int(), temp)
     check(lm, x, tok, None, u, s, n, temp)
+
+
+# --- rows at their ends --------------------------------------------------------
+
+def _one(lm, x, tok, y=None, u=None, s=None, temp=1.0):
+    B, K = tok.shape
+    u = torch.zeros(B, K) if u is None else u
+    s = torch.zeros(B) if s is None else s
+    got = lm.verify_drafts(x.cuda(), tok.cuda(),
+                           None if y is None else y.cuda(), u.cuda(),
+                           s.cuda(), None, temp)
+    return [t.cpu() for t in got]
+
+
+@pytest.mark.parametrize("V", [300, 9000])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("masked", [-INF, None])
+def test_masked_tokens(lm, V, dtype, masked):
+    """Nothing masked, by -inf or the type's lowest value, is taken or drawn,
+    not by random numbers of 0 or next to 1 either."""
+    print("case: masks", V, dtype, masked, flush=True)
+    low = torch.finfo(DT[dtype]).min if masked is None else masked
+    x = torch.full((4, 3, V), low, dtype=DT[dtype])
+    y = x[:, :2].clone()
+    allowed = [3, V // 2, V - 2]
+    x[..., allowed] = torch.tensor([0.5, 1.0, -1.0], dtype=DT[dtype])
+    y[..., allowed] = torch.tensor([1.0, -2.0, -1.0], dtype=DT[dtype])
+    tok = torch.tensor([[allowed[0], 0], [0, 1], [V - 1, 3], [3, V // 2]])
+    top = torch.tensor(1.0 - 2.0 ** -24)
+    for s in (torch.zeros(4), top.expand(4).clone()):
+        for q in (None, y):
+            took, count, chance = (t for t in _one(lm, x, tok, q, None, s))
+            assert count.tolist() == [1, 0, 0, 2]
+            drawn = took.gather(1, count[:, None])[:, 0]
+            assert set(drawn.tolist()) <= set(allowed)
+            assert (took[took >= 0][:, None] ==
+                    torch.tensor(allowed)).any(-1).all()
+            if q is None:  # row 0 draws without token 0, which has nothing
+                last = allowed[0] if float(s[0]) == 0.0 else allowed[2]
+                assert drawn.tolist()[:3] == [last] * 3
+            assert chance[1].tolist() == [0.0, 0.0] or q is not None
+    # certain drafts refused: the drawn token is another one
+    two = torch.full((1, 2, V), low, dtype=DT[dtype])
+    two[..., [5, 7]] = 0.0
+    for s in (0.0, 0.5, float(top)):
+        took, count, _ = _one(lm, two, torch.tensor([[5]]), None,
+                              torch.full((1, 1), 0.75), torch.tensor([s]))
+        assert int(count) == 0 and took.tolist() == [[7, -1]]
+    # one token left in the vocabulary
+    two[..., 7] = low
+    took, count, chance = _one(lm, two, torch.tensor([[5]]), two[:, :1],
+                               torch.full((1, 1), 0.75), torch.tensor([0.9]))
+    assert took.tolist() == [[5, 5]] and float(chance) == 1.0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("temp", [0.0, 0.7])
+@pytest.mark.parametrize("what", ["nan", "inf", "empty"])
+def test_rows_without_a_distribution(lm, dtype, temp, what):
+    print("case: no distribution", dtype, temp, what, flush=True)
+    V = 8200
+    x, tok, y, u, s = make(3, 2, V, dtype, 3)
+    tok[:] = x[:, :2].double().argmax(-1)
+    u *= 0
+
+    def spoil(row):
+        if what == "empty":
+            row[:] = -INF
+        else:
+            row[8195] = float(what)
+
+    for spoiled in range(3):
+        bad = x.clone()
+        spoil(bad[1, spoiled])
+        for q in (None, y):
+            took, count, chance = _one(lm, bad, tok, q, u, s, temp)
+            good = _one(lm, x, tok, q, u, s, temp)
+            assert int(count[1]) == spoiled
+            assert took[1].tolist() == tok[1, :spoiled].tolist() + \
+                [-1] * (3 - spoiled)
+            if spoiled < 2:
+                assert chance[1, spoiled].isnan()
+            for a, b in zip((took, count, chance), good):
+                assert torch.equal(a[[0, 2]], b[[0, 2]])
+    if temp:
+        bad = y.clone()
+        spoil(bad[1, 0])
+        took, count, chance = _one(lm, x, tok, bad, u, s, temp)
+        assert int(count[1]) == 0 and took[1].tolist() == [-1] * 3
+        assert chance[1, 0].isnan()
+
+
+def test_drafts_outside_the_vocabulary(lm):
+    print("case: outside", flush=True)
+    x, tok, y, u, s = make(4, 2, 500, "f32", 4)
+    tok[0, 0], tok[1, 0], tok[2, 1], tok[3, 0] = -1, 500, 2 ** 40, -2 ** 62
+    u *= 0
+    for q in (None, y):
+        took, count, chance = _one(lm, x, tok, q, u, s)
+        assert count.tolist() == [0, 0, 1, 0]
+        assert chance[[0, 1, 2, 3], [0, 0, 1, 0]].tolist() == [0.0] * 4
+        assert bool((took.gather(1, count[:, None]) >= 0).all())
+    took, count, _ = _one(lm, x, tok, temp=0.0)
+    assert count.tolist() == [0, 0, 0, 0] or int(tok[2, 0]) == int(took[2, 0])
+
+
+def test_equal_rows_and_ties(lm):
+    """p = q: nothing is left, every draft is taken below 1; equal logits:
+    the lowest id is the likeliest."""
+    print("case: ties", flush=True)
+    V = 20000
+    x, tok, y, u, s = make(3, 4, V, "bf16", 5)
+    took, count, chance = _one(lm, x, tok, x[:, :4].clone(),
+                               torch.full((3, 4), 1 - 2.0 ** -24), s)
+    assert count.tolist() == [4] * 3 and bool((chance == 1).all())
+    flat = torch.zeros(1, 2, V)
+    flat[0, 1, [9000, 17, 19999]] = 2.0
+    took, count, _ = _one(lm, flat, torch.tensor([[0]]), temp=0.0)
+    assert took.tolist() == [[0, 17]]
+    took, count, _ = _one(lm, flat, torch.tensor([[1]]), temp=0.0)
+    assert took.tolist() == [[0, -1]]
+    # a flat row's draws lie where the running sum says
+    for u_ in (0.0, 0.25, 0.7, 1 - 2.0 ** -24):
+        took, *_ = _one(lm, flat[:, :1], torch.zeros(1, 0).long(),
+                        s=torch.tensor([u_]))
+        at = float(torch.tensor(u_).double()) * V
+        assert int(took) in (int(at), max(int(at) - 1, 0))
+
+
+def test_layouts(lm):
+    """Views with strides of their own, odd starts, and vectors that have to
+    be copied: as contiguous ones."""
+    print("case: layouts", flush=True)
+    x, tok, y, u, s = make(5, 3, 1003, "bf16", 6)
+    big = torch.zeros(5, 4, 1003 + 7).bfloat16()
+    big[..., 3:1006] = x
+    turned = y.transpose(1, 2).contiguous().transpose(1, 2)
+    major = x.transpose(0, 1).contiguous().transpose(0, 1)
+    want = lm.verify_drafts(*(t.cuda() for t in (x, tok, y, u, s)))
+    wide = torch.stack([tok, tok], -1).int().cuda()[..., 0]
+    uu = torch.stack([u, u], 0).cuda()[1]
+    for a, b in ((big.cuda()[..., 3:1006], turned.cuda()),
+                 (major.cuda(), y.cuda())):
+        assert not a.is_contiguous()
+        got = lm.verify_drafts(a, wide, b, uu, s.cuda())
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    one = x[:, :1].cuda().expand(5, 4, 1003)
+    a = lm.verify_drafts(one, tok.cuda(), None, u.cuda(), s.cuda())
+    b = lm.verify_drafts(one.contiguous(), tok.cuda(), None, u.cuda(),
+                         s.cuda())
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_distribution_of_what_is_emitted(lm):
+    """With drafts drawn from q the first token emitted is distributed as p:
+    the shares of q's drafts over a grid of both random numbers.  A grid of n
+    midpoints misses the measure of an interval by at most 1 / n; of u there is
+    one interval a draft (taken or not), 1 / 32, of s one a token, 1 / 512."""
+    print("case: distribution", flush=True)
+    V, n = 5, 512
+    g = _gen(7)
+    p, q = torch.randn(V, generator=g), torch.randn(V, generator=g)
+    mid = (torch.arange(n) + 0.5) / n
+    share = torch.zeros(V, dtype=torch.float64)
+    qs = torch.softmax(q.double(), -1)
+    x = p.cuda().expand(n, 2, V)
+    for draft in range(V):
+        tok = torch.full((n, 1), draft).cuda()
+        for u in mid[::16]:
+            got = lm.verify_drafts(x, tok, q.cuda().expand(n, 1, V),
+                                   torch.full((n, 1), float(u)).cuda(),
+                                   mid.cuda())
+            first = got.tokens[:, 0].cpu()
+            share += qs[draft] * torch.bincount(first, minlength=V) / n / 32
+    off = (share - torch.softmax(p.double(), -1)).abs().max()
+    assert float(off) <= 1 / 32 + 1 / 512, off
+
+
+# --- sizes, streams, graphs ----------------------------------------------------
+
+def test_offsets_past_32_bits(lm):
+    print("case: offsets past 32 bits", flush=True)
+    x, tok, y, u, s = (t.cuda() for t in make(2, 2, 70000, "bf16", 8))
+    apart = 2 ** 31 + 5
+    big = torch.zeros(apart + 3 * 70000, dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((2, 3, 70000), (apart, 70000, 1))
+    far.copy_(x)
+    for q in (y, None):
+        a = lm.verify_drafts(far, tok, q, u, s)
+        b = lm.verify_drafts(x, tok, q, u, s)
+        assert all(torch.equal(m, n) for m, n in zip(a, b))
+
+
+def test_no_sequences_and_many(lm):
+    print("case: none and many", flush=True)
+    x, tok, y, u, s = (t.cuda() for t in make(3000, 1, 33, "f32", 9))
+    got = lm.verify_drafts(x, tok, y, u, s)
+    last = lm.verify_drafts(x[-2:], tok[-2:], y[-2:], u[-2:], s[-2:])
+    assert all(torch.equal(a[-2:], b) for a, b in zip(got, last))
+    none = lm.verify_drafts(x[:0], tok[:0], y[:0], u[:0], s[:0])
+    assert [tuple(t.shape) for t in none] == [(0, 2), (0,), (0, 1)]
+
+
+def test_streams_and_two_graphs(lm):
+    print("case: streams and graphs", flush=True)
+    cases = [[t.cuda() for t in make(6, 3, 30000, "bf16", i)] for i in (1, 2)]
+    want = [lm.verify_drafts(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(lm.verify_drafts(*c))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2]))
+    graphs = []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            out = lm.verify_drafts(*c)
+        graphs.append((graph, out))
+    for rep in range(4):
+        for i in ((0, 1), (1, 0), (1, 1), (0, 0))[rep]:
+            graph, out = graphs[i]
+            for t in out:
+                t.fill_(-7)
+            lm.verify_drafts(*cases[1 - i])
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i])), rep
