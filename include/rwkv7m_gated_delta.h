@@ -85,7 +85,7 @@ int rwkv7m_gated_delta_rule_backward(
  * goes on from state slots[b] (NULL: b) over its first lengths[b] tokens
  * (NULL, or more than T: T); o is 0 behind them.  A slot below 0 is padding:
  * o is 0.  A slot of `pool` or more, or one that an earlier row of the same
- * updating call has, gives NaN in o and leaves the state to the earlier row. */
+ * call updates, gives NaN in o and leaves the state to the earlier row. */
 int rwkv7m_gated_delta_step(const rwkv7m_gated_delta_inputs *in, int64_t pool,
                             float *state, const int64_t *slots,
                             const int64_t *lengths, int update, void *o,

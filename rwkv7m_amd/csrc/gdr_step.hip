@@ -100,7 +100,8 @@ gdr_step_kernel(const GdrStepArgs A, uint32_t parts) {
     const uint32_t bh = blockIdx.x / parts, Hv = uint32_t(A.Hv);
     const int64_t b = bh / Hv, h = bh % Hv,
                   hk = uint32_t(h) / (Hv / uint32_t(A.Hk));
-    const int row = int(blockIdx.x % parts) * ROWS + wave * 16 + (lane >> 4) * 4;
+    const int row =
+        int(blockIdx.x % parts) * ROWS + wave * 16 + (lane >> 4) * 4;
     const bool on = row < A.Dv;  // (Dv is a multiple of 8)
 
     // the first token on its way before the slot and the state are known, and
@@ -129,7 +130,7 @@ gdr_step_kernel(const GdrStepArgs A, uint32_t parts) {
     if (A.update && A.slots && slot >= 0 && len > 0) {
         bool twice = false;
         for (int64_t j = lane; j < b; j += 64)
-            twice |= A.slots[j] == slot;
+            twice |= A.slots[j] == slot && (!A.lengths || A.lengths[j] > 0);
         bad |= __builtin_amdgcn_ballot_w64(twice) != 0;
     }
     E* o = static_cast<E*>(A.o) + (b * A.T * A.Hv + h) * A.Dv + row;

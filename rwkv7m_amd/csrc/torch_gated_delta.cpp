@@ -71,7 +71,6 @@ struct Inputs {
                           in.Dv);
         gate_shape("g", g_, in.B, in.T, in.Hv);
         gate_shape("beta", beta_, in.B, in.T, in.Hv);
-        same_gpu({&q_, &k_, &v_, &g_, &beta_});
         in.scale = scale ? *scale : 1.0 / std::sqrt(double(in.Dk));
         q = q_;
         k = k_;
@@ -109,7 +108,15 @@ Tensor workspace(const Tensor& like, int64_t bytes) {
                      like.options().dtype(at::kByte).requires_grad(false));
 }
 
+// A state as the kernels take it.
+Tensor placed(const Tensor& t) {
+    if (!t.defined()) return t;
+    const Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
 void check_state(const Inputs& x, const Tensor& initial) {
+    same_gpu({&x.q, &x.k, &x.v, &x.g, &x.beta, &initial});
     if (!initial.defined()) return;
     TORCH_CHECK_VALUE(initial.sizes() == at::IntArrayRef(x.state_shape()),
                       "initial_state must have shape ",
@@ -118,7 +125,6 @@ void check_state(const Inputs& x, const Tensor& initial) {
     TORCH_CHECK_TYPE(initial.scalar_type() == at::kFloat,
                      "initial_state must be float32, got ",
                      initial.scalar_type());
-    same_gpu({&x.q, &initial});
 }
 
 // [o, final state, what the backward takes (undefined where not wanted)]
@@ -126,7 +132,7 @@ variable_list rule_forward(Inputs& x, const Tensor& initial, bool train) {
     check_state(x, initial);
     const c10::DeviceGuard guard(x.q.device());
     x.place();
-    const Tensor s0 = dense(initial);
+    const Tensor s0 = placed(initial);
     Tensor o = at::empty(x.o_shape(), x.q.options().requires_grad(false));
     Tensor end = at::empty(x.state_shape(), f32(x.q)), saved;
     if (train) {
@@ -171,7 +177,7 @@ struct GatedDeltaRule : torch::autograd::Function<GatedDeltaRule> {
         if (!dout.defined())
             dout = at::zeros(x.o_shape(), x.q.options().requires_grad(false));
         dout = Inputs::rows(dout, 16);
-        const Tensor dend = dense(d[1]);
+        const Tensor dend = placed(d[1]);
         const auto like = [](const Tensor& t) {
             return at::empty(t.sizes(), t.options().requires_grad(false));
         };
@@ -245,7 +251,7 @@ Tensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v,
         TORCH_CHECK_VALUE(state.size(0) == x.in.B, "a state for each of the ",
                           x.in.B, " rows is needed where slots is None, got ",
                           state.size(0));
-    same_gpu({&x.q, &state, &lengths, &slots});
+    same_gpu({&x.q, &x.k, &x.v, &x.g, &x.beta, &state, &lengths, &slots});
     const c10::DeviceGuard guard(x.q.device());
     x.place();
     const auto ids = [](const Tensor& t) {
@@ -258,6 +264,9 @@ Tensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v,
           rwkv7m_gated_delta_step(&x.in, state.size(0), ptr<float>(state),
                                   ptr<int64_t>(slots), ptr<int64_t>(lengths),
                                   update, ptr(o), stream_of(x.q)));
+    // (a backward that saved the states as they were has to notice)
+    if (update && !state.is_inference())
+        state.unsafeGetTensorImpl()->bump_version();
     return o;
 }
 
