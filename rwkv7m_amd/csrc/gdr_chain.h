@@ -319,10 +319,14 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
     }
 }
 
-// Owning waves of a workgroup: as many workgroups as there are CUs, where the
-// heads are few (a CU's waves share its LDS, whose reads are half of a chunk's
-// time: 32 heads of 1999 tokens take @@ us with one, @@ with two and @@ with
-// four), and as few as possible beyond, since each brings its own K and Q.
+// Owning waves of a workgroup: as few as leave no more workgroups than CUs,
+// and four beyond, since every workgroup brings its own K, Q, T and P and a
+// CU's workgroups share its LDS.  Forward, us with one, two and four (* the
+// rule's), bf16:
+//   1 x 1999 tokens, 32 heads of 128 x 128   77 *   75.5    85
+//   8 x 512, 12 of 64 x 64                   37     22.5 *  25
+//   2 x 1001, 24 of 96 x 128                 87     54 *    65
+//   8 x 4096, 16 of 128 x 128               765    494     370 *
 inline int owning_waves(int64_t heads, int dvp) {
     for (int w = 1; w < 4; w *= 2)
         if (heads * ((dvp + 16 * w - 1) / (16 * w)) <= device_cus()) return w;

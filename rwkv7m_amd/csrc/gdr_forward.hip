@@ -1,6 +1,12 @@
 // The gated delta rule's recurrence over chunks (gdr_common.h has the
 // formulas, gdr_chain.h the division of work): outputs, and the state before
 // each chunk and X where a backward follows.
+//
+// With few heads bound by the way through a chunk, one after the other: 32
+// heads of 128 x 128 over 1999 tokens 77 us, 2.4 a chunk, of which a wave's
+// 132 matrix instructions are 0.9.  With many, where states and X are kept, by
+// memory: 8 x 4096 tokens, 16 heads of 128 x 128, move 1.62 GB in 350 to 370
+// us, 4.5 TB/s.
 #include "gdr_chain.h"
 
 namespace rwkv7m {

