@@ -7,10 +7,15 @@
 //   left = -2^G (dR S0) - N K
 //   right = 2^(G_L - G) (X D) + dP^T Q - (beta N)^T K
 //   dk = beta left + right,  dv = beta dR,  dbeta = k.left + dR.v
-//   dG = q.dq + beta k.left - k.right = q.dq - dv.v (both of the others are
-//   dR.X less or without dv.v), + <D, S_L> at the last token,
+//   dG = q.dq + beta k.left - k.right, + <D, S_L> at the last token,
 //   dg = the sum of dG from the token on,
 //   <D, S_L> = 2^G_L <D, S0> + sum_t k_t.(2^(G_L - G) X D)_t
+//
+// (q.dq - dv.v is dG as well, and cheaper.  But in the running sum of the form
+// above the pairs of tokens on one side of its border cancel, product by
+// product; of the other they do not, and dg, a small sum of large terms, is
+// 1.3e-5 off for 8e-6.  For its sake X and dR are three planes here: 6e-6, at 3
+// to 8 % of this kernel's time.  A third plane of N too: 5.5e-6, 6 % more.)
 //
 // One workgroup a chunk and value head, all of them independent.  A wave owns
 // 32 tokens and a share of the columns of dq, left and right.  S0 and D pass
@@ -19,8 +24,8 @@
 // blocks of N and dP are divided among the waves and meet in LDS, whose rows
 // are operands for dq and left, whose columns for right.
 //
-// 8 x 512 tokens, 12 heads of 64 x 64: 29 us.  8 x 4096, 16 heads of 128 x 128:
-// 2.55 GB in 735 to 795 us, 3.3 TB/s, bound by a workgroup's own steps (one
+// 8 x 512 tokens, 12 heads of 64 x 64: 30.5 us.  8 x 4096, 16 of 128 x 128:
+// 2.55 GB in 760 to 820 us, 3.2 TB/s, bound by a workgroup's own steps (one
 // lives on a CU, its sums fill the registers): the loads of its first block and
 // the gates, a quarter of its time, and four blocks between barriers.
 #include "gdr_common.h"
@@ -44,7 +49,7 @@ struct GradShared {
     union {
         struct {  // a block of 32 columns of v
             Rows<kMade<E>, KT, 32> s, d;  // S0's and D's rows
-            Rows<kMade<E>, 1> x, r;       // X, dR
+            Rows<3, 1> x, r;              // X, dR
             Rows<kIn<E>, 1> o;            // dO
         };
         struct {  // what is made of them
@@ -57,7 +62,7 @@ struct GradShared {
             Rows<kMade<E>, 2> n;  // N, then -beta N
             union {
                 Rows<kMade<E>, 2> p;  // dP
-                float dots[kShares<E, KT>][2][C];  // q.dq, k.left, behind it
+                float dots[kShares<E, KT>][2][C];  // of dG, k.left, behind it
             };
         };
     };
@@ -240,7 +245,7 @@ gdr_gradients_kernel(const GdrArgs A) {
             if (v0 + 32 < DVP) fetch(v0 + 32);
         // operands of the wave's tokens (left or right alike)
         Frag<NI> of[2];
-        Frag<NC> xf[2], rf[2];
+        Frag<3> xf[2], rf[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             of[i] = L.o.rows_in_order(2 * th + i, 0, lane);
@@ -264,10 +269,10 @@ gdr_gradients_kernel(const GdrArgs A) {
             }
         } else {
             const Frag<NI> o = L.o.rows_in_order(2 + th, 0, lane);
-            const Frag<NC> g = L.r.rows_in_order(2 + th, 0, lane);
+            const Frag<3> g = L.r.rows_in_order(2 + th, 0, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const Frag<NC> x = L.x.rows_in_order(i, 0, lane);
+                const Frag<3> x = L.x.rows_in_order(i, 0, lane);
                 mul(dp[i], o, x);
                 mul(nn[i], g, x);
             }
@@ -396,18 +401,20 @@ gdr_gradients_kernel(const GdrArgs A) {
     // the gates' gradients
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        f32x4_t kleft = zero4(), qdq = zero4();
+        f32x4_t kleft = zero4(), dg = zero4();
         const int row = 16 * (2 * th + i);
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
             const f32x4_t kv = L.k.values(row + 4 * q, kh * KW + j, lane);
             left[i][j] = -left[i][j];
-            qdq += L.q.values(row + 4 * q, kh * KW + j, lane) * dq[i][j];
+            dg += L.q.values(row + 4 * q, kh * KW + j, lane) * dq[i][j] -
+                  kv * right[i][j];
             kleft += kv * left[i][j];
         }
+        dg += four(L.beta + row + 4 * q) * kleft;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x = sum16(qdq[e]), y = sum16(kleft[e]);
+            const float x = sum16(dg[e]), y = sum16(kleft[e]);
             if (r < 2) L.dots[kh][r][row + 4 * q + e] = r ? y : x;
         }
     }
@@ -430,8 +437,7 @@ gdr_gradients_kernel(const GdrArgs A) {
             for (int k = 1; k < KQ; ++k) sum += L.dots[k][i][lane];
             return sum;
         };
-        double x = double(dot(0)) - double(L.beta[lane] * L.rv[lane]);
-        double end = 0.0;  // <D, S_L> at the chunk's last token
+        double x = dot(0), end = 0.0;  // <D, S_L> at the chunk's last token
 #pragma unroll
         for (int w = 0; w < 2 * KQ; ++w) end += L.sums[w];
         if (lane == 63) x += end;

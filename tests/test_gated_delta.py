@@ -422,6 +422,31 @@ def test_gradients_wanted_of_some(lm):
         assert torch.equal(got, want[i])
 
 
+@pytest.mark.parametrize("B,T,Hk,Hv,Dk,Dv", [
+    (1, 84, 2, 6, 64, 64), (5, 203, 3, 3, 128, 256), (3, 300, 1, 3, 64, 128)])
+def test_fp32_results_of_bf16_vectors(lm, B, T, Hk, Hv, Dk, Dv):
+    """By their 2-norms.  Two planes leave out 2^-18 of an operand's place at
+    most, 2^-18 / sqrt(3) in the mean, and the product of the second planes as
+    much: with eight products on the longest way 4 2^-18 / sqrt(3) sqrt(2) =
+    1.2e-5 if all had that mean; most places are further from a rounding's
+    border and the ways mostly shorter: 1e-5.  dg is <D, S (I - beta k k^T)> of
+    a token, factor by factor a product of two results off by 1.2e-5, each
+    place by itself: sqrt(2) 1.2e-5 = 1.7e-5 of the sum's size."""
+    print("case: fp32 results", B, T, Hk, Hv, Dk, Dv, flush=True)
+    x = make(B, T, Hk, Hv, Dk, Dv, "bf16", seed=T)
+    s0 = torch.randn(B, Hv, Dv, Dk, generator=_gen(1))
+    do = torch.randn(B, T, Hv, Dv, generator=_gen(2)).bfloat16()
+    ds = torch.randn(B, Hv, Dv, Dk, generator=_gen(3))
+    (_, end), grads, _ = grads64(x, s0, do, ds)
+    leaves = [t.cuda().requires_grad_() for t in (*x, s0)]
+    o, got = lm.gated_delta_rule(*leaves)
+    d = torch.autograd.grad([o, got], leaves, [do.cuda(), ds.cuda()])
+    for name, a, b in (("state", got, end), ("dg", d[3], grads[3]),
+                       ("dbeta", d[4], grads[4]), ("ds0", d[5], grads[5])):
+        off = float((a.detach().double().cpu() - b).norm() / b.norm())
+        assert off <= (1.7e-5 if name == "dg" else 1e-5), (name, off)
+
+
 def test_derivatives_that_are_refused(lm):
     print("case: derivatives refused", flush=True)
     x = [t.cuda().requires_grad_() for t in make(1, 5, 1, 1, 16, 16, "f32")]
