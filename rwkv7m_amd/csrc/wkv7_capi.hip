@@ -912,9 +912,9 @@ int gdr_sizes(const char* fn, const rwkv7m_gated_delta_inputs* in,
                         "Dv up to 256)");
     if (!std::isfinite(in->scale))
         return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": scale is not finite");
-    // (launches have fewer than 2^32 threads along an axis, chunk kernels 256
-    // a chunk, and a few workgroups a head)
-    const int64_t C = rwkv7m::kGdrChunk, most = (int64_t(1) << 24) - 1;
+    // (launches have fewer than 2^32 threads along an axis, chunk kernels up to
+    // 512 a chunk, the chains up to four workgroups of 512 a head)
+    const int64_t C = rwkv7m::kGdrChunk, most = (int64_t(1) << 23) - 1;
     if (in->B > most || in->Hv > most || in->T > (int64_t(1) << 40))
         return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": sizes too large");
     s->chunks = (in->T + C - 1) / C;
