@@ -315,3 +315,34 @@ def test_two_streams_at_once(lm):
     torch.cuda.synchronize()
     for i, out in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2]))
+
+
+def test_inference_mode_and_two_calls_on_one_pool(lm):
+    """States made inside and outside of inference mode, and two streams at
+    work on different slots of one pool."""
+    print("case: inference mode", flush=True)
+    x = [t.cuda() for t in make(4, 2, 1, 2, 64, 64, "bf16", seed=15)]
+    pool = torch.randn(8, 2, 64, 64, generator=_gen(1)).cuda()
+    slots = torch.tensor([5, 0, 7, 2], device="cuda")
+    want = pool.clone()
+    o = lm.gated_delta_step(*x, want, slots=slots)
+    outer = pool.clone()
+    with torch.inference_mode():
+        inner = pool.clone()
+        for state in (inner, outer):
+            assert torch.equal(lm.gated_delta_step(*x, state, slots=slots), o)
+            assert torch.equal(state, want)
+        a, end = lm.gated_delta_rule(*x, pool[slots])
+        tok = torch.zeros(4, 1, dtype=torch.int64, device="cuda")
+        lm.verify_drafts(a.float().flatten(2), tok, temperature=0.0)
+    state = pool.clone()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            outs.append(lm.gated_delta_step(
+                *(t[2 * i:2 * i + 2] for t in x), state,
+                slots=slots[2 * i:2 * i + 2]))
+    torch.cuda.synchronize()
+    assert torch.equal(torch.cat(outs), o) and torch.equal(state, want)
