@@ -27,8 +27,9 @@
  * its chunk of 64 tokens NaN.
  *
  * Sums and states are fp32, products bf16 matrix instructions over sums of
- * bf16 planes: results are off by fp32's rounding or, with bf16 vectors, some
- * 2^-18 of their size, before they are rounded to their own type.  Calls only
+ * three bf16 planes, which hold what fp32 does: results are off as with fp32
+ * products, some 2e-7 of their norm, up to 3e-6 where beta |k|^2 nears 2 and
+ * keys hardly differ, before they are rounded to their own type.  Calls only
  * enqueue work on `stream`, never allocate and never synchronise, so they may
  * be captured in a HIP graph.  Results do not depend on the order in which
  * workgroups run, nor a sequence's on the others in its batch.

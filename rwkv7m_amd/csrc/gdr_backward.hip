@@ -18,7 +18,7 @@ template <typename E, int KT, int OW>
 __global__ void __launch_bounds__(64 * OW + BRING)
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 gdr_backward_kernel(const GdrArgs A, int parts) {
-    constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
+    constexpr int NI = kIn<E>, NC = kMade, DKP = 32 * KT;
     extern __shared__ char lds_raw[];
     const Place at_ = place(blockIdx.x, parts);
     const int64_t head = at_.head;
@@ -45,7 +45,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
 
     chain<E, KT, OW>(
         A, A.dout,
-        static_cast<const Prepared<NC>*>(A.prepared) + head * chunks, head,
+        static_cast<const Prepared*>(A.prepared) + head * chunks, head,
         16 * OW * at_.part, chunks - 1, -1, chunks,
         reinterpret_cast<ChainChunk<E, KT>*>(lds_raw),
         [&](const ChainChunk<E, KT>& L, int64_t c) {
@@ -64,7 +64,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
         const float whole = L.first[C - 1];
         column.take(L, c, c - 1, wave, lane, dO);
         if (DEEP) {
-            triangle<true>(L.p, lane, Pf);
+            triangle<true>(L.m.p, lane, Pf);
             blocks(L.k, 0, lane, kf[0]);
         }
 #pragma unroll
@@ -73,11 +73,11 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
         for (int p = 0; p < 2; ++p)
             of[p] = split8<NI>(dO[2 * p], dO[2 * p + 1]);
         // P^T dO and K D^T, t = spread(tb, 4q + e), v = r
-        if (!DEEP) triangle<true>(L.p, lane, Pf);
+        if (!DEEP) triangle<true>(L.m.p, lane, Pf);
         hold();
         mul_triangle<true>(dX, Pf, of);
         Df[0] = split8<NC>(D[0], D[1]);
-        if (DEEP) interleave<8, 0, 3>();
+        if (DEEP) interleave<4 * NC, 0, 3>();
 #pragma unroll
         for (int p = 0; p < KT; ++p) {
             if (DEEP) hold();
@@ -94,8 +94,8 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
             mul_each(KD, kf[p % TWO], Df[p]);
             if (p + 1 < KT)
                 Df[p + 1] = split8<NC>(D[2 * p + 2], D[2 * p + 3]);
-            if (DEEP && p + 1 < KT) interleave<8, 1, 3>();
-            if (DEEP && p + 1 == KT) interleave<8, 2, 0>();
+            if (DEEP && p + 1 < KT) interleave<4 * NC, 1, 3>();
+            if (DEEP && p + 1 == KT) interleave<4 * NC, 2, 0>();
         }
         // D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K, half of the
         // first product while dX is put together, half while dR is
@@ -115,7 +115,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                               kf[(at + 1) % TWO]);
             else
                 column_blocks(L.k, 0, 0, lane, kf[(at + 1) % TWO]);
-            if (DEEP && at + 1 == HALF) triangle<true>(L.t, lane, Tf);
+            if (DEEP && at + 1 == HALF) triangle<true>(L.m.t, lane, Tf);
             if (!DEEP) hold();
             f32x4_t sum[4];
 #pragma unroll
@@ -133,10 +133,10 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
             for (int i = 2 * at / HALF; i < 2 * (at + 1) / HALF; ++i)
                 xf[i] = split8<NC>(dX[2 * i], dX[2 * i + 1]);
-            if (DEEP && at + 1 < HALF) interleave<8, 1, 8>();
-            if (DEEP && at + 1 == HALF) interleave<8, 4, 8>();
+            if (DEEP && at + 1 < HALF) interleave<4 * NC, 1, 8>();
+            if (DEEP && at + 1 == HALF) interleave<4 * NC, 4, 8>();
         }
-        if (!DEEP) triangle<true>(L.t, lane, Tf);
+        if (!DEEP) triangle<true>(L.m.t, lane, Tf);
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) beta[tb] = four(L.beta + spread(tb, 4 * q));
         hold();
@@ -150,7 +150,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
                 rf[i] = split8<NC>(
                     -(first[2 * i] * beta[2 * i]) * dR[2 * i],
                     -(first[2 * i + 1] * beta[2 * i + 1]) * dR[2 * i + 1]);
-            if (DEEP) interleave<8, 1, 8>();
+            if (DEEP) interleave<4 * NC, 1, 8>();
         }
         put_column(A.dr + (head * chunks + c) * C * DVP, DVP, q, v, dR);
 #pragma unroll
@@ -167,7 +167,7 @@ gdr_backward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = D[4 * n + i];
             mul_each(sum, kf[at % TWO], rf[p]);
-            if (DEEP) interleave<8, 1, 0>();
+            if (DEEP) interleave<4 * NC, 1, 0>();
 #pragma unroll
             for (int i = 0; i < 4; ++i) D[4 * n + i] = sum[i];
         }

@@ -75,7 +75,7 @@ constexpr bool kColumns = sizeof(E) == 2 || KT < 4;
 template <typename E, int KT>
 struct ChainChunk {
     Rows<kIn<E>, KT> k, q;
-    Rows<kMade<E>, 2> t, p;
+    Matrices m;
     std::conditional_t<kColumns<E, KT>, Columns<E>, NoColumns> v;
     alignas(16) float first[C], last[C], beta[C];
 };
@@ -129,16 +129,17 @@ struct OwnColumn {
 // A bringing thread's share of a chunk, for OW owning waves.
 template <typename E, int KT, int OW>
 struct Bring {
-    static constexpr int NC = kMade<E>;
     Staged<E, KT, BRING> k, q;
-    u32x4_t t[2 * NC], p[2 * NC];
+    static constexpr int pieces = sizeof(Matrices) / 16 / BRING;
+    static_assert(pieces * 16 * BRING == sizeof(Matrices), "");
+    u32x4_t m[pieces];
     static constexpr int per_row = 2 * OW, turns = (OW + 1) / 2;
     Eight<E> v[turns];
     float first, last, beta;
 
     // (v0: the workgroup's first column; x: V or dO)
     __device__ __forceinline__ void load(const GdrArgs& A, const GdrTensor& x,
-                                         const Prepared<NC>& M, int64_t b,
+                                         const Prepared& M, int64_t b,
                                          int64_t h, int64_t hk, int64_t c,
                                          int v0, int thread) {
         const int64_t t0 = c * C;
@@ -146,19 +147,8 @@ struct Bring {
         k.load(at<E>(A.k, b, hk, t0), A.k.st, valid, A.Dk, thread);
         q.load(at<E>(A.q, b, hk, t0), A.q.st, valid, A.Dk, thread);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
-            // (the upper right quarters, which nothing reads, hold the lower
-            // left ones' first columns again)
-            const int at_col = row < 32 ? col % 32 : col;
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                t[i * NC + n] =
-                    *reinterpret_cast<const u32x4_t*>(&M.t[n][row][at_col]);
-                p[i * NC + n] =
-                    *reinterpret_cast<const u32x4_t*>(&M.p[n][row][at_col]);
-            }
-        }
+        for (int i = 0; i < pieces; ++i)
+            m[i] = reinterpret_cast<const u32x4_t*>(&M.m)[i * BRING + thread];
         if constexpr (kColumns<E, KT>)
 #pragma unroll
             for (int i = 0; i < turns; ++i) {
@@ -177,16 +167,8 @@ struct Bring {
         k.store(L.k, valid, A.Dk, thread);
         q.store(L.q, valid, A.Dk, thread);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = (i * BRING + thread) / 8, col = 8 * (thread % 8);
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                *reinterpret_cast<u32x4_t*>(&L.t.x[n][row][col]) =
-                    t[i * NC + n];
-                *reinterpret_cast<u32x4_t*>(&L.p.x[n][row][col]) =
-                    p[i * NC + n];
-            }
-        }
+        for (int i = 0; i < pieces; ++i)
+            reinterpret_cast<u32x4_t*>(&L.m)[i * BRING + thread] = m[i];
         if constexpr (kColumns<E, KT>)
 #pragma unroll
             for (int i = 0; i < turns; ++i) {
@@ -207,9 +189,9 @@ struct Bring {
 // The six operands of T or P (or of their transposes) that hold anything, in
 // the order (0, 0) .. (3, 0), (2, 1), (3, 1); transposed (0, 0), (1, 0), (0, 1)
 // .. (3, 1).
-template <bool TRANSPOSED, int NC>
-__device__ __forceinline__ void triangle(const Rows<NC, 2>& x, int lane,
-                                         Frag<NC> (&f)[6]) {
+template <bool TRANSPOSED>
+__device__ __forceinline__ void triangle(const Triangle& x, int lane,
+                                         Frag<kMade> (&f)[6]) {
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
         const int tb = TRANSPOSED ? i < 2 ? i : i - 2 : i < 4 ? i : i - 2;
@@ -281,7 +263,7 @@ __device__ __forceinline__ void column_blocks(const Rows<NI, KT>& x, int n,
 // the threads that own rows, with the chunk in L.
 template <typename E, int KT, int OW, typename F>
 __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
-                                      const Prepared<kMade<E>>* M, int64_t head,
+                                      const Prepared* M, int64_t head,
                                       int v0, int64_t first, int64_t step,
                                       int64_t n, ChainChunk<E, KT>* L, F own) {
     const Head at_head(A, uint32_t(head));

@@ -12,11 +12,14 @@
 //
 // Operands.  All products run on v_mfma_f32_16x16x32_bf16 with fp32 sums.  A
 // number of more bits is a sum of bf16 planes, and a product the sum of the
-// planes' products that count: bf16 q, k and v are one plane (exact), what is
-// computed from them two, the state among it (2^-18 left out); fp32 vectors
-// and what follows from them three (2^-27).  One plane for all would halve the
-// products, and leave the state, an fp32 output that every later chunk reads,
-// 1e-3 off.
+// planes' products that count: bf16 q, k, v and do are one plane (exact), fp32
+// ones and all that is computed, the state among it, three (2^-27 left out,
+// less than fp32 sums round off).  Two planes for what is computed from bf16
+// vectors leave out 2^-18: the final state, an fp32 output, was 4.5e-6 off (its
+// norm) where fp32 products and three planes are 2e-7, and bf16 results, some of
+// them rounded the other way, 1.4e-4 from those of fp32 products for 3.5e-5.
+// They took 92 us for 116 (1 x 1999 tokens, 32 heads of 128 x 128), 1486 for
+// 1567 (8 x 4096 with gradients, 16 of 128 x 128).
 //
 // Register layouts (lane l, r = l % 16, q = l / 16).  An accumulator tile D(X)
 // holds X[4q + e][r], e = 0..3.  An operand of 32 places along the contracted
@@ -50,8 +53,7 @@ typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
 template <typename E>
 constexpr int kIn = sizeof(E) == 2 ? 1 : 3;  // planes of an input
-template <typename E>
-constexpr int kMade = sizeof(E) == 2 ? 2 : 3;  // planes of a computed number
+constexpr int kMade = 3;                      // of a computed number
 
 template <int N>
 struct Frag {
@@ -345,11 +347,59 @@ struct Staged {
 
 // --- what gdr_prepare.hip leaves for a chunk of a head ------------------------
 
-// T and P in planes, row by row, and the gates.  The upper right quarters are
-// zeros that nothing reads.
-template <int NC>
+// A lower triangle of 64 x 64 as the six operands of 16 rows and 32 places that
+// hold anything, (tb, p) = (0, 0) .. (3, 0), (2, 1), (3, 1): rows spread(tb, r),
+// places 32 p + 8q .., lane by lane.  (Row by row, with a pitch that spreads the
+// banks, three planes of two triangles would take half as much again and leave
+// no room for a second chunk in LDS.)
+struct Triangle {
+    alignas(16) bf16_t x[kMade][6][64][8];
+
+    static __device__ __forceinline__ constexpr int operand(int tb, int p) {
+        return tb + 2 * p;
+    }
+    __device__ __forceinline__ bf16_t* at(int n, int row, int col) {
+        const int tb = 2 * (row / 32) + (row >> 2 & 1);
+        const int m = 4 * (row % 32 / 8) + (row & 3);
+        return &x[n][operand(tb, col / 32)][16 * (col % 32 / 8) + m][col % 8];
+    }
+    __device__ __forceinline__ Frag<kMade> rows(int tb, int p, int lane) const {
+        Frag<kMade> f;
+#pragma unroll
+        for (int n = 0; n < kMade; ++n)
+            f.p[n] = *reinterpret_cast<const u32x4_t*>(
+                &x[n][operand(tb, p)][lane][0]);
+        return f;
+    }
+    // The operand of the transpose's rows spread(jb, r), places 32 p ..: rows
+    // 8q + (r >> 2) and four further of pair p, whose tiles are 2 p and 2 p + 1,
+    // four columns a lane, transposed on the way.
+    __device__ __forceinline__ Frag<kMade> columns(int jb, int p,
+                                                   int lane) const {
+        const int slot = 16 * (lane & 3) + 4 * (lane >> 4) + (lane >> 2 & 3);
+        Frag<kMade> f;
+#pragma unroll
+        for (int n = 0; n < kMade; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const bf16_t* from =
+                    &x[n][operand(2 * p + u, jb >> 1)][slot][4 * (jb & 1)];
+                const uint2 w = __builtin_bit_cast(
+                    uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (lds_i16x4_t*)(from)));
+                f.p[n][2 * u] = w.x;
+                f.p[n][2 * u + 1] = w.y;
+            }
+        return f;
+    }
+};
+struct Matrices {
+    Triangle t, p;
+};
+
+// The matrices and the gates.
 struct Prepared {
-    bf16_t t[NC][C][C], p[NC][C][C];
+    Matrices m;
     double G[C];                          // base 2
     float first[C], last[C], beta[C];     // 2^G, 2^(G_L - G)
 };

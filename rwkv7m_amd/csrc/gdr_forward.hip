@@ -18,7 +18,7 @@ template <typename E, int KT, int OW, bool TRAIN>
 __global__ void __launch_bounds__(64 * OW + BRING)
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 gdr_forward_kernel(const GdrArgs A, int parts) {
-    constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
+    constexpr int NI = kIn<E>, NC = kMade, DKP = 32 * KT;
     extern __shared__ char lds_raw[];
     const Place at_ = place(blockIdx.x, parts);
     const int64_t head = at_.head;
@@ -44,7 +44,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
     column.fetch(0, lane);
 
     chain<E, KT, OW>(
-        A, A.v, static_cast<const Prepared<NC>*>(A.prepared) + head * chunks,
+        A, A.v, static_cast<const Prepared*>(A.prepared) + head * chunks,
         head, 16 * OW * at_.part, 0, 1, chunks,
         reinterpret_cast<ChainChunk<E, KT>*>(lds_raw),
         [&](const ChainChunk<E, KT>& L, int64_t c) {
@@ -54,7 +54,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         // What follows is in the order in which it is issued: each step's
         // operands are read from LDS between the products of the step before,
         // and so is what the vector ALU has to do and they do not need.
-        // (bf16: fp32's three planes leave no registers for it.)
+        // (bf16: three planes of fp32 vectors leave no registers for it.)
         constexpr bool DEEP = NI == 1;
         constexpr int TWO = DEEP ? 2 : 1, HALF = KT / 2;
         Frag<NI> kf[TWO][4], qf[TWO][4];
@@ -93,8 +93,8 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             mul_each(B0, kf[p % TWO], Sf[p]);
             if (p + 1 < KT)
                 Sf[p + 1] = split8<NC>(S[2 * p + 2], S[2 * p + 3]);
-            if (DEEP && p + 1 < KT) interleave<8, 1, 3>();
-            if (DEEP && p + 1 == KT) interleave<8, 2, 0>();
+            if (DEEP && p + 1 < KT) interleave<4 * NC, 1, 3>();
+            if (DEEP && p + 1 == KT) interleave<4 * NC, 2, 0>();
         }
         // S Q^T, v = 4q + e, t = spread(tb, r), and meanwhile
         const auto queries = [&](int p) {
@@ -102,7 +102,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
             if (!DEEP) blocks(L.q, p, lane, qf[0]);
             else if (p + 1 < KT) blocks(L.q, p + 1, lane, qf[(p + 1) % TWO]);
             else column_blocks(L.k, 0, 0, lane, kf[0]);
-            if (DEEP && p + 1 == HALF) triangle<false>(L.t, lane, Tf);
+            if (DEEP && p + 1 == HALF) triangle<false>(L.m.t, lane, Tf);
             if (!DEEP) hold();
             mul_each(O, Sf[p], qf[p % TWO]);
         };
@@ -116,13 +116,13 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
 #pragma unroll
             for (int i = 2 * p / HALF; i < 2 * (p + 1) / HALF; ++i)
                 Rf[i] = split8<NC>(V[2 * i], V[2 * i + 1]);
-            if (DEEP && p + 1 < HALF) interleave<8, 1, 6>();
-            if (DEEP && p + 1 == HALF) interleave<8, 2, 8>();
+            if (DEEP && p + 1 < HALF) interleave<4 * NC, 1, 6>();
+            if (DEEP && p + 1 == HALF) interleave<4 * NC, 2, KT == 2 ? 20 : 8>();
         }
         // X = T R
         f32x4_t last[4];
         float own_first[4];
-        if (!DEEP) triangle<false>(L.t, lane, Tf);
+        if (!DEEP) triangle<false>(L.m.t, lane, Tf);
         hold();
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
@@ -132,7 +132,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
         mul_triangle<false>(X, Tf, Rf);
 #pragma unroll
         for (int kb = 0; kb < 2 * KT; ++kb) S[kb] *= whole;
-        if (DEEP) interleave<18, 1, 2>();
+        if (DEEP) interleave<36, 1, 2>();
 #pragma unroll
         for (int p = HALF; p < KT; ++p) {
             queries(p);
@@ -143,7 +143,7 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                                    X[2 * i + 1] * last[2 * i + 1]);
                 Xf[i] = split8<NC>(X[2 * i], X[2 * i + 1]);
             }
-            if (DEEP) interleave<8, 1, 7>();
+            if (DEEP) interleave<4 * NC, 1, KT == 2 ? 16 : 7>();
         }
         if constexpr (TRAIN) {
             put_column(A.x + (head * chunks + c) * C * DVP, DVP, q, v, X);
@@ -164,21 +164,21 @@ gdr_forward_kernel(const GdrArgs A, int parts) {
                     column_blocks(L.k, (at + 1) / 2, (at + 1) & 1, lane,
                                   kf[(at + 1) % TWO]);
                 else
-                    triangle<false>(L.p, lane, Pf);
+                    triangle<false>(L.m.p, lane, Pf);
                 if (!DEEP) hold();
                 mul_each(sum, kf[at % TWO], Rf[p]);
                 if (at == 0)
 #pragma unroll
                     for (int tb = 0; tb < 4; ++tb) O[tb] *= own_first[tb];
-                if (DEEP && at == 0) interleave<8, 1, 2>();
-                if (DEEP && at > 0 && at + 1 < KT) interleave<8, 1, 0>();
-                if (DEEP && at + 1 == KT) interleave<8, 2, 0>();
+                if (DEEP && at == 0) interleave<4 * NC, 1, 2>();
+                if (DEEP && at > 0 && at + 1 < KT) interleave<4 * NC, 1, 0>();
+                if (DEEP && at + 1 == KT) interleave<4 * NC, 2, 0>();
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) S[4 * n + i] = sum[i];
         }
         // O^T = scale (2^G (S Q^T) + X^T P^T)
-        if (!DEEP) triangle<false>(L.p, lane, Pf);
+        if (!DEEP) triangle<false>(L.m.p, lane, Pf);
         hold();
         mul_by_triangle(O, Xf, Pf);
         E* to = op + t0 * A.Hv * A.Dv + int64_t(spread(0, r)) * A.Hv * A.Dv +

@@ -13,9 +13,8 @@
 //
 // (q.dq - dv.v is dG as well, and cheaper.  But in the running sum of the form
 // above the pairs of tokens on one side of its border cancel, product by
-// product; of the other they do not, and dg, a small sum of large terms, is
-// 1.3e-5 off for 8e-6.  For its sake X and dR are three planes here: 6e-6, at 3
-// to 8 % of this kernel's time.  A third plane of N too: 5.5e-6, 6 % more.)
+// product; of the other they do not, and dg, a small sum of large terms, is off
+// by 1.6 times as much.)
 //
 // One workgroup a chunk and value head, all of them independent.  A wave owns
 // 32 tokens and a share of the columns of dq, left and right.  S0 and D pass
@@ -48,8 +47,8 @@ template <typename E, int KT>
 struct GradShared {
     union {
         struct {  // a block of 32 columns of v
-            Rows<kMade<E>, KT, 32> s, d;  // S0's and D's rows
-            Rows<3, 1> x, r;              // X, dR
+            Rows<kMade, KT, 32> s, d;  // S0's and D's rows
+            Rows<kMade, 1> x, r;          // X, dR
             Rows<kIn<E>, 1> o;            // dO
         };
         struct {  // what is made of them
@@ -59,9 +58,9 @@ struct GradShared {
                 };
                 E out[2][C][32 * KT + 8];  // dq and dk, behind them
             };
-            Rows<kMade<E>, 2> n;  // N, then -beta N
+            Rows<kMade, 2> n;  // N, then -beta N
             union {
-                Rows<kMade<E>, 2> p;  // dP
+                Rows<kMade, 2> p;  // dP
                 float dots[kShares<E, KT>][2][C];  // of dG, k.left, behind it
             };
         };
@@ -126,7 +125,7 @@ __device__ __forceinline__ void store_gate(void* p, bool bf16, int64_t i,
 template <typename E, int KT>
 __global__ void __launch_bounds__((128 * kShares<E, KT>), sizeof(E) == 2 ? 2 : 1)
 gdr_gradients_kernel(const GdrArgs A) {
-    constexpr int NI = kIn<E>, NC = kMade<E>, DKP = 32 * KT;
+    constexpr int NI = kIn<E>, NC = kMade, DKP = 32 * KT;
     constexpr int KQ = kShares<E, KT>, NT = 128 * KQ;
     constexpr bool AHEAD = KQ == 4;
     extern __shared__ char lds_raw[];
@@ -142,8 +141,8 @@ gdr_gradients_kernel(const GdrArgs A) {
     const int64_t t0 = c * C;
     const int valid = int(A.T - t0 < C ? A.T - t0 : C);
     const int DVP = (A.Dv + 31) / 32 * 32;
-    const Prepared<NC>& M =
-        static_cast<const Prepared<NC>*>(A.prepared)[head * chunks + c];
+    const Prepared& M =
+        static_cast<const Prepared*>(A.prepared)[head * chunks + c];
 
     const E* dop = at<E>(A.dout, b, h, t0);
     const E* vp = at<E>(A.v, b, h, t0);
@@ -245,7 +244,7 @@ gdr_gradients_kernel(const GdrArgs A) {
             if (v0 + 32 < DVP) fetch(v0 + 32);
         // operands of the wave's tokens (left or right alike)
         Frag<NI> of[2];
-        Frag<3> xf[2], rf[2];
+        Frag<NC> xf[2], rf[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             of[i] = L.o.rows_in_order(2 * th + i, 0, lane);
@@ -269,10 +268,10 @@ gdr_gradients_kernel(const GdrArgs A) {
             }
         } else {
             const Frag<NI> o = L.o.rows_in_order(2 + th, 0, lane);
-            const Frag<3> g = L.r.rows_in_order(2 + th, 0, lane);
+            const Frag<NC> g = L.r.rows_in_order(2 + th, 0, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const Frag<3> x = L.x.rows_in_order(i, 0, lane);
+                const Frag<NC> x = L.x.rows_in_order(i, 0, lane);
                 mul(dp[i], o, x);
                 mul(nn[i], g, x);
             }

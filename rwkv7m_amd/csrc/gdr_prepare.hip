@@ -71,7 +71,7 @@ __device__ __forceinline__ f32x4_t mm32(const f32x4_t& mt, const f32x4_t& y,
 template <typename E, int KT>
 __global__ void __launch_bounds__(NT)
 gdr_prepare_kernel(const GdrArgs A) {
-    constexpr int NI = kIn<E>, NC = kMade<E>;
+    constexpr int NI = kIn<E>, NC = kMade;
     __shared__ Shared S;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
@@ -81,7 +81,7 @@ gdr_prepare_kernel(const GdrArgs A) {
     const int64_t b = at_head.b, h = at_head.h, hk = at_head.hk;
     const int64_t t0 = c * C;
     const int valid = int(A.T - t0 < C ? A.T - t0 : C);
-    auto* out = static_cast<Prepared<NC>*>(A.prepared) + id;
+    auto* out = static_cast<Prepared*>(A.prepared) + id;
 
     // rows of k and q: places 32 p + 8q + i of token 16 tb + r, all loads
     // before the first is waited for
@@ -152,7 +152,7 @@ gdr_prepare_kernel(const GdrArgs A) {
         split2<NC>(pt[2], pt[3], hi);
 #pragma unroll
         for (int n = 0; n < NC; ++n)
-            *reinterpret_cast<uint2*>(&out->p[n][own][16 * j + 4 * q]) =
+            *reinterpret_cast<uint2*>(out->m.p.at(n, own, 16 * j + 4 * q)) =
                 make_uint2(lo[n], hi[n]);
     };
     // the diagonal blocks first: the first wave, which has no other, inverts
@@ -186,8 +186,8 @@ gdr_prepare_kernel(const GdrArgs A) {
         // (the block right of the diagonal that shares a pair with it)
 #pragma unroll
         for (int n = 0; n < NC; ++n)
-            *reinterpret_cast<uint2*>(
-                &out->p[n][own][16 * (wave + 1) + 4 * q]) = make_uint2(0, 0);
+            *reinterpret_cast<uint2*>(out->m.p.at(
+                n, own, 16 * (wave + 1) + 4 * q)) = make_uint2(0, 0);
         *reinterpret_cast<f32x4_t*>(&S.t[own][16 * (wave + 1) + 4 * q]) =
             zero4();
     }
@@ -217,13 +217,15 @@ gdr_prepare_kernel(const GdrArgs A) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int u = i * NT + int(threadIdx.x), row = u / 8, col = 8 * (u % 8);
-        if (row < 32 && col >= 32) continue;
+        const int u = i * NT + int(threadIdx.x), l = u % 64;
+        if (u >= 6 * 64) break;
+        const int tb = u < 256 ? u / 64 : u / 64 - 2, p = u >= 256;
+        const int row = spread(tb, l % 16), col = 32 * p + 8 * (l / 16);
         const Frag<NC> f =
             split8<NC>(four(&S.t[row][col]), four(&S.t[row][col + 4]));
 #pragma unroll
         for (int n = 0; n < NC; ++n)
-            *reinterpret_cast<u32x4_t*>(&out->t[n][row][col]) = f.p[n];
+            *reinterpret_cast<u32x4_t*>(&out->m.t.x[n][u / 64][l][0]) = f.p[n];
     }
 }
 
@@ -232,10 +234,7 @@ gdr_prepare_kernel(const GdrArgs A) {
 int gdr_dkp(int Dk) { return Dk <= 64 ? 64 : 128; }
 int gdr_dvp(int Dv) { return (Dv + 31) / 32 * 32; }
 
-int64_t gdr_prepared_bytes(bool bf16) {
-    return bf16 ? int64_t(sizeof(Prepared<kMade<bf16_t>>))
-                : int64_t(sizeof(Prepared<kMade<float>>));
-}
+int64_t gdr_prepared_bytes() { return int64_t(sizeof(Prepared)); }
 
 hipError_t launch_gdr_prepare(bool bf16, const GdrArgs& A,
                               hipStream_t stream) {

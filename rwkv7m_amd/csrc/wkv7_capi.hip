@@ -925,8 +925,7 @@ int gdr_sizes(const char* fn, const rwkv7m_gated_delta_inputs* in,
                   dvp = rwkv7m::gdr_dvp(int(in->Dv));
     s->states = s->heads * s->chunks * dvp * dkp;
     s->x = s->heads * s->chunks * C * dvp;
-    s->prepared = s->heads * s->chunks *
-                  rwkv7m::gdr_prepared_bytes(in->dtype == RWKV7M_DTYPE_BF16);
+    s->prepared = s->heads * s->chunks * rwkv7m::gdr_prepared_bytes();
     return RWKV7M_OK;
 }
 

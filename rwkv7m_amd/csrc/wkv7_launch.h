@@ -416,7 +416,7 @@ struct GdrArgs {
 };
 int gdr_dkp(int Dk);
 int gdr_dvp(int Dv);
-int64_t gdr_prepared_bytes(bool bf16);
+int64_t gdr_prepared_bytes();
 hipError_t launch_gdr_prepare(bool bf16, const GdrArgs& A,
                               hipStream_t stream);
 hipError_t launch_gdr_forward(bool bf16, const GdrArgs& A, hipStream_t stream);

@@ -1,0 +1,84 @@
+"""The gated delta rule over the whole range that it is documented for: what its
+fp32 results are off by, rates (beta) up to 2, keys that hardly differ, and
+calls large enough for every division of a sequence's work.
+
+Tolerances, of 2-norms.  A product adds up at most 128 + 64 terms in 24 fp32
+additions of a matrix instruction's sums (4 tiles of 32 places, six products of
+planes each), each off by 2^-24 / sqrt(3) in the mean: 1.7e-7.  The longest way
+from an input to a result passes eight products, sqrt(8) 1.7e-7 = 4.8e-7, and
+exponentials of up to 8 in base 2 (smaller weights do not count), 2^-24 8 ln 2 /
+sqrt(3) = 2e-7; a row of the inverse, whose places are as large as beta, doubles
+what comes to it: 1.4e-6, FP32 = 1.5e-6.  dg is the running sum of three such
+terms that cancel: sqrt(3) FP32.  Where beta is up to 2 or keys hardly differ, the
+64 terms of a row of the inverse times what it acts on are each as large as the
+result and differ in sign: sqrt(64) as much.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gated_delta import _gen, close, grads64, make
+
+pytestmark = pytest.mark.gpu
+
+FP32 = 1.5e-6
+
+
+@pytest.fixture(scope="module")
+def lm(hip_lib):
+    import rwkv7m_amd
+    return rwkv7m_amd
+
+
+def results(lm, x, s0, seed):
+    """{name: (got, wanted)} of the fp32 results, and the bf16 ones compared."""
+    g = _gen(seed)
+    B, T, Hv, Dv = x[2].shape
+    do = torch.randn(B, T, Hv, Dv, generator=g).to(x[2].dtype)
+    ds = torch.randn(s0.shape, generator=g)
+    (o, end), grads, _ = grads64(x, s0, do, ds)
+    leaves = [t.cuda().requires_grad_() for t in (*x, s0)]
+    out, got = lm.gated_delta_rule(*leaves)
+    d = torch.autograd.grad([out, got], leaves, [do.cuda(), ds.cuda()])
+    return dict(o=(out, o), state=(got, end), dq=(d[0], grads[0]),
+                dk=(d[1], grads[1]), dv=(d[2], grads[2]),
+                dg=(d[3], grads[3]), dbeta=(d[4], grads[4]),
+                ds0=(d[5], grads[5]))
+
+
+def check_norms(found, factor):
+    for name, (got, want) in found.items():
+        got = got.detach()
+        if got.dtype == torch.bfloat16:
+            close(name, got, want, 16 * factor * FP32)
+            continue
+        off = float((got.double().cpu() - want).norm() / want.norm())
+        tol = factor * FP32 * (3 ** 0.5 if name == "dg" else 1.0)
+        assert off <= tol, (name, off, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,T,Hk,Hv,Dk,Dv", [
+    (1, 84, 2, 6, 64, 64), (2, 203, 2, 2, 128, 128), (2, 300, 1, 3, 40, 72)])
+def test_fp32_results_as_of_fp32_products(lm, B, T, Hk, Hv, Dk, Dv, dtype):
+    print("case: fp32 results", B, T, Hk, Hv, Dk, Dv, dtype, flush=True)
+    x = make(B, T, Hk, Hv, Dk, Dv, dtype, seed=T)
+    s0 = torch.randn(B, Hv, Dv, Dk, generator=_gen(1))
+    check_norms(results(lm, x, s0, 2), 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("alike,decay", [(0.7, 0.0), (0.7, 0.1), (6.0, 0.0),
+                                         (6.0, 0.1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rates_up_to_two(lm, dtype, alike, decay, D):
+    """beta from 1 to 2, keys of length 1: reflections, next to no decay."""
+    print("case: rates", dtype, alike, decay, D, flush=True)
+    x = make(2, 200, 2, 2, D, 64, dtype, seed=5, alike=alike, decay=decay)
+    x[4] = 1.0 + torch.rand(x[4].shape, generator=_gen(6))
+    if dtype == "bf16":  # keys of at most length 1 after their rounding
+        x[1] = (x[1].float() * (1 - 2.0 ** -8)).bfloat16()
+    s0 = torch.randn(2, 2, 64, D, generator=_gen(7))
+    check_norms(results(lm, x, s0, 8), 8.0)
