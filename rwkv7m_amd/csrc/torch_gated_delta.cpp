@@ -25,7 +25,8 @@ struct Inputs {
                     reinterpret_cast<uintptr_t>(t.data_ptr()) % align == 0;
         for (int i = 0; i < 3; ++i)
             fits = fits && (t.size(i) <= 1 || t.stride(i) * unit % align == 0);
-        return fits ? t : t.contiguous();
+        // (a dense tensor that starts elsewhere is its own contiguous())
+        return fits ? t : t.clone(at::MemoryFormat::Contiguous);
     }
 
     static void gate_shape(const char* what, const Tensor& t, int64_t B,

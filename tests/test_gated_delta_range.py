@@ -82,3 +82,39 @@ def test_rates_up_to_two(lm, dtype, alike, decay, D):
         x[1] = (x[1].float() * (1 - 2.0 ** -8)).bfloat16()
     s0 = torch.randn(2, 2, 64, D, generator=_gen(7))
     check_norms(results(lm, x, s0, 8), 8.0)
+
+
+# --- layouts ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_dense_tensors_that_start_anywhere(lm, dtype):
+    """Contiguous vectors, cotangents and gates an element past a 16-byte
+    border: as the same numbers at one."""
+    print("case: odd starts", dtype, flush=True)
+
+    def odd(t):
+        out = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:]
+        out = out.view(t.shape).copy_(t)
+        assert out.is_contiguous() and out.data_ptr() % 16
+        return out
+
+    x = make(2, 70, 1, 2, 32, 40, dtype, seed=21)
+    s0 = torch.randn(2, 2, 40, 32, generator=_gen(1))
+    do = torch.randn(2, 70, 2, 40, generator=_gen(2)).to(x[2].dtype)
+    ds = torch.randn(2, 2, 40, 32, generator=_gen(3))
+    found = []
+    for place in (lambda t: t.cuda(), odd):
+        leaves = [place(t).requires_grad_() for t in (*x, s0)]
+        out = lm.gated_delta_rule(*leaves)
+        found.append([*out, *torch.autograd.grad(out, leaves,
+                                                 [place(do), place(ds)])])
+        with torch.no_grad():
+            found[-1] += lm.gated_delta_rule(*leaves)
+            state = s0.cuda()
+            found[-1] += [lm.gated_delta_step(*(t[:, :3] for t in leaves[:5]),
+                                              state), state]
+            one = [place(t[:, 5:6].contiguous()) for t in x]
+            state = s0.cuda()
+            found[-1] += [lm.gated_delta_step(*one, state), state]
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
