@@ -372,6 +372,11 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(
                          logits.scalar_type(), " and ", draft.scalar_type());
     }
     if (lengths.defined()) check_ids("draft_lengths", lengths, {B});
+    const Tensor given[2] = {or_undefined(accept_), or_undefined(sample_)};
+    no_tangents("verify_drafts", {&logits, &draft, &given[0], &given[1]});
+    TORCH_CHECK(!wants_grad({&logits, &draft, &given[0], &given[1]}),
+                "verify_drafts has no gradient; call it under no_grad, or on "
+                "detached logits");
     same_gpu({&logits, &tokens_, &draft, &lengths});
     const bool greedy = temperature == 0.0;
     Tensor accept, sample;

@@ -123,7 +123,10 @@ def verify_drafts(logits, draft_tokens, draft_logits=None,
     1`` is the number of tokens by which the sequence goes on: the
     ``lengths`` of ``gated_delta_step``.  A token is -1 where its row has no
     distribution (it, or the draft's, holds NaN or +inf, or nothing above
-    -inf); chances of such rows are NaN.  Nothing here has a gradient."""
+    -inf); chances of such rows are NaN.
+
+    There is no gradient: logits that require one are refused where gradients
+    are enabled, as are forward-mode tangents."""
     return VerifiedDrafts(*load_binding().verify_drafts(
         logits, draft_tokens, draft_logits, accept_uniforms, sample_uniforms,
         draft_lengths, temperature))
