@@ -118,3 +118,51 @@ def test_dense_tensors_that_start_anywhere(lm, dtype):
             found[-1] += [lm.gated_delta_step(*one, state), state]
     for a, b in zip(*found):
         assert torch.equal(a, b)
+
+
+# --- division of work ---------------------------------------------------------
+
+# heads and Dv choose how many waves of a workgroup own rows of the state (on
+# 256 CUs, as the name says); in some cases the last workgroup of a head has
+# waves past its rows
+@pytest.mark.parametrize("Dk", [64, 72, 128])
+@pytest.mark.parametrize("B,Hk,Hv,T,Dv", [
+    pytest.param(16, 3, 6, 70, 64, id="two"),
+    pytest.param(16, 5, 5, 70, 40, id="two-part-of-a-tile"),
+    pytest.param(16, 2, 4, 130, 96, id="two-three-workgroups"),
+    pytest.param(5, 2, 6, 70, 200, id="two-of-224-rows"),
+    pytest.param(24, 4, 4, 70, 72, id="four-two-past-the-rows"),
+    pytest.param(24, 2, 4, 70, 200, id="four-of-224-rows"),
+    pytest.param(75, 4, 4, 70, 32, id="four-two-idle"),
+    pytest.param(48, 1, 2, 129, 128, id="four"),
+    pytest.param(33, 8, 8, 66, 256, id="four-256-rows")])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_heads(lm, dtype, B, Hk, Hv, T, Dv, Dk):
+    """Sequences of a large batch against the recurrence, and bit for bit
+    against the same ones in calls of their own."""
+    print("case: many heads", dtype, B, Hk, Hv, T, Dk, Dv, flush=True)
+    x = make(B, T, Hk, Hv, Dk, Dv, dtype, seed=Dk + Dv)
+    s0 = torch.randn(B, Hv, Dv, Dk, generator=_gen(1))
+    do = torch.randn(B, T, Hv, Dv, generator=_gen(2)).to(x[2].dtype)
+    ds = torch.randn(B, Hv, Dv, Dk, generator=_gen(3))
+
+    def call(rows):
+        leaves = [t[rows].cuda().requires_grad_() for t in (*x, s0)]
+        with torch.no_grad():
+            plain = lm.gated_delta_rule(*leaves)
+        out = lm.gated_delta_rule(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip(plain, out))
+        return [*out, *torch.autograd.grad(
+            out, leaves, [do[rows].cuda(), ds[rows].cuda()])]
+
+    names = ("o", "state", "dq", "dk", "dv", "dg", "dbeta", "ds0")
+    whole = call(slice(None))
+    for b in (0, B // 2, B - 1):
+        rows = slice(b, b + 1)
+        alone = call(rows)
+        for name, a, c in zip(names, whole, alone):
+            assert torch.equal(a[rows], c), (name, b)
+        outs, grads, _ = grads64([t[rows] for t in x], s0[rows], do[rows],
+                                 ds[rows])
+        check_norms({n: (a[rows], w) for n, a, w in
+                     zip(names, whole, [*outs, *grads])}, 1.0)
