@@ -312,12 +312,14 @@ verify_draw_kernel(const LmVerifyArgs A) {
                         stop = p == 0.0;
                         if (r.largest != r.largest) p = r.inv;  // NaN
                     } else {
+                        // (outside the vocabulary 0 of 1, or NaN where the
+                        // rows have no distribution)
+                        p = word ? prob(r, S.picked[i], A.c) : 0.0 * r.inv;
                         q = 1.0;
-                        if (word) {
-                            p = prob(r, S.picked[i], A.c);
-                            if (A.draft)
-                                q = prob(S.rows[A.K + 1 + i],
-                                         S.picked[A.K + 1 + i], A.c);
+                        if (A.draft) {
+                            const RowSums& d = S.rows[A.K + 1 + i];
+                            q = word ? prob(d, S.picked[A.K + 1 + i], A.c)
+                                     : 1.0 + 0.0 * d.inv;
                         }
                         stop = !(double(A.accept[b * A.K + i]) * q < p);
                     }

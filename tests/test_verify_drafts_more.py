@@ -35,3 +35,99 @@ def test_derivatives_are_refused():
             verify_drafts(**{**args, name: leaf})
         with pytest.raises(RuntimeError, match="GPU tensors"):
             verify_drafts(**{**args, name: leaf.detach()})
+
+
+@pytest.fixture(scope="module")
+def lm(hip_lib):
+    import rwkv7m_amd
+    return rwkv7m_amd
+
+
+def _call(lm, x, tok, y=None, u=None, s=None, temp=1.0, n=None):
+    B, K = tok.shape
+    u = torch.zeros(B, K) if u is None else u
+    s = torch.zeros(B) if s is None else s
+    got = lm.verify_drafts(x.cuda(), tok.cuda(),
+                           None if y is None else y.cuda(), u.cuda(),
+                           s.cuda(), None if n is None else n.cuda(), temp)
+    return [t.cpu() for t in got]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_greedy_drafts_outside_the_vocabulary(lm, dtype):
+    print("case: greedy, outside", dtype, flush=True)
+    x = torch.randn(4, 3, 500, generator=torch.Generator().manual_seed(4))
+    x = x.to(dtype)
+    best = x.double().argmax(-1)
+    tok = best[:, :2].clone()
+    tok[0, 0], tok[1, 0], tok[2, 1], tok[3, 0] = -1, 500, 2 ** 40, -2 ** 62
+    took, count, chance = _call(lm, x, tok, temp=0.0)
+    assert count.tolist() == [0, 0, 1, 0]
+    assert took.tolist() == [
+        [int(best[0, 0]), -1, -1], [int(best[1, 0]), -1, -1],
+        [int(best[2, 0]), int(best[2, 1]), -1], [int(best[3, 0]), -1, -1]]
+    assert chance.tolist() == [[0.0, 1.0], [0.0, 1.0], [1.0, 0.0], [0.0, 1.0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temp", [0.0, 1.0])
+@pytest.mark.parametrize("what", ["nan", "inf", "empty"])
+def test_drafts_outside_the_vocabulary_of_rows_without_a_distribution(
+        lm, temp, what):
+    """The chance is NaN there, as of any other draft, and the token is -1."""
+    print("case: outside, no distribution", temp, what, flush=True)
+    g = torch.Generator().manual_seed(5)
+    x, y = torch.randn(3, 2, 300, generator=g), torch.randn(3, 1, 300,
+                                                            generator=g)
+    tok = torch.tensor([[-1], [300], [-1]])
+
+    def spoiled(t):
+        t = t.clone()
+        t[:2, 0] = -float("inf") if what == "empty" else t[:2, 0]
+        if what != "empty":
+            t[:2, 0, 7] = float(what)
+        return t
+
+    for a, q in ((spoiled(x), None), (spoiled(x), y), (x, spoiled(y))):
+        if temp == 0.0 and a is x:
+            continue  # (the draft's logits are not looked at)
+        took, count, chance = _call(lm, a, tok, q, temp=temp)
+        assert count.tolist() == [0, 0, 0]
+        assert took[:2].tolist() == [[-1, -1]] * 2 and 0 <= took[2, 0] < 300
+        assert chance[:2].isnan().all() and float(chance[2, 0]) == 0.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,K", [(25000, 1), (70000, 0), (66000, 2)])
+@pytest.mark.parametrize("kind", ["drawn", "certain", "greedy"])
+def test_more_workgroups_than_a_grid_row(lm, B, K, kind):
+    """More than 2^16 workgroups in either launch: sequences from the start, the
+    middle and the end as in small calls."""
+    print("case: grid rows", B, K, kind, flush=True)
+    V = 33
+    g = torch.Generator("cuda").manual_seed(B)
+    x = 2 * torch.randn(B, K + 1, V, generator=g, device="cuda")
+    y = x[:, :K] + torch.randn(B, K, V, generator=g, device="cuda")
+    tok = torch.randint(0, V, (B, K), generator=g, device="cuda")
+    u = torch.rand(B, K, generator=g, device="cuda")
+    s = torch.rand(B, generator=g, device="cuda")
+    n = torch.randint(0, K + 1, (B,), generator=g, device="cuda")
+    temp = 0.0 if kind == "greedy" else 1.0
+    q = y if kind == "drawn" else None
+    got = lm.verify_drafts(x, tok, q, u, s, n, temp)
+    for a in (0, B // 2, 65530, 21840, B - 40):
+        if a > B - 40:
+            continue
+        r = slice(a, a + 40)
+        part = lm.verify_drafts(x[r], tok[r], None if q is None else q[r],
+                                u[r], s[r], n[r], temp)
+        for p, w in zip(got, part):
+            assert torch.equal(p[r], w)
+    # every sequence has its token, and no draft past its length is taken
+    assert bool((got.accepted <= n).all())
+    last = got.tokens.gather(1, got.accepted[:, None])
+    assert bool((last >= 0).all()) and bool((last < V).all())
+    if temp == 0.0:
+        want = x.gather(1, got.accepted[:, None, None].expand(-1, 1, V))
+        assert torch.equal(last[:, 0], want[:, 0].argmax(-1))
