@@ -139,10 +139,11 @@ int rwkv7m_distill_loss_backward(
  * NULL, q_i = 1 at the drafted token: the drafts x_i = tokens[b][i] of sequence
  * b, i < n = draft_lengths[b] (NULL, or more than K: K), are taken from the
  * first on while accept[b][i] q_i(x_i) < p_i(x_i).  accepted[b] = m is their
- * number.  Behind them one token is drawn: from max(p_m - q_m, 0) if m < n,
- * from p_n otherwise, the first whose running sum over the vocabulary passes
- * sample[b] times the whole.  out[b] holds the m drafts, that token, and -1
- * behind; chances[b][i] = min(1, p_i(x_i) / q_i(x_i)) for i < n, 0 behind.
+ * number.  Behind them one token is drawn: from max(p_m - q_m, 0) if m < n (or
+ * p_m where that is 0 everywhere, p_m being q_m), from p_n otherwise, the first
+ * whose running sum over the vocabulary passes sample[b] times the whole.
+ * out[b] holds the m drafts, that token, and -1 behind; chances[b][i] = min(1,
+ * p_i(x_i) / q_i(x_i)) for i < n, 0 behind.
  *
  * temperature 0: a draft is taken where it is the likeliest token (the lowest
  * id of equal ones), which is also the one drawn; draft, accept and sample may
@@ -152,9 +153,10 @@ int rwkv7m_distill_loss_backward(
  * target has rows [B][K + 1] of V logits (outer = B, inner = K + 1), draft
  * [B][K], one dtype; rows past n are not read.  A logit of -inf has p = 0, as
  * has one whose p is less than 2^-1000 of the likeliest token's.  A
- * drafted token outside the vocabulary is never taken.  Where the row that is
- * drawn from, or the draft's, holds NaN or +inf, or nothing above -inf, the
- * token drawn is -1 (and no draft is taken against such a row).  The workspace
+ * drafted token outside the vocabulary is never taken: its chance is 0, and q_i
+ * stays as it is (with draft NULL, 0).  Where the row that is drawn from, or the
+ * draft's, holds NaN or +inf, or nothing above -inf, the token drawn is -1, no
+ * draft is taken against such a row, and its chance is NaN.  The workspace
  * is rwkv7m_verify_drafts_workspace_bytes, 16-byte aligned (-1 for invalid
  * sizes); free again once the call's work is done. */
 int64_t rwkv7m_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);

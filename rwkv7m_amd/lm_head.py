@@ -109,8 +109,10 @@ def verify_drafts(logits, draft_tokens, draft_logits=None,
     drafts are certain, found by lookup, not drawn), draft x of a position is
     taken while ``accept_uniforms * q(x) < p(x)``; behind the ``accepted``
     ones a token is drawn from ``max(p - q, 0)`` of the first position not
-    taken, or from the last row's ``p`` where all were, by ``sample_uniforms``
-    along the running sum over the vocabulary.  ``accept_uniforms`` ``[B,
+    taken (from its ``p`` where nothing is left of that, p being q), or from
+    the last row's ``p`` where all were, by ``sample_uniforms`` along the
+    running sum over the vocabulary.  A draft outside the vocabulary is never
+    taken.  ``accept_uniforms`` ``[B,
     K]`` and ``sample_uniforms`` ``[B]`` are fp32, from 0 to below 1; they are
     compared in float64.  ``draft_lengths`` ``[B]`` (int64 or int32) gives
     sequences with fewer drafts than K; rows past them are not read.

@@ -131,3 +131,26 @@ def test_more_workgroups_than_a_grid_row(lm, B, K, kind):
     if temp == 0.0:
         want = x.gather(1, got.accepted[:, None, None].expand(-1, 1, V))
         assert torch.equal(last[:, 0], want[:, 0].argmax(-1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [7, 9000])
+def test_what_is_drawn_where_nothing_is_left(lm, dtype, V):
+    """A draft that is not taken though p = q: the token comes from p."""
+    print("case: nothing left", dtype, V, flush=True)
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(1, 2, V, generator=g).to(dtype).expand(9, 2, V)
+    tok = torch.full((9, 1), V)
+    s = torch.linspace(0.0, 0.999, 9)
+    took, count, chance = _call(lm, x, tok, x[:, :1], s=s)
+    assert not count.any() and not chance.any()
+    cum = torch.softmax(x[0, 0].double(), -1).cumsum(-1)
+    at = s.double() * cum[-1]
+    assert float((cum[None] - at[:, None]).abs().min(-1).values[1:].min()) \
+        > 1e-9
+    assert took[:, 0].tolist() == (cum[None] <= at[:, None]).sum(-1).tolist()
+    assert (took[:, 1] == -1).all()
+    # without a draft's logits p itself is drawn from: nothing is set aside
+    other, *_ = _call(lm, x, tok, s=s)
+    assert torch.equal(took, other)
