@@ -24,7 +24,7 @@
  * Keys are taken as they come: the recurrence contracts where beta |k|^2 <= 2
  * and g <= 0, and grows where it does not.  g of -inf clears the state.  A
  * number that is not finite makes what it reaches NaN, and may make the rest of
- * its chunk of 64 tokens NaN.
+ * its chunk of 64 tokens NaN, tokens before it among them.
  *
  * Sums and states are fp32, products bf16 matrix instructions over sums of
  * three bf16 planes, which hold what fp32 does: results are off as with fp32

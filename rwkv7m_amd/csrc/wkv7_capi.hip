@@ -2232,6 +2232,9 @@ int rwkv7m_gated_delta_step(const rwkv7m_gated_delta_inputs* in, int64_t pool,
     });
 }
 
+// (lm_verify.hip's LDS holds that many)
+static_assert(RWKV7M_MAX_DRAFTS == rwkv7m::kVerifyMostDrafts, "");
+
 int64_t rwkv7m_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V) {
     if (B < 0 || B > (int64_t(1) << 24) || K < 0 || K > RWKV7M_MAX_DRAFTS ||
         V < 1 || V > (int64_t(1) << 30))

@@ -22,7 +22,7 @@ long as the last axis of a vector is dense and its rows start at multiples of
 16 bytes (views of one fused projection do); others are copied first.  Keys
 are taken as they come: normalise them (the recurrence contracts where ``beta
 |k|^2 <= 2`` and ``g <= 0``).  Padding tokens with ``beta`` and ``g`` 0 leave the
-state as it is.  States are fp32.  Kernels run on the current stream
+state as it is, if their vectors are finite.  States are fp32.  Kernels run on the current stream
 (``csrc/gdr_*.hip``, C ABI in ``include/rwkv7m_gated_delta.h``); there is no
 CPU fallback.
 """
@@ -43,8 +43,13 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None,
     forward-mode tangent raises.  For the backward the call keeps, a value
     head and chunk of 64 tokens, the fp32 state before it and its tokens'
     writes, ``4 Dv (Dk + 64)`` bytes with Dk rounded up to 64 or 128 and Dv to
-    a multiple of 32, and the chunk's matrices, 34 KB with bf16 vectors, 50 KB
-    with fp32; the backward takes the former as much again while it runs.
+    a multiple of 32, and the chunk's matrices, 38 KB; the backward takes the
+    former as much again while it runs, and where value heads share key heads
+    ``8 Hv Dk`` bytes a token.
+
+    A number that is not finite makes what it reaches NaN, and may make the
+    rest of its chunk of 64 tokens in its head NaN, tokens before it among
+    them.
 
     To capture a backward pass in a graph, use leaves that no live eager graph
     holds (detached clones do): the engine would wait across streams, which a
