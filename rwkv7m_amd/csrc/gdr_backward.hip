@@ -5,8 +5,9 @@
 //   dX = scale P^T dO + 2^(G_L - G) (K D^T),  dR = T^T dX
 //   D <- 2^G_L D + scale (2^G dO)^T Q - (beta 2^G dR)^T K
 //
-// Bound as the forward: 8 x 512 tokens, 12 heads of 64 x 64, 21 us, 2.6 a
-// chunk; 8 x 4096, 16 heads of 128 x 128, 1.49 GB in 320 to 345 us, 4.5 TB/s.
+// Bound as the forward: 8 x 512 tokens, 12 heads of 64 x 64, 26.5 us, 3.3 a
+// chunk; 8 x 4096, 16 heads of 128 x 128, 1.52 GB in 355 to 400 us, 3.8 to 4.3
+// TB/s.
 #include "gdr_chain.h"
 
 namespace rwkv7m {

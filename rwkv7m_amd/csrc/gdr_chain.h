@@ -305,10 +305,10 @@ __device__ __forceinline__ void chain(const GdrArgs& A, const GdrTensor& x,
 // and four beyond, since every workgroup brings its own K, Q, T and P and a
 // CU's workgroups share its LDS.  Forward, us with one, two and four (* the
 // rule's), bf16:
-//   1 x 1999 tokens, 32 heads of 128 x 128   77 *   75.5    85
-//   8 x 512, 12 of 64 x 64                   37     22.5 *  25
-//   2 x 1001, 24 of 96 x 128                 87     54 *    65
-//   8 x 4096, 16 of 128 x 128               765    494     370 *
+//   1 x 1999 tokens, 32 heads of 128 x 128  103 *  101.5   105
+//   8 x 512, 12 of 64 x 64                   48     28 *    29
+//   2 x 1001, 24 of 96 x 128                112     62 *    69
+//   8 x 4096, 16 of 128 x 128               898    578     400 *
 inline int owning_waves(int64_t heads, int dvp) {
     for (int w = 1; w < 4; w *= 2)
         if (heads * ((dvp + 16 * w - 1) / (16 * w)) <= device_cus()) return w;

@@ -3,10 +3,10 @@
 // each chunk and X where a backward follows.
 //
 // With few heads bound by the way through a chunk, one after the other: 32
-// heads of 128 x 128 over 1999 tokens 77 us, 2.4 a chunk, of which a wave's
-// 132 matrix instructions are 0.9.  With many, where states and X are kept, by
-// memory: 8 x 4096 tokens, 16 heads of 128 x 128, move 1.62 GB in 350 to 370
-// us, 4.5 TB/s.
+// heads of 128 x 128 over 1999 tokens 103 us, 3.2 a chunk, of which a wave's
+// 216 matrix instructions are half.  With many, where states and X are kept, by
+// memory: 8 x 4096 tokens, 16 heads of 128 x 128, move 1.65 GB in 358 to 400
+// us, 4.1 to 4.6 TB/s.
 #include "gdr_chain.h"
 
 namespace rwkv7m {

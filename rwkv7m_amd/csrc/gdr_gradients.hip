@@ -23,10 +23,11 @@
 // blocks of N and dP are divided among the waves and meet in LDS, whose rows
 // are operands for dq and left, whose columns for right.
 //
-// 8 x 512 tokens, 12 heads of 64 x 64: 30.5 us.  8 x 4096, 16 of 128 x 128:
-// 2.55 GB in 760 to 820 us, 3.2 TB/s, bound by a workgroup's own steps (one
-// lives on a CU, its sums fill the registers): the loads of its first block and
-// the gates, a quarter of its time, and four blocks between barriers.
+// 8 x 512 tokens, 12 heads of 64 x 64: 34.5 us.  8 x 4096, 16 of 128 x 128:
+// 2.55 GB in 790 to 950 us, 2.7 to 3.2 TB/s (matrix units busy 23 % of the
+// time), bound by a workgroup's own steps (one lives on a CU, its sums fill the
+// registers): the loads of its first block and the gates, and four blocks
+// between barriers.
 #include "gdr_common.h"
 
 namespace rwkv7m {
@@ -36,10 +37,10 @@ using namespace gdr;
 
 // Shares of the columns a workgroup's waves are divided over (two rows of
 // waves).  bf16 up to 64 columns: 2, and two workgroups a CU (8 x 512 tokens, 12
-// heads of 64 x 64: 29 us; with 4 and one workgroup 38).  At 128 the sums of
+// heads of 64 x 64: 34.5 us; with 4 and one workgroup 42).  At 128 the sums of
 // half the columns leave no room for a second workgroup's registers: 4, and the
-// next block's loads begun ahead (8 x 4096, 16 of 128 x 128: 735 us; with 2
-// 890).
+// next block's loads begun ahead (8 x 4096, 16 of 128 x 128: 800 us; with 2,
+// which spill, 1720).
 template <typename E, int KT>
 constexpr int kShares = sizeof(E) == 2 && KT == 4 ? 4 : 2;
 

@@ -9,8 +9,8 @@
 //
 // A chunk's way is its latency (loads, products, 16 steps of substitution on
 // one wave, up to three products after each other): 8 x 512 tokens, 12 heads of
-// 64 x 64, 12 us, 1 x 1999, 32 of 128 x 128, 18 us; 8 x 4096, 16 of 128 x 128,
-// 546 MB in 121 to 135 us, 4.3 TB/s.
+// 64 x 64, 13.5 us, 1 x 1999, 32 of 128 x 128, 19.5 us; 8 x 4096, 16 of 128 x
+// 128, 585 MB in 123 to 138 us, 4.2 to 4.8 TB/s.
 #include "gdr_common.h"
 
 namespace rwkv7m {

@@ -12,8 +12,8 @@
 //
 // 192 tokens of 32 heads of 128 x 128: 805 MB of states in 154 us, 5.2 TB/s,
 // above a copy's rate (4.9).  One token of 12 heads of 64 x 64: 4.4 us, a
-// launch's latency.  48 blocks of up to 6 tokens, 32 heads of 64 x 64, read
-// ahead: 14 us for 25 MB, a reduction's wait a token (without the next token's
+// launch's latency.  48 blocks of 0 to 6 tokens, 32 heads of 64 x 64, read
+// ahead: 14 us for 24.5 MB, a reduction's wait a token (without the next token's
 // loads ahead 17).
 #include "wkv7_common.h"
 #include "wkv7_launch.h"

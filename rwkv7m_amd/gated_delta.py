@@ -40,12 +40,13 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None,
 
     Differentiable, first order and reverse mode, in the five inputs and the
     initial state, through both outputs; a second derivative or a
-    forward-mode tangent raises.  For the backward the call keeps, a value
-    head and chunk of 64 tokens, the fp32 state before it and its tokens'
-    writes, ``4 Dv (Dk + 64)`` bytes with Dk rounded up to 64 or 128 and Dv to
-    a multiple of 32, and the chunk's matrices, 38 KB; the backward takes the
-    former as much again while it runs, and where value heads share key heads
-    ``8 Hv Dk`` bytes a token.
+    forward-mode tangent raises.  While it runs the call takes 38 KB a value
+    head and chunk of 64 tokens, the chunk's matrices.  For the backward it
+    keeps these, and a value head and chunk the fp32 state before it and its
+    tokens' writes, ``4 Dv (Dk + 64)`` bytes with Dk rounded up to 64 or 128
+    and Dv to a multiple of 32; the backward takes the latter as much again
+    while it runs, and where value heads share key heads ``8 Hv Dk`` bytes a
+    token.
 
     A number that is not finite makes what it reaches NaN, and may make the
     rest of its chunk of 64 tokens in its head NaN, tokens before it among
