@@ -910,8 +910,9 @@ int gdr_sizes(const char* fn, const rwkv7m_gated_delta_inputs* in,
                         ", Dv=" + std::to_string(in->Dv) +
                         " are not supported (multiples of 8, Dk up to 128, "
                         "Dv up to 256)");
-    if (!std::isfinite(in->scale))
-        return fail(RWKV7M_ERR_INVALID_ARGUMENT, f + ": scale is not finite");
+    if (!std::isfinite(float(in->scale)))
+        return fail(RWKV7M_ERR_INVALID_ARGUMENT,
+                    f + ": scale is not finite in fp32");
     // (launches have fewer than 2^32 threads along an axis, chunk kernels up to
     // 512 a chunk, the chains up to four workgroups of 512 a head)
     const int64_t C = rwkv7m::kGdrChunk, most = (int64_t(1) << 23) - 1;
