@@ -28,8 +28,9 @@
  *
  * Sums and states are fp32, products bf16 matrix instructions over sums of
  * three bf16 planes, which hold what fp32 does: results are off as with fp32
- * products, some 2e-7 of their norm, up to 3e-6 where beta |k|^2 nears 2 and
- * keys hardly differ, before they are rounded to their own type.  Calls only
+ * products, some 2e-7 to 5e-7 of their norm (dg, a small sum of large terms, up
+ * to 2e-6; all up to 3e-6 where beta |k|^2 nears 2 and keys hardly differ),
+ * before they are rounded to their own type.  Calls only
  * enqueue work on `stream`, never allocate and never synchronise, so they may
  * be captured in a HIP graph.  Results do not depend on the order in which
  * workgroups run, nor a sequence's on the others in its batch.
