@@ -166,3 +166,29 @@ def test_many_heads(lm, dtype, B, Hk, Hv, T, Dv, Dk):
                                  ds[rows])
         check_norms({n: (a[rows], w) for n, a, w in
                      zip(names, whole, [*outs, *grads])}, 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_broadcast_gates_and_cotangents(lm, dtype):
+    """One gate for all heads or tokens, one key for all, and the cotangents of
+    sums (all of one number): as the same ones written out."""
+    print("case: broadcast", dtype, flush=True)
+    q, k, v, g, beta = (t.cuda() for t in make(2, 100, 2, 4, 64, 32, dtype,
+                                               seed=31))
+    s0 = torch.randn(1, 4, 32, 64, generator=_gen(1)).cuda()
+    s0 = s0.expand(2, -1, -1, -1)
+    x = (q[:1].expand(2, -1, -1, -1), k[:, :1].expand(-1, 100, -1, -1),
+         v[:, :, :1].expand(-1, -1, 4, -1), g[..., :1].expand(-1, -1, 4),
+         beta[:, :1].expand(-1, 100, -1), s0)
+    found = []
+    for place in (lambda t: t.detach(), lambda t: t.detach().contiguous()):
+        leaves = [place(t).requires_grad_() for t in x]
+        o, end = lm.gated_delta_rule(*leaves)
+        ones = [place(t.new_ones(()).expand(t.shape)) for t in (o, end)]
+        found.append([o, end, *torch.autograd.grad((o, end), leaves, ones)])
+        state = s0.contiguous()
+        with torch.no_grad():
+            found[-1] += [lm.gated_delta_step(*(t[:, :4] for t in leaves[:5]),
+                                              state), state]
+    for a, b in zip(*found):
+        assert torch.equal(a, b)

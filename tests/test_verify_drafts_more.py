@@ -154,3 +154,47 @@ def test_what_is_drawn_where_nothing_is_left(lm, dtype, V):
     # without a draft's logits p itself is drawn from: nothing is set aside
     other, *_ = _call(lm, x, tok, s=s)
     assert torch.equal(took, other)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_ends_of_the_temperatures(lm, dtype):
+    """At 1e-30 as the greedy form, whatever the random numbers and however far
+    the logits, at 1e30 as a flat row."""
+    print("case: temperatures", dtype, flush=True)
+    g = torch.Generator().manual_seed(8)
+    V = 9001
+    x = (3e37 * torch.randn(6, 3, V, generator=g)).to(dtype)
+    x[:, :, 8999] = 3e38  # (one likeliest token each)
+    x[3:, 1, 8999], x[3:, 1, 17] = -float("inf"), 3.1e38
+    tok = torch.full((6, 2), 8999)
+    u, s = torch.rand(6, 2, generator=g), torch.rand(6, generator=g)
+    cold = _call(lm, x, tok, None, u, s, 1e-30)
+    greedy = _call(lm, x, tok, temp=0.0)
+    assert all(torch.equal(a, b) for a, b in zip(cold, greedy))
+    assert cold[1].tolist() == [2, 2, 2, 1, 1, 1]
+    flat = torch.randn(6, 1, V, generator=g).to(dtype)
+    took, *_ = _call(lm, flat, torch.zeros(6, 0).long(), None,
+                     torch.zeros(6, 0), s, 1e30)
+    # (a flat row's running sum is the id, but for rounding)
+    assert bool(((took[:, 0] - (s.double() * V).floor()).abs() <= 1).all())
+
+
+@pytest.mark.gpu
+def test_a_vocabulary_of_a_million(lm):
+    print("case: a million", flush=True)
+    g = torch.Generator().manual_seed(9)
+    V = 1000003
+    x = torch.randn(2, 2, V, generator=g)
+    tok = torch.tensor([[V - 1], [5]])
+    s = torch.tensor([0.25, 0.999])
+    took, count, chance = _call(lm, x, tok, None, torch.full((2, 1), 0.5), s)
+    p = torch.softmax(x.double(), -1)
+    assert not count.any()
+    off = chance[:, 0].double() - p[[0, 1], 0, tok[:, 0]]
+    assert float(off.abs().max()) <= 1e-7 * float(chance.max())
+    p[[0, 1], 0, tok[:, 0]] = 0.0
+    cum = p[:, 0].cumsum(-1)
+    at = s.double()[:, None] * cum[:, -1:]
+    assert float((cum - at).abs().min()) > 1e-9
+    assert took[:, 0].tolist() == (cum <= at).sum(-1).tolist()
